@@ -47,6 +47,8 @@ extern "C" {
 #define QB200_Q4_K 2   /* 256 values / 144 bytes                                          */
 #define QB200_Q6_K 3   /* 256 values / 210 bytes                                          */
 #define QB200_F32 100  /* plain float32 lanes                                             */
+#define QB200_F16 101  /* float16 lanes: rows of the cache operators only                  */
+#define QB200_BF16 102 /* bfloat16 lanes: rows of the cache operators only                 */
 
 /* Argument errors (negative returns). */
 #define QB200_E_FORMAT (-1)     /* format not taken by this entry point                    */
@@ -59,6 +61,8 @@ extern "C" {
 /* Operations, for qb200_lane_name. */
 #define QB200_OP_GEMV 0
 #define QB200_OP_MATMUL 1
+#define QB200_OP_CACHE 2       /* qb200_cache_write, qb200_cache_read */
+#define QB200_OP_ATTENTION 3   /* qb200_cache_attention */
 
 typedef struct qb200_caps {
     int device;              /* ordinal the library is bound to                              */
@@ -87,7 +91,9 @@ const char *qb200_lane_name(int op, int fmt_a);
 
 /* Reads and clears the device-side status word.  0 = every kernel so far ran to the end;
  * non-zero = a bounded wait inside a kernel gave up (bit 0: gemv ring, bit 1: A.B^T pipeline,
- * bit 2: a sharded product's wait for its peers).
+ * bit 2: a sharded product's wait for its peers, bit 3: attention's pipeline), or a cache call met data
+ * it had to leave out (bit 4: a page, length or row outside the cache, the table or the rows given;
+ * bit 5: a NaN or an infinity was written into a cache).
  * Synchronizes the device. */
 int qb200_device_status(int *status);
 
@@ -272,6 +278,70 @@ int qb200_shard_gemv_after(int fmt_a, int fmt_x, const void *a_shard, const void
 int qb200_ipc_export(const void *ptr, void *handle64);
 int qb200_ipc_import(const void *handle64, void **ptr);
 int qb200_ipc_close(void *ptr);
+
+/* ---- a cache of keys and values in 8 bits, and attention over it ---------------------------
+ * No counterpart in the reference, which keeps keys and values in its plain types.  The block products above serve a
+ * model's weights; this is the same idea for what attention keeps: int8 codes with one f32 scale for each block, a block
+ * being `page` consecutive tokens of one sequence in one head.  A stored value is code * scale.
+ *
+ * qb200_cache: the codes are int8 [pages][heads][page][dim], 16-byte aligned; the scales f32 [pages][heads].  page is 16,
+ * 32, 64 or 128 tokens, dim a multiple of 16 up to 256.  Nothing needs initialising: a block's scale and codes are read
+ * only once a token of the sequence has been written into it.
+ *
+ * qb200_sequences: `count` sequences whose rows (a row = one token of the call) lie behind one another.  table[b * width + i]
+ * is the page that holds tokens i*page .. i*page + page - 1 of sequence b; lengths[b] is explained at each call;
+ * offsets[0 .. count] says that the rows of sequence b are offsets[b] .. offsets[b+1] - 1 (NULL: one row a sequence);
+ * rows is how many rows the lane arrays have: rows past offsets[count] are neither read nor written.  All arrays are on
+ * the device, and the calls read them there: nothing is synchronised.  A page or length outside the cache or the table
+ * is left out and sets bit 4 of the status word; nothing is read or written out of bounds.
+ *
+ * Lane arrays (k, v, q, out) are f32, f16 or bf16 (`type`); element (row, head, i) is at row * row_stride + head *
+ * head_stride + i, strides in elements.  Where base and strides are multiples of 16 bytes the loads are wide. */
+typedef struct qb200_cache {
+    void *k_codes, *v_codes;
+    float *k_scales, *v_scales;
+    int pages, heads, page, dim;
+} qb200_cache_t;
+typedef struct qb200_sequences {
+    const int32_t *table;
+    const int32_t *lengths;
+    const int32_t *offsets;
+    int count, width, rows;
+} qb200_sequences_t;
+
+/* Writes the rows of k and v as tokens lengths[b], lengths[b] + 1, ... of their sequences (lengths[b] = tokens that are
+ * in the cache already).  The definition, block by block: let a be the largest magnitude written into the block, s the
+ * block's scale if earlier tokens of the sequence lie in it, else 0, n = a * (1/127) in f32 (both rounded).  Where n <= s the scale stays s;
+ * else it becomes max(n, 1.25 * s), and the earlier tokens' codes c become the integer nearest c * s / scale (a scale
+ * that has to grow grows by a quarter at least, so that however many tokens arrive one by one, rounding again and again
+ * costs a code 2.5 steps at most).  New codes are the integers nearest x / scale, ties to even, from the exact quotients.  A block of zeros has
+ * scale 0.  A NaN is stored as 0 and an infinity as the code +-127; neither enters a, and both set bit 5 of the status word.
+ * Two calls that write the same block must be ordered (one stream, or an event); a page written to must not belong to two
+ * sequences of a call. */
+int qb200_cache_write(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const void *k, int64_t k_row_stride,
+                      int64_t k_head_stride, const void *v, int64_t v_row_stride, int64_t v_head_stride, void *stream);
+/* Reads tokens lengths[b], lengths[b] + 1, ... of the sequences back into the rows of k and v (either may be NULL):
+ * code * scale in f32, rounded once to `type`.  (lengths[b] = the first token read.)  Rows of tokens that lie outside the
+ * table or the cache are left as they were. */
+int qb200_cache_read(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, void *k, int64_t k_row_stride,
+                     int64_t k_head_stride, void *v, int64_t v_row_stride, int64_t v_head_stride, void *stream);
+
+/* out = softmax(scale * q . K^T) . V over the cache, q_heads query heads in groups of q_heads / cache->heads that share a
+ * head of the cache.  lengths[b] = tokens of sequence b to attend to, the call's own among them (write them first).  With
+ * `causal` the rows of a sequence are its last tokens: row i of n sees tokens up to lengths[b] - n + i, and with window
+ * w > 0 only the last w of those (window needs causal).  A row that sees nothing gets zeros, and minus infinity in lse.
+ *   lse: optional, f32 [rows][q_heads]: the logarithm of the sum of exp(scale * q . k) over what the row sees.
+ *   max_queries, max_length: bounds on the rows of a sequence and on lengths[b], for the choice of kernel and the split of
+ *   the work; the results do not depend on them beyond the order of sums.  0: rows (1 without offsets), width * page.
+ *   Sums, softmax statistics and the accumulators are f32; q and the weights enter the tensor cores in f16 (f32 lanes: as
+ *   the sum of two f16), the codes exactly.
+ *   workspace: device scratch of qb200_cache_attention_workspace_bytes(...) bytes, 16-byte aligned, private to the call
+ *   until it completes on `stream`; needed even where no sequence turns out to be split. */
+size_t qb200_cache_attention_workspace_bytes(const qb200_cache_t *cache, int type, int count, int rows, int q_heads, int max_queries, int max_length);
+int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const void *q, int64_t q_row_stride,
+                          int64_t q_head_stride, void *out, int64_t out_row_stride, int64_t out_head_stride, float *lse, int q_heads,
+                          int max_queries, int max_length, float scale, int causal, int window, void *workspace, size_t workspace_bytes,
+                          void *stream);
 
 /* ---- plain device memory for hosts without a CUDA binding of their own (tests, bench) ---- */
 int qb200_malloc(void **ptr, size_t bytes);

@@ -19,6 +19,7 @@ stand in for model weights, which are not available offline.
 import numpy as np
 
 Q8_0, Q4_0, Q4_K, Q6_K, F32 = 0, 1, 2, 3, 100
+F16, BF16 = 101, 102          # lanes of the cache operators' rows (not block formats)
 NAMES = {Q8_0: "q8_0", Q4_0: "q4_0", Q4_K: "q4_k", Q6_K: "q6_k", F32: "f32"}
 IDS = {v: k for k, v in NAMES.items()}
 BLOCK_VALUES = {Q8_0: 32, Q4_0: 32, Q4_K: 256, Q6_K: 256}

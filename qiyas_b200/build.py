@@ -11,8 +11,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIBRARY = os.path.join(HERE, "libqiyas_b200.so")
-SOURCES = ["api.cu", "gemv.cu", "codecs.cu", "matmul.cu", "shard.cu"]
+SOURCES = ["api.cu", "gemv.cu", "codecs.cu", "matmul.cu", "shard.cu", "cache.cu", "attend_rows.cu"]
 HEADERS = ["common.cuh", "launch.h", "encode_blocks.cuh", os.path.join("..", "..", "include", "qiyas_b200.h")]
+# headers that only some sources include
+OWN_HEADERS = {"cache.h": ["api.cu", "cache.cu", "attend_rows.cu"], "cache_device.cuh": ["cache.cu", "attend_rows.cu"],
+               "attend_device.cuh": ["attend_rows.cu"]}
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--compiler-options", "-fPIC",
          "-Xptxas", "-v"]
 
@@ -38,14 +41,15 @@ def _stale_object(src, headers_time):
     if not os.path.exists(obj):
         return True
     built = os.path.getmtime(obj)
-    return os.path.getmtime(os.path.join(CSRC, src)) > built or headers_time > built
+    own = [src] + [h for h, users in OWN_HEADERS.items() if src in users]
+    return headers_time > built or any(os.path.getmtime(os.path.join(CSRC, f)) > built for f in own)
 
 
 def stale():
     if not os.path.exists(LIBRARY):
         return True
     built = os.path.getmtime(LIBRARY)
-    return any(os.path.getmtime(os.path.join(CSRC, f)) > built for f in SOURCES + HEADERS)
+    return any(os.path.getmtime(os.path.join(CSRC, f)) > built for f in SOURCES + HEADERS + list(OWN_HEADERS))
 
 
 def build(force=False, verbose=False):

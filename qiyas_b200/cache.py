@@ -1,0 +1,56 @@
+"""A cache of keys and values in 8 bits: int8 codes with one f32 scale for each block, a block being a page of consecutive
+tokens of one sequence in one head.  ``GpuOps.CacheWrite``, ``CacheRead`` and ``CacheAttention`` work on it; the reference
+has no counterpart (it keeps keys and values in its plain types).
+
+``BlockCache`` holds the four device arrays:
+
+========  ======================================  ============================================================
+k_codes   int8 [pages, heads, page, dim]          page: 16, 32, 64 or 128 tokens; dim: a multiple of 16 up to 256
+v_codes   int8 [pages, heads, page, dim]
+k_scales  float32 [pages, heads]                  a stored value is code * scale
+v_scales  float32 [pages, heads]
+========  ======================================  ============================================================
+
+Which pages belong to which sequence is the caller's: an int32 table [sequences, width] on the device, entry [b, i] naming
+the page that holds tokens i * page .. i * page + page - 1 of sequence b.
+"""
+from . import _lib
+
+PAGES = (16, 32, 64, 128)
+
+
+class BlockCache:
+    """The arrays of a cache, checked once; nothing is copied."""
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales):
+        import torch
+        if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
+            raise ValueError(f"codes are [pages, heads, page, dim] twice: got {tuple(k_codes.shape)}, {tuple(v_codes.shape)}")
+        pages, heads, page, dim = k_codes.shape
+        if tuple(k_scales.shape) != (pages, heads) or tuple(v_scales.shape) != (pages, heads):
+            raise ValueError(f"scales are [pages, heads] = {(pages, heads)}: got {tuple(k_scales.shape)}, {tuple(v_scales.shape)}")
+        if page not in PAGES or dim % 16 or not 0 < dim <= 256:
+            raise NotImplementedError(f"blocks of {page} tokens x {dim}: 16, 32, 64 or 128 tokens, and dim a multiple of 16 up to 256")
+        for name, t, kind in (("k_codes", k_codes, torch.int8), ("v_codes", v_codes, torch.int8),
+                              ("k_scales", k_scales, torch.float32), ("v_scales", v_scales, torch.float32)):
+            if t.dtype != kind or not t.is_contiguous() or t.device != k_codes.device:
+                raise ValueError(f"{name}: contiguous {kind} on {k_codes.device} is needed, got {t.dtype} on {t.device}")
+        self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
+        self.pages, self.heads, self.page, self.dim = pages, heads, page, dim
+        self.device = k_codes.device
+        self.parts = _lib.CacheParts(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages, heads, page, dim)
+
+    @classmethod
+    def empty(cls, pages, heads, page, dim, device="cuda:0"):
+        """A cache of `pages` pages; nothing in it needs initialising."""
+        import torch
+        codes = [torch.empty(pages, heads, page, dim, dtype=torch.int8, device=device) for _ in range(2)]
+        scales = [torch.empty(pages, heads, dtype=torch.float32, device=device) for _ in range(2)]
+        return cls(*codes, *scales)
+
+    @property
+    def nbytes(self):
+        return 2 * self.pages * self.heads * (self.page * self.dim + 4)
+
+
+__all__ = ["BlockCache", "PAGES"]

@@ -6,6 +6,7 @@
 
 #include "common.cuh"
 #include "launch.h"
+#include "cache.h"
 
 namespace {
 
@@ -61,6 +62,8 @@ const char *fmt_name(int fmt)
     case QB200_Q4_K: return "q4_k";
     case QB200_Q6_K: return "q6_k";
     case QB200_F32: return "f32";
+    case QB200_F16: return "f16";
+    case QB200_BF16: return "bf16";
     default: return "?";
     }
 }
@@ -159,6 +162,8 @@ int qb200_init(int device)
     if ((e = qb::gemv_init(g_caps.sm_count, g_caps.max_shared_bytes, g_status))) return cuda_fail(e, "gemv attributes");
     if ((e = qb::matmul_init(g_caps.sm_count, g_caps.max_shared_bytes, g_status))) return cuda_fail(e, "matmul attributes");
     if ((e = qb::shard_init(g_status))) return cuda_fail(e, "shard set-up");
+    if ((e = qb::cache_init(g_status))) return cuda_fail(e, "cache set-up");
+    if ((e = qb::attend_init(g_caps.sm_count, g_caps.max_shared_bytes, g_status))) return cuda_fail(e, "attention set-up");
     g_ready = true;
     t_error[0] = 0;
     return 0;
@@ -179,7 +184,7 @@ int qb200_block_product_available(void) { return g_ready && g_caps.tcgen05 ? 1 :
 const char *qb200_lane_name(int op, int fmt_a)
 {
     (void)fmt_a;
-    return op == QB200_OP_MATMUL ? "s8 tcgen05 blocks" : "s8dp blocks";
+    return op == QB200_OP_MATMUL ? "s8 tcgen05 blocks" : op == QB200_OP_CACHE ? "s8 cache blocks" : op == QB200_OP_ATTENTION ? "f16 mma cache blocks" : "s8dp blocks";
 }
 
 int qb200_device_status(int *status)
@@ -423,6 +428,128 @@ int qb200_decode(int fmt, const void *blocks, float *lanes, int64_t n, void *str
     if (n < 0 || n > 2147483647LL) return fail(QB200_E_SHAPE, "count %lld", (long long)n);
     if (n && (!lanes || !blocks || ((uintptr_t)lanes & 3))) return fail(QB200_E_POINTER, "null or misaligned operand");
     return finish_other(qb::decode_launch(fmt, blocks, lanes, n, (cudaStream_t)stream), "decode", stream);
+}
+
+// ---- the 8-bit cache
+
+// A call's kernels run on the device the library is bound to, whichever is current.
+namespace {
+struct OnDevice {
+    int before = -1;
+    cudaError_t e;
+    OnDevice()
+    {
+        if (!g_ready) { e = cudaErrorInitializationError; return; }
+        e = cudaGetDevice(&before);
+        if (!e && before != g_caps.device) e = cudaSetDevice(g_caps.device);
+    }
+    ~OnDevice()
+    {
+        if (before >= 0 && before != g_caps.device) cudaSetDevice(before);
+    }
+};
+}  // namespace
+
+static int check_cache(const qb200_cache_t *c, const qb200_sequences_t *s, int type)
+{
+    if (!c || !s) return fail(QB200_E_POINTER, "null cache or sequences");
+    if (type != QB200_F32 && type != QB200_F16 && type != QB200_BF16) return fail(QB200_E_FORMAT, "%s: the cache's rows are f32, f16 or bf16 lanes", fmt_name(type));
+    if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128) return fail(QB200_E_SHAPE, "page %d: a block has 16, 32, 64 or 128 tokens", c->page);
+    if (c->dim <= 0 || c->dim > 256 || c->dim % 16) return fail(QB200_E_SHAPE, "dim %d: a multiple of 16 up to 256", c->dim);
+    if (c->pages <= 0 || c->heads <= 0) return fail(QB200_E_SHAPE, "a cache of %d pages and %d heads", c->pages, c->heads);
+    if (c->heads > 65535) return fail(QB200_E_LIMIT, "heads %d: at most 65535", c->heads);
+    if ((int64_t)c->pages * c->heads * c->page > 2147483647LL)
+        return fail(QB200_E_LIMIT, "%d pages x %d heads x %d tokens: at most 2^31 - 1 rows of codes", c->pages, c->heads, c->page);
+    if (!c->k_codes || !c->v_codes || !c->k_scales || !c->v_scales) return fail(QB200_E_POINTER, "the cache has a null part");
+    if (((uintptr_t)c->k_codes & 15) || ((uintptr_t)c->v_codes & 15)) return fail(QB200_E_POINTER, "the cache's codes are 16-byte aligned");
+    if (((uintptr_t)c->k_scales & 3) || ((uintptr_t)c->v_scales & 3)) return fail(QB200_E_POINTER, "misaligned scales");
+    if (s->count < 0 || s->width < 0 || s->rows < 0) return fail(QB200_E_SHAPE, "count %d, width %d, rows %d", s->count, s->width, s->rows);
+    if ((int64_t)s->width * c->page > 2147483647LL - 1024) return fail(QB200_E_LIMIT, "width %d: a sequence has at most 2^31 - 1025 tokens", s->width);
+    if (s->count > (1 << 24)) return fail(QB200_E_LIMIT, "count %d: at most 2^24 sequences", s->count);
+    if (!s->offsets && s->rows < s->count) return fail(QB200_E_SHAPE, "%d sequences of one row each in %d rows", s->count, s->rows);
+    if (s->count > 0 && (!s->lengths || (s->width > 0 && !s->table))) return fail(QB200_E_POINTER, "null table or lengths");
+    if (((uintptr_t)s->table & 3) || ((uintptr_t)s->lengths & 3) || ((uintptr_t)s->offsets & 3)) return fail(QB200_E_POINTER, "misaligned table, lengths or offsets");
+    return 0;
+}
+
+static int check_lanes(const char *name, int type, const void *base, int64_t row, int64_t head, int rows, int heads)
+{
+    if (rows > 0 && !base) return fail(QB200_E_POINTER, "%s: null", name);
+    if ((uintptr_t)base & (type == QB200_F32 ? 3 : 1)) return fail(QB200_E_POINTER, "%s: misaligned", name);
+    const int64_t most = (int64_t)1 << 55;        // products with 32-bit counts stay inside 64 bits of bytes
+    if (row < 0 || head < 0 || row > most / ((int64_t)rows + 1) || head > most / ((int64_t)heads + 1)) return fail(QB200_E_SHAPE, "%s: strides %lld, %lld", name, (long long)row, (long long)head);
+    return 0;
+}
+
+int qb200_cache_write(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const void *k, int64_t k_row_stride,
+                      int64_t k_head_stride, const void *v, int64_t v_row_stride, int64_t v_head_stride, void *stream)
+{
+    int rc = check_cache(cache, sequences, type);
+    if (rc) return rc;
+    if ((rc = check_lanes("k", type, k, k_row_stride, k_head_stride, sequences->rows, cache->heads))) return rc;
+    if ((rc = check_lanes("v", type, v, v_row_stride, v_head_stride, sequences->rows, cache->heads))) return rc;
+    OnDevice on;
+    if (!g_ready) return fail(QB200_E_DEVICE, "qb200_init has not succeeded");
+    if (on.e) return cuda_fail(on.e, "cudaSetDevice");
+    return finish_other(qb::cache_write(*cache, *sequences, type, {const_cast<void *>(k), k_row_stride, k_head_stride},
+                                        {const_cast<void *>(v), v_row_stride, v_head_stride}, (cudaStream_t)stream), "cache_write", stream);
+}
+
+int qb200_cache_read(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, void *k, int64_t k_row_stride,
+                     int64_t k_head_stride, void *v, int64_t v_row_stride, int64_t v_head_stride, void *stream)
+{
+    int rc = check_cache(cache, sequences, type);
+    if (rc) return rc;
+    if (k && (rc = check_lanes("k", type, k, k_row_stride, k_head_stride, sequences->rows, cache->heads))) return rc;
+    if (v && (rc = check_lanes("v", type, v, v_row_stride, v_head_stride, sequences->rows, cache->heads))) return rc;
+    if (!k && !v) return fail(QB200_E_POINTER, "neither k nor v is asked for");
+    OnDevice on;
+    if (!g_ready) return fail(QB200_E_DEVICE, "qb200_init has not succeeded");
+    if (on.e) return cuda_fail(on.e, "cudaSetDevice");
+    return finish_other(qb::cache_read(*cache, *sequences, type, {k, k_row_stride, k_head_stride}, {v, v_row_stride, v_head_stride}, (cudaStream_t)stream),
+                        "cache_read", stream);
+}
+
+// The bounds a caller leaves open.
+static void attention_bounds(const qb200_cache_t *c, const qb200_sequences_t *s, int &max_queries, int &max_length)
+{
+    const int rows = s->offsets ? s->rows : 1, most = s->width * c->page;
+    if (max_queries <= 0 || max_queries > rows) max_queries = rows > 0 ? rows : 1;
+    if (max_length <= 0 || max_length > most) max_length = most > 0 ? most : 1;
+}
+
+size_t qb200_cache_attention_workspace_bytes(const qb200_cache_t *cache, int type, int count, int rows, int q_heads, int max_queries, int max_length)
+{
+    if (!cache || cache->heads <= 0 || q_heads <= 0 || q_heads % cache->heads || cache->dim <= 0 || cache->dim > 256 || count < 0 || rows < 0) return 0;
+    if (max_queries <= 0 || max_queries > rows) max_queries = rows > 0 ? rows : 1;
+    return qb::attend_workspace_bytes(cache->dim, cache->heads, type, count, rows, q_heads, max_queries, max_length);
+}
+
+int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const void *q, int64_t q_row_stride,
+                          int64_t q_head_stride, void *out, int64_t out_row_stride, int64_t out_head_stride, float *lse, int q_heads,
+                          int max_queries, int max_length, float scale, int causal, int window, void *workspace, size_t workspace_bytes,
+                          void *stream)
+{
+    int rc = check_cache(cache, sequences, type);
+    if (rc) return rc;
+    if (q_heads <= 0 || q_heads % cache->heads) return fail(QB200_E_SHAPE, "%d query heads over %d heads of the cache: a whole group each", q_heads, cache->heads);
+    if ((int64_t)q_heads * sequences->rows > 2147483647LL - 65536) return fail(QB200_E_LIMIT, "%d rows x %d heads: at most 2^31 - 65537", sequences->rows, q_heads);
+    if ((rc = check_lanes("q", type, q, q_row_stride, q_head_stride, sequences->rows, q_heads))) return rc;
+    if ((rc = check_lanes("out", type, out, out_row_stride, out_head_stride, sequences->rows, q_heads))) return rc;
+    if ((uintptr_t)lse & 3) return fail(QB200_E_POINTER, "misaligned lse");
+    if (window < 0 || (window > 0 && !causal)) return fail(QB200_E_SHAPE, "window %d: a window looks back from a row's own token, so it needs causal", window);
+    if (!(scale == scale) || scale - scale != 0.f) return fail(QB200_E_SHAPE, "scale is not a finite number");
+    if (max_queries < 0 || max_length < 0) return fail(QB200_E_SHAPE, "max_queries %d, max_length %d", max_queries, max_length);
+    attention_bounds(cache, sequences, max_queries, max_length);
+    const size_t need = qb::attend_workspace_bytes(cache->dim, cache->heads, type, sequences->count, sequences->rows, q_heads, max_queries, max_length);
+    if (!workspace || workspace_bytes < need) return fail(QB200_E_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
+    if ((uintptr_t)workspace & 15) return fail(QB200_E_WORKSPACE, "workspace not 16-byte aligned");
+    OnDevice on;
+    if (!g_ready) return fail(QB200_E_DEVICE, "qb200_init has not succeeded");
+    if (on.e) return cuda_fail(on.e, "cudaSetDevice");
+    qb::AttendCall call = { *cache, *sequences, {const_cast<void *>(q), q_row_stride, q_head_stride}, {out, out_row_stride, out_head_stride}, lse,
+                            type, q_heads, max_queries, max_length, causal != 0, window, scale, workspace };
+    return finish_other(qb::attend(call, (cudaStream_t)stream), "cache_attention", stream);
 }
 
 int qb200_shard_range(int rows, int world, int rank, int *first, int *count)

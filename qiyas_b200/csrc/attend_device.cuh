@@ -1,0 +1,334 @@
+// What the attention kernels share: how a call's work is cut into shares, the rows' limits, and the products' operands.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "cache.h"
+#include "cache_device.cuh"
+
+namespace qb {
+
+constexpr float NOTHING = -1e30f;              // a maximum over nothing (finite: differences of two of them are 0)
+constexpr int TILE_TOKENS = 32;                // tokens a tile of the line of work
+constexpr int LEAST_TILES = 8;                 // tiles a share has at least
+
+struct AttendArgs {
+    qb200_sequences_t seq;
+    Lanes q, out;
+    float *lse;
+    const float *k_scales, *v_scales;
+    int pages, heads, dim, log_page, group, q_heads, causal, window;
+    float scale;
+    int q_wide, out_wide;
+    int whole;                                 // units are not cut: block c takes units c, c + grid, ...
+    int chunks;                                // units a sequence and head, by the caller's bound
+    int grid;
+    void *workspace;
+    int *status;
+};
+
+// R rows of one head of one sequence: rows r0 .. r1 - 1 of its queries x group, and the tokens they see together.
+struct Unit {
+    int b, h, rc;
+    int row, n, len;                           // the sequence: first row, rows, tokens
+    int r0, r1;
+    int lo, hi;                                // tokens that any of the rows sees
+    int t0, nt;                                // tiles: at least one, so that rows that see nothing are written too
+};
+
+__host__ __device__ constexpr size_t part_floats(int r, int dim) { return (size_t)r * (dim + 2); }
+
+template <int R>
+__device__ __forceinline__ Unit unit_of(const AttendArgs &p, int b, int h, int rc)
+{
+    Unit u;
+    u.b = b;
+    u.h = h;
+    u.rc = rc;
+    bool bad;
+    seq_rows(p.seq, b, u.row, u.n, bad);
+    u.len = p.seq.lengths[b];
+    const int most = p.seq.width << p.log_page;
+    bad |= u.len < 0 || u.len > most;
+    u.len = max(0, min(u.len, most));
+    if (bad && (threadIdx.x & 31) == 0) atomicOr(p.status, STATUS_CACHE_RANGE);
+    u.r0 = rc * R;
+    u.r1 = min(u.r0 + R, u.n * p.group);
+    const int first = u.r0 / p.group, last = (max(u.r1, 1) - 1) / p.group;
+    u.hi = p.causal ? max(0, min(u.len, u.len - u.n + last + 1)) : u.len;
+    u.lo = p.window ? max(0, u.len - u.n + first + 1 - p.window) : 0;
+    u.t0 = u.hi > u.lo ? u.lo / TILE_TOKENS : 0;
+    u.nt = u.hi > u.lo ? (u.hi + TILE_TOKENS - 1) / TILE_TOKENS - u.t0 : 1;
+    return u;
+}
+
+// The tokens row `at` of a unit's sequence sees.
+__device__ __forceinline__ void row_limits(const AttendArgs &p, const Unit &u, int at, int &lo, int &hi)
+{
+    const int place = u.len - u.n + at / p.group;
+    hi = p.causal ? max(0, min(u.len, place + 1)) : u.len;
+    lo = p.window ? max(0, place + 1 - p.window) : 0;
+}
+
+// ---------------------------------------------------------------------------------- shares
+template <int R>
+__device__ __forceinline__ int chunks_of(const AttendArgs &p, int b)
+{
+    int row, n;
+    bool bad;
+    seq_rows(p.seq, b, row, n, bad);
+    return (n * p.group + R - 1) / R;
+}
+
+// Tiles of one head of sequence b.
+template <int R>
+__device__ __forceinline__ int64_t tiles_of(const AttendArgs &p, int b)
+{
+    int64_t sum = 0;
+    const int chunks = chunks_of<R>(p, b);
+    for (int rc = 0; rc < chunks; rc++) sum += unit_of<R>(p, b, 0, rc).nt;
+    return sum;
+}
+
+struct Start {
+    int b, h, rc, tile;                        // where a share begins: a unit and a tile inside it
+    int64_t left;                              // tiles it has
+};
+
+// Called by a whole warp: the place `x` on the line of tiles, sequence after sequence, head after head; `total` is its length.
+template <int R>
+__device__ __forceinline__ int64_t line_length(const AttendArgs &p)
+{
+    const int lane = threadIdx.x & 31;
+    int64_t sum = 0;
+    for (int b = lane; b < p.seq.count; b += 32) sum += tiles_of<R>(p, b);
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    return sum * p.heads;
+}
+template <int R>
+__device__ __forceinline__ Start place_on_line(const AttendArgs &p, int64_t x)
+{
+    const int lane = threadIdx.x & 31;
+    Start s = {0, 0, 0, 0, 0};
+    int64_t before = 0;
+    for (int base = 0; base < p.seq.count; base += 32) {
+        const int64_t mine = base + lane < p.seq.count ? tiles_of<R>(p, base + lane) * p.heads : 0;
+        int64_t upto = mine;
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t other = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += other;
+        }
+        const unsigned after = __ballot_sync(0xffffffffu, before + upto > x);
+        if (after) {
+            const int k = __ffs(after) - 1;
+            s.b = base + k;
+            const int64_t tiles = __shfl_sync(0xffffffffu, mine, k) / p.heads;
+            int64_t rest = x - (before + __shfl_sync(0xffffffffu, upto - mine, k));
+            s.h = (int)(rest / tiles);
+            rest -= s.h * tiles;
+            for (;;) {
+                const int nt = unit_of<R>(p, s.b, s.h, s.rc).nt;
+                if (rest < nt) break;
+                rest -= nt;
+                s.rc++;
+            }
+            s.tile = (int)rest;
+            return s;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    s.b = p.seq.count;
+    return s;
+}
+// Shares there are: one a block, but none of less than LEAST_TILES tiles unless every unit has one.
+__device__ __forceinline__ int64_t shares_of(const AttendArgs &p, int64_t total)
+{
+    const int64_t units = (int64_t)p.seq.count * p.heads * p.chunks;
+    return max((int64_t)1, min(min((int64_t)p.grid, total), max(units, total / LEAST_TILES)));
+}
+template <int R>
+__device__ __forceinline__ Start start_of(const AttendArgs &p, int block)
+{
+    const int64_t total = line_length<R>(p), shares = shares_of(p, total);
+    Start s = {0, 0, 0, 0, 0};
+    if (block >= shares) return s;
+    const int64_t from = total * block / shares, to = total * (block + 1) / shares;
+    if (to > from) s = place_on_line<R>(p, from);
+    s.left = to - from;
+    return s;
+}
+
+struct Cut {
+    int b, h, rc;
+    int block, parts;                          // parts: 0, or how many blocks from block - 1 on hold parts of the unit
+};
+template <int R>
+__device__ __forceinline__ Cut cut_of(const AttendArgs &p, int block)
+{
+    const int64_t total = line_length<R>(p), shares = shares_of(p, total);
+    Cut c = {0, 0, 0, block, 0};
+    if (block >= shares) return c;
+    const int64_t from = total * block / shares, before = total * (block - 1) / shares;
+    if (from >= total) return c;
+    const Start s = place_on_line<R>(p, from);
+    if (s.tile == 0 || before > from - s.tile) return c;      // not inside a unit, or not the first boundary inside it
+    const int64_t end = from - s.tile + unit_of<R>(p, s.b, s.h, s.rc).nt;
+    c.b = s.b;
+    c.h = s.h;
+    c.rc = s.rc;
+    c.parts = 1;
+    for (int64_t k = block; k < shares && total * k / shares < end; k++) c.parts++;
+    return c;
+}
+
+struct Piece {                                 // tiles first .. first + count - 1 of a unit
+    Unit unit;
+    int first, count;
+};
+
+// The pieces of a block's share, one after the other.
+template <int R>
+struct Walk {
+    const AttendArgs &p;
+    int b, h, rc, tile;
+    int64_t left;
+    int64_t next_unit;                         // whole: the next unit's number
+
+    __device__ __forceinline__ Walk(const AttendArgs &args, const Start &s) : p(args), b(s.b), h(s.h), rc(s.rc), tile(s.tile), left(s.left), next_unit(blockIdx.x)
+    {
+        if (p.whole) rc = -1;
+    }
+
+    __device__ __forceinline__ bool next(Piece &piece)
+    {
+        if (p.whole) {
+            for (;;) {
+                if (rc >= 0) rc += p.chunks;               // more rows than the caller's bound said
+                else {
+                    if (next_unit >= (int64_t)p.seq.count * p.heads * p.chunks) return false;
+                    rc = (int)(next_unit % p.chunks);
+                    const int64_t bh = next_unit / p.chunks;
+                    h = (int)(bh % p.heads);
+                    b = (int)(bh / p.heads);
+                    next_unit += gridDim.x;
+                }
+                if (rc < chunks_of<R>(p, b)) {
+                    piece.unit = unit_of<R>(p, b, h, rc);
+                    piece.first = 0;
+                    piece.count = piece.unit.nt;
+                    return true;
+                }
+                rc = -1;
+            }
+        }
+        if (left <= 0 || b >= p.seq.count) return false;
+        while (rc >= chunks_of<R>(p, b)) {
+            rc = 0;
+            if (++h == p.heads) { h = 0; b++; }
+            if (b >= p.seq.count) return false;
+        }
+        piece.unit = unit_of<R>(p, b, h, rc);
+        piece.first = tile;
+        piece.count = (int)min((int64_t)(piece.unit.nt - tile), left);
+        if (piece.count <= 0) return false;
+        left -= piece.count;
+        tile = 0;
+        rc++;
+        return true;
+    }
+};
+
+// ---------------------------------------------------------------------------------- arithmetic
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float log2_ratio(float a, float b)
+{
+    return __log2f(__fdiv_rn(a, b));
+}
+// A power of two that brings `top` to 2^13 .. 2^14, and its reciprocal; 1 for zero, infinities and NaN.
+__device__ __forceinline__ void power_scale(float top, float &up, float &down)
+{
+    int e = (__float_as_uint(top) >> 23) & 255;
+    if (top == 0.f || e == 255) e = 140;
+    e = max(e, 14);
+    up = __uint_as_float((uint32_t)(267 - e) << 23);
+    down = __uint_as_float((uint32_t)(e - 13) << 23);
+}
+// Two values as f16 pairs: the nearest, and what is left.
+__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
+    hi = *(const uint32_t *)&h;
+    lo = *(const uint32_t *)&r;
+}
+__device__ __forceinline__ uint32_t minus1152(uint32_t x)
+{
+    uint32_t y;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x64806480u));
+    return y;
+}
+// Bytes 0, 1 (2, 3) of a word, codes + 128, as f16 codes.
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return minus1152(__byte_perm(w, 0x64646464u, 0x4140)); }
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return minus1152(__byte_perm(w, 0x64646464u, 0x4342)); }
+__device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed8(uint32_t x)
+{
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// Byte offset of 16-byte chunk `chunk` of row `row` in a tile of 32 rows that a swizzled tile copy has written.
+template <int DT>
+__device__ __forceinline__ uint32_t swizzled(int sub, int row, int chunk)
+{
+    if (DT == 64) return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+    return sub * (32 * 128) + row * 128 + ((chunk ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const void *map, int x, int y, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+}
+
+// Four dims of a row from the sums: numerator, denominator, and the exponent both are taken against.
+template <typename T>
+__device__ __forceinline__ void finish_row(const AttendArgs &p, const Unit &u, int at, int d, const float4 &acc, float m, float sum)
+{
+    const int row = u.row + at / p.group, head = u.h * p.group + at % p.group;
+    const float inv = sum > 0.f || sum != sum ? __fdiv_rn(1.f, sum) : 0.f;       // nothing seen: zeros
+    const float v[4] = { acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv };
+    T *dst = (T *)p.out.base + (int64_t)row * p.out.row + (int64_t)head * p.out.head + d;
+    if (sizeof(T) == 4) {
+        if (p.out_wide) *(float4 *)dst = make_float4(v[0], v[1], v[2], v[3]);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; i++) ((float *)dst)[i] = v[i];
+    } else {
+        const uint32_t a = bits_of(v[0], dst), b = bits_of(v[1], dst), c = bits_of(v[2], dst), e = bits_of(v[3], dst);
+        if (p.out_wide) *(uint2 *)dst = make_uint2(a | b << 16, c | e << 16);
+        else {
+            ((uint16_t *)dst)[0] = (uint16_t)a;
+            ((uint16_t *)dst)[1] = (uint16_t)b;
+            ((uint16_t *)dst)[2] = (uint16_t)c;
+            ((uint16_t *)dst)[3] = (uint16_t)e;
+        }
+    }
+    if (d == 0 && p.lse) p.lse[(int64_t)row * p.q_heads + head] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+}
+
+}  // namespace qb

@@ -1,0 +1,591 @@
+// Attention over the 8-bit cache for few rows: the query heads that share a head of the cache, for one token or a few.
+//
+// out = softmax(scale * q K^T) V with K = sk * ck, V = sv * cv (int8 codes, one f32 scale for each page and head).  What
+// bounds it is the cache's bytes: at 8 rows 32 operations a byte.  So every byte of the cache is read once for all rows
+// that share it, and the kernel is built to keep copies in flight:
+//  * The work of a call is a line of tiles, 32 tokens of one head of one sequence each.  Block c of the grid takes the
+//    c-th equal share of the line, whatever sequences lie in it: sequences of any lengths load all multiprocessors alike.
+//    Where a share ends inside a sequence, its part goes to the workspace and a second, small kernel joins the parts.
+//  * A producer warp fetches table entries and scales 32 at a time, a lane each, and brings a tile's codes by TMA tile
+//    copies (128-byte swizzle: the reads below touch all banks) into a ring of stages; eight consumer warps take the tiles
+//    in turn, each with a softmax of its own, joined at the end of a share's part.
+//  * A warp takes S^T = K q^T and O^T = V^T P^T with mma.sync m16n8k16 (f16, f32 sums): the tokens, then V's dims, are the
+//    16 rows, the query rows the 8 columns, so 8 rows fill the instruction (tcgen05's 128 rows would be 15/16 padding).
+//    The codes become f16 exactly (byte permute under an exponent of 1024, subtract 1152).  An order of dims or tokens
+//    inside a product is free, so both operands are read as whole 16-byte chunks: lane (g, t) holds K's chunks 2t, 2t+1 of
+//    token g, and V's chunk g of tokens 2t, 2t+1, 2t+8, 2t+9.
+//  * sk goes into the score's factor.  sv goes into the exponent: with v0 the first V scale a warp meets, the weights are
+//    w = 2^(s + log2(sv / v0) - m), the sum of them with v0 / sv as factor is the denominator, and O = v0 * sum w cv.
+//    m is chosen so that w lies at 2^7 at its largest when it is set and is kept while w stays below 2^15: f16 then holds
+//    weights down to 2^-29 of the largest with all its bits, and the accumulators are seldom rescaled.
+//  * q is scaled by a power of two to a row's maximum of 2^13 and cut to f16; with f32 lanes q and w enter as the sum of
+//    two f16 (SPL 2), which loses 2^-22.
+#include <cuda.h>
+#include "common.cuh"
+#include "cache.h"
+#include "cache_device.cuh"
+#include "attend_device.cuh"
+
+namespace qb {
+
+constexpr int RW = 8;                          // consumer warps
+constexpr int RTHREADS = 32 * (RW + 1);
+constexpr uint32_t ROWS_HEADER = 2048;
+
+template <int DT, int NB, int SPL>
+struct RowsCfg {
+    static constexpr int R = 8 * NB;           // rows a unit
+    static constexpr int KS = DT / 16;         // k-steps of a score
+    static constexpr int SUB = DT == 256 ? 2 : 1;               // tile copies of at most 128 bytes of dims
+    static constexpr int SW = DT == 64 ? 64 : 128;              // bytes a row of a copy
+    static constexpr uint32_t HALF = 32 * DT, STAGE = 2 * HALF;  // K, then V
+    static constexpr int S = DT == 64 ? 24 : DT == 128 ? 16 : 8;
+    static constexpr uint32_t MROW = DT + 4;                    // floats a row of the joining buffer
+    static constexpr uint32_t O_RING = 0, O_Q = S * STAGE, O_MERGE = O_Q + KS * NB * SPL * 256, O_ML = O_MERGE + RW * R * MROW * 4;
+    static constexpr uint32_t O_HEAD = O_ML + RW * R * 8, SMEM = O_HEAD + ROWS_HEADER + 1024;
+    static_assert(S % RW == 0, "a stage has one consumer warp");
+    static_assert(SMEM <= 232448, "227 KB of shared memory");
+};
+
+struct RowsHead {                              // at O_HEAD
+    uint64_t full[24], empty[24];
+    float4 scales[24];                         // of a stage: sk, sv of its first and second 16 tokens
+    float factor[16];                          // rows: scale * log2 e / (what q was scaled by)
+    int lo[16], hi[16];                        // rows: tokens they see
+    Start start;
+    int abort;
+};
+static_assert(sizeof(RowsHead) <= ROWS_HEADER, "the header fits");
+
+template <int DT, int NB, int SPL, typename T>
+__global__ void __launch_bounds__(RTHREADS, 1)
+attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap)
+{
+    using C = RowsCfg<DT, NB, SPL>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    RowsHead *head = (RowsHead *)(smem + C::O_HEAD);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ring = smem_u32(smem), full0 = smem_u32(head->full), empty0 = smem_u32(head->empty);
+
+    if (threadIdx.x == 0) {
+        head->abort = 0;
+        for (int i = 0; i < C::S; i++) {
+            mbar_init(full0 + 8 * i, 1);
+            mbar_init(empty0 + 8 * i, 1);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 0) {
+        const Start s = p.whole ? Start{} : start_of<C::R>(p, blockIdx.x);
+        if (lane == 0) head->start = s;
+    }
+    __syncthreads();
+    if (!p.whole) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the joining kernel waits beside this one
+    Walk<C::R> walk(p, head->start);
+    volatile int *abort = &head->abort;
+    uint32_t seq = 0;                          // tiles of this block so far
+
+    if (warp == RW) {
+        // ------------------------------------------------------------------ producer
+        Piece piece;
+        while (walk.next(piece)) {
+            const int per = p.log_page == 4 ? 2 : 1;            // pages a tile
+            const int batch = 32 / per;
+            for (int first = 0; first < piece.count; first += batch) {
+                // a lane a page
+                const int tile = piece.unit.t0 + piece.first + first + lane / per;
+                const int token = tile * 32 + (per == 2 ? (lane & 1) * 16 : 0), slot = token >> p.log_page;
+                int id = -1;
+                float sk = 0.f, sv = -1.f;
+                if (first + lane / per < piece.count && token < piece.unit.hi && (token | (per == 2 ? 15 : 31)) >= piece.unit.lo) {
+                    id = p.seq.table[(int64_t)piece.unit.b * p.seq.width + slot];
+                    if (id < 0 || id >= p.pages) {
+                        id = -1;
+                        atomicOr(p.status, STATUS_CACHE_RANGE);
+                    } else {
+                        const int64_t at = (int64_t)id * p.heads + piece.unit.h;
+                        sk = __ldg(p.k_scales + at);
+                        sv = __ldg(p.v_scales + at);
+                    }
+                }
+                const int n = min(batch, piece.count - first);
+                for (int k = 0; k < n; k++, seq++) {
+                    const int stage = seq % C::S;
+                    if (seq >= C::S && !mbar_wait_warp(empty0 + 8 * stage, (seq / C::S - 1) & 1, abort, p.status, STATUS_ATTEND_WAIT)) goto done;
+                    const int l0 = k * per, l1 = l0 + per - 1;
+                    const int id0 = __shfl_sync(0xffffffffu, id, l0), id1 = __shfl_sync(0xffffffffu, id, l1);
+                    const float k0 = __shfl_sync(0xffffffffu, sk, l0), k1 = __shfl_sync(0xffffffffu, sk, l1);
+                    const float v0 = __shfl_sync(0xffffffffu, sv, l0), v1 = __shfl_sync(0xffffffffu, sv, l1);
+                    const int rows = 32 / per;                  // tokens a copy
+                    const uint32_t bytes = rows * C::SW;
+                    const int live = (id0 >= 0 ? 1 : 0) + (per == 2 && id1 >= 0 ? 1 : 0);
+                    if (lane == 0) {
+                        head->scales[stage] = make_float4(k0, v0, k1, v1);
+                        if (live) mbar_arrive_expect_tx(full0 + 8 * stage, live * 2 * C::SUB * bytes);
+                        else mbar_arrive(full0 + 8 * stage);
+                    }
+                    __syncwarp();
+                    if (lane < 2 * C::SUB * per) {
+                        const int which = lane & 1, sub = (lane >> 1) % C::SUB, pg = lane / (2 * C::SUB);
+                        const int page = pg ? id1 : id0;
+                        if (page >= 0) {
+                            const int inside = ((piece.unit.t0 + piece.first + first + k) * 32 + pg * 16) & ((1 << p.log_page) - 1);
+                            const int row = ((page * p.heads + piece.unit.h) << p.log_page) + inside;
+                            const uint32_t dst = ring + stage * C::STAGE + which * C::HALF + sub * (32 * 128) + pg * 16 * C::SW;
+                            tma_load_2d(dst, which ? &vmap : &kmap, sub * 128, row, full0 + 8 * stage);
+                        }
+                    }
+                }
+            }
+        }
+    done:
+        // no copy may be under way when the block ends, whoever gave up
+        for (uint32_t at = seq > C::S ? seq - C::S : 0; at < seq; at++) {
+            const long long from = clock64();
+            while (!mbar_try_wait(full0 + 8 * (at % C::S), (at / C::S) & 1) && clock64() - from < WAIT_CYCLES) { }
+        }
+        return;
+    }
+
+    // ---------------------------------------------------------------------- consumers
+    const int g = lane >> 2, t = lane & 3;
+    uint2 *qs = (uint2 *)(smem + C::O_Q);
+    float *merge = (float *)(smem + C::O_MERGE);
+    float2 *ml = (float2 *)(smem + C::O_ML);
+    Piece piece;
+    bool gone = false;
+    while (walk.next(piece)) {
+        const Unit &u = piece.unit;
+        // the rows of q, scaled and cut, in the order of the products' operands
+        named_bar_sync(1, 32 * RW);            // the last piece's buffers are free
+        for (int r = warp; r < C::R; r += RW) {
+            const int at = u.r0 + r;
+            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (at < u.r1 && lane < p.dim / 8) {
+                const T *src = (const T *)p.q.base + (int64_t)(u.row + at / p.group) * p.q.row + (int64_t)(u.h * p.group + at % p.group) * p.q.head + lane * 8;
+                const Vec8<T> v = load8<T>(src, p.q_wide);
+                unpack8(v, x);
+            }
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[i]));
+#pragma unroll
+            for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            float up, down;
+            power_scale(top, up, down);
+            if (lane * 8 < DT) {
+                const int sub = lane / 16, chunk = DT == 64 ? lane / 2 : (lane % 16) / 2;
+                const int tt = DT == 64 ? chunk : chunk >> 1, ii = DT == 64 ? 0 : chunk & 1;
+#pragma unroll
+                for (int j = 0; j < 2; j++) {  // four dims each
+                    const int ks = (sub * 2 + ii) * 4 + (lane & 1) * 2 + j;
+                    uint32_t hi0, lo0, hi1, lo1;
+                    split2(x[4 * j] * up, x[4 * j + 1] * up, hi0, lo0);
+                    split2(x[4 * j + 2] * up, x[4 * j + 3] * up, hi1, lo1);
+                    uint2 *dst = qs + ((ks * NB + r / 8) * SPL) * 32 + (r & 7) * 4 + tt;
+                    dst[0] = make_uint2(hi0, hi1);
+                    if (SPL == 2) dst[32] = make_uint2(lo0, lo1);
+                }
+            }
+            if (lane == 0) {
+                head->factor[r] = p.scale * 1.4426950408889634f * down;
+                int lo, hi;
+                row_limits(p, u, at < u.r1 ? at : u.r1 - 1, lo, hi);
+                head->lo[r] = lo;
+                head->hi[r] = hi;
+            }
+        }
+        named_bar_sync(1, 32 * RW);
+        float factor[NB][2];
+        int lo[NB][2], hi[NB][2];
+        int lo_most = 0, hi_least = 0x7fffffff;
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int r = nb * 8 + 2 * t + c;
+                factor[nb][c] = head->factor[r];
+                lo[nb][c] = head->lo[r];
+                hi[nb][c] = head->hi[r];
+            }
+        for (int r = 0; r < C::R; r++) {
+            lo_most = max(lo_most, head->lo[r]);
+            hi_least = min(hi_least, head->hi[r]);
+        }
+
+        float o[C::SUB * (DT == 64 ? 2 : 4)][2][NB][4];          // [16-byte chunk's word][pair of dims]
+#pragma unroll
+        for (int i = 0; i < C::SUB * (DT == 64 ? 2 : 4); i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) o[i][j][nb][c] = 0.f;
+        float mm[NB][2], l[NB][2];             // the exponent that weights are taken against; their sum, this lane's tokens
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) { mm[nb][c] = NOTHING; l[nb][c] = 0.f; }
+        float vref = 0.f;
+
+        const int mine = (int)((warp - seq) & (RW - 1));          // this warp's first tile of the piece
+        for (int j = mine; j < piece.count && !gone; j += RW) {
+            const uint32_t at = seq + j;
+            const int stage = at % C::S;
+            if (!mbar_wait_lanes(full0 + 8 * stage, (at / C::S) & 1, abort, p.status, STATUS_ATTEND_WAIT)) { gone = true; break; }
+            const float4 sc = head->scales[stage];
+            const uint8_t *kt = smem + stage * C::STAGE, *vt = kt + C::HALF;
+            const int base = (u.t0 + piece.first + j) * 32;
+
+            // ---- scores
+            float s[2][NB][4];
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) s[mt][nb][c] = 0.f;
+#pragma unroll
+            for (int sub = 0; sub < C::SUB; sub++)
+#pragma unroll
+                for (int i = 0; i < (DT == 64 ? 1 : 2); i++) {
+                    uint4 a[2][2];             // [tile of 16 tokens][token g, g + 8]
+#pragma unroll
+                    for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) a[mt][e] = *(const uint4 *)(kt + swizzled<DT>(sub, mt * 16 + e * 8 + g, DT == 64 ? t : 2 * t + i));
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        uint2 b[NB][SPL];
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                            for (int x = 0; x < SPL; x++) b[nb][x] = qs[((((sub * 2 + i) * 4 + q) * NB + nb) * SPL + x) * 32 + lane];
+#pragma unroll
+                        for (int mt = 0; mt < 2; mt++) {
+                            const uint32_t w0 = word(a[mt][0], q) ^ 0x80808080u, w1 = word(a[mt][1], q) ^ 0x80808080u;
+                            const uint32_t a0 = codes_lo(w0), a1 = codes_lo(w1), a2 = codes_hi(w0), a3 = codes_hi(w1);
+#pragma unroll
+                            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                                for (int x = 0; x < SPL; x++) mma16816(s[mt][nb], a0, a1, a2, a3, b[nb][x].x, b[nb][x].y);
+                        }
+                    }
+                }
+
+            // ---- weights
+            float lr[2], rinv[2];
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+                const float sk = mt ? sc.z : sc.x, sv = mt ? sc.w : sc.y;
+                if (vref == 0.f && sv > 0.f) vref = sv;
+                lr[mt] = 0.f;
+                rinv[mt] = 1.f;
+                if (sv < 0.f) { lr[mt] = -INFINITY; rinv[mt] = 0.f; }          // a page that is not there
+                else if (sv > 0.f && sv != vref) { lr[mt] = log2_ratio(sv, vref); rinv[mt] = __fdividef(vref, sv); }
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) s[mt][nb][c] = __fmaf_rn(s[mt][nb][c], factor[nb][c & 1] * sk, lr[mt]);
+            }
+            if (base < lo_most || base + 32 > hi_least) {
+#pragma unroll
+                for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const int token = base + mt * 16 + g + (c >> 1) * 8;
+                            if (token < lo[nb][c & 1] || token >= hi[nb][c & 1]) s[mt][nb][c] = -INFINITY;
+                        }
+            }
+            bool above = false;
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) above |= s[mt][nb][c] > mm[nb][c & 1] + 15.f;
+            if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        float top = fmaxf(fmaxf(s[0][nb][c], s[0][nb][c + 2]), fmaxf(s[1][nb][c], s[1][nb][c + 2]));
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        const float next = fmaxf(mm[nb][c], top - 7.f), less = exp2_fast(mm[nb][c] - next);
+                        mm[nb][c] = next;
+                        l[nb][c] *= less;
+#pragma unroll
+                        for (int i = 0; i < C::SUB * (DT == 64 ? 2 : 4); i++)
+#pragma unroll
+                            for (int k = 0; k < 2; k++) {
+                                o[i][k][nb][c] *= less;
+                                o[i][k][nb][c + 2] *= less;
+                            }
+                    }
+            }
+            uint32_t w[2][NB][SPL][2];
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) {
+                    float e[4];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        e[c] = exp2_fast(s[mt][nb][c] - mm[nb][c & 1]);
+                        l[nb][c & 1] = __fmaf_rn(e[c], rinv[mt], l[nb][c & 1]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        uint32_t a, b;
+                        split2(e[2 * k], e[2 * k + 1], a, b);
+                        w[mt][nb][0][k] = transposed8(a);
+                        if (SPL == 2) w[mt][nb][SPL - 1][k] = transposed8(b);
+                    }
+                }
+
+            // ---- O^T += V^T P^T
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int sub = 0; sub < C::SUB; sub++) {
+                    uint4 r[4];                // this lane's dims of tokens 2t, 2t+1, 2t+8, 2t+9
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int token = mt * 16 + 2 * t + (e & 1) + (e >> 1) * 8;
+                        if (DT == 64) {
+                            const uint2 h = *(const uint2 *)(vt + swizzled<DT>(0, token, g >> 1) + (g & 1) * 8);
+                            r[e] = make_uint4(h.x, h.y, 0, 0);
+                        } else r[e] = *(const uint4 *)(vt + swizzled<DT>(sub, token, g));
+                    }
+#pragma unroll
+                    for (int q = 0; q < (DT == 64 ? 2 : 4); q++) {
+                        const uint32_t w0 = word(r[0], q) ^ 0x80808080u, w1 = word(r[1], q) ^ 0x80808080u;
+                        const uint32_t w2 = word(r[2], q) ^ 0x80808080u, w3 = word(r[3], q) ^ 0x80808080u;
+                        const uint32_t x0 = __byte_perm(w0, w1, 0x5140), x1 = __byte_perm(w0, w1, 0x7362);
+                        const uint32_t y0 = __byte_perm(w2, w3, 0x5140), y1 = __byte_perm(w2, w3, 0x7362);
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const uint32_t x = k ? x1 : x0, y = k ? y1 : y0;
+                            const uint32_t a0 = codes_lo(x), a1 = codes_hi(x), a2 = codes_lo(y), a3 = codes_hi(y);
+#pragma unroll
+                            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                                for (int z = 0; z < SPL; z++) mma16816(o[sub * 4 + q][k][nb], a0, a1, a2, a3, w[mt][nb][z][0], w[mt][nb][z][1]);
+                        }
+                    }
+                }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty0 + 8 * stage);
+        }
+        seq += piece.count;
+
+        // ---- the warps' parts of this piece
+        const float v0 = vref > 0.f ? vref : 1.f;
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                float sum = l[nb][c];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                const int r = nb * 8 + 2 * t + c;
+                if (g == 0) ml[warp * C::R + r] = make_float2(mm[nb][c], sum);
+                float *row = merge + (warp * C::R + r) * C::MROW;
+#pragma unroll
+                for (int i = 0; i < C::SUB * (DT == 64 ? 2 : 4); i++) {
+                    const int dim = DT == 64 ? 8 * g + 4 * i : (i / 4) * 128 + 16 * g + 4 * (i % 4);
+                    *(float4 *)(row + dim) = make_float4(o[i][0][nb][c] * v0, o[i][0][nb][c + 2] * v0, o[i][1][nb][c] * v0, o[i][1][nb][c + 2] * v0);
+                }
+            }
+        named_bar_sync(1, 32 * RW);
+        const int rows = u.r1 - u.r0, quads = p.dim / 4;
+        const bool complete = piece.first == 0 && piece.count == u.nt;
+        for (int i = threadIdx.x; i < rows * quads; i += 32 * RW) {
+            const int r = i / quads, d = (i - r * quads) * 4;
+            float m = NOTHING;
+#pragma unroll
+            for (int k = 0; k < RW; k++) m = fmaxf(m, ml[k * C::R + r].x);
+            float sum = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < RW; k++) {
+                const float2 part = ml[k * C::R + r];
+                const float f = exp2_fast(part.x - m);
+                const float4 x = *(const float4 *)(merge + (k * C::R + r) * C::MROW + d);
+                sum = __fmaf_rn(part.y, f, sum);
+                acc.x = __fmaf_rn(x.x, f, acc.x);
+                acc.y = __fmaf_rn(x.y, f, acc.y);
+                acc.z = __fmaf_rn(x.z, f, acc.z);
+                acc.w = __fmaf_rn(x.w, f, acc.w);
+            }
+            if (complete) finish_row<T>(p, u, u.r0 + r, d, acc, m, sum);
+            else {
+                float *slot = (float *)p.workspace + (size_t)(blockIdx.x * 2 + (piece.first ? 0 : 1)) * part_floats(C::R, p.dim);
+                *(float4 *)(slot + C::R * 2 + r * p.dim + d) = acc;
+                if (d == 0) *(float2 *)(slot + r * 2) = make_float2(m, sum);
+            }
+        }
+    }
+}
+
+// Joins the parts of the units that a share's end cuts: block c looks after the unit that the c-th boundary cuts first.
+template <int R, typename T>
+__global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendArgs p)
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    __shared__ Cut cut;
+    if (threadIdx.x < 32) {
+        const Cut c = cut_of<R>(p, blockIdx.x + 1);
+        if (threadIdx.x == 0) cut = c;
+    }
+    __syncthreads();
+    if (cut.parts == 0) return;
+    const Unit u = unit_of<R>(p, cut.b, cut.h, cut.rc);
+    const int rows = u.r1 - u.r0, quads = p.dim / 4;
+    const size_t size = part_floats(R, p.dim);
+    const float *first = (const float *)p.workspace + (size_t)((cut.block - 1) * 2 + 1) * size;      // the part that begins the unit
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * quads; i += 256 * gridDim.y) {
+        const int r = i / quads, d = (i - r * quads) * 4;
+        float m = NOTHING;
+        for (int k = 0; k < cut.parts; k++) m = fmaxf(m, first[(k ? (size_t)(2 * k - 1) * size : 0) + r * 2]);
+        float sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < cut.parts; k++) {
+            const float *part = first + (k ? (size_t)(2 * k - 1) * size : 0);
+            const float2 s = *(const float2 *)(part + r * 2);
+            const float4 x = *(const float4 *)(part + R * 2 + r * p.dim + d);
+            const float f = exp2_fast(s.x - m);
+            sum = __fmaf_rn(s.y, f, sum);
+            acc.x = __fmaf_rn(x.x, f, acc.x);
+            acc.y = __fmaf_rn(x.y, f, acc.y);
+            acc.z = __fmaf_rn(x.z, f, acc.z);
+            acc.w = __fmaf_rn(x.w, f, acc.w);
+        }
+        finish_row<T>(p, u, u.r0 + r, d, acc, m, sum);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- host
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled g_attend_encode = nullptr;
+static int *g_attend_status = nullptr;
+static int g_attend_sms = 0;
+
+template <int DT, int NB, int SPL, typename T>
+static cudaError_t set_rows_attr()
+{
+    return cudaFuncSetAttribute(attend_rows_kernel<DT, NB, SPL, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RowsCfg<DT, NB, SPL>::SMEM);
+}
+template <int DT, int NB>
+static cudaError_t set_rows_attrs()
+{
+    cudaError_t e;
+    if ((e = set_rows_attr<DT, NB, 2, float>()) || (e = set_rows_attr<DT, NB, 1, __half>())) return e;
+    return set_rows_attr<DT, NB, 1, __nv_bfloat16>();
+}
+
+cudaError_t attend_init(int sm_count, int max_smem, int *status)
+{
+    g_attend_status = status;
+    g_attend_sms = sm_count;
+    if (max_smem < 232448) return cudaErrorInvalidValue;
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found);
+    if (e) return e;
+    if (found != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
+    g_attend_encode = (EncodeTiled)fn;
+    if ((e = set_rows_attrs<64, 1>()) || (e = set_rows_attrs<64, 2>()) || (e = set_rows_attrs<128, 1>()) || (e = set_rows_attrs<128, 2>())) return e;
+    return set_rows_attrs<256, 1>();
+}
+
+// rows a unit of the rows kernel: 16 where a group has more than 8 rows (dim <= 128: the accumulators of 16 rows fit beside it)
+static int rows_a_unit(int dim, int rows) { return dim <= 128 && rows > 8 ? 16 : 8; }
+
+size_t attend_workspace_bytes(int dim, int heads, int type, int count, int rows, int q_heads, int max_queries, int max_length)
+{
+    (void)type; (void)count; (void)rows; (void)max_length;
+    const int r = rows_a_unit(dim, q_heads / heads * max_queries);
+    return (size_t)g_attend_sms * 2 * part_floats(r, dim) * 4;
+}
+
+static bool codes_map(CUtensorMap &map, const void *codes, const qb200_cache_t &c, int box_dim, int box_rows)
+{
+    const cuuint64_t dims[2] = { (cuuint64_t)c.dim, (cuuint64_t)c.pages * c.heads * c.page }, strides[1] = { (cuuint64_t)c.dim };
+    const cuuint32_t box[2] = { (cuuint32_t)box_dim, (cuuint32_t)box_rows }, estr[2] = { 1, 1 };
+    return g_attend_encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           box_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DT, int NB, int SPL, typename T>
+static int launch_rows(AttendArgs &args, const qb200_cache_t &c, int grid, cudaStream_t stream)
+{
+    CUtensorMap kmap, vmap;
+    const int box = DT == 64 ? 64 : 128, rows = c.page < 32 ? c.page : 32;
+    if (!codes_map(kmap, c.k_codes, c, box, rows) || !codes_map(vmap, c.v_codes, c, box, rows)) return (int)cudaErrorInvalidValue;
+    attend_rows_kernel<DT, NB, SPL, T><<<grid, RTHREADS, RowsCfg<DT, NB, SPL>::SMEM, stream>>>(args, kmap, vmap);
+    cudaError_t e = cudaGetLastError();
+    if (e || args.whole || grid < 2) return (int)e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(grid - 1); cfg.blockDim = dim3(256); cfg.stream = stream; cfg.attrs = &attr; cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, attend_join_kernel<8 * NB, T>, args);
+}
+
+template <int SPL, typename T>
+static int launch_rows_dim(AttendArgs &args, const qb200_cache_t &c, int r, int grid, cudaStream_t stream)
+{
+    if (c.dim <= 64) return r == 16 ? launch_rows<64, 2, SPL, T>(args, c, grid, stream) : launch_rows<64, 1, SPL, T>(args, c, grid, stream);
+    if (c.dim <= 128) return r == 16 ? launch_rows<128, 2, SPL, T>(args, c, grid, stream) : launch_rows<128, 1, SPL, T>(args, c, grid, stream);
+    return launch_rows<256, 1, SPL, T>(args, c, grid, stream);
+}
+
+int attend(const AttendCall &call, cudaStream_t stream)
+{
+    if (call.seq.count == 0 || call.seq.rows == 0) return 0;
+    const qb200_cache_t &c = call.cache;
+    const int size = call.type == QB200_F32 ? 4 : 2;
+    AttendArgs a;
+    a.seq = call.seq;
+    a.q = call.q;
+    a.out = call.out;
+    a.lse = call.lse;
+    a.k_scales = c.k_scales;
+    a.v_scales = c.v_scales;
+    a.pages = c.pages;
+    a.heads = c.heads;
+    a.dim = c.dim;
+    a.log_page = c.page == 16 ? 4 : c.page == 32 ? 5 : c.page == 64 ? 6 : 7;
+    a.group = call.q_heads / c.heads;
+    a.q_heads = call.q_heads;
+    a.causal = call.causal;
+    a.window = call.window;
+    a.scale = call.scale;
+    a.q_wide = ((uintptr_t)call.q.base & 15) == 0 && call.q.row * size % 16 == 0 && call.q.head * size % 16 == 0;
+    a.out_wide = ((uintptr_t)call.out.base & (4 * size - 1)) == 0 && call.out.row % 4 == 0 && call.out.head % 4 == 0;
+    a.workspace = call.workspace;
+    a.status = g_attend_status;
+    const int r = rows_a_unit(c.dim, a.group * call.max_queries);
+    a.chunks = (a.group * call.max_queries + r - 1) / r;
+    // A unit (the rows r of one head of one sequence) goes to one block whole where it is short: cutting it would cost a
+    // second launch.
+    const int64_t units = (int64_t)call.seq.count * c.heads * a.chunks;
+    a.whole = call.max_length <= 1024;
+    const int grid = a.whole ? (int)(units < 65535 * 8 ? units : 65535 * 8) : g_attend_sms;
+    a.grid = grid;
+    if (call.type == QB200_F32) return launch_rows_dim<2, float>(a, c, r, grid, stream);
+    if (call.type == QB200_F16) return launch_rows_dim<1, __half>(a, c, r, grid, stream);
+    return launch_rows_dim<1, __nv_bfloat16>(a, c, r, grid, stream);
+}
+
+}  // namespace qb
