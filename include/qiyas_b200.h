@@ -336,7 +336,7 @@ int qb200_cache_read(const qb200_cache_t *cache, const qb200_sequences_t *sequen
  *   Sums, softmax statistics and the accumulators are f32; q and the weights enter the tensor cores in f16 (f32 lanes: as
  *   the sum of two f16), the codes exactly.
  *   workspace: device scratch of qb200_cache_attention_workspace_bytes(...) bytes, 16-byte aligned, private to the call
- *   until it completes on `stream`; needed even where no sequence turns out to be split. */
+ *   until it completes on `stream`; the function gives 0, and workspace may be NULL, where no sequence is ever split. */
 size_t qb200_cache_attention_workspace_bytes(const qb200_cache_t *cache, int type, int count, int rows, int q_heads, int max_queries, int max_length);
 int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const void *q, int64_t q_row_stride,
                           int64_t q_head_stride, void *out, int64_t out_row_stride, int64_t out_head_stride, float *lse, int q_heads,

@@ -11,11 +11,13 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIBRARY = os.path.join(HERE, "libqiyas_b200.so")
-SOURCES = ["api.cu", "gemv.cu", "codecs.cu", "matmul.cu", "shard.cu", "cache.cu", "attend_rows.cu"]
+SOURCES = ["api.cu", "gemv.cu", "codecs.cu", "matmul.cu", "shard.cu", "cache.cu", "attend.cu", "attend_rows.cu",
+           "attend_tiles.cu"]
 HEADERS = ["common.cuh", "launch.h", "encode_blocks.cuh", os.path.join("..", "..", "include", "qiyas_b200.h")]
 # headers that only some sources include
-OWN_HEADERS = {"cache.h": ["api.cu", "cache.cu", "attend_rows.cu"], "cache_device.cuh": ["cache.cu", "attend_rows.cu"],
-               "attend_device.cuh": ["attend_rows.cu"]}
+_ATTEND = ["attend.cu", "attend_rows.cu", "attend_tiles.cu"]
+OWN_HEADERS = {"tcgen05.cuh": ["matmul.cu", "attend_tiles.cu"], "cache.h": ["api.cu", "cache.cu"] + _ATTEND, "cache_device.cuh": ["cache.cu"] + _ATTEND,
+               "attend_device.cuh": _ATTEND, "attend_join.cuh": _ATTEND[1:]}
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--compiler-options", "-fPIC",
          "-Xptxas", "-v"]
 

@@ -14,6 +14,8 @@ v_scales  float32 [pages, heads]
 Which pages belong to which sequence is the caller's: an int32 table [sequences, width] on the device, entry [b, i] naming
 the page that holds tokens i * page .. i * page + page - 1 of sequence b.
 """
+import torch
+
 from . import _lib
 
 PAGES = (16, 32, 64, 128)
@@ -23,27 +25,24 @@ class BlockCache:
     """The arrays of a cache, checked once; nothing is copied."""
 
     def __init__(self, k_codes, v_codes, k_scales, v_scales):
-        import torch
-        if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
-            raise ValueError(f"codes are [pages, heads, page, dim] twice: got {tuple(k_codes.shape)}, {tuple(v_codes.shape)}")
-        pages, heads, page, dim = k_codes.shape
-        if tuple(k_scales.shape) != (pages, heads) or tuple(v_scales.shape) != (pages, heads):
+        shape = k_codes.shape
+        if len(shape) != 4 or v_codes.shape != shape:
+            raise ValueError(f"codes are [pages, heads, page, dim] twice: got {tuple(shape)}, {tuple(v_codes.shape)}")
+        self.pages, self.heads, self.page, self.dim = pages, heads, page, dim = tuple(shape)
+        if k_scales.shape != shape[:2] or v_scales.shape != shape[:2]:
             raise ValueError(f"scales are [pages, heads] = {(pages, heads)}: got {tuple(k_scales.shape)}, {tuple(v_scales.shape)}")
         if page not in PAGES or dim % 16 or not 0 < dim <= 256:
             raise NotImplementedError(f"blocks of {page} tokens x {dim}: 16, 32, 64 or 128 tokens, and dim a multiple of 16 up to 256")
-        for name, t, kind in (("k_codes", k_codes, torch.int8), ("v_codes", v_codes, torch.int8),
-                              ("k_scales", k_scales, torch.float32), ("v_scales", v_scales, torch.float32)):
-            if t.dtype != kind or not t.is_contiguous() or t.device != k_codes.device:
-                raise ValueError(f"{name}: contiguous {kind} on {k_codes.device} is needed, got {t.dtype} on {t.device}")
+        self.index = k_codes.get_device()                       # -1: not on a GPU
+        for t, kind in ((k_codes, torch.int8), (v_codes, torch.int8), (k_scales, torch.float32), (v_scales, torch.float32)):
+            if t.dtype is not kind or not t.is_contiguous() or t.get_device() != self.index:
+                raise ValueError(f"contiguous {kind} on one device is needed, got {t.dtype} on {t.device}, strides {t.stride()}")
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
-        self.pages, self.heads, self.page, self.dim = pages, heads, page, dim
-        self.device = k_codes.device
         self.parts = _lib.CacheParts(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages, heads, page, dim)
 
     @classmethod
     def empty(cls, pages, heads, page, dim, device="cuda:0"):
         """A cache of `pages` pages; nothing in it needs initialising."""
-        import torch
         codes = [torch.empty(pages, heads, page, dim, dtype=torch.int8, device=device) for _ in range(2)]
         scales = [torch.empty(pages, heads, dtype=torch.float32, device=device) for _ in range(2)]
         return cls(*codes, *scales)

@@ -542,7 +542,7 @@ int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *s
     if (max_queries < 0 || max_length < 0) return fail(QB200_E_SHAPE, "max_queries %d, max_length %d", max_queries, max_length);
     attention_bounds(cache, sequences, max_queries, max_length);
     const size_t need = qb::attend_workspace_bytes(cache->dim, cache->heads, type, sequences->count, sequences->rows, q_heads, max_queries, max_length);
-    if (!workspace || workspace_bytes < need) return fail(QB200_E_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
+    if (need && (!workspace || workspace_bytes < need)) return fail(QB200_E_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
     if ((uintptr_t)workspace & 15) return fail(QB200_E_WORKSPACE, "workspace not 16-byte aligned");
     OnDevice on;
     if (!g_ready) return fail(QB200_E_DEVICE, "qb200_init has not succeeded");

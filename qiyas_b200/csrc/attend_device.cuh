@@ -1,6 +1,7 @@
 // What the attention kernels share: how a call's work is cut into shares, the rows' limits, and the products' operands.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
 
@@ -10,13 +11,13 @@
 namespace qb {
 
 constexpr float NOTHING = -1e30f;              // a maximum over nothing (finite: differences of two of them are 0)
-constexpr int TILE_TOKENS = 32;                // tokens a tile of the line of work
-constexpr int LEAST_TILES = 8;                 // tiles a share has at least
+constexpr int LEAST_TOKENS = 256;              // tokens a share has at least
 
 struct AttendArgs {
     qb200_sequences_t seq;
     Lanes q, out;
     float *lse;
+    const int8_t *k_codes, *v_codes;
     const float *k_scales, *v_scales;
     int pages, heads, dim, log_page, group, q_heads, causal, window;
     float scale;
@@ -28,7 +29,12 @@ struct AttendArgs {
     int *status;
 };
 
-// R rows of one head of one sequence: rows r0 .. r1 - 1 of its queries x group, and the tokens they see together.
+cudaError_t attend_rows_init();
+int attend_rows(const AttendArgs &args, int type, int r, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t stream);
+cudaError_t attend_tiles_init();
+int attend_tiles(const AttendArgs &args, int type, cudaStream_t stream);
+
+// R rows of one head (R, and TT tokens a tile: the kernel's) of one sequence: rows r0 .. r1 - 1 of its queries x group, and the tokens they see together.
 struct Unit {
     int b, h, rc;
     int row, n, len;                           // the sequence: first row, rows, tokens
@@ -39,28 +45,44 @@ struct Unit {
 
 __host__ __device__ constexpr size_t part_floats(int r, int dim) { return (size_t)r * (dim + 2); }
 
-template <int R>
-__device__ __forceinline__ Unit unit_of(const AttendArgs &p, int b, int h, int rc)
+struct Sequence { int row, n, len; };          // first row, rows, tokens: held to what there is
+
+__device__ __forceinline__ Sequence sequence_at(const AttendArgs &p, int b)
+{
+    Sequence s;
+    bool bad;
+    seq_rows(p.seq, b, s.row, s.n, bad);
+    s.len = p.seq.lengths[b];
+    const int most = p.seq.width << p.log_page;
+    bad |= s.len < 0 || s.len > most;
+    s.len = max(0, min(s.len, most));
+    if (bad && (threadIdx.x & 31) == 0) atomicOr(p.status, STATUS_CACHE_RANGE);
+    return s;
+}
+
+template <int R, int TT>
+__device__ __forceinline__ Unit unit_of(const AttendArgs &p, const Sequence &s, int b, int h, int rc)
 {
     Unit u;
     u.b = b;
     u.h = h;
     u.rc = rc;
-    bool bad;
-    seq_rows(p.seq, b, u.row, u.n, bad);
-    u.len = p.seq.lengths[b];
-    const int most = p.seq.width << p.log_page;
-    bad |= u.len < 0 || u.len > most;
-    u.len = max(0, min(u.len, most));
-    if (bad && (threadIdx.x & 31) == 0) atomicOr(p.status, STATUS_CACHE_RANGE);
+    u.row = s.row;
+    u.n = s.n;
+    u.len = s.len;
     u.r0 = rc * R;
     u.r1 = min(u.r0 + R, u.n * p.group);
     const int first = u.r0 / p.group, last = (max(u.r1, 1) - 1) / p.group;
     u.hi = p.causal ? max(0, min(u.len, u.len - u.n + last + 1)) : u.len;
     u.lo = p.window ? max(0, u.len - u.n + first + 1 - p.window) : 0;
-    u.t0 = u.hi > u.lo ? u.lo / TILE_TOKENS : 0;
-    u.nt = u.hi > u.lo ? (u.hi + TILE_TOKENS - 1) / TILE_TOKENS - u.t0 : 1;
+    u.t0 = u.hi > u.lo ? u.lo / TT : 0;
+    u.nt = u.hi > u.lo ? (u.hi + TT - 1) / TT - u.t0 : 1;
     return u;
+}
+template <int R, int TT>
+__device__ __forceinline__ Unit unit_of(const AttendArgs &p, int b, int h, int rc)
+{
+    return unit_of<R, TT>(p, sequence_at(p, b), b, h, rc);
 }
 
 // The tokens row `at` of a unit's sequence sees.
@@ -82,12 +104,13 @@ __device__ __forceinline__ int chunks_of(const AttendArgs &p, int b)
 }
 
 // Tiles of one head of sequence b.
-template <int R>
+template <int R, int TT>
 __device__ __forceinline__ int64_t tiles_of(const AttendArgs &p, int b)
 {
     int64_t sum = 0;
-    const int chunks = chunks_of<R>(p, b);
-    for (int rc = 0; rc < chunks; rc++) sum += unit_of<R>(p, b, 0, rc).nt;
+    const Sequence s = sequence_at(p, b);
+    const int chunks = (s.n * p.group + R - 1) / R;
+    for (int rc = 0; rc < chunks; rc++) sum += unit_of<R, TT>(p, s, b, 0, rc).nt;
     return sum;
 }
 
@@ -97,23 +120,23 @@ struct Start {
 };
 
 // Called by a whole warp: the place `x` on the line of tiles, sequence after sequence, head after head; `total` is its length.
-template <int R>
+template <int R, int TT>
 __device__ __forceinline__ int64_t line_length(const AttendArgs &p)
 {
     const int lane = threadIdx.x & 31;
     int64_t sum = 0;
-    for (int b = lane; b < p.seq.count; b += 32) sum += tiles_of<R>(p, b);
+    for (int b = lane; b < p.seq.count; b += 32) sum += tiles_of<R, TT>(p, b);
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     return sum * p.heads;
 }
-template <int R>
+template <int R, int TT>
 __device__ __forceinline__ Start place_on_line(const AttendArgs &p, int64_t x)
 {
     const int lane = threadIdx.x & 31;
     Start s = {0, 0, 0, 0, 0};
     int64_t before = 0;
     for (int base = 0; base < p.seq.count; base += 32) {
-        const int64_t mine = base + lane < p.seq.count ? tiles_of<R>(p, base + lane) * p.heads : 0;
+        const int64_t mine = base + lane < p.seq.count ? tiles_of<R, TT>(p, base + lane) * p.heads : 0;
         int64_t upto = mine;
         for (int d = 1; d < 32; d <<= 1) {
             const int64_t other = __shfl_up_sync(0xffffffffu, upto, d);
@@ -127,8 +150,9 @@ __device__ __forceinline__ Start place_on_line(const AttendArgs &p, int64_t x)
             int64_t rest = x - (before + __shfl_sync(0xffffffffu, upto - mine, k));
             s.h = (int)(rest / tiles);
             rest -= s.h * tiles;
+            const Sequence q = sequence_at(p, s.b);
             for (;;) {
-                const int nt = unit_of<R>(p, s.b, s.h, s.rc).nt;
+                const int nt = unit_of<R, TT>(p, q, s.b, s.h, s.rc).nt;
                 if (rest < nt) break;
                 rest -= nt;
                 s.rc++;
@@ -141,20 +165,21 @@ __device__ __forceinline__ Start place_on_line(const AttendArgs &p, int64_t x)
     s.b = p.seq.count;
     return s;
 }
-// Shares there are: one a block, but none of less than LEAST_TILES tiles unless every unit has one.
+// Shares there are: one a block, but none of less than LEAST_TOKENS tokens unless every unit has one.
+template <int TT>
 __device__ __forceinline__ int64_t shares_of(const AttendArgs &p, int64_t total)
 {
     const int64_t units = (int64_t)p.seq.count * p.heads * p.chunks;
-    return max((int64_t)1, min(min((int64_t)p.grid, total), max(units, total / LEAST_TILES)));
+    return max((int64_t)1, min(min((int64_t)p.grid, total), max(units, total / (LEAST_TOKENS / TT))));
 }
-template <int R>
+template <int R, int TT>
 __device__ __forceinline__ Start start_of(const AttendArgs &p, int block)
 {
-    const int64_t total = line_length<R>(p), shares = shares_of(p, total);
+    const int64_t total = line_length<R, TT>(p), shares = shares_of<TT>(p, total);
     Start s = {0, 0, 0, 0, 0};
     if (block >= shares) return s;
     const int64_t from = total * block / shares, to = total * (block + 1) / shares;
-    if (to > from) s = place_on_line<R>(p, from);
+    if (to > from) s = place_on_line<R, TT>(p, from);
     s.left = to - from;
     return s;
 }
@@ -163,17 +188,17 @@ struct Cut {
     int b, h, rc;
     int block, parts;                          // parts: 0, or how many blocks from block - 1 on hold parts of the unit
 };
-template <int R>
+template <int R, int TT>
 __device__ __forceinline__ Cut cut_of(const AttendArgs &p, int block)
 {
-    const int64_t total = line_length<R>(p), shares = shares_of(p, total);
+    const int64_t total = line_length<R, TT>(p), shares = shares_of<TT>(p, total);
     Cut c = {0, 0, 0, block, 0};
     if (block >= shares) return c;
     const int64_t from = total * block / shares, before = total * (block - 1) / shares;
     if (from >= total) return c;
-    const Start s = place_on_line<R>(p, from);
+    const Start s = place_on_line<R, TT>(p, from);
     if (s.tile == 0 || before > from - s.tile) return c;      // not inside a unit, or not the first boundary inside it
-    const int64_t end = from - s.tile + unit_of<R>(p, s.b, s.h, s.rc).nt;
+    const int64_t end = from - s.tile + unit_of<R, TT>(p, s.b, s.h, s.rc).nt;
     c.b = s.b;
     c.h = s.h;
     c.rc = s.rc;
@@ -188,7 +213,7 @@ struct Piece {                                 // tiles first .. first + count -
 };
 
 // The pieces of a block's share, one after the other.
-template <int R>
+template <int R, int TT>
 struct Walk {
     const AttendArgs &p;
     int b, h, rc, tile;
@@ -214,7 +239,7 @@ struct Walk {
                     next_unit += gridDim.x;
                 }
                 if (rc < chunks_of<R>(p, b)) {
-                    piece.unit = unit_of<R>(p, b, h, rc);
+                    piece.unit = unit_of<R, TT>(p, b, h, rc);
                     piece.first = 0;
                     piece.count = piece.unit.nt;
                     return true;
@@ -228,7 +253,7 @@ struct Walk {
             if (++h == p.heads) { h = 0; b++; }
             if (b >= p.seq.count) return false;
         }
-        piece.unit = unit_of<R>(p, b, h, rc);
+        piece.unit = unit_of<R, TT>(p, b, h, rc);
         piece.first = tile;
         piece.count = (int)min((int64_t)(piece.unit.nt - tile), left);
         if (piece.count <= 0) return false;

@@ -1,0 +1,62 @@
+// The second kernel of an attention call whose work was cut inside sequences.
+#pragma once
+
+#include "attend_device.cuh"
+
+namespace qb {
+
+// Joins the parts of the units that a share's end cuts: block c looks after the unit that the c-th boundary cuts first.
+template <int R, int TT, typename T>
+__global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendArgs p)
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    __shared__ Cut cut;
+    if (threadIdx.x < 32) {
+        const Cut c = cut_of<R, TT>(p, blockIdx.x + 1);
+        if (threadIdx.x == 0) cut = c;
+    }
+    __syncthreads();
+    if (cut.parts == 0) return;
+    const Unit u = unit_of<R, TT>(p, cut.b, cut.h, cut.rc);
+    const int rows = u.r1 - u.r0, quads = p.dim / 4;
+    const size_t size = part_floats(R, p.dim);
+    const float *first = (const float *)p.workspace + (size_t)((cut.block - 1) * 2 + 1) * size;      // the part that begins the unit
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * quads; i += 256 * gridDim.y) {
+        const int r = i / quads, d = (i - r * quads) * 4;
+        float m = NOTHING;
+        for (int k = 0; k < cut.parts; k++) m = fmaxf(m, first[(k ? (size_t)(2 * k - 1) * size : 0) + r * 2]);
+        float sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < cut.parts; k++) {
+            const float *part = first + (k ? (size_t)(2 * k - 1) * size : 0);
+            const float2 s = *(const float2 *)(part + r * 2);
+            const float4 x = *(const float4 *)(part + R * 2 + r * p.dim + d);
+            const float f = exp2_fast(s.x - m);
+            sum = __fmaf_rn(s.y, f, sum);
+            acc.x = __fmaf_rn(x.x, f, acc.x);
+            acc.y = __fmaf_rn(x.y, f, acc.y);
+            acc.z = __fmaf_rn(x.z, f, acc.z);
+            acc.w = __fmaf_rn(x.w, f, acc.w);
+        }
+        finish_row<T>(p, u, u.r0 + r, d, acc, m, sum);
+    }
+}
+
+// Launched beside the kernel whose parts it joins (a programmatic dependent: it waits for that kernel's end itself).
+template <int R, int TT, typename T>
+static int launch_join(const AttendArgs &args, cudaStream_t stream)
+{
+    if (args.grid < 2) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(args.grid - 1, R > 16 ? R / 16 : 1);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, attend_join_kernel<R, TT, T>, args);
+}
+
+}  // namespace qb

@@ -20,11 +20,9 @@
 //    weights down to 2^-29 of the largest with all its bits, and the accumulators are seldom rescaled.
 //  * q is scaled by a power of two to a row's maximum of 2^13 and cut to f16; with f32 lanes q and w enter as the sum of
 //    two f16 (SPL 2), which loses 2^-22.
-#include <cuda.h>
 #include "common.cuh"
-#include "cache.h"
-#include "cache_device.cuh"
 #include "attend_device.cuh"
+#include "attend_join.cuh"
 
 namespace qb {
 
@@ -77,12 +75,12 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
         mbar_fence_init();
     }
     if (warp == 0) {
-        const Start s = p.whole ? Start{} : start_of<C::R>(p, blockIdx.x);
+        const Start s = p.whole ? Start{} : start_of<C::R, 32>(p, blockIdx.x);
         if (lane == 0) head->start = s;
     }
     __syncthreads();
     if (!p.whole) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the joining kernel waits beside this one
-    Walk<C::R> walk(p, head->start);
+    Walk<C::R, 32> walk(p, head->start);
     volatile int *abort = &head->abort;
     uint32_t seq = 0;                          // tiles of this block so far
 
@@ -433,50 +431,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
     }
 }
 
-// Joins the parts of the units that a share's end cuts: block c looks after the unit that the c-th boundary cuts first.
-template <int R, typename T>
-__global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendArgs p)
-{
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    __shared__ Cut cut;
-    if (threadIdx.x < 32) {
-        const Cut c = cut_of<R>(p, blockIdx.x + 1);
-        if (threadIdx.x == 0) cut = c;
-    }
-    __syncthreads();
-    if (cut.parts == 0) return;
-    const Unit u = unit_of<R>(p, cut.b, cut.h, cut.rc);
-    const int rows = u.r1 - u.r0, quads = p.dim / 4;
-    const size_t size = part_floats(R, p.dim);
-    const float *first = (const float *)p.workspace + (size_t)((cut.block - 1) * 2 + 1) * size;      // the part that begins the unit
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * quads; i += 256 * gridDim.y) {
-        const int r = i / quads, d = (i - r * quads) * 4;
-        float m = NOTHING;
-        for (int k = 0; k < cut.parts; k++) m = fmaxf(m, first[(k ? (size_t)(2 * k - 1) * size : 0) + r * 2]);
-        float sum = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < cut.parts; k++) {
-            const float *part = first + (k ? (size_t)(2 * k - 1) * size : 0);
-            const float2 s = *(const float2 *)(part + r * 2);
-            const float4 x = *(const float4 *)(part + R * 2 + r * p.dim + d);
-            const float f = exp2_fast(s.x - m);
-            sum = __fmaf_rn(s.y, f, sum);
-            acc.x = __fmaf_rn(x.x, f, acc.x);
-            acc.y = __fmaf_rn(x.y, f, acc.y);
-            acc.z = __fmaf_rn(x.z, f, acc.z);
-            acc.w = __fmaf_rn(x.w, f, acc.w);
-        }
-        finish_row<T>(p, u, u.r0 + r, d, acc, m, sum);
-    }
-}
-
 // ---------------------------------------------------------------------------------------------- host
-
-typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiled g_attend_encode = nullptr;
-static int *g_attend_status = nullptr;
-static int g_attend_sms = 0;
 
 template <int DT, int NB, int SPL, typename T>
 static cudaError_t set_rows_attr()
@@ -491,101 +446,34 @@ static cudaError_t set_rows_attrs()
     return set_rows_attr<DT, NB, 1, __nv_bfloat16>();
 }
 
-cudaError_t attend_init(int sm_count, int max_smem, int *status)
+cudaError_t attend_rows_init()
 {
-    g_attend_status = status;
-    g_attend_sms = sm_count;
-    if (max_smem < 232448) return cudaErrorInvalidValue;
-    void *fn = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found);
-    if (e) return e;
-    if (found != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
-    g_attend_encode = (EncodeTiled)fn;
+    cudaError_t e;
     if ((e = set_rows_attrs<64, 1>()) || (e = set_rows_attrs<64, 2>()) || (e = set_rows_attrs<128, 1>()) || (e = set_rows_attrs<128, 2>())) return e;
     return set_rows_attrs<256, 1>();
 }
 
-// rows a unit of the rows kernel: 16 where a group has more than 8 rows (dim <= 128: the accumulators of 16 rows fit beside it)
-static int rows_a_unit(int dim, int rows) { return dim <= 128 && rows > 8 ? 16 : 8; }
-
-size_t attend_workspace_bytes(int dim, int heads, int type, int count, int rows, int q_heads, int max_queries, int max_length)
-{
-    (void)type; (void)count; (void)rows; (void)max_length;
-    const int r = rows_a_unit(dim, q_heads / heads * max_queries);
-    return (size_t)g_attend_sms * 2 * part_floats(r, dim) * 4;
-}
-
-static bool codes_map(CUtensorMap &map, const void *codes, const qb200_cache_t &c, int box_dim, int box_rows)
-{
-    const cuuint64_t dims[2] = { (cuuint64_t)c.dim, (cuuint64_t)c.pages * c.heads * c.page }, strides[1] = { (cuuint64_t)c.dim };
-    const cuuint32_t box[2] = { (cuuint32_t)box_dim, (cuuint32_t)box_rows }, estr[2] = { 1, 1 };
-    return g_attend_encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           box_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int DT, int NB, int SPL, typename T>
-static int launch_rows(AttendArgs &args, const qb200_cache_t &c, int grid, cudaStream_t stream)
+static int launch_rows(const AttendArgs &args, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t stream)
 {
-    CUtensorMap kmap, vmap;
-    const int box = DT == 64 ? 64 : 128, rows = c.page < 32 ? c.page : 32;
-    if (!codes_map(kmap, c.k_codes, c, box, rows) || !codes_map(vmap, c.v_codes, c, box, rows)) return (int)cudaErrorInvalidValue;
-    attend_rows_kernel<DT, NB, SPL, T><<<grid, RTHREADS, RowsCfg<DT, NB, SPL>::SMEM, stream>>>(args, kmap, vmap);
-    cudaError_t e = cudaGetLastError();
-    if (e || args.whole || grid < 2) return (int)e;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(grid - 1); cfg.blockDim = dim3(256); cfg.stream = stream; cfg.attrs = &attr; cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, attend_join_kernel<8 * NB, T>, args);
+    attend_rows_kernel<DT, NB, SPL, T><<<args.grid, RTHREADS, RowsCfg<DT, NB, SPL>::SMEM, stream>>>(args, kmap, vmap);
+    const cudaError_t e = cudaGetLastError();
+    return e || args.whole ? (int)e : launch_join<8 * NB, 32, T>(args, stream);
 }
 
 template <int SPL, typename T>
-static int launch_rows_dim(AttendArgs &args, const qb200_cache_t &c, int r, int grid, cudaStream_t stream)
+static int launch_rows_dim(const AttendArgs &args, int r, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t stream)
 {
-    if (c.dim <= 64) return r == 16 ? launch_rows<64, 2, SPL, T>(args, c, grid, stream) : launch_rows<64, 1, SPL, T>(args, c, grid, stream);
-    if (c.dim <= 128) return r == 16 ? launch_rows<128, 2, SPL, T>(args, c, grid, stream) : launch_rows<128, 1, SPL, T>(args, c, grid, stream);
-    return launch_rows<256, 1, SPL, T>(args, c, grid, stream);
+    if (args.dim <= 64) return r == 16 ? launch_rows<64, 2, SPL, T>(args, kmap, vmap, stream) : launch_rows<64, 1, SPL, T>(args, kmap, vmap, stream);
+    if (args.dim <= 128) return r == 16 ? launch_rows<128, 2, SPL, T>(args, kmap, vmap, stream) : launch_rows<128, 1, SPL, T>(args, kmap, vmap, stream);
+    return launch_rows<256, 1, SPL, T>(args, kmap, vmap, stream);
 }
 
-int attend(const AttendCall &call, cudaStream_t stream)
+int attend_rows(const AttendArgs &args, int type, int r, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t stream)
 {
-    if (call.seq.count == 0 || call.seq.rows == 0) return 0;
-    const qb200_cache_t &c = call.cache;
-    const int size = call.type == QB200_F32 ? 4 : 2;
-    AttendArgs a;
-    a.seq = call.seq;
-    a.q = call.q;
-    a.out = call.out;
-    a.lse = call.lse;
-    a.k_scales = c.k_scales;
-    a.v_scales = c.v_scales;
-    a.pages = c.pages;
-    a.heads = c.heads;
-    a.dim = c.dim;
-    a.log_page = c.page == 16 ? 4 : c.page == 32 ? 5 : c.page == 64 ? 6 : 7;
-    a.group = call.q_heads / c.heads;
-    a.q_heads = call.q_heads;
-    a.causal = call.causal;
-    a.window = call.window;
-    a.scale = call.scale;
-    a.q_wide = ((uintptr_t)call.q.base & 15) == 0 && call.q.row * size % 16 == 0 && call.q.head * size % 16 == 0;
-    a.out_wide = ((uintptr_t)call.out.base & (4 * size - 1)) == 0 && call.out.row % 4 == 0 && call.out.head % 4 == 0;
-    a.workspace = call.workspace;
-    a.status = g_attend_status;
-    const int r = rows_a_unit(c.dim, a.group * call.max_queries);
-    a.chunks = (a.group * call.max_queries + r - 1) / r;
-    // A unit (the rows r of one head of one sequence) goes to one block whole where it is short: cutting it would cost a
-    // second launch.
-    const int64_t units = (int64_t)call.seq.count * c.heads * a.chunks;
-    a.whole = call.max_length <= 1024;
-    const int grid = a.whole ? (int)(units < 65535 * 8 ? units : 65535 * 8) : g_attend_sms;
-    a.grid = grid;
-    if (call.type == QB200_F32) return launch_rows_dim<2, float>(a, c, r, grid, stream);
-    if (call.type == QB200_F16) return launch_rows_dim<1, __half>(a, c, r, grid, stream);
-    return launch_rows_dim<1, __nv_bfloat16>(a, c, r, grid, stream);
+    if (type == QB200_F32) return launch_rows_dim<2, float>(args, r, kmap, vmap, stream);
+    if (type == QB200_F16) return launch_rows_dim<1, __half>(args, r, kmap, vmap, stream);
+    return launch_rows_dim<1, __nv_bfloat16>(args, r, kmap, vmap, stream);
 }
 
 }  // namespace qb

@@ -1,0 +1,541 @@
+// Attention over the 8-bit cache for many rows (prompts, guessed tokens, large groups) on the fifth-generation tensor cores.
+//
+// out = softmax(scale * q K^T) V as in attend_rows.cu, with 128 rows (tokens x the query heads of a group) a tile and tiles
+// of TT tokens of the cache.  Here the operations bound it: a pair of row tiles and 128 tokens of 128 dims are 2 x 2 products
+// of 128 x 128 x 128, 2048 cycles of the tensor pipe, and as many cycles of the exponential unit.  So:
+//  * S = q K^T and O += P V are tcgen05.mma kind::f16 (codes are exact in f16), issued by one thread, S, P and O in tensor
+//    memory: P replaces S in place as f16 and is read from there as the second product's A operand.
+//  * Eight converter warps fetch the codes (16 bytes a load, a tile ahead in registers) and store them as f16 core matrices
+//    (8 tokens x 8 dims): one layout that is K-major for K (a row a token) and MN-major for V (a row a dim).  Every byte of
+//    the cache is converted once for the 256 rows of a block.
+//  * Two groups of four softmax warps, a thread a row, work on the two row tiles in turn with the tensor pipe: while one
+//    takes exponentials the pipe has the other's products.  With one row tile (NQ 1, or a unit of at most 128 rows) the two
+//    S buffers take the tiles of tokens alternately instead.
+//  * A thread reads its row of S twice, for the maximum and for the weights: the second reading costs less than the 64
+//    registers that would hold the row.  The maximum is kept while weights stay below 2^15, so O is seldom rescaled.
+// Scales, exponents and the cut of q and w are those of attend_rows.cu; so are the shares of the grid's blocks.
+#include "common.cuh"
+#include "attend_device.cuh"
+#include "attend_join.cuh"
+#include "tcgen05.cuh"
+
+namespace qb {
+
+constexpr int CW = 8;                          // converter warps: four for K, four for V
+
+template <int DC, int SPL>
+struct TilesCfg {
+    static constexpr int TT = DC == 128 ? 128 : 64;             // tokens a tile
+    static constexpr int NQ = DC == 128 ? 2 : 1;                // row tiles a block
+    static constexpr int R = 128 * NQ;
+    static constexpr int SLOTS = SPL == 1 ? 2 : 1;              // of K and of V
+    static constexpr int NG = TT / 16;
+    static constexpr int WARPS = 4 * NQ + CW + 1, THREADS = 32 * WARPS;
+    static constexpr uint32_t QTILE = 128 * DC * 2, SLOT = TT * DC * 2;
+    static constexpr uint32_t O_Q = 0, O_K = NQ * SPL * QTILE, O_V = O_K + SLOTS * SLOT, O_HEAD = O_V + SLOTS * SLOT, SMEM = O_HEAD + 2048 + 128;
+    static_assert(SMEM <= 232448, "227 KB of shared memory");
+    __host__ __device__ static constexpr uint32_t s_col(int b) { return b * TT; }
+    __host__ __device__ static constexpr uint32_t o_col(int t) { return 256 + t * 128; }
+};
+
+struct TilesHead {
+    uint64_t qfull, ofull, drain;
+    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], odone[2];
+    Start start;
+    uint32_t tmem;
+    int abort;
+    float factor[256];
+};
+static_assert(sizeof(TilesHead) <= 2048, "the header fits");
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+                   "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[tmem] . B, A's row of 16 f16 in eight columns.
+__device__ __forceinline__ void mma_issue_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// The tiles of a block's share in order, for the converters.
+template <int R, int TT>
+struct KvTile {
+    int b, h, base, lo, hi;
+    bool there;
+};
+template <int R, int TT>
+struct KvWalk {
+    Walk<R, TT> walk;
+    Piece piece;
+    int at;
+    bool more;
+    __device__ __forceinline__ KvWalk(const AttendArgs &p, const Start &s) : walk(p, s), at(0) { more = walk.next(piece); }
+    __device__ __forceinline__ KvTile<R, TT> next()
+    {
+        KvTile<R, TT> t;
+        if (more && at == piece.count) {
+            at = 0;
+            more = walk.next(piece);
+        }
+        t.there = more;
+        if (more) {
+            t.b = piece.unit.b;
+            t.h = piece.unit.h;
+            t.base = (piece.unit.t0 + piece.first + at) * TT;
+            t.lo = piece.unit.lo;
+            t.hi = piece.unit.hi;
+            at++;
+        }
+        return t;
+    }
+};
+
+// The page that holds token `token` of sequence b, or -1.
+__device__ __forceinline__ int page_at(const AttendArgs &p, int b, int token, int lo, int hi, int tokens, bool report)
+{
+    if (token >= hi || token + tokens <= lo) return -1;
+    const int id = p.seq.table[(int64_t)b * p.seq.width + (token >> p.log_page)];
+    if (id >= 0 && id < p.pages) return id;
+    if (report) atomicOr(p.status, STATUS_CACHE_RANGE);
+    return -1;
+}
+
+template <int DC, int SPL, typename T>
+__global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_kernel(const __grid_constant__ AttendArgs p)
+{
+    using C = TilesCfg<DC, SPL>;
+    constexpr int TT = C::TT, NQ = C::NQ, R = C::R, SLOTS = C::SLOTS, NG = C::NG;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
+    TilesHead *head = (TilesHead *)(smem + C::O_HEAD);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base_u32 = smem_u32(smem);
+    const uint32_t qfull = smem_u32(&head->qfull), ofull = smem_u32(&head->ofull), drain = smem_u32(&head->drain);
+    const uint32_t kfull = smem_u32(head->kfull), kempty = smem_u32(head->kempty), vfull = smem_u32(head->vfull), vempty = smem_u32(head->vempty);
+    const uint32_t sfull = smem_u32(head->sfull), pfull = smem_u32(head->pfull), odone = smem_u32(head->odone);
+
+    if (threadIdx.x == 0) {
+        head->abort = 0;
+        mbar_init(qfull, 4 * NQ);
+        mbar_init(ofull, 1);
+        mbar_init(drain, 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(kfull + 8 * i, 4);
+            mbar_init(kempty + 8 * i, 1);
+            mbar_init(vfull + 8 * i, 4);
+            mbar_init(vempty + 8 * i, 1);
+            mbar_init(sfull + 8 * i, 1);
+            mbar_init(pfull + 8 * i, 4);
+            mbar_init(odone + 8 * i, 1);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 0) {
+        const Start s = start_of<R, TT>(p, blockIdx.x);
+        if (lane == 0) head->start = s;
+    }
+    if (warp == C::WARPS - 1) tmem_alloc(smem_u32(&head->tmem), 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");           // the joining kernel waits beside this one
+    const uint32_t tmem = head->tmem;
+    volatile int *abort = &head->abort;
+    int *status = p.status;
+
+    if (warp < 4 * NQ) {
+        // ------------------------------------------------------------------ softmax: a thread a row
+        const int t = warp >> 2, quarter = warp & 3;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        Walk<R, TT> walk(p, head->start);
+        Piece piece;
+        uint32_t pieces = 0, uses[2] = {0, 0}, done = 0;         // uses of the S buffers and of this group's O so far
+        while (walk.next(piece)) {
+            const Unit &u = piece.unit;
+            const int nq = NQ == 2 && u.r1 - u.r0 > 128 ? 2 : 1;
+            const bool active = t < nq;
+            const int n = piece.count;
+            if (active) {
+                // q: half a warp a row of up to 128 dims, a warp a row beyond
+                constexpr int PER = DC == 128 ? 2 : 1, WIDTH = 32 / PER;
+                uint8_t *tile = smem + C::O_Q + t * SPL * C::QTILE;
+                const int col = lane % WIDTH;
+#pragma unroll 4
+                for (int i = 0; i < 32 / PER; i++) {
+                    const int r = quarter * 32 + i * PER + lane / WIDTH, at = u.r0 + t * 128 + r;
+                    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    if (at < u.r1 && col < p.dim / 8) {
+                        const T *src = (const T *)p.q.base + (int64_t)(u.row + at / p.group) * p.q.row + (int64_t)(u.h * p.group + at % p.group) * p.q.head + col * 8;
+                        unpack8(load8<T>(src, p.q_wide), x);
+                    }
+                    float top = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[k]));
+#pragma unroll
+                    for (int d = WIDTH / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    float up, down;
+                    power_scale(top, up, down);
+                    if (p.scale < 0.f) up = -up;               // a factor below stays positive, so maxima can be taken of the sums
+                    if (col < p.dim / 8) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) split2(x[2 * k] * up, x[2 * k + 1] * up, hi[k], lo[k]);
+                        uint8_t *dst = tile + col * 2048 + (r >> 3) * 128 + (r & 7) * 16;
+                        *(uint4 *)dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        if (SPL == 2) *(uint4 *)(dst + C::QTILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                    if (col == 0) head->factor[t * 128 + r] = fabsf(p.scale) * 1.4426950408889634f * down;
+                }
+                fence_proxy_async();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(qfull);
+
+            float l = 0.f, mm = 0.f, vref = 0.f;
+            bool fresh = true;                                   // nothing seen yet: mm says nothing
+            const int at = u.r0 + t * 128 + quarter * 32 + lane;
+            bool ok = true;
+            if (active) {
+                const float factor = head->factor[t * 128 + quarter * 32 + lane];
+                int lo, hi;
+                row_limits(p, u, min(at, u.r1 - 1), lo, hi);
+                const int lo_most = __reduce_max_sync(0xffffffffu, lo), hi_least = __reduce_min_sync(0xffffffffu, hi);
+                // a lane a group of 16 tokens: page a tile of tokens ahead of the scales, scales a tile ahead of their use
+                const int first = (u.t0 + piece.first) * TT, mine = lane * 16;
+                auto page_of = [&](int j) { return lane < NG && j < n ? page_at(p, u.b, first + j * TT + mine, u.lo, u.hi, 16, quarter == 0) : -1; };
+                auto scales_of = [&](int id) {
+                    if (id < 0) return make_float2(0.f, -1.f);
+                    const int64_t i = (int64_t)id * p.heads + u.h;
+                    return make_float2(__ldg(p.k_scales + i), __ldg(p.v_scales + i));
+                };
+                float2 sc = scales_of(page_of(0));
+                int id = page_of(1);
+                for (int j = 0; j < n; j++) {
+                    const float2 sc_next = scales_of(id);
+                    id = page_of(j + 2);
+                    const int base = first + j * TT;
+                    const int buf = nq == 2 ? t : j & 1;
+                    const uint32_t use = uses[buf] + (nq == 2 ? j : j >> 1);
+                    if (!mbar_wait_lanes(sfull + 8 * buf, use & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
+                    tc_fence_after();
+                    // V's scales against the first of them
+                    const unsigned some = __ballot_sync(0xffffffffu, sc.y > 0.f);
+                    const float found = __shfl_sync(0xffffffffu, sc.y, some ? __ffs(some) - 1 : 0);
+                    if (vref == 0.f && some) vref = found;
+                    float lr_mine = 0.f, rinv_mine = 1.f;
+                    if (sc.y < 0.f) { lr_mine = -INFINITY; rinv_mine = 0.f; }
+                    else if (sc.y > 0.f && sc.y != vref) { lr_mine = log2_ratio(sc.y, vref); rinv_mine = __fdividef(vref, sc.y); }
+                    const bool whole = base >= lo_most && base + TT <= hi_least;
+                    const uint32_t s_at = tmem + lanes + C::s_col(buf);
+
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < TT / 32; c++) {
+                        uint32_t v[32];
+                        tmem_ld32(s_at + 32 * c, v);
+                        tmem_ld_landed32(v);
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float f = factor * __shfl_sync(0xffffffffu, sc.x, 2 * c + e), lr = __shfl_sync(0xffffffffu, lr_mine, 2 * c + e);
+                            if (whole) {
+                                float most = __uint_as_float(v[16 * e]);
+#pragma unroll
+                                for (int i = 1; i < 16; i++) most = fmaxf(most, __uint_as_float(v[16 * e + i]));
+                                top = fmaxf(top, __fmaf_rn(most, f, lr));
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 16; i++) {
+                                    const int token = base + 32 * c + 16 * e + i;
+                                    const float s = __fmaf_rn(__uint_as_float(v[16 * e + i]), f, lr);
+                                    if (token >= lo && token < hi) top = fmaxf(top, s);
+                                }
+                            }
+                        }
+                    }
+                    const bool above = fresh ? top > -INFINITY : top > mm + 15.f;
+                    if (__any_sync(0xffffffffu, above)) {
+                        float less = 1.f;
+                        if (above) {
+                            const float next = top - 7.f;
+                            if (!fresh) less = exp2_fast(mm - next);
+                            l *= less;
+                            mm = next;
+                            fresh = false;
+                        }
+                        if (j > 0) {                             // O so far, once the product before has ended
+                            if (!mbar_wait_lanes(odone + 8 * t, (done + j - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
+                            tc_fence_after();
+                            for (int d = 0; d < p.dim; d += 16) {
+                                uint32_t v[16];
+                                tmem_ld16(tmem + lanes + C::o_col(t) + d, v);
+                                tmem_ld_landed16(v);
+#pragma unroll
+                                for (int i = 0; i < 16; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * less);
+                                tmem_st16(tmem + lanes + C::o_col(t) + d, v);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < TT / 32; c++) {
+                        uint32_t v[32], w[16], w2[16];
+                        tmem_ld32(s_at + 32 * c, v);
+                        tmem_ld_landed32(v);
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float f = factor * __shfl_sync(0xffffffffu, sc.x, 2 * c + e);
+                            const float a = __shfl_sync(0xffffffffu, lr_mine, 2 * c + e) - mm, rinv = __shfl_sync(0xffffffffu, rinv_mine, 2 * c + e);
+                            float sum = 0.f;
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                float s0 = __fmaf_rn(__uint_as_float(v[16 * e + i]), f, a), s1 = __fmaf_rn(__uint_as_float(v[16 * e + i + 1]), f, a);
+                                if (!whole) {
+                                    const int token = base + 32 * c + 16 * e + i;
+                                    if (token < lo || token >= hi) s0 = -INFINITY;
+                                    if (token + 1 < lo || token + 1 >= hi) s1 = -INFINITY;
+                                }
+                                const float e0 = exp2_fast(s0), e1 = exp2_fast(s1);
+                                sum += e0 + e1;
+                                split2(e0, e1, w[8 * e + i / 2], w2[8 * e + i / 2]);
+                            }
+                            l = __fmaf_rn(sum, rinv, l);
+                        }
+                        tmem_st16(s_at + (SPL == 2 ? 32 : 16) * c, w);
+                        if (SPL == 2) tmem_st16(s_at + 32 * c + 16, w2);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(pfull + 8 * buf);
+                    sc = sc_next;
+                }
+            }
+            // the buffers' uses, whoever had them
+            if (nq == 2) { uses[0] += n; uses[1] += n; }
+            else { uses[0] += (n + 1) / 2; uses[1] += n / 2; }
+            if (active) done += n;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok || !mbar_wait_lanes(ofull, pieces & 1, abort, status, STATUS_ATTEND_WAIT)) break;
+            pieces++;
+            if (!active) continue;
+            tc_fence_after();
+            const float v0 = vref > 0.f ? vref : 1.f;
+            const bool complete = piece.first == 0 && n == u.nt;
+            const int r = at - u.r0;
+            float *slot = (float *)p.workspace + (size_t)(blockIdx.x * 2 + (piece.first ? 0 : 1)) * part_floats(R, p.dim);
+            for (int d = 0; d < p.dim; d += 16) {
+                uint32_t v[16];
+                tmem_ld16(tmem + lanes + C::o_col(t) + d, v);
+                tmem_ld_landed16(v);
+                if (at < u.r1) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 acc = make_float4(__uint_as_float(v[i]) * v0, __uint_as_float(v[i + 1]) * v0, __uint_as_float(v[i + 2]) * v0, __uint_as_float(v[i + 3]) * v0);
+                        if (complete) finish_row<T>(p, u, at, d + i, acc, mm, l);
+                        else *(float4 *)(slot + R * 2 + (size_t)r * p.dim + d + i) = acc;
+                    }
+                }
+            }
+            if (!complete && at < u.r1) *(float2 *)(slot + r * 2) = make_float2(fresh ? NOTHING : mm, l);
+        }
+    } else if (warp < 4 * NQ + CW) {
+        // ------------------------------------------------------------------ converters
+        const int kv = (warp - 4 * NQ) >> 2, w = (warp - 4 * NQ) & 3;
+        const int8_t *codes = kv ? p.v_codes : p.k_codes;
+        const uint32_t full = kv ? vfull : kfull, empty = kv ? vempty : kempty;
+        uint8_t *slots = smem + (kv ? C::O_V : C::O_K);
+        constexpr int GROUPS = TT / 32, HALVES = DC / 64;        // groups of 8 tokens a warp; a lane: a token and every fourth chunk of 16 dims
+        static_assert(GROUPS * HALVES == 8, "eight loads a lane");
+        const int r8 = lane & 7, c4 = lane >> 3, chunks = p.dim >> 4;
+        KvWalk<R, TT> tiles(p, head->start);
+        auto page_of = [&](const KvTile<R, TT> &t) {             // lane i: the page of this warp's i-th group
+            return t.there && lane < GROUPS ? page_at(p, t.b, t.base + (lane * 4 + w) * 8, t.lo, t.hi, 8, false) : -1;
+        };
+        auto load = [&](const KvTile<R, TT> &t, int id, uint4 (&raw)[8]) {
+#pragma unroll
+            for (int i = 0; i < GROUPS; i++) {
+                const int page = __shfl_sync(0xffffffffu, id, i);
+                const int token = t.base + (i * 4 + w) * 8 + r8;
+                const int8_t *row = codes + ((((int64_t)page * p.heads + t.h) << p.log_page) + (token & ((1 << p.log_page) - 1))) * p.dim;
+#pragma unroll
+                for (int k = 0; k < HALVES; k++)
+                    raw[i * HALVES + k] = page >= 0 && c4 + 4 * k < chunks ? __ldg((const uint4 *)row + c4 + 4 * k) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        KvTile<R, TT> now = tiles.next();
+        KvTile<R, TT> next = now;
+        int id = page_of(now);
+        uint4 raw[8], coming[8];
+        if (now.there) {
+            load(now, id, raw);
+            next = tiles.next();
+            id = page_of(next);
+        }
+        for (uint32_t seq = 0; now.there; seq++) {
+            const KvTile<R, TT> here = next;
+            if (here.there) {
+                load(here, id, coming);
+                next = tiles.next();
+                id = page_of(next);
+            }
+            const int slot = seq % SLOTS;
+            if (seq >= SLOTS && !mbar_wait_warp(empty + 8 * slot, (seq / SLOTS - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) break;
+            uint8_t *dst = slots + slot * C::SLOT;
+#pragma unroll
+            for (int i = 0; i < GROUPS; i++)
+#pragma unroll
+                for (int k = 0; k < HALVES; k++) {
+                    if (c4 + 4 * k < chunks) {
+                        uint32_t h[8];
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const uint32_t x = word(raw[i * HALVES + k], q) ^ 0x80808080u;
+                            h[2 * q] = codes_lo(x);
+                            h[2 * q + 1] = codes_hi(x);
+                        }
+                        uint8_t *at = dst + (2 * (c4 + 4 * k)) * (TT * 16) + (i * 4 + w) * 128 + r8 * 16;
+                        *(uint4 *)at = make_uint4(h[0], h[1], h[2], h[3]);
+                        *(uint4 *)(at + TT * 16) = make_uint4(h[4], h[5], h[6], h[7]);
+                    }
+                }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + 8 * slot);
+            now = here;
+#pragma unroll
+            for (int i = 0; i < 8; i++) raw[i] = coming[i];
+        }
+    } else if (lane == 0) {
+        // ------------------------------------------------------------------ one thread issues the products
+        Walk<R, TT> walk(p, head->start);
+        Piece piece;
+        const uint32_t s_desc = idesc_of(1, 128, TT), o_desc = idesc_of(1, 128, p.dim) | 1u << 16;      // B of the second: a row a dim
+        uint32_t kseq = 0, vseq = 0, uses[2] = {0, 0}, pieces = 0;
+        bool ok = true;
+        auto wait = [&](uint32_t bar, uint32_t parity) { ok = ok && mbar_wait(bar, parity & 1, abort, status, STATUS_ATTEND_WAIT); return ok; };
+        auto scores = [&](int t, int buf, uint32_t slot) {
+            const uint32_t k_at = base_u32 + C::O_K + slot * C::SLOT;
+#pragma unroll 1
+            for (int x = 0; x < SPL; x++) {
+                const uint32_t q_at = base_u32 + C::O_Q + (t * SPL + x) * C::QTILE;
+                for (int d = 0; d < p.dim / 16; d++)
+                    mma_issue<1>(tmem + C::s_col(buf), smem_desc(q_at + d * 4096, 2048, 128), smem_desc(k_at + d * (TT * 32), TT * 16, 128), s_desc, x | d);
+            }
+            mma_commit(sfull + 8 * buf);
+        };
+        auto sums = [&](int t, int buf, uint32_t slot, int j) {
+            const uint32_t v_at = base_u32 + C::O_V + slot * C::SLOT;
+#pragma unroll 1
+            for (int s = 0; s < TT / 16; s++) {
+                const uint64_t desc = smem_desc(v_at + s * 256, 128, TT * 16);
+                const uint32_t col = tmem + C::s_col(buf) + (SPL == 2 ? (s >> 1) * 32 + (s & 1) * 8 : s * 8);
+                mma_issue_ts(tmem + C::o_col(t), col, desc, o_desc, j | s);
+                if (SPL == 2) mma_issue_ts(tmem + C::o_col(t), col + 16, desc, o_desc, 1);
+            }
+            mma_commit(odone + 8 * t);
+        };
+        while (ok && walk.next(piece)) {
+            const int n = piece.count, nq = NQ == 2 && piece.unit.r1 - piece.unit.r0 > 128 ? 2 : 1;
+            if (!wait(qfull, pieces)) break;
+            tc_fence_after();
+            if (!wait(kfull + 8 * (kseq % SLOTS), kseq / SLOTS)) break;
+            for (int t = 0; t < nq; t++) scores(t, t, kseq % SLOTS);
+            mma_commit(kempty + 8 * (kseq % SLOTS));
+            kseq++;
+            for (int j = 0; j < n && ok; j++) {
+                const uint32_t vs = vseq % SLOTS, ks = kseq % SLOTS;
+                const bool more = j + 1 < n;
+                if (nq == 2) {
+                    for (int t = 0; t < 2; t++) {
+                        if (t == 0 && !wait(vfull + 8 * vs, vseq / SLOTS)) break;
+                        if (!wait(pfull + 8 * t, uses[t] + j)) break;
+                        tc_fence_after();
+                        sums(t, t, vs, j);
+                        if (more) {
+                            if (t == 0 && !wait(kfull + 8 * ks, kseq / SLOTS)) break;
+                            tc_fence_after();
+                            scores(t, t, ks);
+                        }
+                    }
+                } else {
+                    const int buf = j & 1;
+                    if (more) {
+                        if (!wait(kfull + 8 * ks, kseq / SLOTS)) break;
+                        tc_fence_after();
+                        scores(0, buf ^ 1, ks);
+                    }
+                    if (!wait(vfull + 8 * vs, vseq / SLOTS) || !wait(pfull + 8 * buf, uses[buf] + (j >> 1))) break;
+                    tc_fence_after();
+                    sums(0, buf, vs, j);
+                }
+                if (!ok) break;
+                mma_commit(vempty + 8 * vs);
+                vseq++;
+                if (more) {
+                    mma_commit(kempty + 8 * ks);
+                    kseq++;
+                }
+            }
+            if (!ok) break;
+            if (nq == 2) { uses[0] += n; uses[1] += n; }
+            else { uses[0] += (n + 1) / 2; uses[1] += n / 2; }
+            mma_commit(ofull);
+            pieces++;
+        }
+        // nothing may run on the tensor cores when the block gives its memory back
+        mma_commit(drain);
+        const long long from = clock64();
+        while (!mbar_try_wait(drain, 0) && clock64() - from < WAIT_CYCLES) { }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == C::WARPS - 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- host
+
+template <int DC, int SPL, typename T>
+static cudaError_t set_tiles_attr()
+{
+    return cudaFuncSetAttribute(attend_tiles_kernel<DC, SPL, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TilesCfg<DC, SPL>::SMEM);
+}
+
+cudaError_t attend_tiles_init()
+{
+    cudaError_t e;
+    if ((e = set_tiles_attr<128, 2, float>()) || (e = set_tiles_attr<128, 1, __half>()) || (e = set_tiles_attr<128, 1, __nv_bfloat16>())) return e;
+    if ((e = set_tiles_attr<256, 2, float>()) || (e = set_tiles_attr<256, 1, __half>())) return e;
+    return set_tiles_attr<256, 1, __nv_bfloat16>();
+}
+
+template <int DC, int SPL, typename T>
+static int launch_tiles(const AttendArgs &args, cudaStream_t stream)
+{
+    using C = TilesCfg<DC, SPL>;
+    attend_tiles_kernel<DC, SPL, T><<<args.grid, C::THREADS, C::SMEM, stream>>>(args);
+    const cudaError_t e = cudaGetLastError();
+    return e ? (int)e : launch_join<C::R, C::TT, T>(args, stream);
+}
+
+int attend_tiles(const AttendArgs &args, int type, cudaStream_t stream)
+{
+    if (type == QB200_F32) return args.dim <= 128 ? launch_tiles<128, 2, float>(args, stream) : launch_tiles<256, 2, float>(args, stream);
+    if (type == QB200_F16) return args.dim <= 128 ? launch_tiles<128, 1, __half>(args, stream) : launch_tiles<256, 1, __half>(args, stream);
+    return args.dim <= 128 ? launch_tiles<128, 1, __nv_bfloat16>(args, stream) : launch_tiles<256, 1, __nv_bfloat16>(args, stream);
+}
+
+}  // namespace qb

@@ -256,27 +256,29 @@ class GpuOps:
         """Quantises the rows of k and v ([rows, heads, dim], f32, f16 or bf16) into `cache` as tokens lengths[b], lengths[b] + 1,
         ... of their sequences.  table: int32 [sequences, width] of pages; lengths: int32, tokens already there; offsets: int32
         [sequences + 1], the rows of each sequence (None: one row each).  All on the device; nothing is synchronised."""
-        kind = self._lanes(cache, k, "k", cache.heads)
-        if self._lanes(cache, v, "v", cache.heads) != kind or v.shape[0] != k.shape[0]:
+        kind, rows, *at = self._lanes(cache, k, "k", cache.heads)
+        other, same, *v_at = self._lanes(cache, v, "v", cache.heads)
+        if other != kind or same != rows:
             raise ValueError("k and v have the same rows and type")
-        seq = self._sequences(cache, table, lengths, offsets, k.shape[0])
-        rc = self.lib.qb200_cache_write(cache.parts, seq, kind, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                                        _stream(stream))
-        self.gpu.check(rc, "CacheWrite")
+        seq = self._sequences(cache, table, lengths, offsets, rows)
+        self.gpu.check(self.lib.qb200_cache_write(cache.parts, seq, kind, *at, *v_at, _stream(stream)), "CacheWrite")
         return "s8 cache blocks"
 
     def CacheRead(self, cache, k, v, table, starts, offsets=None, stream=None):
         """Reads tokens starts[b], starts[b] + 1, ... of the sequences back into the rows of k and v (either may be None)."""
-        some = k if k is not None else v
-        if some is None:
+        if k is None and v is None:
             raise ValueError("neither k nor v is asked for")
-        kind = self._lanes(cache, some, "k" if some is k else "v", cache.heads)
-        if k is not None and v is not None and (self._lanes(cache, v, "v", cache.heads) != kind or v.shape[0] != k.shape[0]):
-            raise ValueError("k and v have the same rows and type")
-        seq = self._sequences(cache, table, starts, offsets, some.shape[0])
-        at = [(t.data_ptr(), t.stride(0), t.stride(1)) if t is not None else (None, 0, 0) for t in (k, v)]
-        rc = self.lib.qb200_cache_read(cache.parts, seq, kind, *at[0], *at[1], _stream(stream))
-        self.gpu.check(rc, "CacheRead")
+        kind, rows, *at = self._lanes(cache, v if k is None else k, "v" if k is None else "k", cache.heads)
+        if k is None:
+            at, v_at = (None, 0, 0), at
+        elif v is None:
+            v_at = (None, 0, 0)
+        else:
+            other, same, *v_at = self._lanes(cache, v, "v", cache.heads)
+            if other != kind or same != rows:
+                raise ValueError("k and v have the same rows and type")
+        seq = self._sequences(cache, table, starts, offsets, rows)
+        self.gpu.check(self.lib.qb200_cache_read(cache.parts, seq, kind, *at, *v_at, _stream(stream)), "CacheRead")
         return "s8 cache blocks"
 
     def CacheAttention(self, cache, q, out, table, lengths, offsets=None, max_queries=0, max_length=0, scale=None, causal=True, window=0,
@@ -287,50 +289,50 @@ class GpuOps:
         lengths, known to the host, for the choice of kernel (0: rows, or 1 without offsets; all the table holds).  scale None:
         1 / sqrt(dim).  workspace None: one of the call's own, from torch's allocator on the call's stream."""
         heads = q.shape[1] if q.dim() == 3 else 0
-        kind = self._lanes(cache, q, "q", heads)
-        if self._lanes(cache, out, "out", heads) != kind or out.shape[0] != q.shape[0]:
+        kind, rows, *at = self._lanes(cache, q, "q", heads)
+        other, same, *out_at = self._lanes(cache, out, "out", heads)
+        if other != kind or same != rows:
             raise ValueError("q and out have the same shape and type")
-        rows = q.shape[0]
-        if lse is not None:
-            import torch
-            if lse.dtype != torch.float32 or tuple(lse.shape) != (rows, heads) or not lse.is_contiguous() or lse.device != cache.device:
-                raise ValueError(f"lse: contiguous float32 {(rows, heads)} on {cache.device}")
         seq = self._sequences(cache, table, lengths, offsets, rows)
+        lse_at = None
+        if lse is not None:
+            if str(lse.dtype) != "torch.float32" or tuple(lse.shape) != (rows, heads) or not lse.is_contiguous() or lse.get_device() != cache.index:
+                raise ValueError(f"lse: contiguous float32 {(rows, heads)} on the cache's device")
+            lse_at = lse.data_ptr()
         if workspace is None:
-            need = self.lib.qb200_cache_attention_workspace_bytes(cache.parts, kind, seq.count, rows if offsets is not None else 1, heads,
-                                                                  int(max_queries), int(max_length) or seq.width * cache.page)
-            workspace, workspace_bytes = self._scratch_on(stream, need), need
-        rc = self.lib.qb200_cache_attention(cache.parts, seq, kind, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
-                                            out.stride(1), None if lse is None else lse.data_ptr(), heads, int(max_queries), int(max_length),
-                                            float(cache.dim ** -0.5 if scale is None else scale), int(bool(causal)), int(window), _ptr(workspace),
-                                            int(workspace_bytes), _stream(stream))
-        self.gpu.check(rc, "CacheAttention")
+            workspace_bytes = self.lib.qb200_cache_attention_workspace_bytes(cache.parts, kind, seq.count, rows if offsets is not None else 1, heads,
+                                                                             max_queries, max_length or seq.width * cache.page)
+            if workspace_bytes:
+                workspace = self._scratch_on(stream, workspace_bytes)
+        self.gpu.check(self.lib.qb200_cache_attention(cache.parts, seq, kind, *at, *out_at, lse_at, heads, max_queries, max_length,
+                                                      cache.dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, _ptr(workspace),
+                                                      workspace_bytes, _stream(stream)), "CacheAttention")
         return self.lib.qb200_lane_name(OP_ATTENTION, kind).decode()
 
     def _lanes(self, cache, t, name, heads):
-        """The lane type of rows [rows, heads, dim] of a cache operator; refuses what the C ABI cannot be told."""
+        """Rows [rows, heads, dim] of a cache operator as the C ABI takes them: (lane type, rows, address, row stride, head stride)."""
         kind = _LANES.get(str(t.dtype))
         if kind is None:
             raise NotImplementedError(f"{name}: {t.dtype}; rows are float32, float16 or bfloat16")
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != cache.dim:
-            raise ValueError(f"{name}: [rows, {heads}, {cache.dim}] is needed, got {tuple(t.shape)}")
-        if t.stride(2) != 1 and cache.dim > 1:
-            raise ValueError(f"{name}: the values of a head lie side by side (stride {t.stride(2)})")
-        if t.device != cache.device or t.device.index != self.gpu.device:
-            raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}, the library bound to cuda:{self.gpu.device}")
-        return kind
+        shape, strides = t.shape, t.stride()
+        if len(shape) != 3 or shape[1] != heads or shape[2] != cache.dim:
+            raise ValueError(f"{name}: [rows, {heads}, {cache.dim}] is needed, got {tuple(shape)}")
+        if strides[2] != 1:
+            raise ValueError(f"{name}: the values of a head lie side by side (stride {strides[2]})")
+        if t.get_device() != cache.index or cache.index != self.gpu.device:
+            raise ValueError(f"{name} is on {t.device}, the cache on {cache.k_codes.device}, the library bound to cuda:{self.gpu.device}")
+        return kind, shape[0], t.data_ptr(), strides[0], strides[1]
 
     def _sequences(self, cache, table, lengths, offsets, rows):
-        import torch
-        count = lengths.shape[0] if lengths.dim() == 1 else -1
-        if table.dim() != 2 or table.shape[0] != count or (table.stride(1) != 1 and table.shape[1] > 1) or (count > 1 and table.stride(0) != table.shape[1]):
-            raise ValueError(f"table: contiguous [sequences, width] for {count} sequences, got {tuple(table.shape)}")
-        if offsets is not None and tuple(offsets.shape) != (count + 1,):
-            raise ValueError(f"offsets: [{count + 1}], got {tuple(offsets.shape)}")
-        for t in (table, lengths, offsets):
-            if t is not None and (t.dtype != torch.int32 or t.device != cache.device or (t.dim() == 1 and t.shape[0] > 1 and t.stride(0) != 1)):
-                raise ValueError(f"table, lengths and offsets are contiguous int32 on {cache.device}")
-        return _lib.Sequences(table.data_ptr(), lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), count, table.shape[1], rows)
+        shape, counts = table.shape, lengths.shape
+        if len(counts) != 1 or len(shape) != 2 or shape[0] != counts[0]:
+            raise ValueError(f"table [sequences, width] and lengths [sequences]: got {tuple(shape)}, {tuple(counts)}")
+        if offsets is not None and tuple(offsets.shape) != (counts[0] + 1,):
+            raise ValueError(f"offsets: [{counts[0] + 1}], got {tuple(offsets.shape)}")
+        for t in (table, lengths) if offsets is None else (table, lengths, offsets):
+            if str(t.dtype) != "torch.int32" or not t.is_contiguous() or t.get_device() != cache.index:
+                raise ValueError(f"table, lengths and offsets are contiguous int32 on the cache's device: got {t.dtype} on {t.device}, strides {t.stride()}")
+        return _lib.Sequences(table.data_ptr(), lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), counts[0], shape[1], rows)
 
     def _scratch_on(self, stream, nbytes_):
         """A buffer of torch's allocator that belongs to `stream`: freed in its order, and the graph's own under capture."""
@@ -338,9 +340,9 @@ class GpuOps:
         device = torch.device("cuda", self.gpu.device)
         want = _stream(stream) or 0
         if torch.cuda.current_stream(device).cuda_stream == want:
-            return torch.empty(max(int(nbytes_), 16), dtype=torch.uint8, device=device)
+            return torch.empty(nbytes_, dtype=torch.uint8, device=device)
         with torch.cuda.stream(torch.cuda.ExternalStream(want, device=device) if want else torch.cuda.default_stream(device)):
-            return torch.empty(max(int(nbytes_), 16), dtype=torch.uint8, device=device)
+            return torch.empty(nbytes_, dtype=torch.uint8, device=device)
 
     # -- host-buffer form (upload, product, download), for callers that hold numpy arrays ---------
     def GemvBlocksHost(self, fmt, a, x, y, rows, cols, fmt_x=None):
