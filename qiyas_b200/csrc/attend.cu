@@ -82,6 +82,10 @@ int attend(const AttendCall &call, cudaStream_t stream)
     a.log_page = c.page == 16 ? 4 : c.page == 32 ? 5 : c.page == 64 ? 6 : 7;
     a.group = call.q_heads / c.heads;
     a.q_heads = call.q_heads;
+    int log_group = 0;
+    while ((1 << log_group) < a.group) log_group++;
+    a.group_shift = 31 + log_group;
+    a.group_magic = (uint32_t)((((uint64_t)1 << a.group_shift) + a.group - 1) / a.group);
     a.causal = call.causal;
     a.window = call.window;
     a.scale = call.scale;

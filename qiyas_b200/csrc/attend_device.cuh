@@ -25,9 +25,13 @@ struct AttendArgs {
     int whole;                                 // units are not cut: block c takes units c, c + grid, ...
     int chunks;                                // units a sequence and head, by the caller's bound
     int grid;
+    uint32_t group_magic;                      // n / group = n * magic >> shift for 0 <= n < 2^31
+    int group_shift;
     void *workspace;
     int *status;
 };
+
+__device__ __forceinline__ int by_group(const AttendArgs &p, int n) { return (int)(((uint64_t)(uint32_t)n * p.group_magic) >> p.group_shift); }
 
 cudaError_t attend_rows_init();
 int attend_rows(const AttendArgs &args, int type, int r, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t stream);
@@ -72,7 +76,7 @@ __device__ __forceinline__ Unit unit_of(const AttendArgs &p, const Sequence &s, 
     u.len = s.len;
     u.r0 = rc * R;
     u.r1 = min(u.r0 + R, u.n * p.group);
-    const int first = u.r0 / p.group, last = (max(u.r1, 1) - 1) / p.group;
+    const int first = by_group(p, u.r0), last = by_group(p, max(u.r1, 1) - 1);
     u.hi = p.causal ? max(0, min(u.len, u.len - u.n + last + 1)) : u.len;
     u.lo = p.window ? max(0, u.len - u.n + first + 1 - p.window) : 0;
     u.t0 = u.hi > u.lo ? u.lo / TT : 0;
@@ -88,7 +92,7 @@ __device__ __forceinline__ Unit unit_of(const AttendArgs &p, int b, int h, int r
 // The tokens row `at` of a unit's sequence sees.
 __device__ __forceinline__ void row_limits(const AttendArgs &p, const Unit &u, int at, int &lo, int &hi)
 {
-    const int place = u.len - u.n + at / p.group;
+    const int place = u.len - u.n + by_group(p, at);
     hi = p.causal ? max(0, min(u.len, place + 1)) : u.len;
     lo = p.window ? max(0, place + 1 - p.window) : 0;
 }
@@ -103,64 +107,95 @@ __device__ __forceinline__ int chunks_of(const AttendArgs &p, int b)
     return (n * p.group + R - 1) / R;
 }
 
-// Tiles of one head of sequence b.
-template <int R, int TT>
-__device__ __forceinline__ int64_t tiles_of(const AttendArgs &p, int b)
-{
-    int64_t sum = 0;
-    const Sequence s = sequence_at(p, b);
-    const int chunks = (s.n * p.group + R - 1) / R;
-    for (int rc = 0; rc < chunks; rc++) sum += unit_of<R, TT>(p, s, b, 0, rc).nt;
-    return sum;
-}
-
 struct Start {
     int b, h, rc, tile;                        // where a share begins: a unit and a tile inside it
     int64_t left;                              // tiles it has
 };
 
-// Called by a whole warp: the place `x` on the line of tiles, sequence after sequence, head after head; `total` is its length.
+// The line of tiles: sequence after sequence, head after head, unit after unit.  The functions below are called by a whole
+// warp.  Few sequences: a lane a unit; many: a lane a sequence.
+constexpr int FEW_SEQUENCES = 8;
+
+// Tiles of one head of sequence b: this lane's part of them (few sequences), or all.
+template <int R, int TT>
+__device__ __forceinline__ int64_t tiles_of(const AttendArgs &p, int b, int first, int step)
+{
+    int64_t sum = 0;
+    const Sequence s = sequence_at(p, b);
+    const int chunks = (s.n * p.group + R - 1) / R;
+    for (int rc = first; rc < chunks; rc += step) sum += unit_of<R, TT>(p, s, b, 0, rc).nt;
+    return sum;
+}
+__device__ __forceinline__ int64_t warp_sum(int64_t x)
+{
+#pragma unroll
+    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+}
+__device__ __forceinline__ int64_t warp_upto(int64_t x)          // the sum over this lane and those before it
+{
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t other = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += other;
+    }
+    return x;
+}
 template <int R, int TT>
 __device__ __forceinline__ int64_t line_length(const AttendArgs &p)
 {
     const int lane = threadIdx.x & 31;
     int64_t sum = 0;
-    for (int b = lane; b < p.seq.count; b += 32) sum += tiles_of<R, TT>(p, b);
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    return sum * p.heads;
+    if (p.seq.count <= FEW_SEQUENCES)
+        for (int b = 0; b < p.seq.count; b++) sum += tiles_of<R, TT>(p, b, lane, 32);
+    else
+        for (int b = lane; b < p.seq.count; b += 32) sum += tiles_of<R, TT>(p, b, 0, 1);
+    return warp_sum(sum) * p.heads;
 }
+// Where place x of the line is; x is below its length.
 template <int R, int TT>
 __device__ __forceinline__ Start place_on_line(const AttendArgs &p, int64_t x)
 {
     const int lane = threadIdx.x & 31;
-    Start s = {0, 0, 0, 0, 0};
-    int64_t before = 0;
-    for (int base = 0; base < p.seq.count; base += 32) {
-        const int64_t mine = base + lane < p.seq.count ? tiles_of<R, TT>(p, base + lane) * p.heads : 0;
-        int64_t upto = mine;
-        for (int d = 1; d < 32; d <<= 1) {
-            const int64_t other = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += other;
+    Start s = {p.seq.count, 0, 0, 0, 0};
+    int64_t tiles = 0;                         // of one head of the sequence found
+    if (p.seq.count <= FEW_SEQUENCES) {
+        for (int b = 0; b < p.seq.count; b++) {
+            tiles = warp_sum(tiles_of<R, TT>(p, b, lane, 32));
+            if (x < tiles * p.heads) { s.b = b; break; }
+            x -= tiles * p.heads;
         }
-        const unsigned after = __ballot_sync(0xffffffffu, before + upto > x);
+    } else {
+        for (int base = 0; base < p.seq.count; base += 32) {
+            const int64_t mine = base + lane < p.seq.count ? tiles_of<R, TT>(p, base + lane, 0, 1) : 0, upto = warp_upto(mine) * p.heads;
+            const unsigned after = __ballot_sync(0xffffffffu, upto > x);
+            if (after) {
+                const int k = __ffs(after) - 1;
+                s.b = base + k;
+                tiles = __shfl_sync(0xffffffffu, mine, k);
+                x -= __shfl_sync(0xffffffffu, upto, k) - tiles * p.heads;
+                break;
+            }
+            x -= __shfl_sync(0xffffffffu, upto, 31);
+        }
+    }
+    if (s.b == p.seq.count || tiles == 0) { s.b = p.seq.count; return s; }
+    s.h = (int)(x / tiles);
+    x -= s.h * tiles;
+    const Sequence q = sequence_at(p, s.b);
+    const int chunks = (q.n * p.group + R - 1) / R;
+    for (int base = 0; base < chunks; base += 32) {
+        const int64_t upto = warp_upto(base + lane < chunks ? unit_of<R, TT>(p, q, s.b, s.h, base + lane).nt : 0);
+        const unsigned after = __ballot_sync(0xffffffffu, upto > x);
         if (after) {
             const int k = __ffs(after) - 1;
-            s.b = base + k;
-            const int64_t tiles = __shfl_sync(0xffffffffu, mine, k) / p.heads;
-            int64_t rest = x - (before + __shfl_sync(0xffffffffu, upto - mine, k));
-            s.h = (int)(rest / tiles);
-            rest -= s.h * tiles;
-            const Sequence q = sequence_at(p, s.b);
-            for (;;) {
-                const int nt = unit_of<R, TT>(p, q, s.b, s.h, s.rc).nt;
-                if (rest < nt) break;
-                rest -= nt;
-                s.rc++;
-            }
-            s.tile = (int)rest;
+            s.rc = base + k;
+            const int64_t before = __shfl_sync(0xffffffffu, upto, k > 0 ? k - 1 : 0);
+            s.tile = (int)(x - (k > 0 ? before : 0));
             return s;
         }
-        before += __shfl_sync(0xffffffffu, upto, 31);
+        x -= __shfl_sync(0xffffffffu, upto, 31);
     }
     s.b = p.seq.count;
     return s;
@@ -330,22 +365,43 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void *map, int x
                  : "memory");
 }
 
-// Four dims of a row from the sums: numerator, denominator, and the exponent both are taken against.
+// Where row `at` of a unit's sequence goes, and its logarithm of the sum.
 template <typename T>
-__device__ __forceinline__ void finish_row(const AttendArgs &p, const Unit &u, int at, int d, const float4 &acc, float m, float sum)
+__device__ __forceinline__ T *out_row(const AttendArgs &p, const Unit &u, int at)
 {
-    const int row = u.row + at / p.group, head = u.h * p.group + at % p.group;
-    const float inv = sum > 0.f || sum != sum ? __fdiv_rn(1.f, sum) : 0.f;       // nothing seen: zeros
-    const float v[4] = { acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv };
-    T *dst = (T *)p.out.base + (int64_t)row * p.out.row + (int64_t)head * p.out.head + d;
+    const int token = by_group(p, at);
+    return (T *)p.out.base + (int64_t)(u.row + token) * p.out.row + (int64_t)(u.h * p.group + at - token * p.group) * p.out.head;
+}
+template <typename T>
+__device__ __forceinline__ const T *q_row(const AttendArgs &p, const Unit &u, int at)
+{
+    const int token = by_group(p, at);
+    return (const T *)p.q.base + (int64_t)(u.row + token) * p.q.row + (int64_t)(u.h * p.group + at - token * p.group) * p.q.head;
+}
+__device__ __forceinline__ void store_lse(const AttendArgs &p, const Unit &u, int at, float m, float sum)
+{
+    if (!p.lse) return;
+    const int token = by_group(p, at);
+    p.lse[(int64_t)(u.row + token) * p.q_heads + u.h * p.group + at - token * p.group] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+}
+// What the sums are divided by; rows that see nothing get zeros.
+__device__ __forceinline__ float inverse_of(float sum) { return sum > 0.f || sum != sum ? __fdiv_rn(1.f, sum) : 0.f; }
+
+// Four dims of a row.
+template <typename T>
+__device__ __forceinline__ void store4(T *dst, const float4 &v, bool wide)
+{
     if (sizeof(T) == 4) {
-        if (p.out_wide) *(float4 *)dst = make_float4(v[0], v[1], v[2], v[3]);
-        else
-#pragma unroll
-            for (int i = 0; i < 4; i++) ((float *)dst)[i] = v[i];
+        if (wide) *(float4 *)dst = v;
+        else {
+            ((float *)dst)[0] = v.x;
+            ((float *)dst)[1] = v.y;
+            ((float *)dst)[2] = v.z;
+            ((float *)dst)[3] = v.w;
+        }
     } else {
-        const uint32_t a = bits_of(v[0], dst), b = bits_of(v[1], dst), c = bits_of(v[2], dst), e = bits_of(v[3], dst);
-        if (p.out_wide) *(uint2 *)dst = make_uint2(a | b << 16, c | e << 16);
+        const uint32_t a = bits_of(v.x, dst), b = bits_of(v.y, dst), c = bits_of(v.z, dst), e = bits_of(v.w, dst);
+        if (wide) *(uint2 *)dst = make_uint2(a | b << 16, c | e << 16);
         else {
             ((uint16_t *)dst)[0] = (uint16_t)a;
             ((uint16_t *)dst)[1] = (uint16_t)b;
@@ -353,7 +409,35 @@ __device__ __forceinline__ void finish_row(const AttendArgs &p, const Unit &u, i
             ((uint16_t *)dst)[3] = (uint16_t)e;
         }
     }
-    if (d == 0 && p.lse) p.lse[(int64_t)row * p.q_heads + head] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+}
+template <typename T>
+__device__ __forceinline__ void finish_row(const AttendArgs &p, const Unit &u, int at, int d, const float4 &acc, float m, float sum)
+{
+    const float inv = inverse_of(sum);
+    store4<T>(out_row<T>(p, u, at) + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv), p.out_wide);
+    if (d == 0) store_lse(p, u, at, m, sum);
+}
+
+// ---------------------------------------------------------------------------------- waits
+// As mbar_wait, but polled without a suspended thread first: these waits are short.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity)
+{
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool mbar_wait_soon(uint32_t bar, uint32_t parity, volatile int *abort, int *status, int status_bit)
+{
+#pragma unroll 1
+    for (int i = 0; i < 64; i++)
+        if (mbar_test(bar, parity)) return true;
+    return mbar_wait(bar, parity, abort, status, status_bit);
+}
+// The same for the lanes of a warp, which leave together.
+__device__ __forceinline__ bool mbar_wait_soon_lanes(uint32_t bar, uint32_t parity, volatile int *abort, int *status, int status_bit)
+{
+    return __all_sync(0xffffffffu, mbar_wait_soon(bar, parity, abort, status, status_bit));
 }
 
 }  // namespace qb

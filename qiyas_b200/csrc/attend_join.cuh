@@ -9,13 +9,13 @@ namespace qb {
 template <int R, int TT, typename T>
 __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendArgs p)
 {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     __shared__ Cut cut;
     if (threadIdx.x < 32) {
         const Cut c = cut_of<R, TT>(p, blockIdx.x + 1);
         if (threadIdx.x == 0) cut = c;
     }
     __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");         // (what a call is cut by was there before either kernel)
     if (cut.parts == 0) return;
     const Unit u = unit_of<R, TT>(p, cut.b, cut.h, cut.rc);
     const int rows = u.r1 - u.r0, quads = p.dim / 4;

@@ -161,7 +161,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
             const int at = u.r0 + r;
             float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             if (at < u.r1 && lane < p.dim / 8) {
-                const T *src = (const T *)p.q.base + (int64_t)(u.row + at / p.group) * p.q.row + (int64_t)(u.h * p.group + at % p.group) * p.q.head + lane * 8;
+                const T *src = q_row<T>(p, u, at) + lane * 8;
                 const Vec8<T> v = load8<T>(src, p.q_wide);
                 unpack8(v, x);
             }

@@ -30,7 +30,10 @@ struct TilesCfg {
     static constexpr int R = 128 * NQ;
     static constexpr int SLOTS = SPL == 1 ? 2 : 1;              // of K and of V
     static constexpr int NG = TT / 16;
-    static constexpr int WARPS = 4 * NQ + CW + 1, THREADS = 32 * WARPS;
+    static constexpr int WARPS = 4 * NQ + CW + 4, THREADS = 32 * WARPS;       // the last four: one issues the products
+    // registers a thread: of the launch (65536 over the threads, whole eights), and of the softmax, converter and last warps
+    static constexpr int REGS = NQ == 2 ? 96 : 128, SOFT_REGS = NQ == 2 ? 144 : 200, CONV_REGS = NQ == 2 ? 72 : 104, REST_REGS = 48;
+    static_assert(NQ * SOFT_REGS + 2 * CONV_REGS + REST_REGS <= (NQ + 3) * REGS, "the shares of the registers fit the launch's");
     static constexpr uint32_t QTILE = 128 * DC * 2, SLOT = TT * DC * 2;
     static constexpr uint32_t O_Q = 0, O_K = NQ * SPL * QTILE, O_V = O_K + SLOTS * SLOT, O_HEAD = O_V + SLOTS * SLOT, SMEM = O_HEAD + 2048 + 128;
     static_assert(SMEM <= 232448, "227 KB of shared memory");
@@ -110,6 +113,91 @@ __device__ __forceinline__ int page_at(const AttendArgs &p, int b, int token, in
     return -1;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// The largest score (in powers of two) of this lane's row in a tile of S: a group of 16 tokens has one factor sk and one
+// shift log2(sv / v0), which lane `group` holds.
+template <int TT, bool MASKED>
+__device__ __forceinline__ float row_top(uint32_t s_at, float factor, float sk, float lr_mine, int base, int lo, int hi)
+{
+    float top = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < TT / 32; c += 2) {
+        uint32_t v[2][32];
+        tmem_ld32(s_at + 32 * c, v[0]);
+        tmem_ld32(s_at + 32 * c + 32, v[1]);
+        tmem_ld_landed32(v[0]);
+        tmem_ld_landed32(v[1]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t *x = v[e >> 1] + 16 * (e & 1);
+            const float f = factor * __shfl_sync(0xffffffffu, sk, 2 * c + e), lr = __shfl_sync(0xffffffffu, lr_mine, 2 * c + e);
+            if (MASKED) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int token = base + 32 * c + 16 * e + i;
+                    const float s = __fmaf_rn(__uint_as_float(x[i]), f, lr);
+                    top = fmaxf(top, token >= lo && token < hi ? s : -INFINITY);
+                }
+            } else {
+                float a = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2])), b = max3(__uint_as_float(x[3]), __uint_as_float(x[4]), __uint_as_float(x[5]));
+                a = max3(a, __uint_as_float(x[6]), __uint_as_float(x[7]));
+                b = max3(b, __uint_as_float(x[8]), __uint_as_float(x[9]));
+                a = max3(a, __uint_as_float(x[10]), __uint_as_float(x[11]));
+                b = max3(b, __uint_as_float(x[12]), __uint_as_float(x[13]));
+                a = max3(a, __uint_as_float(x[14]), __uint_as_float(x[15]));
+                top = fmaxf(top, __fmaf_rn(fmaxf(a, b), f, lr));
+            }
+        }
+    }
+    return top;
+}
+
+// The row's weights 2^(s - mm), in place of its scores as f16; returns their sum over sv / v0.
+template <int TT, int SPL, bool MASKED>
+__device__ __forceinline__ float row_weights(uint32_t s_at, float factor, float sk, float lr_mine, float rinv_mine, float mm, int base, int lo, int hi)
+{
+    float l = 0.f;
+    uint32_t v[2][32];
+    tmem_ld32(s_at, v[0]);
+    tmem_ld_landed32(v[0]);
+#pragma unroll
+    for (int c = 0; c < TT / 32; c++) {
+        if (c + 1 < TT / 32) tmem_ld32(s_at + 32 * c + 32, v[(c + 1) & 1]);
+        uint32_t w[16], w2[16];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const uint32_t *x = v[c & 1] + 16 * e;
+            const float f = factor * __shfl_sync(0xffffffffu, sk, 2 * c + e);
+            const float a = __shfl_sync(0xffffffffu, lr_mine, 2 * c + e) - mm, rinv = __shfl_sync(0xffffffffu, rinv_mine, 2 * c + e);
+            float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                float s0 = __fmaf_rn(__uint_as_float(x[i]), f, a), s1 = __fmaf_rn(__uint_as_float(x[i + 1]), f, a);
+                if (MASKED) {
+                    const int token = base + 32 * c + 16 * e + i;
+                    if (token < lo || token >= hi) s0 = -INFINITY;
+                    if (token + 1 < lo || token + 1 >= hi) s1 = -INFINITY;
+                }
+                const float e0 = exp2_fast(s0), e1 = exp2_fast(s1);
+                sum0 += e0;
+                sum1 += e1;
+                split2(e0, e1, w[8 * e + i / 2], w2[8 * e + i / 2]);
+            }
+            l = __fmaf_rn(sum0 + sum1, rinv, l);
+        }
+        tmem_st16(s_at + (SPL == 2 ? 32 : 16) * c, w);
+        if (SPL == 2) tmem_st16(s_at + 32 * c + 16, w2);
+        if (c + 1 < TT / 32) tmem_ld_landed32(v[(c + 1) & 1]);
+    }
+    return l;
+}
+
 template <int DC, int SPL, typename T>
 __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_kernel(const __grid_constant__ AttendArgs p)
 {
@@ -144,7 +232,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         const Start s = start_of<R, TT>(p, blockIdx.x);
         if (lane == 0) head->start = s;
     }
-    if (warp == C::WARPS - 1) tmem_alloc(smem_u32(&head->tmem), 512);
+    if (warp == 4 * NQ + CW) tmem_alloc(smem_u32(&head->tmem), 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -155,6 +243,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
 
     if (warp < 4 * NQ) {
         // ------------------------------------------------------------------ softmax: a thread a row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFT_REGS));
         const int t = warp >> 2, quarter = warp & 3;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         Walk<R, TT> walk(p, head->start);
@@ -165,36 +254,45 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             const int nq = NQ == 2 && u.r1 - u.r0 > 128 ? 2 : 1;
             const bool active = t < nq;
             const int n = piece.count;
+            const int at = u.r0 + t * 128 + quarter * 32 + lane;
             if (active) {
-                // q: half a warp a row of up to 128 dims, a warp a row beyond
-                constexpr int PER = DC == 128 ? 2 : 1, WIDTH = 32 / PER;
+                // q: half a warp a row of up to 128 dims, a warp a row beyond; a row's address comes from the lane whose row it is
+                constexpr int PER = DC == 128 ? 2 : 1, WIDTH = 32 / PER, BATCH = sizeof(T) == 4 ? 4 : 8;
                 uint8_t *tile = smem + C::O_Q + t * SPL * C::QTILE;
                 const int col = lane % WIDTH;
-#pragma unroll 4
-                for (int i = 0; i < 32 / PER; i++) {
-                    const int r = quarter * 32 + i * PER + lane / WIDTH, at = u.r0 + t * 128 + r;
-                    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    if (at < u.r1 && col < p.dim / 8) {
-                        const T *src = (const T *)p.q.base + (int64_t)(u.row + at / p.group) * p.q.row + (int64_t)(u.h * p.group + at % p.group) * p.q.head + col * 8;
-                        unpack8(load8<T>(src, p.q_wide), x);
+                const T *mine = q_row<T>(p, u, min(at, u.r1 - 1));
+#pragma unroll 1
+                for (int i0 = 0; i0 < 32 / PER; i0 += BATCH) {
+                    Vec8<T> raw[BATCH];
+#pragma unroll
+                    for (int i = 0; i < BATCH; i++) {
+                        const int r = (i0 + i) * PER + lane / WIDTH;
+                        const T *src = (const T *)__shfl_sync(0xffffffffu, (unsigned long long)mine, r);
+                        raw[i] = u.r0 + t * 128 + quarter * 32 + r < u.r1 && col < p.dim / 8 ? load8<T>(src + col * 8, p.q_wide) : zero8<T>();
                     }
-                    float top = 0.f;
 #pragma unroll
-                    for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[k]));
+                    for (int i = 0; i < BATCH; i++) {
+                        const int r = quarter * 32 + (i0 + i) * PER + lane / WIDTH;
+                        float x[8];
+                        unpack8(raw[i], x);
+                        float top = 0.f;
 #pragma unroll
-                    for (int d = WIDTH / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    float up, down;
-                    power_scale(top, up, down);
-                    if (p.scale < 0.f) up = -up;               // a factor below stays positive, so maxima can be taken of the sums
-                    if (col < p.dim / 8) {
-                        uint32_t hi[4], lo[4];
+                        for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[k]));
 #pragma unroll
-                        for (int k = 0; k < 4; k++) split2(x[2 * k] * up, x[2 * k + 1] * up, hi[k], lo[k]);
-                        uint8_t *dst = tile + col * 2048 + (r >> 3) * 128 + (r & 7) * 16;
-                        *(uint4 *)dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        if (SPL == 2) *(uint4 *)(dst + C::QTILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        for (int d = WIDTH / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        float up, down;
+                        power_scale(top, up, down);
+                        if (p.scale < 0.f) up = -up;           // the factor stays positive, so maxima can be taken of the sums
+                        if (col < p.dim / 8) {
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) split2(x[2 * k] * up, x[2 * k + 1] * up, hi[k], lo[k]);
+                            uint8_t *dst = tile + col * 2048 + (r >> 3) * 128 + (r & 7) * 16;
+                            *(uint4 *)dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            if (SPL == 2) *(uint4 *)(dst + C::QTILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        }
+                        if (col == 0) head->factor[t * 128 + r] = fabsf(p.scale) * 1.4426950408889634f * down;
                     }
-                    if (col == 0) head->factor[t * 128 + r] = fabsf(p.scale) * 1.4426950408889634f * down;
                 }
                 fence_proxy_async();
             }
@@ -204,7 +302,6 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
 
             float l = 0.f, mm = 0.f, vref = 0.f;
             bool fresh = true;                                   // nothing seen yet: mm says nothing
-            const int at = u.r0 + t * 128 + quarter * 32 + lane;
             bool ok = true;
             if (active) {
                 const float factor = head->factor[t * 128 + quarter * 32 + lane];
@@ -227,7 +324,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                     const int base = first + j * TT;
                     const int buf = nq == 2 ? t : j & 1;
                     const uint32_t use = uses[buf] + (nq == 2 ? j : j >> 1);
-                    if (!mbar_wait_lanes(sfull + 8 * buf, use & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
+                    if (!mbar_wait_soon_lanes(sfull + 8 * buf, use & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
                     tc_fence_after();
                     // V's scales against the first of them
                     const unsigned some = __ballot_sync(0xffffffffu, sc.y > 0.f);
@@ -239,30 +336,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                     const bool whole = base >= lo_most && base + TT <= hi_least;
                     const uint32_t s_at = tmem + lanes + C::s_col(buf);
 
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < TT / 32; c++) {
-                        uint32_t v[32];
-                        tmem_ld32(s_at + 32 * c, v);
-                        tmem_ld_landed32(v);
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const float f = factor * __shfl_sync(0xffffffffu, sc.x, 2 * c + e), lr = __shfl_sync(0xffffffffu, lr_mine, 2 * c + e);
-                            if (whole) {
-                                float most = __uint_as_float(v[16 * e]);
-#pragma unroll
-                                for (int i = 1; i < 16; i++) most = fmaxf(most, __uint_as_float(v[16 * e + i]));
-                                top = fmaxf(top, __fmaf_rn(most, f, lr));
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 16; i++) {
-                                    const int token = base + 32 * c + 16 * e + i;
-                                    const float s = __fmaf_rn(__uint_as_float(v[16 * e + i]), f, lr);
-                                    if (token >= lo && token < hi) top = fmaxf(top, s);
-                                }
-                            }
-                        }
-                    }
+                    float top = whole ? row_top<TT, false>(s_at, factor, sc.x, lr_mine, base, lo, hi) : row_top<TT, true>(s_at, factor, sc.x, lr_mine, base, lo, hi);
                     const bool above = fresh ? top > -INFINITY : top > mm + 15.f;
                     if (__any_sync(0xffffffffu, above)) {
                         float less = 1.f;
@@ -286,33 +360,8 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                             }
                         }
                     }
-#pragma unroll
-                    for (int c = 0; c < TT / 32; c++) {
-                        uint32_t v[32], w[16], w2[16];
-                        tmem_ld32(s_at + 32 * c, v);
-                        tmem_ld_landed32(v);
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const float f = factor * __shfl_sync(0xffffffffu, sc.x, 2 * c + e);
-                            const float a = __shfl_sync(0xffffffffu, lr_mine, 2 * c + e) - mm, rinv = __shfl_sync(0xffffffffu, rinv_mine, 2 * c + e);
-                            float sum = 0.f;
-#pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                float s0 = __fmaf_rn(__uint_as_float(v[16 * e + i]), f, a), s1 = __fmaf_rn(__uint_as_float(v[16 * e + i + 1]), f, a);
-                                if (!whole) {
-                                    const int token = base + 32 * c + 16 * e + i;
-                                    if (token < lo || token >= hi) s0 = -INFINITY;
-                                    if (token + 1 < lo || token + 1 >= hi) s1 = -INFINITY;
-                                }
-                                const float e0 = exp2_fast(s0), e1 = exp2_fast(s1);
-                                sum += e0 + e1;
-                                split2(e0, e1, w[8 * e + i / 2], w2[8 * e + i / 2]);
-                            }
-                            l = __fmaf_rn(sum, rinv, l);
-                        }
-                        tmem_st16(s_at + (SPL == 2 ? 32 : 16) * c, w);
-                        if (SPL == 2) tmem_st16(s_at + 32 * c + 16, w2);
-                    }
+                    l += whole ? row_weights<TT, SPL, false>(s_at, factor, sc.x, lr_mine, rinv_mine, mm, base, lo, hi)
+                               : row_weights<TT, SPL, true>(s_at, factor, sc.x, lr_mine, rinv_mine, mm, base, lo, hi);
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
@@ -333,6 +382,9 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             const bool complete = piece.first == 0 && n == u.nt;
             const int r = at - u.r0;
             float *slot = (float *)p.workspace + (size_t)(blockIdx.x * 2 + (piece.first ? 0 : 1)) * part_floats(R, p.dim);
+            float *part = slot + R * 2 + (size_t)r * p.dim;
+            const float f = complete ? v0 * inverse_of(l) : v0;
+            T *dst = out_row<T>(p, u, min(at, u.r1 - 1));
             for (int d = 0; d < p.dim; d += 16) {
                 uint32_t v[16];
                 tmem_ld16(tmem + lanes + C::o_col(t) + d, v);
@@ -340,16 +392,20 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 if (at < u.r1) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
-                        const float4 acc = make_float4(__uint_as_float(v[i]) * v0, __uint_as_float(v[i + 1]) * v0, __uint_as_float(v[i + 2]) * v0, __uint_as_float(v[i + 3]) * v0);
-                        if (complete) finish_row<T>(p, u, at, d + i, acc, mm, l);
-                        else *(float4 *)(slot + R * 2 + (size_t)r * p.dim + d + i) = acc;
+                        const float4 x = make_float4(__uint_as_float(v[i]) * f, __uint_as_float(v[i + 1]) * f, __uint_as_float(v[i + 2]) * f, __uint_as_float(v[i + 3]) * f);
+                        if (complete) store4<T>(dst + d + i, x, p.out_wide);
+                        else *(float4 *)(part + d + i) = x;
                     }
                 }
             }
-            if (!complete && at < u.r1) *(float2 *)(slot + r * 2) = make_float2(fresh ? NOTHING : mm, l);
+            if (at < u.r1) {
+                if (complete) store_lse(p, u, at, mm, l);
+                else *(float2 *)(slot + r * 2) = make_float2(fresh ? NOTHING : mm, l);
+            }
         }
     } else if (warp < 4 * NQ + CW) {
         // ------------------------------------------------------------------ converters
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::CONV_REGS));
         const int kv = (warp - 4 * NQ) >> 2, w = (warp - 4 * NQ) & 3;
         const int8_t *codes = kv ? p.v_codes : p.k_codes;
         const uint32_t full = kv ? vfull : kfull, empty = kv ? vempty : kempty;
@@ -372,24 +428,16 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                     raw[i * HALVES + k] = page >= 0 && c4 + 4 * k < chunks ? __ldg((const uint4 *)row + c4 + 4 * k) : make_uint4(0, 0, 0, 0);
             }
         };
-        KvTile<R, TT> now = tiles.next();
-        KvTile<R, TT> next = now;
-        int id = page_of(now);
-        uint4 raw[8], coming[8];
-        if (now.there) {
-            load(now, id, raw);
+        KvTile<R, TT> next = tiles.next();
+        int id = page_of(next);
+        for (uint32_t seq = 0; next.there; seq++) {
+            // the loads are under way while the slot is waited for
+            uint4 raw[8];
+            load(next, id, raw);
             next = tiles.next();
             id = page_of(next);
-        }
-        for (uint32_t seq = 0; now.there; seq++) {
-            const KvTile<R, TT> here = next;
-            if (here.there) {
-                load(here, id, coming);
-                next = tiles.next();
-                id = page_of(next);
-            }
             const int slot = seq % SLOTS;
-            if (seq >= SLOTS && !mbar_wait_warp(empty + 8 * slot, (seq / SLOTS - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) break;
+            if (seq >= SLOTS && !mbar_wait_soon_lanes(empty + 8 * slot, (seq / SLOTS - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) break;
             uint8_t *dst = slots + slot * C::SLOT;
 #pragma unroll
             for (int i = 0; i < GROUPS; i++)
@@ -411,36 +459,44 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(full + 8 * slot);
-            now = here;
-#pragma unroll
-            for (int i = 0; i < 8; i++) raw[i] = coming[i];
         }
-    } else if (lane == 0) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REST_REGS));
+        if (warp == 4 * NQ + CW && lane == 0) {
         // ------------------------------------------------------------------ one thread issues the products
         Walk<R, TT> walk(p, head->start);
         Piece piece;
         const uint32_t s_desc = idesc_of(1, 128, TT), o_desc = idesc_of(1, 128, p.dim) | 1u << 16;      // B of the second: a row a dim
         uint32_t kseq = 0, vseq = 0, uses[2] = {0, 0}, pieces = 0;
         bool ok = true;
-        auto wait = [&](uint32_t bar, uint32_t parity) { ok = ok && mbar_wait(bar, parity & 1, abort, status, STATUS_ATTEND_WAIT); return ok; };
+        auto wait = [&](uint32_t bar, uint32_t parity) { ok = ok && mbar_wait_soon(bar, parity & 1, abort, status, STATUS_ATTEND_WAIT); return ok; };
+        // descriptors count addresses in 16 bytes: a step of 16 dims (tokens) is an addition
+        const uint64_t q_desc = smem_desc(base_u32 + C::O_Q, 2048, 128), k_desc = smem_desc(base_u32 + C::O_K, TT * 16, 128);
+        const uint64_t v_desc = smem_desc(base_u32 + C::O_V, 128, TT * 16);
+        const int steps = p.dim / 16;
         auto scores = [&](int t, int buf, uint32_t slot) {
-            const uint32_t k_at = base_u32 + C::O_K + slot * C::SLOT;
-#pragma unroll 1
+            uint32_t accumulate = 0;
+#pragma unroll
             for (int x = 0; x < SPL; x++) {
-                const uint32_t q_at = base_u32 + C::O_Q + (t * SPL + x) * C::QTILE;
-                for (int d = 0; d < p.dim / 16; d++)
-                    mma_issue<1>(tmem + C::s_col(buf), smem_desc(q_at + d * 4096, 2048, 128), smem_desc(k_at + d * (TT * 32), TT * 16, 128), s_desc, x | d);
+                uint64_t qd = q_desc + (t * SPL + x) * (C::QTILE >> 4), kd = k_desc + slot * (C::SLOT >> 4);
+#pragma unroll 4
+                for (int d = 0; d < steps; d++) {
+                    mma_issue<1>(tmem + C::s_col(buf), qd, kd, s_desc, accumulate);
+                    accumulate = 1;
+                    qd += 4096 >> 4;
+                    kd += TT * 32 >> 4;
+                }
             }
             mma_commit(sfull + 8 * buf);
         };
         auto sums = [&](int t, int buf, uint32_t slot, int j) {
-            const uint32_t v_at = base_u32 + C::O_V + slot * C::SLOT;
-#pragma unroll 1
+            const uint64_t vd = v_desc + slot * (C::SLOT >> 4);
+            const uint32_t p_at = tmem + C::s_col(buf), o_at = tmem + C::o_col(t);
+#pragma unroll
             for (int s = 0; s < TT / 16; s++) {
-                const uint64_t desc = smem_desc(v_at + s * 256, 128, TT * 16);
-                const uint32_t col = tmem + C::s_col(buf) + (SPL == 2 ? (s >> 1) * 32 + (s & 1) * 8 : s * 8);
-                mma_issue_ts(tmem + C::o_col(t), col, desc, o_desc, j | s);
-                if (SPL == 2) mma_issue_ts(tmem + C::o_col(t), col + 16, desc, o_desc, 1);
+                const uint32_t col = p_at + (SPL == 2 ? (s >> 1) * 32 + (s & 1) * 8 : s * 8);
+                mma_issue_ts(o_at, col, vd + s * (256 >> 4), o_desc, s ? 1 : j);
+                if (SPL == 2) mma_issue_ts(o_at, col + 16, vd + s * (256 >> 4), o_desc, 1);
             }
             mma_commit(odone + 8 * t);
         };
@@ -496,11 +552,12 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         mma_commit(drain);
         const long long from = clock64();
         while (!mbar_try_wait(drain, 0) && clock64() - from < WAIT_CYCLES) { }
+        }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == C::WARPS - 1) {
+    if (warp == 4 * NQ + CW) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -511,6 +568,10 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
 template <int DC, int SPL, typename T>
 static cudaError_t set_tiles_attr()
 {
+    cudaFuncAttributes is;
+    cudaError_t e = cudaFuncGetAttributes(&is, attend_tiles_kernel<DC, SPL, T>);
+    if (e) return e;
+    if (is.numRegs != TilesCfg<DC, SPL>::REGS) return cudaErrorInvalidConfiguration;      // its warps share out just these
     return cudaFuncSetAttribute(attend_tiles_kernel<DC, SPL, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TilesCfg<DC, SPL>::SMEM);
 }
 
