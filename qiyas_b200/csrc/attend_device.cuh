@@ -1,7 +1,6 @@
 // What the attention kernels share: how a call's work is cut into shares, the rows' limits, and the products' operands.
 #pragma once
 
-#include <cuda.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
 
@@ -34,7 +33,7 @@ struct AttendArgs {
 __device__ __forceinline__ int by_group(const AttendArgs &p, int n) { return (int)(((uint64_t)(uint32_t)n * p.group_magic) >> p.group_shift); }
 
 cudaError_t attend_rows_init();
-int attend_rows(const AttendArgs &args, int type, int r, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t stream);
+int attend_rows(const AttendArgs &args, int type, int r, cudaStream_t stream);
 cudaError_t attend_tiles_init();
 int attend_tiles(const AttendArgs &args, int type, cudaStream_t stream);
 
@@ -123,6 +122,7 @@ __device__ __forceinline__ int64_t tiles_of(const AttendArgs &p, int b, int firs
     int64_t sum = 0;
     const Sequence s = sequence_at(p, b);
     const int chunks = (s.n * p.group + R - 1) / R;
+#pragma unroll 1
     for (int rc = first; rc < chunks; rc += step) sum += unit_of<R, TT>(p, s, b, 0, rc).nt;
     return sum;
 }
@@ -148,8 +148,10 @@ __device__ __forceinline__ int64_t line_length(const AttendArgs &p)
     const int lane = threadIdx.x & 31;
     int64_t sum = 0;
     if (p.seq.count <= FEW_SEQUENCES)
+#pragma unroll 1
         for (int b = 0; b < p.seq.count; b++) sum += tiles_of<R, TT>(p, b, lane, 32);
     else
+#pragma unroll 1
         for (int b = lane; b < p.seq.count; b += 32) sum += tiles_of<R, TT>(p, b, 0, 1);
     return warp_sum(sum) * p.heads;
 }
@@ -161,12 +163,14 @@ __device__ __forceinline__ Start place_on_line(const AttendArgs &p, int64_t x)
     Start s = {p.seq.count, 0, 0, 0, 0};
     int64_t tiles = 0;                         // of one head of the sequence found
     if (p.seq.count <= FEW_SEQUENCES) {
+#pragma unroll 1
         for (int b = 0; b < p.seq.count; b++) {
             tiles = warp_sum(tiles_of<R, TT>(p, b, lane, 32));
             if (x < tiles * p.heads) { s.b = b; break; }
             x -= tiles * p.heads;
         }
     } else {
+#pragma unroll 1
         for (int base = 0; base < p.seq.count; base += 32) {
             const int64_t mine = base + lane < p.seq.count ? tiles_of<R, TT>(p, base + lane, 0, 1) : 0, upto = warp_upto(mine) * p.heads;
             const unsigned after = __ballot_sync(0xffffffffu, upto > x);
@@ -185,6 +189,7 @@ __device__ __forceinline__ Start place_on_line(const AttendArgs &p, int64_t x)
     x -= s.h * tiles;
     const Sequence q = sequence_at(p, s.b);
     const int chunks = (q.n * p.group + R - 1) / R;
+#pragma unroll 1
     for (int base = 0; base < chunks; base += 32) {
         const int64_t upto = warp_upto(base + lane < chunks ? unit_of<R, TT>(p, q, s.b, s.h, base + lane).nt : 0);
         const unsigned after = __ballot_sync(0xffffffffu, upto > x);
@@ -208,7 +213,7 @@ __device__ __forceinline__ int64_t shares_of(const AttendArgs &p, int64_t total)
     return max((int64_t)1, min(min((int64_t)p.grid, total), max(units, total / (LEAST_TOKENS / TT))));
 }
 template <int R, int TT>
-__device__ __forceinline__ Start start_of(const AttendArgs &p, int block)
+__device__ __noinline__ Start start_of(const AttendArgs &p, int block)
 {
     const int64_t total = line_length<R, TT>(p), shares = shares_of<TT>(p, total);
     Start s = {0, 0, 0, 0, 0};
@@ -224,7 +229,7 @@ struct Cut {
     int block, parts;                          // parts: 0, or how many blocks from block - 1 on hold parts of the unit
 };
 template <int R, int TT>
-__device__ __forceinline__ Cut cut_of(const AttendArgs &p, int block)
+__device__ __noinline__ Cut cut_of(const AttendArgs &p, int block)
 {
     const int64_t total = line_length<R, TT>(p), shares = shares_of<TT>(p, total);
     Cut c = {0, 0, 0, block, 0};
@@ -232,12 +237,13 @@ __device__ __forceinline__ Cut cut_of(const AttendArgs &p, int block)
     const int64_t from = total * block / shares, before = total * (block - 1) / shares;
     if (from >= total) return c;
     const Start s = place_on_line<R, TT>(p, from);
-    if (s.tile == 0 || before > from - s.tile) return c;      // not inside a unit, or not the first boundary inside it
+    if (s.b >= p.seq.count || s.tile == 0 || before > from - s.tile) return c;      // not inside a unit, or not the first boundary inside it
     const int64_t end = from - s.tile + unit_of<R, TT>(p, s.b, s.h, s.rc).nt;
     c.b = s.b;
     c.h = s.h;
     c.rc = s.rc;
     c.parts = 1;
+#pragma unroll 1
     for (int64_t k = block; k < shares && total * k / shares < end; k++) c.parts++;
     return c;
 }
@@ -247,48 +253,58 @@ struct Piece {                                 // tiles first .. first + count -
     int first, count;
 };
 
-// The pieces of a block's share, one after the other.
-template <int R, int TT>
+// The pieces of a block's share, one after the other.  WHOLE: the call's units may be uncut (args.whole).
+template <int R, int TT, bool WHOLE>
 struct Walk {
     const AttendArgs &p;
-    int b, h, rc, tile;
-    int64_t left;
-    int64_t next_unit;                         // whole: the next unit's number
+    Sequence seq;
+    int b, h, rc, chunks, tile;
+    int64_t left;                              // tiles; whole: the next unit's number
 
-    __device__ __forceinline__ Walk(const AttendArgs &args, const Start &s) : p(args), b(s.b), h(s.h), rc(s.rc), tile(s.tile), left(s.left), next_unit(blockIdx.x)
+    __device__ __forceinline__ Walk(const AttendArgs &args, const Start &s) : p(args), b(s.b), h(s.h), rc(s.rc), chunks(0), tile(s.tile), left(s.left)
     {
-        if (p.whole) rc = -1;
+        if (WHOLE && p.whole) {
+            left = blockIdx.x;
+            rc = 0;
+        } else if (b >= p.seq.count) left = 0;
+        else if (left > 0) look();
     }
-
+    __device__ __forceinline__ void look()
+    {
+        seq = sequence_at(p, b);
+        chunks = (seq.n * p.group + R - 1) / R;
+    }
     __device__ __forceinline__ bool next(Piece &piece)
     {
-        if (p.whole) {
-            for (;;) {
-                if (rc >= 0) rc += p.chunks;               // more rows than the caller's bound said
-                else {
-                    if (next_unit >= (int64_t)p.seq.count * p.heads * p.chunks) return false;
-                    rc = (int)(next_unit % p.chunks);
-                    const int64_t bh = next_unit / p.chunks;
-                    h = (int)(bh % p.heads);
-                    b = (int)(bh / p.heads);
-                    next_unit += gridDim.x;
-                }
-                if (rc < chunks_of<R>(p, b)) {
-                    piece.unit = unit_of<R, TT>(p, b, h, rc);
-                    piece.first = 0;
-                    piece.count = piece.unit.nt;
-                    return true;
-                }
-                rc = -1;
+        if (WHOLE && p.whole) {
+            rc += p.chunks;                                    // more rows than the caller's bound said
+#pragma unroll 1
+            while (rc >= chunks) {
+                if (left >= (int64_t)p.seq.count * p.heads * p.chunks) return false;
+                const int unit = (int)left;                    // fewer than 2^31: seen to on the host
+                const int bh = unit / p.chunks;
+                rc = unit - bh * p.chunks;
+                b = bh / p.heads;
+                h = bh - b * p.heads;
+                left += gridDim.x;
+                look();
+            }
+            piece.unit = unit_of<R, TT>(p, seq, b, h, rc);
+            piece.first = 0;
+            piece.count = piece.unit.nt;
+            return true;
+        }
+        if (left <= 0) return false;
+#pragma unroll 1
+        while (rc >= chunks) {
+            rc = 0;
+            if (++h == p.heads) {
+                h = 0;
+                if (++b >= p.seq.count) return false;
+                look();
             }
         }
-        if (left <= 0 || b >= p.seq.count) return false;
-        while (rc >= chunks_of<R>(p, b)) {
-            rc = 0;
-            if (++h == p.heads) { h = 0; b++; }
-            if (b >= p.seq.count) return false;
-        }
-        piece.unit = unit_of<R, TT>(p, b, h, rc);
+        piece.unit = unit_of<R, TT>(p, seq, b, h, rc);
         piece.first = tile;
         piece.count = (int)min((int64_t)(piece.unit.nt - tile), left);
         if (piece.count <= 0) return false;
@@ -337,6 +353,32 @@ __device__ __forceinline__ uint32_t minus1152(uint32_t x)
 // Bytes 0, 1 (2, 3) of a word, codes + 128, as f16 codes.
 __device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return minus1152(__byte_perm(w, 0x64646464u, 0x4140)); }
 __device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return minus1152(__byte_perm(w, 0x64646464u, 0x4342)); }
+// A page number from the table.  It is fetched ahead, and looked at only where it is used, so that nothing waits for the
+// table where the next pages are asked for.
+struct Page {
+    int id;
+    bool wanted;                               // tokens that a row sees lie in it
+};
+__device__ __forceinline__ Page page_at(const AttendArgs &p, int b, int token, int tokens, int lo, int hi, bool there)
+{
+    Page g;
+    g.wanted = there && token < hi && token + tokens > lo;
+    g.id = -1;
+    if (g.wanted) g.id = __ldg(p.seq.table + (int64_t)b * p.seq.width + (token >> p.log_page));
+    return g;
+}
+__device__ __forceinline__ int page_number(const AttendArgs &p, const Page &g, bool report)        // -1: none
+{
+    if (g.id >= 0 && g.id < p.pages) return g.id;
+    if (g.wanted && report) atomicOr(p.status, STATUS_CACHE_RANGE);
+    return -1;
+}
+__device__ __forceinline__ float2 scales_at(const AttendArgs &p, int page, int h)      // of K and of V; V's below zero: no page
+{
+    if (page < 0) return make_float2(0.f, -1.f);
+    const int64_t i = (int64_t)page * p.heads + h;
+    return make_float2(__ldg(p.k_scales + i), __ldg(p.v_scales + i));
+}
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
@@ -351,20 +393,13 @@ __device__ __forceinline__ uint32_t transposed8(uint32_t x)
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-// Byte offset of 16-byte chunk `chunk` of row `row` in a tile of 32 rows that a swizzled tile copy has written.
+// Byte offset of 16-byte chunk `chunk` of row `row` in a tile of 32 rows: rows of 128 bytes (64), chunks exchanged so that a column of rows lies in different banks.
 template <int DT>
 __device__ __forceinline__ uint32_t swizzled(int sub, int row, int chunk)
 {
     if (DT == 64) return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
     return sub * (32 * 128) + row * 128 + ((chunk ^ (row & 7)) << 4);
 }
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const void *map, int x, int y, uint32_t bar)
-{
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
-                 : "memory");
-}
-
 // Where row `at` of a unit's sequence goes, and its logarithm of the sum.
 template <typename T>
 __device__ __forceinline__ T *out_row(const AttendArgs &p, const Unit &u, int at)

@@ -6,9 +6,10 @@
 //  * The work of a call is a line of tiles, 32 tokens of one head of one sequence each.  Block c of the grid takes the
 //    c-th equal share of the line, whatever sequences lie in it: sequences of any lengths load all multiprocessors alike.
 //    Where a share ends inside a sequence, its part goes to the workspace and a second, small kernel joins the parts.
-//  * A producer warp fetches table entries and scales 32 at a time, a lane each, and brings a tile's codes by TMA tile
-//    copies (128-byte swizzle: the reads below touch all banks) into a ring of stages; eight consumer warps take the tiles
-//    in turn, each with a softmax of its own, joined at the end of a share's part.
+//  * A producer warp fetches table entries and scales 32 at a time, a lane each, and brings a tile's codes by asynchronous
+//    16-byte copies into a ring of stages, swizzled so that the reads below touch all banks (TMA tile copies, the first form,
+//    cost their issuing warp 600 to 700 cycles a tile of 8 KB, where the memory's pace is 350); eight consumer warps take the
+//    tiles in turn, each with a softmax of its own, joined at the end of a share's part.
 //  * A warp takes S^T = K q^T and O^T = V^T P^T with mma.sync m16n8k16 (f16, f32 sums): the tokens, then V's dims, are the
 //    16 rows, the query rows the 8 columns, so 8 rows fill the instruction (tcgen05's 128 rows would be 15/16 padding).
 //    The codes become f16 exactly (byte permute under an exponent of 1024, subtract 1152).  An order of dims or tokens
@@ -27,7 +28,8 @@
 namespace qb {
 
 constexpr int RW = 8;                          // consumer warps
-constexpr int RTHREADS = 32 * (RW + 1);
+constexpr int RP = 4;                          // producer warps
+constexpr int RTHREADS = 32 * (RW + RP);
 constexpr uint32_t ROWS_HEADER = 2048;
 
 template <int DT, int NB, int SPL>
@@ -41,7 +43,7 @@ struct RowsCfg {
     static constexpr uint32_t MROW = DT + 4;                    // floats a row of the joining buffer
     static constexpr uint32_t O_RING = 0, O_Q = S * STAGE, O_MERGE = O_Q + KS * NB * SPL * 256, O_ML = O_MERGE + RW * R * MROW * 4;
     static constexpr uint32_t O_HEAD = O_ML + RW * R * 8, SMEM = O_HEAD + ROWS_HEADER + 1024;
-    static_assert(S % RW == 0, "a stage has one consumer warp");
+    static_assert(S % RW == 0 && S % RP == 0, "a stage has one consumer warp and one producer");
     static_assert(SMEM <= 232448, "227 KB of shared memory");
 };
 
@@ -55,9 +57,22 @@ struct RowsHead {                              // at O_HEAD
 };
 static_assert(sizeof(RowsHead) <= ROWS_HEADER, "the header fits");
 
+struct Batch { int b, h, lo, hi, tile, count; };       // tiles of one piece
+
+// 16 bytes of global memory into shared memory, past the L1 cache; and this thread's arrival on a barrier once all it has
+// copied so far is there.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src)
+{
+    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_arrive(uint32_t bar)
+{
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 template <int DT, int NB, int SPL, typename T>
 __global__ void __launch_bounds__(RTHREADS, 1)
-attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap)
+attend_rows_kernel(const __grid_constant__ AttendArgs p)
 {
     using C = RowsCfg<DT, NB, SPL>;
     extern __shared__ uint8_t smem_raw[];
@@ -69,7 +84,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
     if (threadIdx.x == 0) {
         head->abort = 0;
         for (int i = 0; i < C::S; i++) {
-            mbar_init(full0 + 8 * i, 1);
+            mbar_init(full0 + 8 * i, 33);        // the producer's lanes, as their copies land, and its word that the scales are there
             mbar_init(empty0 + 8 * i, 1);
         }
         mbar_fence_init();
@@ -80,69 +95,92 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
     }
     __syncthreads();
     if (!p.whole) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the joining kernel waits beside this one
-    Walk<C::R, 32> walk(p, head->start);
+    Walk<C::R, 32, true> walk(p, head->start);
     volatile int *abort = &head->abort;
     uint32_t seq = 0;                          // tiles of this block so far
 
-    if (warp == RW) {
-        // ------------------------------------------------------------------ producer
+    if (warp >= RW) {
+        // ------------------------------------------------------------------ producers: every RP-th tile each
+        // A batch: as many tiles of a piece as 32 pages hold, a lane a page.  Its page numbers are fetched two batches
+        // ahead, its scales one ahead.
+        const int per = p.log_page == 4 ? 2 : 1, most = 32 / per, mine = warp - RW;      // pages a tile, tiles a batch
         Piece piece;
-        while (walk.next(piece)) {
-            const int per = p.log_page == 4 ? 2 : 1;            // pages a tile
-            const int batch = 32 / per;
-            for (int first = 0; first < piece.count; first += batch) {
-                // a lane a page
-                const int tile = piece.unit.t0 + piece.first + first + lane / per;
-                const int token = tile * 32 + (per == 2 ? (lane & 1) * 16 : 0), slot = token >> p.log_page;
-                int id = -1;
-                float sk = 0.f, sv = -1.f;
-                if (first + lane / per < piece.count && token < piece.unit.hi && (token | (per == 2 ? 15 : 31)) >= piece.unit.lo) {
-                    id = p.seq.table[(int64_t)piece.unit.b * p.seq.width + slot];
-                    if (id < 0 || id >= p.pages) {
-                        id = -1;
-                        atomicOr(p.status, STATUS_CACHE_RANGE);
-                    } else {
-                        const int64_t at = (int64_t)id * p.heads + piece.unit.h;
-                        sk = __ldg(p.k_scales + at);
-                        sv = __ldg(p.v_scales + at);
+        int at = 0;
+        bool more = walk.next(piece);
+        auto next_batch = [&]() {
+            Batch t;
+            if (more && at >= piece.count) {
+                at = 0;
+                more = walk.next(piece);
+            }
+            t.b = piece.unit.b;
+            t.h = piece.unit.h;
+            t.lo = piece.unit.lo;
+            t.hi = piece.unit.hi;
+            t.tile = piece.unit.t0 + piece.first + at;
+            t.count = more ? min(most, piece.count - at) : 0;
+            at += t.count;
+            return t;
+        };
+        auto page_of = [&](const Batch &t) {
+            const int token = (t.tile + lane / per) * 32 + (per == 2 ? (lane & 1) * 16 : 0);
+            return page_at(p, t.b, token, 32 / per, t.lo, t.hi, lane / per < t.count);
+        };
+        constexpr int CHUNKS = DT / 16, ROWS = 32 / CHUNKS;              // 16-byte chunks a token, tokens an instruction of the warp
+        const int chunk = lane % CHUNKS, row0 = lane / CHUNKS;
+        const bool has = chunk * 16 < p.dim;
+        const int step = ROWS * p.dim;
+        Batch now = next_batch();
+        int id = page_number(p, page_of(now), mine == 0);
+        float2 sc = scales_at(p, id, now.h);
+        Batch next = next_batch();
+        Page id_next = page_of(next);
+        while (now.count) {
+            const Batch after = next_batch();
+            const int id_then = page_number(p, id_next, mine == 0);
+            const float2 sc_then = scales_at(p, id_then, next.h);
+            id_next = page_of(after);
+            for (int k = (mine - seq) & (RP - 1); k < now.count; k += RP) {
+                const uint32_t tile = seq + k;
+                const int stage = tile % C::S;
+                if (tile >= C::S && !mbar_wait_soon_lanes(empty0 + 8 * stage, (tile / C::S - 1) & 1, abort, p.status, STATUS_ATTEND_WAIT)) goto done;
+                const int base = (now.tile + k) * 32, l0 = k * per, l1 = l0 + per - 1;
+                const int id0 = __shfl_sync(0xffffffffu, id, l0), id1 = __shfl_sync(0xffffffffu, id, l1);
+                // tokens 0 .. 15 of the tile, and 16 .. 31: in pages of 16 they lie apart
+                const int inside = base & ((1 << p.log_page) - 1), inside1 = per == 2 ? 0 : inside + 16;
+                int64_t from = ((((int64_t)id0 * p.heads + now.h) << p.log_page) + inside + row0) * p.dim + chunk * 16;
+                const int64_t from1 = ((((int64_t)id1 * p.heads + now.h) << p.log_page) + inside1 + row0) * p.dim + chunk * 16;
+                const uint32_t to = ring + stage * C::STAGE;
+                const bool whole = base >= now.lo && base + 32 <= now.hi;
+#pragma unroll
+                for (int i = 0; i < 32 / ROWS; i++, from += step) {
+                    if (i * ROWS == 16) from = from1;
+                    const int row = i * ROWS + row0;
+                    bool copy = has && (i * ROWS >= 16 ? id1 : id0) >= 0;
+                    if (!whole) copy &= base + row >= now.lo && base + row < now.hi;
+                    if (copy) {
+                        const uint32_t dst = to + swizzled<DT>(DT == 256 ? chunk >> 3 : 0, row, DT == 256 ? chunk & 7 : chunk);
+                        copy16(dst, p.k_codes + from);
+                        copy16(dst + C::HALF, p.v_codes + from);
                     }
                 }
-                const int n = min(batch, piece.count - first);
-                for (int k = 0; k < n; k++, seq++) {
-                    const int stage = seq % C::S;
-                    if (seq >= C::S && !mbar_wait_warp(empty0 + 8 * stage, (seq / C::S - 1) & 1, abort, p.status, STATUS_ATTEND_WAIT)) goto done;
-                    const int l0 = k * per, l1 = l0 + per - 1;
-                    const int id0 = __shfl_sync(0xffffffffu, id, l0), id1 = __shfl_sync(0xffffffffu, id, l1);
-                    const float k0 = __shfl_sync(0xffffffffu, sk, l0), k1 = __shfl_sync(0xffffffffu, sk, l1);
-                    const float v0 = __shfl_sync(0xffffffffu, sv, l0), v1 = __shfl_sync(0xffffffffu, sv, l1);
-                    const int rows = 32 / per;                  // tokens a copy
-                    const uint32_t bytes = rows * C::SW;
-                    const int live = (id0 >= 0 ? 1 : 0) + (per == 2 && id1 >= 0 ? 1 : 0);
-                    if (lane == 0) {
-                        head->scales[stage] = make_float4(k0, v0, k1, v1);
-                        if (live) mbar_arrive_expect_tx(full0 + 8 * stage, live * 2 * C::SUB * bytes);
-                        else mbar_arrive(full0 + 8 * stage);
-                    }
-                    __syncwarp();
-                    if (lane < 2 * C::SUB * per) {
-                        const int which = lane & 1, sub = (lane >> 1) % C::SUB, pg = lane / (2 * C::SUB);
-                        const int page = pg ? id1 : id0;
-                        if (page >= 0) {
-                            const int inside = ((piece.unit.t0 + piece.first + first + k) * 32 + pg * 16) & ((1 << p.log_page) - 1);
-                            const int row = ((page * p.heads + piece.unit.h) << p.log_page) + inside;
-                            const uint32_t dst = ring + stage * C::STAGE + which * C::HALF + sub * (32 * 128) + pg * 16 * C::SW;
-                            tma_load_2d(dst, which ? &vmap : &kmap, sub * 128, row, full0 + 8 * stage);
-                        }
-                    }
+                copies_arrive(full0 + 8 * stage);
+                const float k0 = __shfl_sync(0xffffffffu, sc.x, l0), k1 = __shfl_sync(0xffffffffu, sc.x, l1);
+                const float v0 = __shfl_sync(0xffffffffu, sc.y, l0), v1 = __shfl_sync(0xffffffffu, sc.y, l1);
+                if (lane == 0) {
+                    head->scales[stage] = make_float4(k0, v0, k1, v1);
+                    mbar_arrive(full0 + 8 * stage);
                 }
             }
+            seq += now.count;
+            now = next;
+            id = id_then;
+            sc = sc_then;
+            next = after;
         }
     done:
-        // no copy may be under way when the block ends, whoever gave up
-        for (uint32_t at = seq > C::S ? seq - C::S : 0; at < seq; at++) {
-            const long long from = clock64();
-            while (!mbar_try_wait(full0 + 8 * (at % C::S), (at / C::S) & 1) && clock64() - from < WAIT_CYCLES) { }
-        }
+        // no copy may be under way when the block ends, whoever gave up: a thread waits for its own
+        asm volatile("cp.async.wait_all;" ::: "memory");
         return;
     }
 
@@ -232,7 +270,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
         for (int j = mine; j < piece.count && !gone; j += RW) {
             const uint32_t at = seq + j;
             const int stage = at % C::S;
-            if (!mbar_wait_lanes(full0 + 8 * stage, (at / C::S) & 1, abort, p.status, STATUS_ATTEND_WAIT)) { gone = true; break; }
+            if (!mbar_wait_soon_lanes(full0 + 8 * stage, (at / C::S) & 1, abort, p.status, STATUS_ATTEND_WAIT)) { gone = true; break; }
             const float4 sc = head->scales[stage];
             const uint8_t *kt = smem + stage * C::STAGE, *vt = kt + C::HALF;
             const int base = (u.t0 + piece.first + j) * 32;
@@ -454,26 +492,26 @@ cudaError_t attend_rows_init()
 }
 
 template <int DT, int NB, int SPL, typename T>
-static int launch_rows(const AttendArgs &args, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t stream)
+static int launch_rows(const AttendArgs &args, cudaStream_t stream)
 {
-    attend_rows_kernel<DT, NB, SPL, T><<<args.grid, RTHREADS, RowsCfg<DT, NB, SPL>::SMEM, stream>>>(args, kmap, vmap);
+    attend_rows_kernel<DT, NB, SPL, T><<<args.grid, RTHREADS, RowsCfg<DT, NB, SPL>::SMEM, stream>>>(args);
     const cudaError_t e = cudaGetLastError();
     return e || args.whole ? (int)e : launch_join<8 * NB, 32, T>(args, stream);
 }
 
 template <int SPL, typename T>
-static int launch_rows_dim(const AttendArgs &args, int r, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t stream)
+static int launch_rows_dim(const AttendArgs &args, int r, cudaStream_t stream)
 {
-    if (args.dim <= 64) return r == 16 ? launch_rows<64, 2, SPL, T>(args, kmap, vmap, stream) : launch_rows<64, 1, SPL, T>(args, kmap, vmap, stream);
-    if (args.dim <= 128) return r == 16 ? launch_rows<128, 2, SPL, T>(args, kmap, vmap, stream) : launch_rows<128, 1, SPL, T>(args, kmap, vmap, stream);
-    return launch_rows<256, 1, SPL, T>(args, kmap, vmap, stream);
+    if (args.dim <= 64) return r == 16 ? launch_rows<64, 2, SPL, T>(args, stream) : launch_rows<64, 1, SPL, T>(args, stream);
+    if (args.dim <= 128) return r == 16 ? launch_rows<128, 2, SPL, T>(args, stream) : launch_rows<128, 1, SPL, T>(args, stream);
+    return launch_rows<256, 1, SPL, T>(args, stream);
 }
 
-int attend_rows(const AttendArgs &args, int type, int r, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t stream)
+int attend_rows(const AttendArgs &args, int type, int r, cudaStream_t stream)
 {
-    if (type == QB200_F32) return launch_rows_dim<2, float>(args, r, kmap, vmap, stream);
-    if (type == QB200_F16) return launch_rows_dim<1, __half>(args, r, kmap, vmap, stream);
-    return launch_rows_dim<1, __nv_bfloat16>(args, r, kmap, vmap, stream);
+    if (type == QB200_F32) return launch_rows_dim<2, float>(args, r, stream);
+    if (type == QB200_F16) return launch_rows_dim<1, __half>(args, r, stream);
+    return launch_rows_dim<1, __nv_bfloat16>(args, r, stream);
 }
 
 }  // namespace qb

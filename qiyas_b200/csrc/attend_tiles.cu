@@ -5,14 +5,14 @@
 // of 128 x 128 x 128, 2048 cycles of the tensor pipe, and as many cycles of the exponential unit.  So:
 //  * S = q K^T and O += P V are tcgen05.mma kind::f16 (codes are exact in f16), issued by one thread, S, P and O in tensor
 //    memory: P replaces S in place as f16 and is read from there as the second product's A operand.
-//  * Eight converter warps fetch the codes (16 bytes a load, a tile ahead in registers) and store them as f16 core matrices
-//    (8 tokens x 8 dims): one layout that is K-major for K (a row a token) and MN-major for V (a row a dim).  Every byte of
-//    the cache is converted once for the 256 rows of a block.
+//  * Eight converter warps fetch the codes (16 bytes a load) and store them as f16: K as core matrices of 8 tokens x 8 dims,
+//    V as rows of 64 dims with the 128-byte swizzle, which the second product reads across (a row a dim: MN-major).  Every
+//    byte of the cache is converted once for the 256 rows of a block.
 //  * Two groups of four softmax warps, a thread a row, work on the two row tiles in turn with the tensor pipe: while one
 //    takes exponentials the pipe has the other's products.  With one row tile (NQ 1, or a unit of at most 128 rows) the two
 //    S buffers take the tiles of tokens alternately instead.
-//  * A thread reads its row of S twice, for the maximum and for the weights: the second reading costs less than the 64
-//    registers that would hold the row.  The maximum is kept while weights stay below 2^15, so O is seldom rescaled.
+//  * A thread reads its row of S once, 32 tokens at a time, and takes the weights against the exponent it has: only where one
+//    would pass 2^15 does it go back over what the row has of O and of the tile's weights, in place, by a power of two.
 // Scales, exponents and the cut of q and w are those of attend_rows.cu; so are the shares of the grid's blocks.
 #include "common.cuh"
 #include "attend_device.cuh"
@@ -35,7 +35,7 @@ struct TilesCfg {
     static constexpr int REGS = NQ == 2 ? 96 : 128, SOFT_REGS = NQ == 2 ? 144 : 200, CONV_REGS = NQ == 2 ? 72 : 104, REST_REGS = 48;
     static_assert(NQ * SOFT_REGS + 2 * CONV_REGS + REST_REGS <= (NQ + 3) * REGS, "the shares of the registers fit the launch's");
     static constexpr uint32_t QTILE = 128 * DC * 2, SLOT = TT * DC * 2;
-    static constexpr uint32_t O_Q = 0, O_K = NQ * SPL * QTILE, O_V = O_K + SLOTS * SLOT, O_HEAD = O_V + SLOTS * SLOT, SMEM = O_HEAD + 2048 + 128;
+    static constexpr uint32_t O_Q = 0, O_K = NQ * SPL * QTILE, O_V = O_K + SLOTS * SLOT, O_HEAD = O_V + SLOTS * SLOT, SMEM = O_HEAD + 2048 + 1024;
     static_assert(SMEM <= 232448, "227 KB of shared memory");
     __host__ __device__ static constexpr uint32_t s_col(int b) { return b * TT; }
     __host__ __device__ static constexpr uint32_t o_col(int t) { return 256 + t * 128; }
@@ -78,7 +78,7 @@ struct KvTile {
 };
 template <int R, int TT>
 struct KvWalk {
-    Walk<R, TT> walk;
+    Walk<R, TT, false> walk;
     Piece piece;
     int at;
     bool more;
@@ -103,16 +103,6 @@ struct KvWalk {
     }
 };
 
-// The page that holds token `token` of sequence b, or -1.
-__device__ __forceinline__ int page_at(const AttendArgs &p, int b, int token, int lo, int hi, int tokens, bool report)
-{
-    if (token >= hi || token + tokens <= lo) return -1;
-    const int id = p.seq.table[(int64_t)b * p.seq.width + (token >> p.log_page)];
-    if (id >= 0 && id < p.pages) return id;
-    if (report) atomicOr(p.status, STATUS_CACHE_RANGE);
-    return -1;
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
     float d;
@@ -120,82 +110,25 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return d;
 }
 
-// The largest score (in powers of two) of this lane's row in a tile of S: a group of 16 tokens has one factor sk and one
-// shift log2(sv / v0), which lane `group` holds.
-template <int TT, bool MASKED>
-__device__ __forceinline__ float row_top(uint32_t s_at, float factor, float sk, float lr_mine, int base, int lo, int hi)
+// Pairs of f32 in one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b)
 {
-    float top = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < TT / 32; c += 2) {
-        uint32_t v[2][32];
-        tmem_ld32(s_at + 32 * c, v[0]);
-        tmem_ld32(s_at + 32 * c + 32, v[1]);
-        tmem_ld_landed32(v[0]);
-        tmem_ld_landed32(v[1]);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const uint32_t *x = v[e >> 1] + 16 * (e & 1);
-            const float f = factor * __shfl_sync(0xffffffffu, sk, 2 * c + e), lr = __shfl_sync(0xffffffffu, lr_mine, 2 * c + e);
-            if (MASKED) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int token = base + 32 * c + 16 * e + i;
-                    const float s = __fmaf_rn(__uint_as_float(x[i]), f, lr);
-                    top = fmaxf(top, token >= lo && token < hi ? s : -INFINITY);
-                }
-            } else {
-                float a = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2])), b = max3(__uint_as_float(x[3]), __uint_as_float(x[4]), __uint_as_float(x[5]));
-                a = max3(a, __uint_as_float(x[6]), __uint_as_float(x[7]));
-                b = max3(b, __uint_as_float(x[8]), __uint_as_float(x[9]));
-                a = max3(a, __uint_as_float(x[10]), __uint_as_float(x[11]));
-                b = max3(b, __uint_as_float(x[12]), __uint_as_float(x[13]));
-                a = max3(a, __uint_as_float(x[14]), __uint_as_float(x[15]));
-                top = fmaxf(top, __fmaf_rn(fmaxf(a, b), f, lr));
-            }
-        }
-    }
-    return top;
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
 }
-
-// The row's weights 2^(s - mm), in place of its scores as f16; returns their sum over sv / v0.
-template <int TT, int SPL, bool MASKED>
-__device__ __forceinline__ float row_weights(uint32_t s_at, float factor, float sk, float lr_mine, float rinv_mine, float mm, int base, int lo, int hi)
+__device__ __forceinline__ void unpair(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c)
 {
-    float l = 0.f;
-    uint32_t v[2][32];
-    tmem_ld32(s_at, v[0]);
-    tmem_ld_landed32(v[0]);
-#pragma unroll
-    for (int c = 0; c < TT / 32; c++) {
-        if (c + 1 < TT / 32) tmem_ld32(s_at + 32 * c + 32, v[(c + 1) & 1]);
-        uint32_t w[16], w2[16];
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const uint32_t *x = v[c & 1] + 16 * e;
-            const float f = factor * __shfl_sync(0xffffffffu, sk, 2 * c + e);
-            const float a = __shfl_sync(0xffffffffu, lr_mine, 2 * c + e) - mm, rinv = __shfl_sync(0xffffffffu, rinv_mine, 2 * c + e);
-            float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                float s0 = __fmaf_rn(__uint_as_float(x[i]), f, a), s1 = __fmaf_rn(__uint_as_float(x[i + 1]), f, a);
-                if (MASKED) {
-                    const int token = base + 32 * c + 16 * e + i;
-                    if (token < lo || token >= hi) s0 = -INFINITY;
-                    if (token + 1 < lo || token + 1 >= hi) s1 = -INFINITY;
-                }
-                const float e0 = exp2_fast(s0), e1 = exp2_fast(s1);
-                sum0 += e0;
-                sum1 += e1;
-                split2(e0, e1, w[8 * e + i / 2], w2[8 * e + i / 2]);
-            }
-            l = __fmaf_rn(sum0 + sum1, rinv, l);
-        }
-        tmem_st16(s_at + (SPL == 2 ? 32 : 16) * c, w);
-        if (SPL == 2) tmem_st16(s_at + 32 * c + 16, w2);
-        if (c + 1 < TT / 32) tmem_ld_landed32(v[(c + 1) & 1]);
-    }
-    return l;
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 
 template <int DC, int SPL, typename T>
@@ -204,7 +137,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
     using C = TilesCfg<DC, SPL>;
     constexpr int TT = C::TT, NQ = C::NQ, R = C::R, SLOTS = C::SLOTS, NG = C::NG;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
+    uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     TilesHead *head = (TilesHead *)(smem + C::O_HEAD);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base_u32 = smem_u32(smem);
@@ -246,9 +179,9 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFT_REGS));
         const int t = warp >> 2, quarter = warp & 3;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        Walk<R, TT> walk(p, head->start);
+        Walk<R, TT, false> walk(p, head->start);
         Piece piece;
-        uint32_t pieces = 0, uses[2] = {0, 0}, done = 0;         // uses of the S buffers and of this group's O so far
+        uint32_t pieces = 0, uses0 = 0, uses1 = 0, done = 0;     // uses of the S buffers and of this group's O so far
         while (walk.next(piece)) {
             const Unit &u = piece.unit;
             const int nq = NQ == 2 && u.r1 - u.r0 > 128 ? 2 : 1;
@@ -309,23 +242,16 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 row_limits(p, u, min(at, u.r1 - 1), lo, hi);
                 const int lo_most = __reduce_max_sync(0xffffffffu, lo), hi_least = __reduce_min_sync(0xffffffffu, hi);
                 // a lane a group of 16 tokens: page a tile of tokens ahead of the scales, scales a tile ahead of their use
-                const int first = (u.t0 + piece.first) * TT, mine = lane * 16;
-                auto page_of = [&](int j) { return lane < NG && j < n ? page_at(p, u.b, first + j * TT + mine, u.lo, u.hi, 16, quarter == 0) : -1; };
-                auto scales_of = [&](int id) {
-                    if (id < 0) return make_float2(0.f, -1.f);
-                    const int64_t i = (int64_t)id * p.heads + u.h;
-                    return make_float2(__ldg(p.k_scales + i), __ldg(p.v_scales + i));
-                };
-                float2 sc = scales_of(page_of(0));
-                int id = page_of(1);
+                const int first = (u.t0 + piece.first) * TT;
+                auto page_of = [&](int j) { return page_at(p, u.b, first + j * TT + lane * 16, 16, u.lo, u.hi, lane < NG && j < n); };
+                float2 sc = scales_at(p, page_number(p, page_of(0), quarter == 0), u.h);
+                Page page = page_of(1);
                 for (int j = 0; j < n; j++) {
-                    const float2 sc_next = scales_of(id);
-                    id = page_of(j + 2);
+                    const float2 sc_next = scales_at(p, page_number(p, page, quarter == 0), u.h);
+                    page = page_of(j + 2);
                     const int base = first + j * TT;
                     const int buf = nq == 2 ? t : j & 1;
-                    const uint32_t use = uses[buf] + (nq == 2 ? j : j >> 1);
-                    if (!mbar_wait_soon_lanes(sfull + 8 * buf, use & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
-                    tc_fence_after();
+                    const uint32_t use = (buf ? uses1 : uses0) + (nq == 2 ? j : j >> 1);
                     // V's scales against the first of them
                     const unsigned some = __ballot_sync(0xffffffffu, sc.y > 0.f);
                     const float found = __shfl_sync(0xffffffffu, sc.y, some ? __ffs(some) - 1 : 0);
@@ -334,34 +260,100 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                     if (sc.y < 0.f) { lr_mine = -INFINITY; rinv_mine = 0.f; }
                     else if (sc.y > 0.f && sc.y != vref) { lr_mine = log2_ratio(sc.y, vref); rinv_mine = __fdividef(vref, sc.y); }
                     const bool whole = base >= lo_most && base + TT <= hi_least;
-                    const uint32_t s_at = tmem + lanes + C::s_col(buf);
+                    const uint32_t s_at = tmem + lanes + C::s_col(buf), o_at = tmem + lanes + C::o_col(t);
+                    if (!mbar_wait_soon_lanes(sfull + 8 * buf, use & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
+                    tc_fence_after();
 
-                    float top = whole ? row_top<TT, false>(s_at, factor, sc.x, lr_mine, base, lo, hi) : row_top<TT, true>(s_at, factor, sc.x, lr_mine, base, lo, hi);
-                    const bool above = fresh ? top > -INFINITY : top > mm + 15.f;
-                    if (__any_sync(0xffffffffu, above)) {
-                        float less = 1.f;
-                        if (above) {
-                            const float next = top - 7.f;
-                            if (!fresh) less = exp2_fast(mm - next);
-                            l *= less;
-                            mm = next;
-                            fresh = false;
-                        }
-                        if (j > 0) {                             // O so far, once the product before has ended
-                            if (!mbar_wait_lanes(odone + 8 * t, (done + j - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
-                            tc_fence_after();
-                            for (int d = 0; d < p.dim; d += 16) {
-                                uint32_t v[16];
-                                tmem_ld16(tmem + lanes + C::o_col(t) + d, v);
-                                tmem_ld_landed16(v);
+                    uint32_t v[32];
+                    tmem_ld32(s_at, v);
+#pragma unroll 1
+                    for (int c = 0; c < TT / 32; c++) {
+                        float x[32];                             // scores, in powers of two against mm
+                        tmem_ld_landed32(v);
 #pragma unroll
-                                for (int i = 0; i < 16; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * less);
-                                tmem_st16(tmem + lanes + C::o_col(t) + d, v);
+                        for (int e = 0; e < 2; e++) {
+                            const float f = factor * __shfl_sync(0xffffffffu, sc.x, 2 * c + e), a = __shfl_sync(0xffffffffu, lr_mine, 2 * c + e) - mm;
+                            const uint64_t f2 = pair(f, f), a2 = pair(a, a);
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2)
+                                unpair(pair_fma(pair(__uint_as_float(v[16 * e + i]), __uint_as_float(v[16 * e + i + 1])), f2, a2), x[16 * e + i], x[16 * e + i + 1]);
+                        }
+                        if (c + 1 < TT / 32) tmem_ld32(s_at + 32 * c + 32, v);
+                        if (!whole) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) {
+                                const int token = base + 32 * c + i;
+                                x[i] = token >= lo && token < hi ? x[i] : -INFINITY;
                             }
                         }
+                        float top = max3(x[0], x[1], x[2]), top2 = max3(x[3], x[4], x[5]);
+#pragma unroll
+                        for (int i = 6; i < 30; i += 4) {
+                            top = max3(top, x[i], x[i + 1]);
+                            top2 = max3(top2, x[i + 2], x[i + 3]);
+                        }
+                        top = max3(fmaxf(top, top2), x[30], x[31]);
+                        // seldom: the exponent the weights are taken against goes up, by whole powers of two
+                        const bool above = fresh ? top > -INFINITY : top > 15.f;
+                        if (__any_sync(0xffffffffu, above)) {
+                            float up = 0.f, less = 1.f;
+                            if (above) {
+                                up = ceilf(top) - 7.f;
+                                if (!fresh) less = exp2_fast(-up);
+                                fresh = false;
+                            }
+                            mm += up;
+                            l *= less;
+#pragma unroll
+                            for (int i = 0; i < 32; i++) x[i] -= up;
+                            tmem_st_wait();
+#pragma unroll 1
+                            for (int k = 0; k < c * (SPL == 2 ? 32 : 16); k += 16) {          // this tile's weights so far
+                                uint32_t w[16];
+                                tmem_ld16(s_at + k, w);
+                                tmem_ld_landed16(w);
+#pragma unroll
+                                for (int i = 0; i < 16; i++) {
+                                    const float2 y = __half22float2(*(const __half2 *)&w[i]);
+                                    const __half2 z = __floats2half2_rn(y.x * less, y.y * less);
+                                    w[i] = *(const uint32_t *)&z;
+                                }
+                                tmem_st16(s_at + k, w);
+                            }
+                            if (j > 0) {                         // O so far, once the product before has ended
+                                if (!mbar_wait_soon_lanes(odone + 8 * t, (done + j - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
+                                tc_fence_after();
+#pragma unroll 1
+                                for (int d = 0; d < p.dim; d += 16) {
+                                    uint32_t w[16];
+                                    tmem_ld16(o_at + d, w);
+                                    tmem_ld_landed16(w);
+#pragma unroll
+                                    for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__uint_as_float(w[i]) * less);
+                                    tmem_st16(o_at + d, w);
+                                }
+                            }
+                            if (c + 1 < TT / 32) tmem_ld_landed32(v);
+                        }
+                        uint32_t w[16], w2[16];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float rinv = __shfl_sync(0xffffffffu, rinv_mine, 2 * c + e);
+                            uint64_t sum = 0;
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                const float e0 = exp2_fast(x[16 * e + i]), e1 = exp2_fast(x[16 * e + i + 1]);
+                                sum = pair_add(sum, pair(e0, e1));
+                                split2(e0, e1, w[8 * e + i / 2], w2[8 * e + i / 2]);
+                            }
+                            float s0, s1;
+                            unpair(sum, s0, s1);
+                            l = __fmaf_rn(s0 + s1, rinv, l);
+                        }
+                        tmem_st16(s_at + (SPL == 2 ? 32 : 16) * c, w);
+                        if (SPL == 2) tmem_st16(s_at + 32 * c + 16, w2);
                     }
-                    l += whole ? row_weights<TT, SPL, false>(s_at, factor, sc.x, lr_mine, rinv_mine, mm, base, lo, hi)
-                               : row_weights<TT, SPL, true>(s_at, factor, sc.x, lr_mine, rinv_mine, mm, base, lo, hi);
+                    if (!ok) break;
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
@@ -370,8 +362,8 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 }
             }
             // the buffers' uses, whoever had them
-            if (nq == 2) { uses[0] += n; uses[1] += n; }
-            else { uses[0] += (n + 1) / 2; uses[1] += n / 2; }
+            uses0 += nq == 2 ? n : (n + 1) / 2;
+            uses1 += nq == 2 ? n : n / 2;
             if (active) done += n;
             ok = __all_sync(0xffffffffu, ok);
             if (!ok || !mbar_wait_lanes(ofull, pieces & 1, abort, status, STATUS_ATTEND_WAIT)) break;
@@ -413,9 +405,13 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         constexpr int GROUPS = TT / 32, HALVES = DC / 64;        // groups of 8 tokens a warp; a lane: a token and every fourth chunk of 16 dims
         static_assert(GROUPS * HALVES == 8, "eight loads a lane");
         const int r8 = lane & 7, c4 = lane >> 3, chunks = p.dim >> 4;
+        // where a chunk's two halves of 8 dims go.  K: core matrices, [8 dims][8 tokens]; V: rows of 64 dims, 128 bytes, with
+        // the chunks of a row exchanged by its number (the 128-byte swizzle)
+        const int at0 = kv ? w * 1024 + r8 * 128 + ((2 * c4 ^ r8) << 4) : 2 * c4 * (TT * 16) + w * 128 + r8 * 16;
+        const int at1 = kv ? w * 1024 + r8 * 128 + (((2 * c4 + 1) ^ r8) << 4) : at0 + TT * 16;
         KvWalk<R, TT> tiles(p, head->start);
         auto page_of = [&](const KvTile<R, TT> &t) {             // lane i: the page of this warp's i-th group
-            return t.there && lane < GROUPS ? page_at(p, t.b, t.base + (lane * 4 + w) * 8, t.lo, t.hi, 8, false) : -1;
+            return page_at(p, t.b, t.base + (lane * 4 + w) * 8, 8, t.lo, t.hi, t.there && lane < GROUPS);
         };
         auto load = [&](const KvTile<R, TT> &t, int id, uint4 (&raw)[8]) {
 #pragma unroll
@@ -429,13 +425,13 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             }
         };
         KvTile<R, TT> next = tiles.next();
-        int id = page_of(next);
+        Page page = page_of(next);
         for (uint32_t seq = 0; next.there; seq++) {
             // the loads are under way while the slot is waited for
             uint4 raw[8];
-            load(next, id, raw);
+            load(next, page_number(p, page, false), raw);
             next = tiles.next();
-            id = page_of(next);
+            page = page_of(next);
             const int slot = seq % SLOTS;
             if (seq >= SLOTS && !mbar_wait_soon_lanes(empty + 8 * slot, (seq / SLOTS - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) break;
             uint8_t *dst = slots + slot * C::SLOT;
@@ -451,9 +447,9 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                             h[2 * q] = codes_lo(x);
                             h[2 * q + 1] = codes_hi(x);
                         }
-                        uint8_t *at = dst + (2 * (c4 + 4 * k)) * (TT * 16) + (i * 4 + w) * 128 + r8 * 16;
-                        *(uint4 *)at = make_uint4(h[0], h[1], h[2], h[3]);
-                        *(uint4 *)(at + TT * 16) = make_uint4(h[4], h[5], h[6], h[7]);
+                        uint8_t *at = dst + i * (kv ? 4096 : 512) + k * (TT * 128);
+                        *(uint4 *)(at + at0) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *(uint4 *)(at + at1) = make_uint4(h[4], h[5], h[6], h[7]);
                     }
                 }
             fence_proxy_async();
@@ -464,22 +460,22 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REST_REGS));
         if (warp == 4 * NQ + CW && lane == 0) {
         // ------------------------------------------------------------------ one thread issues the products
-        Walk<R, TT> walk(p, head->start);
+        Walk<R, TT, false> walk(p, head->start);
         Piece piece;
         const uint32_t s_desc = idesc_of(1, 128, TT), o_desc = idesc_of(1, 128, p.dim) | 1u << 16;      // B of the second: a row a dim
-        uint32_t kseq = 0, vseq = 0, uses[2] = {0, 0}, pieces = 0;
+        uint32_t kseq = 0, vseq = 0, uses0 = 0, uses1 = 0, pieces = 0;
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) { ok = ok && mbar_wait_soon(bar, parity & 1, abort, status, STATUS_ATTEND_WAIT); return ok; };
         // descriptors count addresses in 16 bytes: a step of 16 dims (tokens) is an addition
         const uint64_t q_desc = smem_desc(base_u32 + C::O_Q, 2048, 128), k_desc = smem_desc(base_u32 + C::O_K, TT * 16, 128);
-        const uint64_t v_desc = smem_desc(base_u32 + C::O_V, 128, TT * 16);
+        const uint64_t v_desc = smem_desc(base_u32 + C::O_V, TT * 128, 1024) | (uint64_t)2 << 61;      // 128-byte swizzle
         const int steps = p.dim / 16;
         auto scores = [&](int t, int buf, uint32_t slot) {
             uint32_t accumulate = 0;
 #pragma unroll
             for (int x = 0; x < SPL; x++) {
                 uint64_t qd = q_desc + (t * SPL + x) * (C::QTILE >> 4), kd = k_desc + slot * (C::SLOT >> 4);
-#pragma unroll 4
+#pragma unroll 1
                 for (int d = 0; d < steps; d++) {
                     mma_issue<1>(tmem + C::s_col(buf), qd, kd, s_desc, accumulate);
                     accumulate = 1;
@@ -490,13 +486,13 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             mma_commit(sfull + 8 * buf);
         };
         auto sums = [&](int t, int buf, uint32_t slot, int j) {
-            const uint64_t vd = v_desc + slot * (C::SLOT >> 4);
+            uint64_t vd = v_desc + slot * (C::SLOT >> 4);
             const uint32_t p_at = tmem + C::s_col(buf), o_at = tmem + C::o_col(t);
-#pragma unroll
-            for (int s = 0; s < TT / 16; s++) {
+#pragma unroll 1
+            for (int s = 0; s < TT / 16; s++, vd += 2048 >> 4) {
                 const uint32_t col = p_at + (SPL == 2 ? (s >> 1) * 32 + (s & 1) * 8 : s * 8);
-                mma_issue_ts(o_at, col, vd + s * (256 >> 4), o_desc, s ? 1 : j);
-                if (SPL == 2) mma_issue_ts(o_at, col + 16, vd + s * (256 >> 4), o_desc, 1);
+                mma_issue_ts(o_at, col, vd, o_desc, s ? 1 : j);
+                if (SPL == 2) mma_issue_ts(o_at, col + 16, vd, o_desc, 1);
             }
             mma_commit(odone + 8 * t);
         };
@@ -514,7 +510,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 if (nq == 2) {
                     for (int t = 0; t < 2; t++) {
                         if (t == 0 && !wait(vfull + 8 * vs, vseq / SLOTS)) break;
-                        if (!wait(pfull + 8 * t, uses[t] + j)) break;
+                        if (!wait(pfull + 8 * t, (t ? uses1 : uses0) + j)) break;
                         tc_fence_after();
                         sums(t, t, vs, j);
                         if (more) {
@@ -530,7 +526,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                         tc_fence_after();
                         scores(0, buf ^ 1, ks);
                     }
-                    if (!wait(vfull + 8 * vs, vseq / SLOTS) || !wait(pfull + 8 * buf, uses[buf] + (j >> 1))) break;
+                    if (!wait(vfull + 8 * vs, vseq / SLOTS) || !wait(pfull + 8 * buf, (buf ? uses1 : uses0) + (j >> 1))) break;
                     tc_fence_after();
                     sums(0, buf, vs, j);
                 }
@@ -543,8 +539,8 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 }
             }
             if (!ok) break;
-            if (nq == 2) { uses[0] += n; uses[1] += n; }
-            else { uses[0] += (n + 1) / 2; uses[1] += n / 2; }
+            uses0 += nq == 2 ? n : (n + 1) / 2;
+            uses1 += nq == 2 ? n : n / 2;
             mma_commit(ofull);
             pieces++;
         }
