@@ -11,6 +11,10 @@ namespace qb {
 
 constexpr float NOTHING = -1e30f;              // a maximum over nothing (finite: differences of two of them are 0)
 constexpr int LEAST_TOKENS = 256;              // tokens a share has at least
+// What a unit costs a block besides its tiles, in tiles of TT tokens: its rows of q, the join of its sums.  Measured: 3000
+// cycles at 350 a tile in attend_rows.cu (32 tokens a tile), 25000 at 7000 in attend_tiles.cu.  The line of work below
+// counts it, or a block that gets many short sequences ends long after the others.
+__host__ __device__ constexpr int unit_pad(int tt) { return tt == 32 ? 8 : 4; }
 
 struct AttendArgs {
     qb200_sequences_t seq;
@@ -106,16 +110,25 @@ __device__ __forceinline__ int chunks_of(const AttendArgs &p, int b)
     return (n * p.group + R - 1) / R;
 }
 
+// a / b for 0 <= a < 2^52, b > 0: a double's quotient, put right
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b)
+{
+    int64_t q = (int64_t)((double)a / (double)b);
+    if (q * b > a) q--;
+    if ((q + 1) * b <= a) q++;
+    return q;
+}
+
 struct Start {
-    int b, h, rc, tile;                        // where a share begins: a unit and a tile inside it
-    int64_t left;                              // tiles it has
+    int b, h, rc, at;                          // where a share begins: a unit, and a place in it
+    int64_t left;                              // how long it is
 };
 
-// The line of tiles: sequence after sequence, head after head, unit after unit.  The functions below are called by a whole
-// warp.  Few sequences: a lane a unit; many: a lane a sequence.
+// The line of work: sequence after sequence, head after head, unit after unit, a unit taking unit_pad places for itself and
+// then one a tile.  The functions below are called by a whole warp.  Few sequences: a lane a unit; many: a lane a sequence.
 constexpr int FEW_SEQUENCES = 8;
 
-// Tiles of one head of sequence b: this lane's part of them (few sequences), or all.
+// The length of one head of sequence b: this lane's part of it (few sequences), or all.
 template <int R, int TT>
 __device__ __forceinline__ int64_t tiles_of(const AttendArgs &p, int b, int first, int step)
 {
@@ -123,7 +136,7 @@ __device__ __forceinline__ int64_t tiles_of(const AttendArgs &p, int b, int firs
     const Sequence s = sequence_at(p, b);
     const int chunks = (s.n * p.group + R - 1) / R;
 #pragma unroll 1
-    for (int rc = first; rc < chunks; rc += step) sum += unit_of<R, TT>(p, s, b, 0, rc).nt;
+    for (int rc = first; rc < chunks; rc += step) sum += unit_of<R, TT>(p, s, b, 0, rc).nt + unit_pad(TT);
     return sum;
 }
 __device__ __forceinline__ int64_t warp_sum(int64_t x)
@@ -161,7 +174,7 @@ __device__ __forceinline__ Start place_on_line(const AttendArgs &p, int64_t x)
 {
     const int lane = threadIdx.x & 31;
     Start s = {p.seq.count, 0, 0, 0, 0};
-    int64_t tiles = 0;                         // of one head of the sequence found
+    int64_t tiles = 0;                         // the length of one head of the sequence found
     if (p.seq.count <= FEW_SEQUENCES) {
 #pragma unroll 1
         for (int b = 0; b < p.seq.count; b++) {
@@ -185,19 +198,19 @@ __device__ __forceinline__ Start place_on_line(const AttendArgs &p, int64_t x)
         }
     }
     if (s.b == p.seq.count || tiles == 0) { s.b = p.seq.count; return s; }
-    s.h = (int)(x / tiles);
+    s.h = (int)quotient(x, tiles);
     x -= s.h * tiles;
     const Sequence q = sequence_at(p, s.b);
     const int chunks = (q.n * p.group + R - 1) / R;
 #pragma unroll 1
     for (int base = 0; base < chunks; base += 32) {
-        const int64_t upto = warp_upto(base + lane < chunks ? unit_of<R, TT>(p, q, s.b, s.h, base + lane).nt : 0);
+        const int64_t upto = warp_upto(base + lane < chunks ? unit_of<R, TT>(p, q, s.b, s.h, base + lane).nt + unit_pad(TT) : 0);
         const unsigned after = __ballot_sync(0xffffffffu, upto > x);
         if (after) {
             const int k = __ffs(after) - 1;
             s.rc = base + k;
             const int64_t before = __shfl_sync(0xffffffffu, upto, k > 0 ? k - 1 : 0);
-            s.tile = (int)(x - (k > 0 ? before : 0));
+            s.at = (int)(x - (k > 0 ? before : 0));
             return s;
         }
         x -= __shfl_sync(0xffffffffu, upto, 31);
@@ -207,18 +220,27 @@ __device__ __forceinline__ Start place_on_line(const AttendArgs &p, int64_t x)
 }
 // Shares there are: one a block, but none of less than LEAST_TOKENS tokens unless every unit has one.
 template <int TT>
-__device__ __forceinline__ int64_t shares_of(const AttendArgs &p, int64_t total)
+__device__ __forceinline__ int shares_of(const AttendArgs &p, int64_t total)
 {
     const int64_t units = (int64_t)p.seq.count * p.heads * p.chunks;
-    return max((int64_t)1, min(min((int64_t)p.grid, total), max(units, total / (LEAST_TOKENS / TT))));
+    return (int)max((int64_t)1, min(min((int64_t)p.grid, total), max(units, total / (LEAST_TOKENS / TT))));
 }
+// Where share `block` begins: shares are equally long, but for one place.
+struct Shares {
+    int64_t each;
+    int more;                                  // the first `more` of them have one place more
+    __device__ __forceinline__ Shares(int64_t total, int shares) { each = quotient(total, shares); more = (int)(total - each * shares); }
+    __device__ __forceinline__ int64_t at(int block) const { return each * block + min(block, more); }
+};
 template <int R, int TT>
 __device__ __noinline__ Start start_of(const AttendArgs &p, int block)
 {
-    const int64_t total = line_length<R, TT>(p), shares = shares_of<TT>(p, total);
+    const int64_t total = line_length<R, TT>(p);
+    const int shares = shares_of<TT>(p, total);
     Start s = {0, 0, 0, 0, 0};
     if (block >= shares) return s;
-    const int64_t from = total * block / shares, to = total * (block + 1) / shares;
+    const Shares cuts(total, shares);
+    const int64_t from = cuts.at(block), to = cuts.at(block + 1);
     if (to > from) s = place_on_line<R, TT>(p, from);
     s.left = to - from;
     return s;
@@ -231,20 +253,22 @@ struct Cut {
 template <int R, int TT>
 __device__ __noinline__ Cut cut_of(const AttendArgs &p, int block)
 {
-    const int64_t total = line_length<R, TT>(p), shares = shares_of<TT>(p, total);
+    const int64_t total = line_length<R, TT>(p);
+    const int shares = shares_of<TT>(p, total);
     Cut c = {0, 0, 0, block, 0};
     if (block >= shares) return c;
-    const int64_t from = total * block / shares, before = total * (block - 1) / shares;
-    if (from >= total) return c;
+    const Shares cuts(total, shares);
+    const int64_t from = cuts.at(block), before = cuts.at(block - 1);
     const Start s = place_on_line<R, TT>(p, from);
-    if (s.b >= p.seq.count || s.tile == 0 || before > from - s.tile) return c;      // not inside a unit, or not the first boundary inside it
-    const int64_t end = from - s.tile + unit_of<R, TT>(p, s.b, s.h, s.rc).nt;
+    // not inside a unit's tiles, or not the first boundary inside them
+    if (s.b >= p.seq.count || s.at <= unit_pad(TT) || before > from - s.at + unit_pad(TT)) return c;
+    const int64_t end = from - s.at + unit_pad(TT) + unit_of<R, TT>(p, s.b, s.h, s.rc).nt;
     c.b = s.b;
     c.h = s.h;
     c.rc = s.rc;
     c.parts = 1;
 #pragma unroll 1
-    for (int64_t k = block; k < shares && total * k / shares < end; k++) c.parts++;
+    for (int k = block; k < shares && cuts.at(k) < end; k++) c.parts++;
     return c;
 }
 
@@ -258,10 +282,10 @@ template <int R, int TT, bool WHOLE>
 struct Walk {
     const AttendArgs &p;
     Sequence seq;
-    int b, h, rc, chunks, tile;
-    int64_t left;                              // tiles; whole: the next unit's number
+    int b, h, rc, chunks, at;
+    int64_t left;                              // of the share; whole: the next unit's number
 
-    __device__ __forceinline__ Walk(const AttendArgs &args, const Start &s) : p(args), b(s.b), h(s.h), rc(s.rc), chunks(0), tile(s.tile), left(s.left)
+    __device__ __forceinline__ Walk(const AttendArgs &args, const Start &s) : p(args), b(s.b), h(s.h), rc(s.rc), chunks(0), at(s.at), left(s.left)
     {
         if (WHOLE && p.whole) {
             left = blockIdx.x;
@@ -294,24 +318,28 @@ struct Walk {
             piece.count = piece.unit.nt;
             return true;
         }
-        if (left <= 0) return false;
 #pragma unroll 1
-        while (rc >= chunks) {
-            rc = 0;
-            if (++h == p.heads) {
-                h = 0;
-                if (++b >= p.seq.count) return false;
-                look();
+        while (left > 0) {
+#pragma unroll 1
+            while (rc >= chunks) {
+                rc = 0;
+                if (++h == p.heads) {
+                    h = 0;
+                    if (++b >= p.seq.count) return false;
+                    look();
+                }
             }
+            piece.unit = unit_of<R, TT>(p, seq, b, h, rc);
+            const int to = (int)min((int64_t)(piece.unit.nt + unit_pad(TT)), at + left);
+            if (to <= at) return false;
+            piece.first = max(0, at - unit_pad(TT));
+            piece.count = max(0, to - unit_pad(TT)) - piece.first;
+            left -= to - at;
+            at = 0;
+            rc++;
+            if (piece.count > 0) return true;
         }
-        piece.unit = unit_of<R, TT>(p, seq, b, h, rc);
-        piece.first = tile;
-        piece.count = (int)min((int64_t)(piece.unit.nt - tile), left);
-        if (piece.count <= 0) return false;
-        left -= piece.count;
-        tile = 0;
-        rc++;
-        return true;
+        return false;
     }
 };
 

@@ -23,20 +23,38 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     const float *first = (const float *)p.workspace + (size_t)((cut.block - 1) * 2 + 1) * size;      // the part that begins the unit
     for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * quads; i += 256 * gridDim.y) {
         const int r = i / quads, d = (i - r * quads) * 4;
-        float m = NOTHING;
-        for (int k = 0; k < cut.parts; k++) m = fmaxf(m, first[(k ? (size_t)(2 * k - 1) * size : 0) + r * 2]);
-        float sum = 0.f;
+        float m = NOTHING, sum = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < cut.parts; k++) {
-            const float *part = first + (k ? (size_t)(2 * k - 1) * size : 0);
-            const float2 s = *(const float2 *)(part + r * 2);
-            const float4 x = *(const float4 *)(part + R * 2 + r * p.dim + d);
-            const float f = exp2_fast(s.x - m);
-            sum = __fmaf_rn(s.y, f, sum);
-            acc.x = __fmaf_rn(x.x, f, acc.x);
-            acc.y = __fmaf_rn(x.y, f, acc.y);
-            acc.z = __fmaf_rn(x.z, f, acc.z);
-            acc.w = __fmaf_rn(x.w, f, acc.w);
+#pragma unroll 1
+        for (int k0 = 0; k0 < cut.parts; k0 += 8) {            // eight parts' loads at a time, in the order of the tokens
+            float2 s[8];
+            float4 x[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                s[k] = make_float2(NOTHING, 0.f);
+                x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k0 + k < cut.parts) {
+                    const float *part = first + (k0 + k ? (size_t)(2 * (k0 + k) - 1) * size : 0);
+                    s[k] = *(const float2 *)(part + r * 2);
+                    x[k] = *(const float4 *)(part + R * 2 + r * p.dim + d);
+                }
+            }
+            float top = m;
+#pragma unroll
+            for (int k = 0; k < 8; k++) top = fmaxf(top, s[k].x);
+            const float less = exp2_fast(m - top);
+            m = top;
+            sum *= less;
+            acc = make_float4(acc.x * less, acc.y * less, acc.z * less, acc.w * less);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float f = exp2_fast(s[k].x - m);
+                sum = __fmaf_rn(s[k].y, f, sum);
+                acc.x = __fmaf_rn(x[k].x, f, acc.x);
+                acc.y = __fmaf_rn(x[k].y, f, acc.y);
+                acc.z = __fmaf_rn(x[k].z, f, acc.z);
+                acc.w = __fmaf_rn(x[k].w, f, acc.w);
+            }
         }
         finish_row<T>(p, u, u.r0 + r, d, acc, m, sum);
     }
