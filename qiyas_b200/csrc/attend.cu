@@ -2,11 +2,15 @@
 //
 //  * attend_rows.cu: at most 16 rows (query heads x tokens that share a head of the cache): the cache's bytes bound it.
 //  * attend_tiles.cu: more rows: the tensor cores (tcgen05) take 128 rows of queries at a time.
+#include <cuda.h>
 #include "common.cuh"
 #include "attend_device.cuh"
 
 namespace qb {
 
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled g_attend_encode = nullptr;
 static int *g_attend_status = nullptr;
 static int g_attend_sms = 0;
 
@@ -15,7 +19,12 @@ cudaError_t attend_init(int sm_count, int max_smem, int *status)
     g_attend_status = status;
     g_attend_sms = sm_count;
     if (max_smem < 232448) return cudaErrorInvalidValue;
-    cudaError_t e;
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found);
+    if (e) return e;
+    if (found != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
+    g_attend_encode = (EncodeTiled)fn;
     if ((e = attend_rows_init())) return e;
     return attend_tiles_init();
 }
@@ -42,6 +51,16 @@ size_t attend_workspace_bytes(int dim, int heads, int type, int count, int rows,
     (void)type; (void)rows;
     const Plan plan = plan_of(dim, heads, q_heads / heads, count, max_queries, max_length);
     return plan.whole ? 0 : (size_t)g_attend_sms * 2 * part_floats(plan.r, dim) * 4;
+}
+
+// The codes as rows of dim bytes, fetched box_rows tokens and box_dim dims at a time (zeros past dim).
+static bool codes_map(CUtensorMap &map, const void *codes, const qb200_cache_t &c, int box_dim, int box_rows)
+{
+    const cuuint64_t dims[2] = { (cuuint64_t)c.dim, (cuuint64_t)c.pages * c.heads * c.page }, strides[1] = { (cuuint64_t)c.dim };
+    const cuuint32_t box[2] = { (cuuint32_t)box_dim, (cuuint32_t)box_rows }, estr[2] = { 1, 1 };
+    return g_attend_encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           box_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 int attend(const AttendCall &call, cudaStream_t stream)
@@ -81,7 +100,10 @@ int attend(const AttendCall &call, cudaStream_t stream)
     const int64_t units = (int64_t)call.seq.count * c.heads * a.chunks;
     a.grid = plan.whole ? (int)(units < 1 << 20 ? units : 1 << 20) : g_attend_sms;
     if (plan.tiles) return attend_tiles(a, call.type, stream);
-    return attend_rows(a, call.type, plan.r, stream);
+    CUtensorMap kmap, vmap;
+    const int box = c.dim <= 64 ? 64 : 128, rows = c.page < 32 ? c.page : 32;
+    if (!codes_map(kmap, c.k_codes, c, box, rows) || !codes_map(vmap, c.v_codes, c, box, rows)) return (int)cudaErrorInvalidValue;
+    return attend_rows(a, call.type, plan.r, kmap, vmap, stream);
 }
 
 }  // namespace qb

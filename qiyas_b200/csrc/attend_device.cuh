@@ -1,6 +1,7 @@
 // What the attention kernels share: how a call's work is cut into shares, the rows' limits, and the products' operands.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
 
@@ -37,7 +38,7 @@ struct AttendArgs {
 __device__ __forceinline__ int by_group(const AttendArgs &p, int n) { return (int)(((uint64_t)(uint32_t)n * p.group_magic) >> p.group_shift); }
 
 cudaError_t attend_rows_init();
-int attend_rows(const AttendArgs &args, int type, int r, cudaStream_t stream);
+int attend_rows(const AttendArgs &args, int type, int r, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t stream);
 cudaError_t attend_tiles_init();
 int attend_tiles(const AttendArgs &args, int type, cudaStream_t stream);
 

@@ -21,6 +21,7 @@
 //    weights down to 2^-29 of the largest with all its bits, and the accumulators are seldom rescaled.
 //  * q is scaled by a power of two to a row's maximum of 2^13 and cut to f16; with f32 lanes q and w enter as the sum of
 //    two f16 (SPL 2), which loses 2^-22.
+#include <cuda.h>
 #include "common.cuh"
 #include "attend_device.cuh"
 #include "attend_join.cuh"
@@ -59,20 +60,16 @@ static_assert(sizeof(RowsHead) <= ROWS_HEADER, "the header fits");
 
 struct Batch { int b, h, lo, hi, tile, count; };       // tiles of one piece
 
-// 16 bytes of global memory into shared memory, past the L1 cache; and this thread's arrival on a barrier once all it has
-// copied so far is there.
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src)
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const void *map, int x, int y, uint32_t bar)
 {
-    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copies_arrive(uint32_t bar)
-{
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
 }
 
 template <int DT, int NB, int SPL, typename T>
 __global__ void __launch_bounds__(RTHREADS, 1)
-attend_rows_kernel(const __grid_constant__ AttendArgs p)
+attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap)
 {
     using C = RowsCfg<DT, NB, SPL>;
     extern __shared__ uint8_t smem_raw[];
@@ -84,7 +81,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p)
     if (threadIdx.x == 0) {
         head->abort = 0;
         for (int i = 0; i < C::S; i++) {
-            mbar_init(full0 + 8 * i, 33);        // the producer's lanes, as their copies land, and its word that the scales are there
+            mbar_init(full0 + 8 * i, 1);
             mbar_init(empty0 + 8 * i, 1);
         }
         mbar_fence_init();
@@ -126,10 +123,10 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p)
             const int token = (t.tile + lane / per) * 32 + (per == 2 ? (lane & 1) * 16 : 0);
             return page_at(p, t.b, token, 32 / per, t.lo, t.hi, lane / per < t.count);
         };
-        constexpr int CHUNKS = DT / 16, ROWS = 32 / CHUNKS;              // 16-byte chunks a token, tokens an instruction of the warp
-        const int chunk = lane % CHUNKS, row0 = lane / CHUNKS;
-        const bool has = chunk * 16 < p.dim;
-        const int step = ROWS * p.dim;
+        // a copy: the tokens of one page in the tile, up to 128 bytes of each; a lane a copy
+        const int rows = 32 / per, which = lane & 1, sub = (lane >> 1) % C::SUB, second = lane / (2 * C::SUB);
+        const uint32_t bytes = rows * C::SW, offset = which * C::HALF + sub * (32 * 128) + second * 16 * C::SW;
+        uint32_t issued = 0;                   // this warp's tiles so far: stages mine, mine + RP, ... in turn
         Batch now = next_batch();
         int id = page_number(p, page_of(now), mine == 0);
         float2 sc = scales_at(p, id, now.h);
@@ -146,30 +143,20 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p)
                 if (tile >= C::S && !mbar_wait_soon_lanes(empty0 + 8 * stage, (tile / C::S - 1) & 1, abort, p.status, STATUS_ATTEND_WAIT)) goto done;
                 const int base = (now.tile + k) * 32, l0 = k * per, l1 = l0 + per - 1;
                 const int id0 = __shfl_sync(0xffffffffu, id, l0), id1 = __shfl_sync(0xffffffffu, id, l1);
-                // tokens 0 .. 15 of the tile, and 16 .. 31: in pages of 16 they lie apart
-                const int inside = base & ((1 << p.log_page) - 1), inside1 = per == 2 ? 0 : inside + 16;
-                int64_t from = ((((int64_t)id0 * p.heads + now.h) << p.log_page) + inside + row0) * p.dim + chunk * 16;
-                const int64_t from1 = ((((int64_t)id1 * p.heads + now.h) << p.log_page) + inside1 + row0) * p.dim + chunk * 16;
-                const uint32_t to = ring + stage * C::STAGE;
-                const bool whole = base >= now.lo && base + 32 <= now.hi;
-#pragma unroll
-                for (int i = 0; i < 32 / ROWS; i++, from += step) {
-                    if (i * ROWS == 16) from = from1;
-                    const int row = i * ROWS + row0;
-                    bool copy = has && (i * ROWS >= 16 ? id1 : id0) >= 0;
-                    if (!whole) copy &= base + row >= now.lo && base + row < now.hi;
-                    if (copy) {
-                        const uint32_t dst = to + swizzled<DT>(DT == 256 ? chunk >> 3 : 0, row, DT == 256 ? chunk & 7 : chunk);
-                        copy16(dst, p.k_codes + from);
-                        copy16(dst + C::HALF, p.v_codes + from);
-                    }
-                }
-                copies_arrive(full0 + 8 * stage);
                 const float k0 = __shfl_sync(0xffffffffu, sc.x, l0), k1 = __shfl_sync(0xffffffffu, sc.x, l1);
                 const float v0 = __shfl_sync(0xffffffffu, sc.y, l0), v1 = __shfl_sync(0xffffffffu, sc.y, l1);
                 if (lane == 0) {
+                    const int live = (id0 >= 0 ? 1 : 0) + (per == 2 && id1 >= 0 ? 1 : 0);
                     head->scales[stage] = make_float4(k0, v0, k1, v1);
-                    mbar_arrive(full0 + 8 * stage);
+                    if (live) mbar_arrive_expect_tx(full0 + 8 * stage, live * 2 * C::SUB * bytes);
+                    else mbar_arrive(full0 + 8 * stage);
+                }
+                issued++;
+                __syncwarp();
+                const int page = second ? id1 : id0;
+                if (lane < 2 * C::SUB * per && page >= 0) {
+                    const int row = ((page * p.heads + now.h) << p.log_page) + ((base + second * 16) & ((1 << p.log_page) - 1));
+                    tma_load_2d(ring + stage * C::STAGE + offset, which ? &vmap : &kmap, sub * 128, row, full0 + 8 * stage);
                 }
             }
             seq += now.count;
@@ -179,8 +166,14 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p)
             next = after;
         }
     done:
-        // no copy may be under way when the block ends, whoever gave up: a thread waits for its own
-        asm volatile("cp.async.wait_all;" ::: "memory");
+        // no copy may be under way when the block ends, whoever gave up
+        for (int i = 0; i < C::S; i++)
+            if (i % RP == mine && issued > i / RP) {
+                // the newest of this warp's tiles in stage i
+                const uint32_t uses = (issued - 1 - i / RP) / (C::S / RP);
+                const long long from = clock64();
+                while (!mbar_try_wait(full0 + 8 * i, uses & 1) && clock64() - from < WAIT_CYCLES) { }
+            }
         return;
     }
 
@@ -492,26 +485,26 @@ cudaError_t attend_rows_init()
 }
 
 template <int DT, int NB, int SPL, typename T>
-static int launch_rows(const AttendArgs &args, cudaStream_t stream)
+static int launch_rows(const AttendArgs &args, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t stream)
 {
-    attend_rows_kernel<DT, NB, SPL, T><<<args.grid, RTHREADS, RowsCfg<DT, NB, SPL>::SMEM, stream>>>(args);
+    attend_rows_kernel<DT, NB, SPL, T><<<args.grid, RTHREADS, RowsCfg<DT, NB, SPL>::SMEM, stream>>>(args, kmap, vmap);
     const cudaError_t e = cudaGetLastError();
     return e || args.whole ? (int)e : launch_join<8 * NB, 32, T>(args, stream);
 }
 
 template <int SPL, typename T>
-static int launch_rows_dim(const AttendArgs &args, int r, cudaStream_t stream)
+static int launch_rows_dim(const AttendArgs &args, int r, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t stream)
 {
-    if (args.dim <= 64) return r == 16 ? launch_rows<64, 2, SPL, T>(args, stream) : launch_rows<64, 1, SPL, T>(args, stream);
-    if (args.dim <= 128) return r == 16 ? launch_rows<128, 2, SPL, T>(args, stream) : launch_rows<128, 1, SPL, T>(args, stream);
-    return launch_rows<256, 1, SPL, T>(args, stream);
+    if (args.dim <= 64) return r == 16 ? launch_rows<64, 2, SPL, T>(args, kmap, vmap, stream) : launch_rows<64, 1, SPL, T>(args, kmap, vmap, stream);
+    if (args.dim <= 128) return r == 16 ? launch_rows<128, 2, SPL, T>(args, kmap, vmap, stream) : launch_rows<128, 1, SPL, T>(args, kmap, vmap, stream);
+    return launch_rows<256, 1, SPL, T>(args, kmap, vmap, stream);
 }
 
-int attend_rows(const AttendArgs &args, int type, int r, cudaStream_t stream)
+int attend_rows(const AttendArgs &args, int type, int r, const CUtensorMap &kmap, const CUtensorMap &vmap, cudaStream_t stream)
 {
-    if (type == QB200_F32) return launch_rows_dim<2, float>(args, r, stream);
-    if (type == QB200_F16) return launch_rows_dim<1, __half>(args, r, stream);
-    return launch_rows_dim<1, __nv_bfloat16>(args, r, stream);
+    if (type == QB200_F32) return launch_rows_dim<2, float>(args, r, kmap, vmap, stream);
+    if (type == QB200_F16) return launch_rows_dim<1, __half>(args, r, kmap, vmap, stream);
+    return launch_rows_dim<1, __nv_bfloat16>(args, r, kmap, vmap, stream);
 }
 
 }  // namespace qb
