@@ -89,21 +89,33 @@ __device__ __forceinline__ Item item_of(const CacheArgs &p, int item)
     return it;
 }
 
-// x / scale to the nearest integer, ties to even, from the exact quotient: the product with the reciprocal is off by less
-// than 2^-16, so only a quotient next to a half can round to the wrong side, and the remainder x - q * scale, which an fma
-// gives exactly here, says so.  Adding 1.5 * 2^23 rounds; the sum's low byte is the code.
-__device__ __forceinline__ uint32_t code_of(float x, float scale, float inverse, float half)
+// Eight x / scale to the nearest integers, ties to even, from the exact quotients.  Adding 1.5 * 2^23 to the product with
+// the reciprocal rounds it; the sum's low byte is the code.  The product is off by less than 2^-16, so only a quotient next to
+// a half can go to the wrong side, and the remainder x - q * scale, which an fma gives exactly here, says so.  That is looked
+// at for the eight together: seldom is there one.
+__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float scale, float inverse, float half)
 {
     constexpr float MAGIC = 12582912.f;
-    const float m = __fmaf_rn(x, inverse, MAGIC);
-    const float q = __fsub_rn(m, MAGIC);
-    const float r = __fmaf_rn(-q, scale, x);
-    uint32_t bits = __float_as_uint(m);
-    if (fabsf(r) >= half) {
-        const uint32_t away = r > 0.f ? 1u : 0xffffffffu;
-        if (fabsf(r) > half || (bits & 1u)) bits += away;
+    float m[8], most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        m[i] = __fmaf_rn(x[i], inverse, MAGIC);
+        most = fmaxf(most, fabsf(__fmaf_rn(-__fsub_rn(m[i], MAGIC), scale, x[i])));
     }
-    return bits & 0xffu;
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) c[i] = __float_as_uint(m[i]);
+    if (most >= half) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float r = __fmaf_rn(-__fsub_rn(m[i], MAGIC), scale, x[i]);
+            if (fabsf(r) > half || (fabsf(r) == half && (c[i] & 1u))) c[i] += r > 0.f ? 1u : 0xffffffffu;
+        }
+    }
+    uint2 w;
+    w.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    w.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+    return w;
 }
 
 // The same for scales whose reciprocal leaves the type's range or whose half is not exact, and for NaN and infinities.
@@ -125,8 +137,7 @@ __global__ void __launch_bounds__(item_threads(LANES)) cache_write_kernel(const 
 {
     constexpr int THREADS = item_threads(LANES);
     constexpr int PER = THREADS / LANES;
-    __shared__ float s_max[32];
-    __shared__ int s_odd[32];
+    __shared__ uint32_t s_max[32];
     const int group = threadIdx.x / LANES, tid = threadIdx.x % LANES;
     const Item it = item_of(p, blockIdx.x * PER + group);
     if (it.page < 0) return;                       // uniform over the group; with one group a block, over the block
@@ -153,28 +164,41 @@ __global__ void __launch_bounds__(item_threads(LANES)) cache_write_kernel(const 
             if (col >= vecs) { col -= vecs; row++; }
         }
     }
-    float top = 0.f;
-    bool odd = false;
+    // magnitudes compare as their bits do, and infinities and NaN lie above all others
+    uint32_t bits = 0;
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        float v[8];
-        unpack8(x[j], v);
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float a = fabsf(v[i]);
-            const bool finite = a <= 3.402823466e38f;
-            odd |= !finite;
-            top = finite ? fmaxf(top, a) : top;
-        }
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    odd = __any_sync(0xffffffffu, odd);
+    for (int j = 0; j < NV; j++) bits = largest8(x[j], bits);
+    bits = largest_of(bits, (const T *)nullptr);
+    bits = __reduce_max_sync(0xffffffffu, bits);
     if (LANES > 32) {
-        if ((tid & 31) == 0) { s_max[tid >> 5] = top; s_odd[tid >> 5] = odd; }
+        if ((tid & 31) == 0) s_max[tid >> 5] = bits;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < LANES / 32; w++) { top = fmaxf(top, s_max[w]); odd |= s_odd[w] != 0; }
+        for (int w = 0; w < LANES / 32; w++) bits = max(bits, s_max[w]);
+    }
+    float top = magnitude(bits, (const T *)nullptr);
+    const bool odd = !(top <= 3.402823466e38f);
+    if (odd) {                                     // seldom: the largest of the finite ones
+        top = 0.f;
+#pragma unroll 1
+        for (int j = 0; j < NV; j++) {
+            float v[8];
+            unpack8(x[0], v);
+#pragma unroll
+            for (int k = 1; k < NV; k++)
+                if (k == j) unpack8(x[k], v);
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fabsf(v[i]) <= 3.402823466e38f ? fmaxf(top, fabsf(v[i])) : top;
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (LANES > 32) {
+            __syncthreads();
+            if ((tid & 31) == 0) s_max[tid >> 5] = __float_as_uint(top);
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < LANES / 32; w++) top = fmaxf(top, __uint_as_float(s_max[w]));
+        }
     }
     if (odd && tid == 0) atomicOr(p.status, STATUS_CACHE_VALUE);
 
@@ -204,17 +228,15 @@ __global__ void __launch_bounds__(item_threads(LANES)) cache_write_kernel(const 
         if (tid + j * LANES >= total) break;
         float v[8];
         unpack8(x[j], v);
-        uint32_t c[8];
-        if (plain) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) c[i] = code_of(v[i], scale, inverse, half);
-        } else {
+        uint2 w;
+        if (plain) w = codes_of(v, scale, inverse, half);
+        else {
+            uint32_t c[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) c[i] = code_of_any(v[i], scale);
+            w.x = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+            w.y = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
         }
-        uint2 w;
-        w.x = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-        w.y = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
         dst[tid + j * LANES] = w;
     }
 }

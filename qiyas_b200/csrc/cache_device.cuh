@@ -64,6 +64,20 @@ __device__ __forceinline__ void unpack8(const Vec8<__nv_bfloat16> &x, float (&v)
     }
 }
 
+// The largest magnitude's bits, of eight values and of what was there: two 16-bit halves, or one word.
+template <typename T>
+__device__ __forceinline__ uint32_t largest8(const Vec8<T> &x, uint32_t bits)
+{
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) * 2; i++) bits = sizeof(T) == 4 ? max(bits, x.w[i] & 0x7fffffffu) : __vmaxu2(bits, x.w[i] & 0x7fff7fffu);
+    return bits;
+}
+__device__ __forceinline__ uint32_t largest_of(uint32_t bits, const float *) { return bits; }
+__device__ __forceinline__ uint32_t largest_of(uint32_t bits, const void *) { return max(bits & 0xffffu, bits >> 16); }
+__device__ __forceinline__ float magnitude(uint32_t bits, const float *) { return __uint_as_float(bits); }
+__device__ __forceinline__ float magnitude(uint32_t bits, const __half *) { return __half2float(__ushort_as_half((unsigned short)bits)); }
+__device__ __forceinline__ float magnitude(uint32_t bits, const __nv_bfloat16 *) { return __uint_as_float(bits << 16); }
+
 __device__ __forceinline__ uint32_t bits_of(float x, const __half *) { return __half_as_ushort(__float2half_rn(x)); }
 __device__ __forceinline__ uint32_t bits_of(float x, const __nv_bfloat16 *) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
 __device__ __forceinline__ uint32_t bits_of(float x, const float *) { return __float_as_uint(x); }
