@@ -295,8 +295,9 @@ int qb200_ipc_close(void *ptr);
  * the device, and the calls read them there: nothing is synchronised.  A page or length outside the cache or the table
  * is left out and sets bit 4 of the status word; nothing is read or written out of bounds.
  *
- * Lane arrays (k, v, q, out) are f32, f16 or bf16 (`type`); element (row, head, i) is at row * row_stride + head *
- * head_stride + i, strides in elements.  Where base and strides are multiples of 16 bytes the loads are wide. */
+ * qb200_lanes: an array of rows in f32, f16 or bf16 (`type` of the call); element (row, head, i) is at base + row *
+ * row_stride + head * head_stride + i, strides in elements.  Where base and strides are multiples of 16 bytes the loads
+ * are wide. */
 typedef struct qb200_cache {
     void *k_codes, *v_codes;
     float *k_scales, *v_scales;
@@ -308,6 +309,10 @@ typedef struct qb200_sequences {
     const int32_t *offsets;
     int count, width, rows;
 } qb200_sequences_t;
+typedef struct qb200_lanes {
+    void *base;
+    int64_t row_stride, head_stride;
+} qb200_lanes_t;
 
 /* Writes the rows of k and v as tokens lengths[b], lengths[b] + 1, ... of their sequences (lengths[b] = tokens that are
  * in the cache already).  The definition, block by block: let a be the largest magnitude written into the block, s the
@@ -318,13 +323,13 @@ typedef struct qb200_sequences {
  * scale 0.  A NaN is stored as 0 and an infinity as the code +-127; neither enters a, and both set bit 5 of the status word.
  * Two calls that write the same block must be ordered (one stream, or an event); a page written to must not belong to two
  * sequences of a call. */
-int qb200_cache_write(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const void *k, int64_t k_row_stride,
-                      int64_t k_head_stride, const void *v, int64_t v_row_stride, int64_t v_head_stride, void *stream);
+int qb200_cache_write(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const qb200_lanes_t *k, const qb200_lanes_t *v,
+                      void *stream);
 /* Reads tokens lengths[b], lengths[b] + 1, ... of the sequences back into the rows of k and v (either may be NULL):
  * code * scale in f32, rounded once to `type`.  (lengths[b] = the first token read.)  Rows of tokens that lie outside the
  * table or the cache are left as they were. */
-int qb200_cache_read(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, void *k, int64_t k_row_stride,
-                     int64_t k_head_stride, void *v, int64_t v_row_stride, int64_t v_head_stride, void *stream);
+int qb200_cache_read(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const qb200_lanes_t *k, const qb200_lanes_t *v,
+                     void *stream);
 
 /* out = softmax(scale * q . K^T) . V over the cache, q_heads query heads in groups of q_heads / cache->heads that share a
  * head of the cache.  lengths[b] = tokens of sequence b to attend to, the call's own among them (write them first).  With
@@ -337,11 +342,17 @@ int qb200_cache_read(const qb200_cache_t *cache, const qb200_sequences_t *sequen
  *   the sum of two f16), the codes exactly.
  *   workspace: device scratch of qb200_cache_attention_workspace_bytes(...) bytes, 16-byte aligned, private to the call
  *   until it completes on `stream`; the function gives 0, and workspace may be NULL, where no sequence is ever split. */
-size_t qb200_cache_attention_workspace_bytes(const qb200_cache_t *cache, int type, int count, int rows, int q_heads, int max_queries, int max_length);
-int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const void *q, int64_t q_row_stride,
-                          int64_t q_head_stride, void *out, int64_t out_row_stride, int64_t out_head_stride, float *lse, int q_heads,
-                          int max_queries, int max_length, float scale, int causal, int window, void *workspace, size_t workspace_bytes,
-                          void *stream);
+typedef struct qb200_attention {
+    qb200_lanes_t q, out;
+    float *lse;
+    void *workspace;
+    size_t workspace_bytes;
+    int q_heads, max_queries, max_length;
+    float scale;
+    int causal, window;
+} qb200_attention_t;
+size_t qb200_cache_attention_workspace_bytes(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const qb200_attention_t *attention);
+int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const qb200_attention_t *attention, void *stream);
 
 /* ---- plain device memory for hosts without a CUDA binding of their own (tests, bench) ---- */
 int qb200_malloc(void **ptr, size_t bytes);

@@ -5,6 +5,7 @@ machine without an sm_100 device makes qb200_init fail.
 """
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY = os.path.join(HERE, "libqiyas_b200.so")
@@ -23,16 +24,11 @@ class Caps(C.Structure):
                 ("tcgen05", C.c_int), ("max_shared_bytes", C.c_int), ("l2_bytes", C.c_int64), ("global_bytes", C.c_int64)]
 
 
-class CacheParts(C.Structure):
-    """qb200_cache_t: the codes and scales of a cache and its sizes."""
-    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
-                ("pages", C.c_int), ("heads", C.c_int), ("page", C.c_int), ("dim", C.c_int)]
-
-
-class Sequences(C.Structure):
-    """qb200_sequences_t: which pages and which rows of a call belong to which sequence."""
-    _fields_ = [("table", C.c_void_p), ("lengths", C.c_void_p), ("offsets", C.c_void_p), ("count", C.c_int), ("width", C.c_int), ("rows", C.c_int)]
-
+# The structures of the cache operators, packed by `struct` as the C compiler lays them out: a call hands their bytes over.
+CACHE = struct.Struct("@4P4i").pack            # qb200_cache_t: k_codes, v_codes, k_scales, v_scales, pages, heads, page, dim
+SEQUENCES = struct.Struct("@3P3i4x").pack      # qb200_sequences_t: table, lengths, offsets, count, width, rows
+LANES = struct.Struct("@P2q").pack             # qb200_lanes_t: base, row stride, head stride
+ATTENTION = struct.Struct("@P2qP2q2PN3if2i").pack       # qb200_attention_t: q, out, lse, workspace, bytes, q_heads, max_queries, max_length, scale, causal, window
 
 _P, _I, _Z, _L = C.c_void_p, C.c_int, C.c_size_t, C.c_int64
 
@@ -70,10 +66,10 @@ SIGNATURES = {
     "qb200_tensor_rate": (_I, [C.POINTER(C.c_double)]),
     "qb200_encode": (_I, [_I, _P, _P, _L, _P]),
     "qb200_decode": (_I, [_I, _P, _P, _L, _P]),
-    "qb200_cache_write": (_I, [C.POINTER(CacheParts), C.POINTER(Sequences), _I, _P, _L, _L, _P, _L, _L, _P]),
-    "qb200_cache_read": (_I, [C.POINTER(CacheParts), C.POINTER(Sequences), _I, _P, _L, _L, _P, _L, _L, _P]),
-    "qb200_cache_attention_workspace_bytes": (_Z, [C.POINTER(CacheParts), _I, _I, _I, _I, _I, _I]),
-    "qb200_cache_attention": (_I, [C.POINTER(CacheParts), C.POINTER(Sequences), _I, _P, _L, _L, _P, _L, _L, _P, _I, _I, _I, C.c_float, _I, _I, _P, _Z, _P]),
+    "qb200_cache_write": (_I, [_P, _P, _I, _P, _P, _P]),
+    "qb200_cache_read": (_I, [_P, _P, _I, _P, _P, _P]),
+    "qb200_cache_attention_workspace_bytes": (_Z, [_P, _P, _I, _P]),
+    "qb200_cache_attention": (_I, [_P, _P, _I, _P, _P]),
     "qb200_malloc": (_I, [C.POINTER(_P), _Z]),
     "qb200_free": (_I, [_P]),
     "qb200_malloc_host": (_I, [C.POINTER(_P), _Z]),

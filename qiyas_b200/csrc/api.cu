@@ -472,84 +472,81 @@ static int check_cache(const qb200_cache_t *c, const qb200_sequences_t *s, int t
     return 0;
 }
 
-static int check_lanes(const char *name, int type, const void *base, int64_t row, int64_t head, int rows, int heads)
+static int check_lanes(const char *name, int type, const qb200_lanes_t &x, int rows, int heads)
 {
-    if (rows > 0 && !base) return fail(QB200_E_POINTER, "%s: null", name);
-    if ((uintptr_t)base & (type == QB200_F32 ? 3 : 1)) return fail(QB200_E_POINTER, "%s: misaligned", name);
+    if (rows > 0 && !x.base) return fail(QB200_E_POINTER, "%s: null", name);
+    if ((uintptr_t)x.base & (type == QB200_F32 ? 3 : 1)) return fail(QB200_E_POINTER, "%s: misaligned", name);
     const int64_t most = (int64_t)1 << 55;        // products with 32-bit counts stay inside 64 bits of bytes
-    if (row < 0 || head < 0 || row > most / ((int64_t)rows + 1) || head > most / ((int64_t)heads + 1)) return fail(QB200_E_SHAPE, "%s: strides %lld, %lld", name, (long long)row, (long long)head);
+    if (x.row_stride < 0 || x.head_stride < 0 || x.row_stride > most / ((int64_t)rows + 1) || x.head_stride > most / ((int64_t)heads + 1))
+        return fail(QB200_E_SHAPE, "%s: strides %lld, %lld", name, (long long)x.row_stride, (long long)x.head_stride);
     return 0;
 }
 
-int qb200_cache_write(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const void *k, int64_t k_row_stride,
-                      int64_t k_head_stride, const void *v, int64_t v_row_stride, int64_t v_head_stride, void *stream)
+int qb200_cache_write(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const qb200_lanes_t *k, const qb200_lanes_t *v, void *stream)
 {
     int rc = check_cache(cache, sequences, type);
     if (rc) return rc;
-    if ((rc = check_lanes("k", type, k, k_row_stride, k_head_stride, sequences->rows, cache->heads))) return rc;
-    if ((rc = check_lanes("v", type, v, v_row_stride, v_head_stride, sequences->rows, cache->heads))) return rc;
+    if (!k || !v) return fail(QB200_E_POINTER, "null k or v");
+    if ((rc = check_lanes("k", type, *k, sequences->rows, cache->heads)) || (rc = check_lanes("v", type, *v, sequences->rows, cache->heads))) return rc;
     OnDevice on;
     if (!g_ready) return fail(QB200_E_DEVICE, "qb200_init has not succeeded");
     if (on.e) return cuda_fail(on.e, "cudaSetDevice");
-    return finish_other(qb::cache_write(*cache, *sequences, type, {const_cast<void *>(k), k_row_stride, k_head_stride},
-                                        {const_cast<void *>(v), v_row_stride, v_head_stride}, (cudaStream_t)stream), "cache_write", stream);
+    return finish_other(qb::cache_write(*cache, *sequences, type, *k, *v, (cudaStream_t)stream), "cache_write", stream);
 }
 
-int qb200_cache_read(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, void *k, int64_t k_row_stride,
-                     int64_t k_head_stride, void *v, int64_t v_row_stride, int64_t v_head_stride, void *stream)
+int qb200_cache_read(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const qb200_lanes_t *k, const qb200_lanes_t *v, void *stream)
 {
     int rc = check_cache(cache, sequences, type);
     if (rc) return rc;
-    if (k && (rc = check_lanes("k", type, k, k_row_stride, k_head_stride, sequences->rows, cache->heads))) return rc;
-    if (v && (rc = check_lanes("v", type, v, v_row_stride, v_head_stride, sequences->rows, cache->heads))) return rc;
     if (!k && !v) return fail(QB200_E_POINTER, "neither k nor v is asked for");
+    if (k && (rc = check_lanes("k", type, *k, sequences->rows, cache->heads))) return rc;
+    if (v && (rc = check_lanes("v", type, *v, sequences->rows, cache->heads))) return rc;
     OnDevice on;
     if (!g_ready) return fail(QB200_E_DEVICE, "qb200_init has not succeeded");
     if (on.e) return cuda_fail(on.e, "cudaSetDevice");
-    return finish_other(qb::cache_read(*cache, *sequences, type, {k, k_row_stride, k_head_stride}, {v, v_row_stride, v_head_stride}, (cudaStream_t)stream),
-                        "cache_read", stream);
+    const qb200_lanes_t none = { nullptr, 0, 0 };
+    return finish_other(qb::cache_read(*cache, *sequences, type, k ? *k : none, v ? *v : none, (cudaStream_t)stream), "cache_read", stream);
 }
 
 // The bounds a caller leaves open.
-static void attention_bounds(const qb200_cache_t *c, const qb200_sequences_t *s, int &max_queries, int &max_length)
+static void attention_bounds(const qb200_cache_t &c, const qb200_sequences_t &s, qb200_attention_t &a)
 {
-    const int rows = s->offsets ? s->rows : 1, most = s->width * c->page;
-    if (max_queries <= 0 || max_queries > rows) max_queries = rows > 0 ? rows : 1;
-    if (max_length <= 0 || max_length > most) max_length = most > 0 ? most : 1;
+    const int rows = s.offsets ? s.rows : 1;
+    const int64_t most = (int64_t)s.width * c.page;
+    if (a.max_queries <= 0 || a.max_queries > rows) a.max_queries = rows > 0 ? rows : 1;
+    if (a.max_length <= 0 || a.max_length > most) a.max_length = most > 0 ? (int)most : 1;
 }
 
-size_t qb200_cache_attention_workspace_bytes(const qb200_cache_t *cache, int type, int count, int rows, int q_heads, int max_queries, int max_length)
+size_t qb200_cache_attention_workspace_bytes(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const qb200_attention_t *attention)
 {
-    if (!cache || cache->heads <= 0 || q_heads <= 0 || q_heads % cache->heads || cache->dim <= 0 || cache->dim > 256 || count < 0 || rows < 0) return 0;
-    if (max_queries <= 0 || max_queries > rows) max_queries = rows > 0 ? rows : 1;
-    return qb::attend_workspace_bytes(cache->dim, cache->heads, type, count, rows, q_heads, max_queries, max_length);
+    if (!attention || check_cache(cache, sequences, type) || attention->q_heads <= 0 || attention->q_heads % cache->heads) return 0;
+    qb200_attention_t a = *attention;
+    attention_bounds(*cache, *sequences, a);
+    return qb::attend_workspace_bytes(*cache, *sequences, a);
 }
 
-int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const void *q, int64_t q_row_stride,
-                          int64_t q_head_stride, void *out, int64_t out_row_stride, int64_t out_head_stride, float *lse, int q_heads,
-                          int max_queries, int max_length, float scale, int causal, int window, void *workspace, size_t workspace_bytes,
-                          void *stream)
+int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const qb200_attention_t *attention, void *stream)
 {
     int rc = check_cache(cache, sequences, type);
     if (rc) return rc;
-    if (q_heads <= 0 || q_heads % cache->heads) return fail(QB200_E_SHAPE, "%d query heads over %d heads of the cache: a whole group each", q_heads, cache->heads);
-    if ((int64_t)q_heads * sequences->rows > 2147483647LL - 65536) return fail(QB200_E_LIMIT, "%d rows x %d heads: at most 2^31 - 65537", sequences->rows, q_heads);
-    if ((rc = check_lanes("q", type, q, q_row_stride, q_head_stride, sequences->rows, q_heads))) return rc;
-    if ((rc = check_lanes("out", type, out, out_row_stride, out_head_stride, sequences->rows, q_heads))) return rc;
-    if ((uintptr_t)lse & 3) return fail(QB200_E_POINTER, "misaligned lse");
-    if (window < 0 || (window > 0 && !causal)) return fail(QB200_E_SHAPE, "window %d: a window looks back from a row's own token, so it needs causal", window);
-    if (!(scale == scale) || scale - scale != 0.f) return fail(QB200_E_SHAPE, "scale is not a finite number");
-    if (max_queries < 0 || max_length < 0) return fail(QB200_E_SHAPE, "max_queries %d, max_length %d", max_queries, max_length);
-    attention_bounds(cache, sequences, max_queries, max_length);
-    const size_t need = qb::attend_workspace_bytes(cache->dim, cache->heads, type, sequences->count, sequences->rows, q_heads, max_queries, max_length);
-    if (need && (!workspace || workspace_bytes < need)) return fail(QB200_E_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
-    if ((uintptr_t)workspace & 15) return fail(QB200_E_WORKSPACE, "workspace not 16-byte aligned");
+    if (!attention) return fail(QB200_E_POINTER, "null attention");
+    qb200_attention_t a = *attention;
+    if (a.q_heads <= 0 || a.q_heads % cache->heads) return fail(QB200_E_SHAPE, "%d query heads over %d heads of the cache: a whole group each", a.q_heads, cache->heads);
+    if ((int64_t)a.q_heads * sequences->rows > 2147483647LL - 65536) return fail(QB200_E_LIMIT, "%d rows x %d heads: at most 2^31 - 65537", sequences->rows, a.q_heads);
+    if ((rc = check_lanes("q", type, a.q, sequences->rows, a.q_heads)) || (rc = check_lanes("out", type, a.out, sequences->rows, a.q_heads))) return rc;
+    if ((uintptr_t)a.lse & 3) return fail(QB200_E_POINTER, "misaligned lse");
+    if (a.window < 0 || (a.window > 0 && !a.causal)) return fail(QB200_E_SHAPE, "window %d: a window looks back from a row's own token, so it needs causal", a.window);
+    if (!(a.scale == a.scale) || a.scale - a.scale != 0.f) return fail(QB200_E_SHAPE, "scale is not a finite number");
+    if (a.max_queries < 0 || a.max_length < 0) return fail(QB200_E_SHAPE, "max_queries %d, max_length %d", a.max_queries, a.max_length);
+    attention_bounds(*cache, *sequences, a);
+    const size_t need = qb::attend_workspace_bytes(*cache, *sequences, a);
+    if (need && (!a.workspace || a.workspace_bytes < need))
+        return fail(QB200_E_WORKSPACE, "workspace of %zu bytes, %zu needed", a.workspace ? a.workspace_bytes : (size_t)0, need);
+    if ((uintptr_t)a.workspace & 15) return fail(QB200_E_WORKSPACE, "workspace not 16-byte aligned");
     OnDevice on;
     if (!g_ready) return fail(QB200_E_DEVICE, "qb200_init has not succeeded");
     if (on.e) return cuda_fail(on.e, "cudaSetDevice");
-    qb::AttendCall call = { *cache, *sequences, {const_cast<void *>(q), q_row_stride, q_head_stride}, {out, out_row_stride, out_head_stride}, lse,
-                            type, q_heads, max_queries, max_length, causal != 0, window, scale, workspace };
-    return finish_other(qb::attend(call, (cudaStream_t)stream), "cache_attention", stream);
+    return finish_other(qb::attend(*cache, *sequences, type, a, (cudaStream_t)stream), "cache_attention", stream);
 }
 
 int qb200_shard_range(int rows, int world, int rank, int *first, int *count)

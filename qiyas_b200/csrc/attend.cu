@@ -36,21 +36,20 @@ struct Plan {
     bool whole;                // no unit is cut: units are short, and cutting them would cost a second launch
 };
 
-static Plan plan_of(int dim, int heads, int group, int count, int max_queries, int max_length)
+static Plan plan_of(const qb200_cache_t &c, const qb200_sequences_t &s, const qb200_attention_t &a)
 {
-    const int64_t rows = (int64_t)group * max_queries;
+    const int64_t rows = (int64_t)(a.q_heads / c.heads) * a.max_queries;
     Plan plan;
     plan.tiles = rows > 16;
-    plan.r = plan.tiles ? (dim <= 128 ? 256 : 128) : dim <= 128 && rows > 8 ? 16 : 8;
-    plan.whole = !plan.tiles && max_length <= 1024 && (int64_t)count * heads * rows < 1 << 30;
+    plan.r = plan.tiles ? (c.dim <= 128 ? 256 : 128) : c.dim <= 128 && rows > 8 ? 16 : 8;
+    plan.whole = !plan.tiles && a.max_length <= 1024 && (int64_t)s.count * c.heads * rows < 1 << 30;
     return plan;
 }
 
-size_t attend_workspace_bytes(int dim, int heads, int type, int count, int rows, int q_heads, int max_queries, int max_length)
+size_t attend_workspace_bytes(const qb200_cache_t &c, const qb200_sequences_t &s, const qb200_attention_t &a)
 {
-    (void)type; (void)rows;
-    const Plan plan = plan_of(dim, heads, q_heads / heads, count, max_queries, max_length);
-    return plan.whole ? 0 : (size_t)g_attend_sms * 2 * part_floats(plan.r, dim) * 4;
+    const Plan plan = plan_of(c, s, a);
+    return plan.whole ? 0 : (size_t)g_attend_sms * 2 * part_floats(plan.r, c.dim) * 4;
 }
 
 // The codes as rows of dim bytes, fetched box_rows tokens and box_dim dims at a time (zeros past dim).
@@ -63,13 +62,12 @@ static bool codes_map(CUtensorMap &map, const void *codes, const qb200_cache_t &
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int attend(const AttendCall &call, cudaStream_t stream)
+int attend(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const qb200_attention_t &call, cudaStream_t stream)
 {
-    if (call.seq.count == 0 || call.seq.rows == 0) return 0;
-    const qb200_cache_t &c = call.cache;
-    const int size = call.type == QB200_F32 ? 4 : 2;
+    if (s.count == 0 || s.rows == 0) return 0;
+    const int size = type == QB200_F32 ? 4 : 2;
     AttendArgs a;
-    a.seq = call.seq;
+    a.seq = s;
     a.q = call.q;
     a.out = call.out;
     a.lse = call.lse;
@@ -84,26 +82,26 @@ int attend(const AttendCall &call, cudaStream_t stream)
     a.group = call.q_heads / c.heads;
     a.q_heads = call.q_heads;
     int log_group = 0;
-    while ((1 << log_group) < a.group) log_group++;
+    while (((int64_t)1 << log_group) < a.group) log_group++;
     a.group_shift = 31 + log_group;
     a.group_magic = (uint32_t)((((uint64_t)1 << a.group_shift) + a.group - 1) / a.group);
-    a.causal = call.causal;
+    a.causal = call.causal != 0;
     a.window = call.window;
     a.scale = call.scale;
-    a.q_wide = ((uintptr_t)call.q.base & 15) == 0 && call.q.row * size % 16 == 0 && call.q.head * size % 16 == 0;
-    a.out_wide = ((uintptr_t)call.out.base & (4 * size - 1)) == 0 && call.out.row % 4 == 0 && call.out.head % 4 == 0;
+    a.q_wide = ((uintptr_t)call.q.base & 15) == 0 && call.q.row_stride * size % 16 == 0 && call.q.head_stride * size % 16 == 0;
+    a.out_wide = ((uintptr_t)call.out.base & (4 * size - 1)) == 0 && call.out.row_stride % 4 == 0 && call.out.head_stride % 4 == 0;
     a.workspace = call.workspace;
     a.status = g_attend_status;
-    const Plan plan = plan_of(c.dim, c.heads, a.group, call.seq.count, call.max_queries, call.max_length);
+    const Plan plan = plan_of(c, s, call);
     a.chunks = (int)(((int64_t)a.group * call.max_queries + plan.r - 1) / plan.r);
     a.whole = plan.whole;
-    const int64_t units = (int64_t)call.seq.count * c.heads * a.chunks;
+    const int64_t units = (int64_t)s.count * c.heads * a.chunks;
     a.grid = plan.whole ? (int)(units < 1 << 20 ? units : 1 << 20) : g_attend_sms;
-    if (plan.tiles) return attend_tiles(a, call.type, stream);
+    if (plan.tiles) return attend_tiles(a, type, stream);
     CUtensorMap kmap, vmap;
     const int box = c.dim <= 64 ? 64 : 128, rows = c.page < 32 ? c.page : 32;
     if (!codes_map(kmap, c.k_codes, c, box, rows) || !codes_map(vmap, c.v_codes, c, box, rows)) return (int)cudaErrorInvalidValue;
-    return attend_rows(a, call.type, plan.r, kmap, vmap, stream);
+    return attend_rows(a, type, plan.r, kmap, vmap, stream);
 }
 
 }  // namespace qb

@@ -19,7 +19,7 @@ __host__ __device__ constexpr int unit_pad(int tt) { return tt == 32 ? 8 : 4; }
 
 struct AttendArgs {
     qb200_sequences_t seq;
-    Lanes q, out;
+    qb200_lanes_t q, out;
     float *lse;
     const int8_t *k_codes, *v_codes;
     const float *k_scales, *v_scales;
@@ -434,13 +434,13 @@ template <typename T>
 __device__ __forceinline__ T *out_row(const AttendArgs &p, const Unit &u, int at)
 {
     const int token = by_group(p, at);
-    return (T *)p.out.base + (int64_t)(u.row + token) * p.out.row + (int64_t)(u.h * p.group + at - token * p.group) * p.out.head;
+    return (T *)p.out.base + (int64_t)(u.row + token) * p.out.row_stride + (int64_t)(u.h * p.group + at - token * p.group) * p.out.head_stride;
 }
 template <typename T>
 __device__ __forceinline__ const T *q_row(const AttendArgs &p, const Unit &u, int at)
 {
     const int token = by_group(p, at);
-    return (const T *)p.q.base + (int64_t)(u.row + token) * p.q.row + (int64_t)(u.h * p.group + at - token * p.group) * p.q.head;
+    return (const T *)p.q.base + (int64_t)(u.row + token) * p.q.row_stride + (int64_t)(u.h * p.group + at - token * p.group) * p.q.head_stride;
 }
 __device__ __forceinline__ void store_lse(const AttendArgs &p, const Unit &u, int at, float m, float sum)
 {

@@ -18,7 +18,7 @@ namespace qb {
 static int *g_cache_status = nullptr;
 
 struct CacheArgs {
-    Lanes lanes[2];
+    qb200_lanes_t lanes[2];
     int8_t *codes[2];
     float *scales[2];
     qb200_sequences_t seq;
@@ -143,8 +143,8 @@ __global__ void __launch_bounds__(item_threads(LANES)) cache_write_kernel(const 
     if (it.page < 0) return;                       // uniform over the group; with one group a block, over the block
     const int head = blockIdx.y, kv = blockIdx.z;
     const int vecs = p.dim >> 3, total = it.count * vecs;
-    const T *src = (const T *)p.lanes[kv].base + (int64_t)it.row * p.lanes[kv].row + (int64_t)head * p.lanes[kv].head;
-    const int64_t stride = p.lanes[kv].row;
+    const T *src = (const T *)p.lanes[kv].base + (int64_t)it.row * p.lanes[kv].row_stride + (int64_t)head * p.lanes[kv].head_stride;
+    const int64_t stride = p.lanes[kv].row_stride;
     const bool wide = (p.wide >> kv) & 1;
     const int64_t block = (int64_t)it.page * p.heads + head;
     int8_t *codes = p.codes[kv] + (block << p.log_page) * p.dim;
@@ -256,8 +256,8 @@ __global__ void __launch_bounds__(item_threads(LANES)) cache_read_kernel(const _
     const int64_t block = (int64_t)it.page * p.heads + head;
     const uint2 *src = (const uint2 *)(p.codes[kv] + (block << p.log_page) * p.dim + it.first * p.dim);
     const float scale = p.scales[kv][block];
-    T *dst = (T *)p.lanes[kv].base + (int64_t)it.row * p.lanes[kv].row + (int64_t)head * p.lanes[kv].head;
-    const int64_t stride = p.lanes[kv].row;
+    T *dst = (T *)p.lanes[kv].base + (int64_t)it.row * p.lanes[kv].row_stride + (int64_t)head * p.lanes[kv].head_stride;
+    const int64_t stride = p.lanes[kv].row_stride;
     const bool wide = (p.wide >> kv) & 1;
     uint2 c[NV];
 #pragma unroll
@@ -283,7 +283,7 @@ cudaError_t cache_init(int *status)
     return cudaSuccess;
 }
 
-static CacheArgs args_of(const qb200_cache_t &c, const qb200_sequences_t &s, int size, const Lanes &k, const Lanes &v)
+static CacheArgs args_of(const qb200_cache_t &c, const qb200_sequences_t &s, int size, const qb200_lanes_t &k, const qb200_lanes_t &v)
 {
     CacheArgs p;
     p.lanes[0] = k;
@@ -301,7 +301,7 @@ static CacheArgs args_of(const qb200_cache_t &c, const qb200_sequences_t &s, int
     p.items = s.offsets ? s.rows / c.page + 2 * s.count : s.count;
     p.wide = 0;
     for (int i = 0; i < 2; i++)
-        if (((uintptr_t)p.lanes[i].base & 15) == 0 && p.lanes[i].row * size % 16 == 0 && p.lanes[i].head * size % 16 == 0) p.wide |= 1 << i;
+        if (((uintptr_t)p.lanes[i].base & 15) == 0 && p.lanes[i].row_stride * size % 16 == 0 && p.lanes[i].head_stride * size % 16 == 0) p.wide |= 1 << i;
     p.status = g_cache_status;
     return p;
 }
@@ -335,12 +335,12 @@ static int dispatch(bool write, int type, const CacheArgs &p, cudaStream_t strea
     return run<__nv_bfloat16>(write, p, stream);
 }
 
-int cache_write(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const Lanes &k, const Lanes &v, cudaStream_t stream)
+int cache_write(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const qb200_lanes_t &k, const qb200_lanes_t &v, cudaStream_t stream)
 {
     return dispatch(true, type, args_of(c, s, type == QB200_F32 ? 4 : 2, k, v), stream);
 }
 
-int cache_read(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const Lanes &k, const Lanes &v, cudaStream_t stream)
+int cache_read(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const qb200_lanes_t &k, const qb200_lanes_t &v, cudaStream_t stream)
 {
     return dispatch(false, type, args_of(c, s, type == QB200_F32 ? 4 : 2, k, v), stream);
 }

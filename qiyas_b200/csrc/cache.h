@@ -15,26 +15,14 @@ constexpr int STATUS_ATTEND_WAIT = 8;
 constexpr int STATUS_CACHE_RANGE = 16;
 constexpr int STATUS_CACHE_VALUE = 32;
 
-struct Lanes {                  // element (row, head, i) at base + row * row + head * head + i
-    void *base;
-    int64_t row, head;
-};
-
 cudaError_t cache_init(int *status);
-int cache_write(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const Lanes &k, const Lanes &v, cudaStream_t stream);
-int cache_read(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const Lanes &k, const Lanes &v, cudaStream_t stream);
+int cache_write(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const qb200_lanes_t &k, const qb200_lanes_t &v, cudaStream_t stream);
+// either of k and v may have no base
+int cache_read(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const qb200_lanes_t &k, const qb200_lanes_t &v, cudaStream_t stream);
 
-struct AttendCall {
-    qb200_cache_t cache;
-    qb200_sequences_t seq;
-    Lanes q, out;
-    float *lse;
-    int type, q_heads, max_queries, max_length, causal, window;
-    float scale;
-    void *workspace;
-};
+// max_queries and max_length have been given values
 cudaError_t attend_init(int sm_count, int max_smem, int *status);
-size_t attend_workspace_bytes(int dim, int heads, int type, int count, int rows, int q_heads, int max_queries, int max_length);
-int attend(const AttendCall &call, cudaStream_t stream);
+size_t attend_workspace_bytes(const qb200_cache_t &c, const qb200_sequences_t &s, const qb200_attention_t &a);
+int attend(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const qb200_attention_t &a, cudaStream_t stream);
 
 }  // namespace qb

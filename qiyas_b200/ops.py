@@ -19,7 +19,16 @@ from .blocks import BF16, BLOCK_VALUES, F16, F32, NAMES, Q4_0, Q8_0, fmt_id, nby
 OP_GEMV, OP_MATMUL, OP_CACHE, OP_ATTENTION = 0, 1, 2, 3
 
 
-_LANES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+_kinds = {}
+
+
+def _lane_kinds():
+    """Lane types by torch's: filled on first use, since importing this module needs no torch."""
+    if not _kinds:
+        import torch
+        _kinds.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+        _kinds["i32"] = torch.int32
+    return _kinds
 
 
 @dataclass(frozen=True)
@@ -256,29 +265,34 @@ class GpuOps:
         """Quantises the rows of k and v ([rows, heads, dim], f32, f16 or bf16) into `cache` as tokens lengths[b], lengths[b] + 1,
         ... of their sequences.  table: int32 [sequences, width] of pages; lengths: int32, tokens already there; offsets: int32
         [sequences + 1], the rows of each sequence (None: one row each).  All on the device; nothing is synchronised."""
-        kind, rows, *at = self._lanes(cache, k, "k", cache.heads)
-        other, same, *v_at = self._lanes(cache, v, "v", cache.heads)
+        kind, rows, base, row, head = self._lanes(cache, k, "k", cache.heads)
+        other, same, v_base, v_row, v_head = self._lanes(cache, v, "v", cache.heads)
         if other != kind or same != rows:
             raise ValueError("k and v have the same rows and type")
-        seq = self._sequences(cache, table, lengths, offsets, rows)
-        self.gpu.check(self.lib.qb200_cache_write(cache.parts, seq, kind, *at, *v_at, _stream(stream)), "CacheWrite")
+        rc = self.lib.qb200_cache_write(cache.parts, self._sequences(cache, table, lengths, offsets, rows), kind, _lib.LANES(base, row, head),
+                                        _lib.LANES(v_base, v_row, v_head), _stream(stream))
+        if rc:
+            self.gpu.check(rc, "CacheWrite")
         return "s8 cache blocks"
 
     def CacheRead(self, cache, k, v, table, starts, offsets=None, stream=None):
         """Reads tokens starts[b], starts[b] + 1, ... of the sequences back into the rows of k and v (either may be None)."""
         if k is None and v is None:
             raise ValueError("neither k nor v is asked for")
-        kind, rows, *at = self._lanes(cache, v if k is None else k, "v" if k is None else "k", cache.heads)
+        kind, rows, base, row, head = self._lanes(cache, v if k is None else k, "v" if k is None else "k", cache.heads)
+        at = v_at = _lib.LANES(base, row, head)
         if k is None:
-            at, v_at = (None, 0, 0), at
+            at = None
         elif v is None:
-            v_at = (None, 0, 0)
+            v_at = None
         else:
-            other, same, *v_at = self._lanes(cache, v, "v", cache.heads)
+            other, same, base, row, head = self._lanes(cache, v, "v", cache.heads)
             if other != kind or same != rows:
                 raise ValueError("k and v have the same rows and type")
-        seq = self._sequences(cache, table, starts, offsets, rows)
-        self.gpu.check(self.lib.qb200_cache_read(cache.parts, seq, kind, *at, *v_at, _stream(stream)), "CacheRead")
+            v_at = _lib.LANES(base, row, head)
+        rc = self.lib.qb200_cache_read(cache.parts, self._sequences(cache, table, starts, offsets, rows), kind, at, v_at, _stream(stream))
+        if rc:
+            self.gpu.check(rc, "CacheRead")
         return "s8 cache blocks"
 
     def CacheAttention(self, cache, q, out, table, lengths, offsets=None, max_queries=0, max_length=0, scale=None, causal=True, window=0,
@@ -289,29 +303,33 @@ class GpuOps:
         lengths, known to the host, for the choice of kernel (0: rows, or 1 without offsets; all the table holds).  scale None:
         1 / sqrt(dim).  workspace None: one of the call's own, from torch's allocator on the call's stream."""
         heads = q.shape[1] if q.dim() == 3 else 0
-        kind, rows, *at = self._lanes(cache, q, "q", heads)
-        other, same, *out_at = self._lanes(cache, out, "out", heads)
+        kind, rows, base, row, head = self._lanes(cache, q, "q", heads)
+        other, same, out_base, out_row, out_head = self._lanes(cache, out, "out", heads)
         if other != kind or same != rows:
             raise ValueError("q and out have the same shape and type")
         seq = self._sequences(cache, table, lengths, offsets, rows)
-        lse_at = None
+        lse_at = 0
         if lse is not None:
-            if str(lse.dtype) != "torch.float32" or tuple(lse.shape) != (rows, heads) or not lse.is_contiguous() or lse.get_device() != cache.index:
+            if _lane_kinds().get(lse.dtype) != F32 or lse.shape != (rows, heads) or not lse.is_contiguous() or lse.get_device() != cache.index:
                 raise ValueError(f"lse: contiguous float32 {(rows, heads)} on the cache's device")
             lse_at = lse.data_ptr()
-        if workspace is None:
-            workspace_bytes = self.lib.qb200_cache_attention_workspace_bytes(cache.parts, kind, seq.count, rows if offsets is not None else 1, heads,
-                                                                             max_queries, max_length or seq.width * cache.page)
-            if workspace_bytes:
-                workspace = self._scratch_on(stream, workspace_bytes)
-        self.gpu.check(self.lib.qb200_cache_attention(cache.parts, seq, kind, *at, *out_at, lse_at, heads, max_queries, max_length,
-                                                      cache.dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, _ptr(workspace),
-                                                      workspace_bytes, _stream(stream)), "CacheAttention")
-        return self.lib.qb200_lane_name(OP_ATTENTION, kind).decode()
+        scale = cache.dim ** -0.5 if scale is None else scale
+        workspace = _ptr(workspace) or 0
+        rest = (heads, max_queries, max_length, scale, 1 if causal else 0, window)
+        args = _lib.ATTENTION(base, row, head, out_base, out_row, out_head, lse_at, workspace, workspace_bytes, *rest)
+        if not workspace:
+            need = self.lib.qb200_cache_attention_workspace_bytes(cache.parts, seq, kind, args)
+            if need:
+                held = self._scratch_on(stream, need)          # until the call is in its stream
+                args = _lib.ATTENTION(base, row, head, out_base, out_row, out_head, lse_at, held.data_ptr(), need, *rest)
+        rc = self.lib.qb200_cache_attention(cache.parts, seq, kind, args, _stream(stream))
+        if rc:
+            self.gpu.check(rc, "CacheAttention")
+        return "f16 mma cache blocks"
 
     def _lanes(self, cache, t, name, heads):
         """Rows [rows, heads, dim] of a cache operator as the C ABI takes them: (lane type, rows, address, row stride, head stride)."""
-        kind = _LANES.get(str(t.dtype))
+        kind = _lane_kinds().get(t.dtype)
         if kind is None:
             raise NotImplementedError(f"{name}: {t.dtype}; rows are float32, float16 or bfloat16")
         shape, strides = t.shape, t.stride()
@@ -324,15 +342,21 @@ class GpuOps:
         return kind, shape[0], t.data_ptr(), strides[0], strides[1]
 
     def _sequences(self, cache, table, lengths, offsets, rows):
-        shape, counts = table.shape, lengths.shape
-        if len(counts) != 1 or len(shape) != 2 or shape[0] != counts[0]:
-            raise ValueError(f"table [sequences, width] and lengths [sequences]: got {tuple(shape)}, {tuple(counts)}")
-        if offsets is not None and tuple(offsets.shape) != (counts[0] + 1,):
-            raise ValueError(f"offsets: [{counts[0] + 1}], got {tuple(offsets.shape)}")
-        for t in (table, lengths) if offsets is None else (table, lengths, offsets):
-            if str(t.dtype) != "torch.int32" or not t.is_contiguous() or t.get_device() != cache.index:
-                raise ValueError(f"table, lengths and offsets are contiguous int32 on the cache's device: got {t.dtype} on {t.device}, strides {t.stride()}")
-        return _lib.Sequences(table.data_ptr(), lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), counts[0], shape[1], rows)
+        if lengths.dim() != 1 or table.dim() != 2 or table.shape[0] != lengths.shape[0]:
+            raise ValueError(f"table [sequences, width] and lengths [sequences]: got {tuple(table.shape)}, {tuple(lengths.shape)}")
+        count, width = table.shape
+        index, i32 = cache.index, _lane_kinds()["i32"]
+        at = 0
+        good = table.dtype is lengths.dtype is i32 and table.is_contiguous() and lengths.is_contiguous() and table.get_device() == lengths.get_device() == index
+        if offsets is not None:
+            if offsets.shape != (count + 1,):
+                raise ValueError(f"offsets: [{count + 1}], got {tuple(offsets.shape)}")
+            good = good and offsets.dtype is i32 and offsets.is_contiguous() and offsets.get_device() == index
+            at = offsets.data_ptr()
+        if not good:
+            raise ValueError("table, lengths and offsets are contiguous int32 on the cache's device: got " +
+                             ", ".join(f"{t.dtype} {t.stride()} on {t.device}" for t in (table, lengths, offsets) if t is not None))
+        return _lib.SEQUENCES(table.data_ptr(), lengths.data_ptr(), at, count, width, rows)
 
     def _scratch_on(self, stream, nbytes_):
         """A buffer of torch's allocator that belongs to `stream`: freed in its order, and the graph's own under capture."""

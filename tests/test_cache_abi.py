@@ -19,37 +19,43 @@ def parts(**change):
     from qiyas_b200 import _lib
     want = dict(k_codes=256, v_codes=512, k_scales=1024, v_scales=2048, pages=4, heads=2, page=16, dim=64)
     want.update(change)
-    return _lib.CacheParts(**want)
+    return _lib.CACHE(*want.values())
 
 
 def sequences(**change):
     from qiyas_b200 import _lib
     want = dict(table=256, lengths=512, offsets=1024, count=3, width=2, rows=9)
     want.update(change)
-    return _lib.Sequences(**want)
+    return _lib.SEQUENCES(*want.values())
+
+
+def lanes(base=256, row=128, head=64):
+    from qiyas_b200 import _lib
+    return _lib.LANES(base, row, head)
 
 
 def write(lib, cache=None, seq=None, kind=B.F16, k=256, row=128, head=64, v=256):
-    return lib.qb200_cache_write(cache or parts(), seq or sequences(), kind, k, row, head, v, row, head, None)
+    return lib.qb200_cache_write(cache or parts(), seq or sequences(), kind, lanes(k, row, head), lanes(v, row, head), None)
 
 
-def attention(lib, cache=None, seq=None, kind=B.F16, q=256, row=512, head=64, out=256, lse=None, heads=8, max_queries=0, max_length=0, scale=0.125, causal=1,
+def attention(lib, cache=None, seq=None, kind=B.F16, q=256, row=512, head=64, out=256, lse=0, heads=8, max_queries=0, max_length=0, scale=0.125, causal=1,
               window=0, workspace=4096, size=1 << 40):
-    return lib.qb200_cache_attention(cache or parts(), seq or sequences(), kind, q, row, head, out, row, head, lse, heads, max_queries, max_length, scale,
-                                     causal, window, workspace, size, None)
+    from qiyas_b200 import _lib
+    args = _lib.ATTENTION(q, row, head, out, row, head, lse, workspace, size, heads, max_queries, max_length, scale, causal, window)
+    return lib.qb200_cache_attention(cache or parts(), seq or sequences(), kind, args, None)
 
 
 CACHES = [(dict(page=8), SHAPE), (dict(page=48), SHAPE), (dict(dim=24), SHAPE), (dict(dim=272), SHAPE), (dict(dim=0), SHAPE), (dict(pages=0), SHAPE),
-          (dict(heads=-1), SHAPE), (dict(heads=70000), LIMIT), (dict(pages=2 ** 30), LIMIT), (dict(k_codes=None), POINTER), (dict(v_scales=None), POINTER),
+          (dict(heads=-1), SHAPE), (dict(heads=70000), LIMIT), (dict(pages=2 ** 30), LIMIT), (dict(k_codes=0), POINTER), (dict(v_scales=0), POINTER),
           (dict(k_codes=264), POINTER), (dict(v_scales=1026), POINTER)]
 SEQUENCES = [(dict(count=-1), SHAPE), (dict(width=-1), SHAPE), (dict(rows=-1), SHAPE), (dict(width=2 ** 28), LIMIT), (dict(count=2 ** 25, rows=2 ** 26), LIMIT),
-             (dict(offsets=None, rows=2), SHAPE), (dict(lengths=None), POINTER), (dict(table=None), POINTER), (dict(table=258), POINTER), (dict(offsets=1025), POINTER)]
+             (dict(offsets=0, rows=2), SHAPE), (dict(lengths=0), POINTER), (dict(table=0), POINTER), (dict(table=258), POINTER), (dict(offsets=1025), POINTER)]
 
 
 @pytest.mark.parametrize("change,code", CACHES)
 def test_caches_that_are_refused(lib, change, code):
     assert write(lib, cache=parts(**change)) == code
-    assert attention(lib, cache=parts(**change), heads=max(1, parts(**change).heads) * 2) == code
+    assert attention(lib, cache=parts(**change), heads=max(1, change.get("heads", 2)) * 2) == code
     assert lib.qb200_last_error()
 
 
@@ -57,19 +63,21 @@ def test_caches_that_are_refused(lib, change, code):
 def test_sequences_that_are_refused(lib, change, code):
     assert write(lib, seq=sequences(**change)) == code
     assert attention(lib, seq=sequences(**change)) == code
-    assert lib.qb200_cache_read(parts(), sequences(**change), B.F16, 256, 128, 64, 256, 128, 64, None) == code
+    assert lib.qb200_cache_read(parts(), sequences(**change), B.F16, lanes(), lanes(), None) == code
 
 
 def test_rows_that_are_refused(lib):
     assert write(lib, kind=B.Q8_0) == FORMAT
-    assert write(lib, k=None) == POINTER
+    assert write(lib, k=0) == POINTER
     assert write(lib, v=257) == POINTER
     assert write(lib, kind=B.F32, k=258) == POINTER
     assert write(lib, row=-1) == SHAPE
     assert write(lib, head=1 << 60) == SHAPE
-    assert lib.qb200_cache_read(parts(), sequences(), B.F16, None, 0, 0, None, 0, 0, None) == POINTER
-    assert lib.qb200_cache_write(None, sequences(), B.F16, 256, 1, 1, 256, 1, 1, None) == POINTER
-    assert lib.qb200_cache_write(parts(), None, B.F16, 256, 1, 1, 256, 1, 1, None) == POINTER
+    assert lib.qb200_cache_read(parts(), sequences(), B.F16, None, None, None) == POINTER
+    assert lib.qb200_cache_write(None, sequences(), B.F16, lanes(), lanes(), None) == POINTER
+    assert lib.qb200_cache_write(parts(), None, B.F16, lanes(), lanes(), None) == POINTER
+    assert lib.qb200_cache_write(parts(), sequences(), B.F16, lanes(), None, None) == POINTER
+    assert lib.qb200_cache_attention(parts(), sequences(), B.F16, None, None) == POINTER
 
 
 def test_attention_refuses(lib):
@@ -82,7 +90,7 @@ def test_attention_refuses(lib):
     assert attention(lib, max_queries=-1) == SHAPE
     assert attention(lib, max_length=-1) == SHAPE
     assert attention(lib, lse=1026) == POINTER
-    assert attention(lib, q=None) == POINTER
+    assert attention(lib, q=0) == POINTER
     assert attention(lib, kind=B.BF16, out=257) == POINTER
     assert attention(lib, kind=100 + 7) == FORMAT
     assert attention(lib, seq=sequences(rows=2 ** 30), heads=8) == LIMIT
@@ -94,7 +102,7 @@ def test_a_good_call_needs_a_device(lib):
     if torch.cuda.is_available():
         pytest.skip("a device is present")
     assert write(lib) == DEVICE
-    assert lib.qb200_cache_read(parts(), sequences(), B.F32, 256, 128, 64, None, 0, 0, None) == DEVICE
+    assert lib.qb200_cache_read(parts(), sequences(), B.F32, lanes(), None, None) == DEVICE
     assert attention(lib) == DEVICE
 
 
@@ -127,3 +135,24 @@ def test_the_mirror_refuses_what_the_abi_cannot_be_told():
                       (table.t(), lengths, None), (table, lengths[None], None), (torch.zeros(3, 4, dtype=torch.int32)[:, ::2], lengths, None)):
         with pytest.raises(ValueError):
             ops._sequences(cache, t, n, off, 3)
+
+
+def test_packed_structures_have_the_headers_sizes():
+    """The header compiled as C: sizes and offsets are those the mirror packs."""
+    import os
+    import subprocess
+    import sys
+    import tempfile
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = """#include <stdio.h>
+#include <stddef.h>
+#include "qiyas_b200.h"
+int main(void) { printf("%zu %zu %zu %zu %zu %zu %zu", sizeof(qb200_cache_t), sizeof(qb200_sequences_t), sizeof(qb200_lanes_t), sizeof(qb200_attention_t),
+ offsetof(qb200_sequences_t, count), offsetof(qb200_attention_t, q_heads), offsetof(qb200_attention_t, scale)); return 0; }"""
+    with tempfile.TemporaryDirectory() as d:
+        with open(os.path.join(d, "a.c"), "w") as f:
+            f.write(text)
+        subprocess.check_call(["gcc", "-I", os.path.join(root, "include"), "-o", os.path.join(d, "a"), os.path.join(d, "a.c")])
+        got = [int(x) for x in subprocess.check_output([os.path.join(d, "a")]).split()]
+    assert sys.maxsize > 2 ** 32
+    assert got == [len(parts()), len(sequences()), len(lanes()), 96, 24, 72, 84]
