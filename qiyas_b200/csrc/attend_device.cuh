@@ -15,7 +15,7 @@ constexpr int LEAST_TOKENS = 256;              // tokens a share has at least
 // What a unit costs a block besides its tiles, in tiles of TT tokens: its rows of q, the join of its sums.  Measured: 3000
 // cycles at 350 a tile in attend_rows.cu (32 tokens a tile), 25000 at 7000 in attend_tiles.cu.  The line of work below
 // counts it, or a block that gets many short sequences ends long after the others.
-__host__ __device__ constexpr int unit_pad(int tt) { return tt == 32 ? 8 : 4; }
+__host__ __device__ constexpr int unit_pad(int tt) { return tt == 32 ? 8 : 10; }
 
 struct AttendArgs {
     qb200_sequences_t seq;

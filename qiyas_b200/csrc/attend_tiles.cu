@@ -8,9 +8,9 @@
 //  * Eight converter warps fetch the codes (16 bytes a load) and store them as f16: K as core matrices of 8 tokens x 8 dims,
 //    V as rows of 64 dims with the 128-byte swizzle, which the second product reads across (a row a dim: MN-major).  Every
 //    byte of the cache is converted once for the 256 rows of a block.
-//  * Two groups of four softmax warps, a thread a row, work on the two row tiles in turn with the tensor pipe: while one
-//    takes exponentials the pipe has the other's products.  With one row tile (NQ 1, or a unit of at most 128 rows) the two
-//    S buffers take the tiles of tokens alternately instead.
+//  * A group of four softmax warps a row tile, a thread a row, with two buffers of S: the tensor pipe is a tile of tokens
+//    ahead, so the chain from a product's end through the barrier, the softmax and the next product's issue is hidden (with
+//    one buffer of 128 tokens a row tile it was not: 7700 cycles for 128 tokens, 2048 of them the tensor pipe's).
 //  * A thread reads its row of S once, 32 tokens at a time, and takes the weights against the exponent it has: only where one
 //    would pass 2^15 does it go back over what the row has of O and of the tile's weights, in place, by a power of two.
 // Scales, exponents and the cut of q and w are those of attend_rows.cu; so are the shares of the grid's blocks.
@@ -25,10 +25,10 @@ constexpr int CW = 8;                          // converter warps: four for K, f
 
 template <int DC, int SPL>
 struct TilesCfg {
-    static constexpr int TT = DC == 128 ? 128 : 64;             // tokens a tile
+    static constexpr int TT = 64;                               // tokens a tile
     static constexpr int NQ = DC == 128 ? 2 : 1;                // row tiles a block
     static constexpr int R = 128 * NQ;
-    static constexpr int SLOTS = SPL == 1 ? 2 : 1;              // of K and of V
+    static constexpr int SLOTS = (SPL == 1 ? 2 : 1) * (DC == 128 ? 2 : 1);      // of K and of V
     static constexpr int NG = TT / 16;
     static constexpr int WARPS = 4 * NQ + CW + 4, THREADS = 32 * WARPS;       // the last four: one issues the products
     // registers a thread: of the launch (65536 over the threads, whole eights), and of the softmax, converter and last warps
@@ -37,13 +37,16 @@ struct TilesCfg {
     static constexpr uint32_t QTILE = 128 * DC * 2, SLOT = TT * DC * 2;
     static constexpr uint32_t O_Q = 0, O_K = NQ * SPL * QTILE, O_V = O_K + SLOTS * SLOT, O_HEAD = O_V + SLOTS * SLOT, SMEM = O_HEAD + 2048 + 1024;
     static_assert(SMEM <= 232448, "227 KB of shared memory");
-    __host__ __device__ static constexpr uint32_t s_col(int b) { return b * TT; }
+    __host__ __device__ static constexpr uint32_t s_col(int t, int b) { return (2 * t + b) * TT; }
     __host__ __device__ static constexpr uint32_t o_col(int t) { return 256 + t * 128; }
 };
 
 struct TilesHead {
     uint64_t qfull, ofull, drain;
-    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], odone[2];
+    uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
+    uint64_t sfull[4], pfull[4], odone[2];     // of the S buffers, two a row tile; of O, one a row tile
+    uint64_t sempty[4];                        // of `scales`
+    float4 scales[4][4];                       // of a tile's groups of 16 tokens: sk, log2(sv / v0), v0 / sv, v0
     Start start;
     uint32_t tmem;
     int abort;
@@ -74,7 +77,7 @@ __device__ __forceinline__ void mma_issue_ts(uint32_t tmem_d, uint32_t tmem_a, u
 template <int R, int TT>
 struct KvTile {
     int b, h, base, lo, hi;
-    bool there;
+    bool there, starts;                        // starts: the first of a piece
 };
 template <int R, int TT>
 struct KvWalk {
@@ -91,6 +94,7 @@ struct KvWalk {
             more = walk.next(piece);
         }
         t.there = more;
+        t.starts = at == 0;
         if (more) {
             t.b = piece.unit.b;
             t.h = piece.unit.h;
@@ -131,6 +135,25 @@ __device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b)
     return d;
 }
 
+// 2^x0, 2^x1 without the exponential unit: x = n + f with |f| <= 1/2, 2^f by its Taylor polynomial of degree 5 (what is
+// left out is below 0.00016 * 2^-6, 4e-6 of the value), n added to the exponent.  Below 2^-120: 2^-120.
+__device__ __forceinline__ void exp2_pair(float x0, float x1, float &e0, float &e1)
+{
+    constexpr float MAGIC = 12582912.f;                        // 1.5 * 2^23: the sum's low bits are the integer
+    const uint64_t x = pair(fmaxf(x0, -120.f), fmaxf(x1, -120.f)), n = pair_add(x, pair(MAGIC, MAGIC));
+    const uint64_t f = pair_fma(pair_add(n, pair(-MAGIC, -MAGIC)), pair(-1.f, -1.f), x);
+    uint64_t y = pair_fma(f, pair(0.0013333558f, 0.0013333558f), pair(0.009618129f, 0.009618129f));
+    y = pair_fma(y, f, pair(0.055504109f, 0.055504109f));
+    y = pair_fma(y, f, pair(0.240226507f, 0.240226507f));
+    y = pair_fma(y, f, pair(0.693147181f, 0.693147181f));
+    y = pair_fma(y, f, pair(1.f, 1.f));
+    float n0, n1, y0, y1;
+    unpair(n, n0, n1);
+    unpair(y, y0, y1);
+    e0 = __int_as_float(__float_as_int(y0) + (__float_as_int(n0) << 23));
+    e1 = __int_as_float(__float_as_int(y1) + (__float_as_int(n1) << 23));
+}
+
 template <int DC, int SPL, typename T>
 __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_kernel(const __grid_constant__ AttendArgs p)
 {
@@ -143,21 +166,22 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
     const uint32_t base_u32 = smem_u32(smem);
     const uint32_t qfull = smem_u32(&head->qfull), ofull = smem_u32(&head->ofull), drain = smem_u32(&head->drain);
     const uint32_t kfull = smem_u32(head->kfull), kempty = smem_u32(head->kempty), vfull = smem_u32(head->vfull), vempty = smem_u32(head->vempty);
-    const uint32_t sfull = smem_u32(head->sfull), pfull = smem_u32(head->pfull), odone = smem_u32(head->odone);
+    const uint32_t sfull = smem_u32(head->sfull), pfull = smem_u32(head->pfull), odone = smem_u32(head->odone), sempty = smem_u32(head->sempty);
 
     if (threadIdx.x == 0) {
         head->abort = 0;
         mbar_init(qfull, 4 * NQ);
-        mbar_init(ofull, 1);
-        mbar_init(drain, 1);
-        for (int i = 0; i < 2; i++) {
-            mbar_init(kfull + 8 * i, 4);
-            mbar_init(kempty + 8 * i, 1);
+        mbar_init(ofull, 2);
+        mbar_init(drain, 2);
+        for (int i = 0; i < 2; i++) mbar_init(odone + 8 * i, 1);
+        for (int i = 0; i < 4; i++) {
+            mbar_init(kfull + 8 * i, 5);           // the converters', and the tile's scales
+            mbar_init(sempty + 8 * i, 2);
+            mbar_init(kempty + 8 * i, 2);
             mbar_init(vfull + 8 * i, 4);
-            mbar_init(vempty + 8 * i, 1);
+            mbar_init(vempty + 8 * i, 2);
             mbar_init(sfull + 8 * i, 1);
             mbar_init(pfull + 8 * i, 4);
-            mbar_init(odone + 8 * i, 1);
         }
         mbar_fence_init();
     }
@@ -181,7 +205,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         Walk<R, TT, false> walk(p, head->start);
         Piece piece;
-        uint32_t pieces = 0, uses0 = 0, uses1 = 0, done = 0;     // uses of the S buffers and of this group's O so far
+        uint32_t pieces = 0, seq = 0, tiles = 0;                 // so far: pieces, tiles of the block, of this row tile
         while (walk.next(piece)) {
             const Unit &u = piece.unit;
             const int nq = NQ == 2 && u.r1 - u.r0 > 128 ? 2 : 1;
@@ -241,135 +265,111 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 int lo, hi;
                 row_limits(p, u, min(at, u.r1 - 1), lo, hi);
                 const int lo_most = __reduce_max_sync(0xffffffffu, lo), hi_least = __reduce_min_sync(0xffffffffu, hi);
-                // a lane a group of 16 tokens: page a tile of tokens ahead of the scales, scales a tile ahead of their use
                 const int first = (u.t0 + piece.first) * TT;
-                auto page_of = [&](int j) { return page_at(p, u.b, first + j * TT + lane * 16, 16, u.lo, u.hi, lane < NG && j < n); };
-                float2 sc = scales_at(p, page_number(p, page_of(0), quarter == 0), u.h);
-                Page page = page_of(1);
                 for (int j = 0; j < n; j++) {
-                    const float2 sc_next = scales_at(p, page_number(p, page, quarter == 0), u.h);
-                    page = page_of(j + 2);
                     const int base = first + j * TT;
-                    const int buf = nq == 2 ? t : j & 1;
-                    const uint32_t use = (buf ? uses1 : uses0) + (nq == 2 ? j : j >> 1);
-                    // V's scales against the first of them
-                    const unsigned some = __ballot_sync(0xffffffffu, sc.y > 0.f);
-                    const float found = __shfl_sync(0xffffffffu, sc.y, some ? __ffs(some) - 1 : 0);
-                    if (vref == 0.f && some) vref = found;
-                    float lr_mine = 0.f, rinv_mine = 1.f;
-                    if (sc.y < 0.f) { lr_mine = -INFINITY; rinv_mine = 0.f; }
-                    else if (sc.y > 0.f && sc.y != vref) { lr_mine = log2_ratio(sc.y, vref); rinv_mine = __fdividef(vref, sc.y); }
+                    const int buf = (tiles + j) & 1;
+                    const uint32_t sbar = sfull + 8 * (2 * t + buf), use = (tiles + j) >> 1;
                     const bool whole = base >= lo_most && base + TT <= hi_least;
-                    const uint32_t s_at = tmem + lanes + C::s_col(buf), o_at = tmem + lanes + C::o_col(t);
-                    if (!mbar_wait_soon_lanes(sfull + 8 * buf, use & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
+                    const uint32_t s_at = tmem + lanes + C::s_col(t, buf), o_at = tmem + lanes + C::o_col(t);
+                    if (!mbar_wait_soon_lanes(sbar, use & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
                     tc_fence_after();
 
-                    uint32_t v[32];
-                    tmem_ld32(s_at, v);
+                    uint32_t v[2][32];
+                    tmem_ld32(s_at, v[0]);
+                    tmem_ld32(s_at + 32, v[1]);
+                    float4 sc[NG];
+#pragma unroll
+                    for (int e = 0; e < NG; e++) sc[e] = head->scales[(seq + j) & 3][e];
+                    vref = sc[NG - 1].w;
+                    tmem_ld_landed32(v[0]);
+                    tmem_ld_landed32(v[1]);
+                    float x[64];                                 // scores, in powers of two against mm
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) {
+                        const float f = factor * sc[i / 16].x, a = sc[i / 16].y - mm;
+                        unpair(pair_fma(pair(__uint_as_float(v[i / 32][i % 32]), __uint_as_float(v[i / 32][i % 32 + 1])), pair(f, f), pair(a, a)), x[i], x[i + 1]);
+                    }
+                    if (!whole) {
+                        const int from = lo - base, to = hi - base;
+#pragma unroll
+                        for (int i = 0; i < 64; i++) x[i] = i >= from && i < to ? x[i] : -INFINITY;
+                    }
+                    float tops[4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        tops[q] = max3(x[16 * q], x[16 * q + 1], x[16 * q + 2]);
+#pragma unroll
+                        for (int i = 3; i < 15; i += 2) tops[q] = max3(tops[q], x[16 * q + i], x[16 * q + i + 1]);
+                        tops[q] = fmaxf(tops[q], x[16 * q + 15]);
+                    }
+                    const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
+                    // seldom: the exponent the weights are taken against goes up, by whole powers of two
+                    const bool above = fresh ? top > -INFINITY : top > 15.f;
+                    if (__any_sync(0xffffffffu, above)) {
+                        float up = 0.f, less = 1.f;
+                        if (above) {
+                            up = ceilf(top) - 7.f;
+                            if (!fresh) less = exp2_fast(-up);
+                            fresh = false;
+                        }
+                        mm += up;
+                        l *= less;
+#pragma unroll
+                        for (int i = 0; i < 64; i++) x[i] -= up;
+                        if (j > 0) {                             // O so far, once the product before has ended
+                            if (!mbar_wait_soon_lanes(odone + 8 * t, (tiles + j - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
+                            tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < TT / 32; c++) {
-                        float x[32];                             // scores, in powers of two against mm
-                        tmem_ld_landed32(v);
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const float f = factor * __shfl_sync(0xffffffffu, sc.x, 2 * c + e), a = __shfl_sync(0xffffffffu, lr_mine, 2 * c + e) - mm;
-                            const uint64_t f2 = pair(f, f), a2 = pair(a, a);
-#pragma unroll
-                            for (int i = 0; i < 16; i += 2)
-                                unpair(pair_fma(pair(__uint_as_float(v[16 * e + i]), __uint_as_float(v[16 * e + i + 1])), f2, a2), x[16 * e + i], x[16 * e + i + 1]);
-                        }
-                        if (c + 1 < TT / 32) tmem_ld32(s_at + 32 * c + 32, v);
-                        if (!whole) {
-#pragma unroll
-                            for (int i = 0; i < 32; i++) {
-                                const int token = base + 32 * c + i;
-                                x[i] = token >= lo && token < hi ? x[i] : -INFINITY;
-                            }
-                        }
-                        float top = max3(x[0], x[1], x[2]), top2 = max3(x[3], x[4], x[5]);
-#pragma unroll
-                        for (int i = 6; i < 30; i += 4) {
-                            top = max3(top, x[i], x[i + 1]);
-                            top2 = max3(top2, x[i + 2], x[i + 3]);
-                        }
-                        top = max3(fmaxf(top, top2), x[30], x[31]);
-                        // seldom: the exponent the weights are taken against goes up, by whole powers of two
-                        const bool above = fresh ? top > -INFINITY : top > 15.f;
-                        if (__any_sync(0xffffffffu, above)) {
-                            float up = 0.f, less = 1.f;
-                            if (above) {
-                                up = ceilf(top) - 7.f;
-                                if (!fresh) less = exp2_fast(-up);
-                                fresh = false;
-                            }
-                            mm += up;
-                            l *= less;
-#pragma unroll
-                            for (int i = 0; i < 32; i++) x[i] -= up;
-                            tmem_st_wait();
-#pragma unroll 1
-                            for (int k = 0; k < c * (SPL == 2 ? 32 : 16); k += 16) {          // this tile's weights so far
+                            for (int d = 0; d < p.dim; d += 16) {
                                 uint32_t w[16];
-                                tmem_ld16(s_at + k, w);
+                                tmem_ld16(o_at + d, w);
                                 tmem_ld_landed16(w);
 #pragma unroll
-                                for (int i = 0; i < 16; i++) {
-                                    const float2 y = __half22float2(*(const __half2 *)&w[i]);
-                                    const __half2 z = __floats2half2_rn(y.x * less, y.y * less);
-                                    w[i] = *(const uint32_t *)&z;
-                                }
-                                tmem_st16(s_at + k, w);
+                                for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__uint_as_float(w[i]) * less);
+                                tmem_st16(o_at + d, w);
                             }
-                            if (j > 0) {                         // O so far, once the product before has ended
-                                if (!mbar_wait_soon_lanes(odone + 8 * t, (done + j - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
-                                tc_fence_after();
-#pragma unroll 1
-                                for (int d = 0; d < p.dim; d += 16) {
-                                    uint32_t w[16];
-                                    tmem_ld16(o_at + d, w);
-                                    tmem_ld_landed16(w);
-#pragma unroll
-                                    for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__uint_as_float(w[i]) * less);
-                                    tmem_st16(o_at + d, w);
-                                }
-                            }
-                            if (c + 1 < TT / 32) tmem_ld_landed32(v);
                         }
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {                // 32 tokens: 16 columns of weights (32: the two f16)
                         uint32_t w[16], w2[16];
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            const float rinv = __shfl_sync(0xffffffffu, rinv_mine, 2 * c + e);
-                            uint64_t sum = 0;
+                            uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                const float e0 = exp2_fast(x[16 * e + i]), e1 = exp2_fast(x[16 * e + i + 1]);
-                                sum = pair_add(sum, pair(e0, e1));
+                            for (int i = 0; i < 16; i += 4) {
+                                const float *y = x + 32 * c + 16 * e + i;
+                                float e0 = exp2_fast(y[0]), e1 = exp2_fast(y[1]), e2, e3;
+                                // a quarter of the exponentials on the fma pipe, where their cut to f16 hides the polynomial's error
+                                if (SPL == 1 && i % 8 == 0) exp2_pair(y[2], y[3], e2, e3);
+                                else { e2 = exp2_fast(y[2]); e3 = exp2_fast(y[3]); }
+                                sum0 = pair_add(sum0, pair(e0, e1));
+                                sum1 = pair_add(sum1, pair(e2, e3));
                                 split2(e0, e1, w[8 * e + i / 2], w2[8 * e + i / 2]);
+                                split2(e2, e3, w[8 * e + i / 2 + 1], w2[8 * e + i / 2 + 1]);
                             }
                             float s0, s1;
-                            unpair(sum, s0, s1);
-                            l = __fmaf_rn(s0 + s1, rinv, l);
+                            unpair(pair_add(sum0, sum1), s0, s1);
+                            l = __fmaf_rn(s0 + s1, sc[2 * c + e].z, l);
                         }
                         tmem_st16(s_at + (SPL == 2 ? 32 : 16) * c, w);
                         if (SPL == 2) tmem_st16(s_at + 32 * c + 16, w2);
                     }
-                    if (!ok) break;
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(pfull + 8 * buf);
-                    sc = sc_next;
+                    if (lane == 0) mbar_arrive(pfull + 8 * (2 * t + buf));
                 }
             }
-            // the buffers' uses, whoever had them
-            uses0 += nq == 2 ? n : (n + 1) / 2;
-            uses1 += nq == 2 ? n : n / 2;
-            if (active) done += n;
+            seq += n;
+            if (active) tiles += n;
             ok = __all_sync(0xffffffffu, ok);
             if (!ok || !mbar_wait_lanes(ofull, pieces & 1, abort, status, STATUS_ATTEND_WAIT)) break;
             pieces++;
             if (!active) continue;
             tc_fence_after();
+            if (fresh) l = 0.f;                                  // (what is hidden weighs 2^-120 at most, not always nothing)
             const float v0 = vref > 0.f ? vref : 1.f;
             const bool complete = piece.first == 0 && n == u.nt;
             const int r = at - u.r0;
@@ -403,7 +403,8 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         const uint32_t full = kv ? vfull : kfull, empty = kv ? vempty : kempty;
         uint8_t *slots = smem + (kv ? C::O_V : C::O_K);
         constexpr int GROUPS = TT / 32, HALVES = DC / 64;        // groups of 8 tokens a warp; a lane: a token and every fourth chunk of 16 dims
-        static_assert(GROUPS * HALVES == 8, "eight loads a lane");
+        constexpr int BATCH = 8 / (GROUPS * HALVES), LOADS = GROUPS * HALVES;        // tiles whose loads, eight a lane, are under way together
+        static_assert(BATCH * LOADS == 8 && BATCH <= SLOTS, "eight loads a lane");
         const int r8 = lane & 7, c4 = lane >> 3, chunks = p.dim >> 4;
         // where a chunk's two halves of 8 dims go.  K: core matrices, [8 dims][8 tokens]; V: rows of 64 dims, 128 bytes, with
         // the chunks of a row exchanged by its number (the 128-byte swizzle)
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         auto page_of = [&](const KvTile<R, TT> &t) {             // lane i: the page of this warp's i-th group
             return page_at(p, t.b, t.base + (lane * 4 + w) * 8, 8, t.lo, t.hi, t.there && lane < GROUPS);
         };
-        auto load = [&](const KvTile<R, TT> &t, int id, uint4 (&raw)[8]) {
+        auto load = [&](const KvTile<R, TT> &t, int id, uint4 *raw) {
 #pragma unroll
             for (int i = 0; i < GROUPS; i++) {
                 const int page = __shfl_sync(0xffffffffu, id, i);
@@ -424,124 +425,170 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                     raw[i * HALVES + k] = page >= 0 && c4 + 4 * k < chunks ? __ldg((const uint4 *)row + c4 + 4 * k) : make_uint4(0, 0, 0, 0);
             }
         };
-        KvTile<R, TT> next = tiles.next();
-        Page page = page_of(next);
-        for (uint32_t seq = 0; next.there; seq++) {
-            // the loads are under way while the slot is waited for
+        KvTile<R, TT> next[BATCH];
+        Page page[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) {
+            next[i] = tiles.next();
+            page[i] = page_of(next[i]);
+        }
+        for (uint32_t seq = 0; next[0].there; seq += BATCH) {
+            // the loads are under way while the slots are waited for
             uint4 raw[8];
-            load(next, page_number(p, page, false), raw);
-            next = tiles.next();
-            page = page_of(next);
-            const int slot = seq % SLOTS;
-            if (seq >= SLOTS && !mbar_wait_soon_lanes(empty + 8 * slot, (seq / SLOTS - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) break;
-            uint8_t *dst = slots + slot * C::SLOT;
+            bool there[BATCH];
 #pragma unroll
-            for (int i = 0; i < GROUPS; i++)
+            for (int i = 0; i < BATCH; i++) {
+                there[i] = next[i].there;
+                load(next[i], page_number(p, page[i], false), raw + i * LOADS);
+            }
 #pragma unroll
-                for (int k = 0; k < HALVES; k++) {
-                    if (c4 + 4 * k < chunks) {
-                        uint32_t h[8];
+            for (int i = 0; i < BATCH; i++) {
+                next[i] = tiles.next();
+                page[i] = page_of(next[i]);
+            }
+            bool ok = true;
 #pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const uint32_t x = word(raw[i * HALVES + k], q) ^ 0x80808080u;
-                            h[2 * q] = codes_lo(x);
-                            h[2 * q + 1] = codes_hi(x);
+            for (int n = 0; n < BATCH; n++) {
+                if (!there[n]) break;
+                const uint32_t slot = (seq + n) % SLOTS, use = (seq + n) / SLOTS;
+                if (use > 0 && !mbar_wait_soon_lanes(empty + 8 * slot, (use - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
+                uint8_t *dst = slots + slot * C::SLOT;
+#pragma unroll
+                for (int i = 0; i < GROUPS; i++)
+#pragma unroll
+                    for (int k = 0; k < HALVES; k++) {
+                        if (c4 + 4 * k < chunks) {
+                            uint32_t h[8];
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const uint32_t x = word(raw[n * LOADS + i * HALVES + k], q) ^ 0x80808080u;
+                                h[2 * q] = codes_lo(x);
+                                h[2 * q + 1] = codes_hi(x);
+                            }
+                            uint8_t *at = dst + i * (kv ? 4096 : 512) + k * (TT * 128);
+                            *(uint4 *)(at + at0) = make_uint4(h[0], h[1], h[2], h[3]);
+                            *(uint4 *)(at + at1) = make_uint4(h[4], h[5], h[6], h[7]);
                         }
-                        uint8_t *at = dst + i * (kv ? 4096 : 512) + k * (TT * 128);
-                        *(uint4 *)(at + at0) = make_uint4(h[0], h[1], h[2], h[3]);
-                        *(uint4 *)(at + at1) = make_uint4(h[4], h[5], h[6], h[7]);
                     }
-                }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full + 8 * slot);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + 8 * slot);
+            }
+            if (!ok) break;
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REST_REGS));
-        if (warp == 4 * NQ + CW && lane == 0) {
-        // ------------------------------------------------------------------ one thread issues the products
+        const int issuer = warp - 4 * NQ - CW;
+        if (issuer == 2) {
+            // -------------------------------------------------------------- a warp fetches the tiles' scales
+            // a lane a group of 16 tokens; pages are asked for two tiles ahead, scales one
+            KvWalk<R, TT> walk(p, head->start);
+            auto page_of = [&](const KvTile<R, TT> &t) { return page_at(p, t.b, t.base + lane * 16, 16, t.lo, t.hi, t.there && lane < NG); };
+            KvTile<R, TT> now = walk.next();
+            float2 sc = scales_at(p, page_number(p, page_of(now), true), now.h);
+            KvTile<R, TT> next = walk.next();
+            Page page = page_of(next);
+            float vref = 0.f;
+            for (uint32_t seq = 0; now.there; seq++) {
+                const float2 sc_next = scales_at(p, page_number(p, page, true), next.h);
+                const KvTile<R, TT> after = walk.next();
+                page = page_of(after);
+                if (now.starts) vref = 0.f;
+                // V's scales against the first of the piece that is not zero
+                const unsigned some = __ballot_sync(0xffffffffu, sc.y > 0.f);
+                const float found = __shfl_sync(0xffffffffu, sc.y, some ? __ffs(some) - 1 : 0);
+                if (vref == 0.f && some) vref = found;
+                float lr = 0.f, rinv = 1.f;
+                if (sc.y < 0.f) { lr = -INFINITY; rinv = 0.f; }
+                else if (sc.y > 0.f && sc.y != vref) { lr = log2_ratio(sc.y, vref); rinv = __fdividef(vref, sc.y); }
+                if (seq >= 4 && !mbar_wait_soon_lanes(sempty + 8 * (seq & 3), (seq / 4 - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) break;
+                if (lane < NG) head->scales[seq & 3][lane] = make_float4(sc.x, lr, rinv, vref);
+                __syncwarp();
+                // (an arrival of the slot's next use must not count for this one)
+                if (seq >= SLOTS && !mbar_wait_soon_lanes(kempty + 8 * (seq % SLOTS), (seq / SLOTS - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) break;
+                if (lane == 0) mbar_arrive(kfull + 8 * (seq % SLOTS));
+                now = next;
+                sc = sc_next;
+                next = after;
+            }
+        }
+        if (issuer < 2 && lane == 0) {
+        // ------------------------------------------------------------------ a thread a row tile issues its products
         Walk<R, TT, false> walk(p, head->start);
         Piece piece;
         const uint32_t s_desc = idesc_of(1, 128, TT), o_desc = idesc_of(1, 128, p.dim) | 1u << 16;      // B of the second: a row a dim
-        uint32_t kseq = 0, vseq = 0, uses0 = 0, uses1 = 0, pieces = 0;
+        const int t = issuer;
+        uint32_t seq = 0, tiles = 0, pieces = 0;               // tiles of the block, of this row tile; pieces
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) { ok = ok && mbar_wait_soon(bar, parity & 1, abort, status, STATUS_ATTEND_WAIT); return ok; };
         // descriptors count addresses in 16 bytes: a step of 16 dims (tokens) is an addition
         const uint64_t q_desc = smem_desc(base_u32 + C::O_Q, 2048, 128), k_desc = smem_desc(base_u32 + C::O_K, TT * 16, 128);
         const uint64_t v_desc = smem_desc(base_u32 + C::O_V, TT * 128, 1024) | (uint64_t)2 << 61;      // 128-byte swizzle
         const int steps = p.dim / 16;
-        auto scores = [&](int t, int buf, uint32_t slot) {
+        // K's slots, and V's, are released by two arrivals: with one row tile both come from its thread
+        auto release = [&](uint32_t bar, int nq) {
+            mma_commit(bar);
+            if (nq == 1) mma_commit(bar);
+        };
+        auto scores = [&](int j, int nq) {
+            const uint32_t slot = (seq + j) % SLOTS;
+            const int buf = (tiles + j) & 1;
+            if (!wait(kfull + 8 * slot, (seq + j) / SLOTS)) return;
+            tc_fence_after();
             uint32_t accumulate = 0;
 #pragma unroll
             for (int x = 0; x < SPL; x++) {
                 uint64_t qd = q_desc + (t * SPL + x) * (C::QTILE >> 4), kd = k_desc + slot * (C::SLOT >> 4);
 #pragma unroll 1
                 for (int d = 0; d < steps; d++) {
-                    mma_issue<1>(tmem + C::s_col(buf), qd, kd, s_desc, accumulate);
+                    mma_issue<1>(tmem + C::s_col(t, buf), qd, kd, s_desc, accumulate);
                     accumulate = 1;
                     qd += 4096 >> 4;
                     kd += TT * 32 >> 4;
                 }
             }
-            mma_commit(sfull + 8 * buf);
+            mma_commit(sfull + 8 * (2 * t + buf));
+            release(kempty + 8 * slot, nq);
         };
-        auto sums = [&](int t, int buf, uint32_t slot, int j) {
+        auto sums = [&](int j, int nq) {
+            const uint32_t slot = (seq + j) % SLOTS;
+            const int buf = (tiles + j) & 1;
+            if (!wait(vfull + 8 * slot, (seq + j) / SLOTS) || !wait(pfull + 8 * (2 * t + buf), (tiles + j) >> 1)) return;
+            tc_fence_after();
             uint64_t vd = v_desc + slot * (C::SLOT >> 4);
-            const uint32_t p_at = tmem + C::s_col(buf), o_at = tmem + C::o_col(t);
+            uint32_t col = tmem + C::s_col(t, buf), accumulate = j;
+            const uint32_t o_at = tmem + C::o_col(t);
 #pragma unroll 1
-            for (int s = 0; s < TT / 16; s++, vd += 2048 >> 4) {
-                const uint32_t col = p_at + (SPL == 2 ? (s >> 1) * 32 + (s & 1) * 8 : s * 8);
-                mma_issue_ts(o_at, col, vd, o_desc, s ? 1 : j);
+            for (int s = 0; s < TT / 32; s++) {                // 32 tokens: their weights lie in 16 columns (32: the two f16)
+                mma_issue_ts(o_at, col, vd, o_desc, accumulate);
                 if (SPL == 2) mma_issue_ts(o_at, col + 16, vd, o_desc, 1);
+                vd += 2048 >> 4;
+                mma_issue_ts(o_at, col + 8, vd, o_desc, 1);
+                if (SPL == 2) mma_issue_ts(o_at, col + 24, vd, o_desc, 1);
+                vd += 2048 >> 4;
+                col += SPL == 2 ? 32 : 16;
+                accumulate = 1;
             }
             mma_commit(odone + 8 * t);
+            release(vempty + 8 * slot, nq);
+            release(sempty + 8 * ((seq + j) & 3), nq);
         };
         while (ok && walk.next(piece)) {
             const int n = piece.count, nq = NQ == 2 && piece.unit.r1 - piece.unit.r0 > 128 ? 2 : 1;
             if (!wait(qfull, pieces)) break;
             tc_fence_after();
-            if (!wait(kfull + 8 * (kseq % SLOTS), kseq / SLOTS)) break;
-            for (int t = 0; t < nq; t++) scores(t, t, kseq % SLOTS);
-            mma_commit(kempty + 8 * (kseq % SLOTS));
-            kseq++;
-            for (int j = 0; j < n && ok; j++) {
-                const uint32_t vs = vseq % SLOTS, ks = kseq % SLOTS;
-                const bool more = j + 1 < n;
-                if (nq == 2) {
-                    for (int t = 0; t < 2; t++) {
-                        if (t == 0 && !wait(vfull + 8 * vs, vseq / SLOTS)) break;
-                        if (!wait(pfull + 8 * t, (t ? uses1 : uses0) + j)) break;
-                        tc_fence_after();
-                        sums(t, t, vs, j);
-                        if (more) {
-                            if (t == 0 && !wait(kfull + 8 * ks, kseq / SLOTS)) break;
-                            tc_fence_after();
-                            scores(t, t, ks);
-                        }
-                    }
-                } else {
-                    const int buf = j & 1;
-                    if (more) {
-                        if (!wait(kfull + 8 * ks, kseq / SLOTS)) break;
-                        tc_fence_after();
-                        scores(0, buf ^ 1, ks);
-                    }
-                    if (!wait(vfull + 8 * vs, vseq / SLOTS) || !wait(pfull + 8 * buf, (buf ? uses1 : uses0) + (j >> 1))) break;
-                    tc_fence_after();
-                    sums(0, buf, vs, j);
+            if (t < nq) {
+                // S of a tile takes the place of the weights two tiles back: behind their product, in this thread's order
+                scores(0, nq);
+                for (int j = 0; j < n && ok; j++) {
+                    if (j + 1 < n) scores(j + 1, nq);
+                    if (ok) sums(j, nq);
                 }
                 if (!ok) break;
-                mma_commit(vempty + 8 * vs);
-                vseq++;
-                if (more) {
-                    mma_commit(kempty + 8 * ks);
-                    kseq++;
-                }
+                release(ofull, nq);
+                tiles += n;
             }
-            if (!ok) break;
-            uses0 += nq == 2 ? n : (n + 1) / 2;
-            uses1 += nq == 2 ? n : n / 2;
-            mma_commit(ofull);
+            seq += n;
             pieces++;
         }
         // nothing may run on the tensor cores when the block gives its memory back
