@@ -483,20 +483,29 @@ __device__ __forceinline__ void finish_row(const AttendArgs &p, const Unit &u, i
 }
 
 // ---------------------------------------------------------------------------------- waits
-// As mbar_wait, but polled without a suspended thread first: these waits are short.
+// Bounded as mbar_wait is, with little code at each place (the warps of a block run different code and share the caches of
+// instructions): a poll takes 20 cycles or more, so 2^26 of them are about a second at least.
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity)
 {
     uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done != 0;
+}
+static __device__ __noinline__ bool gives_up(uint32_t polls, volatile int *abort, int *status, int status_bit)
+{
+    if (*abort) return true;
+    if (polls < 1u << 26) return false;
+    *abort = 1;
+    atomicOr(status, status_bit);
+    return true;
 }
 __device__ __forceinline__ bool mbar_wait_soon(uint32_t bar, uint32_t parity, volatile int *abort, int *status, int status_bit)
 {
 #pragma unroll 1
-    for (int i = 0; i < 64; i++)
-        if (mbar_test(bar, parity)) return true;
-    return mbar_wait(bar, parity, abort, status, status_bit);
+    for (uint32_t polls = 1; !mbar_test(bar, parity); polls++)
+        if ((polls & 1023) == 0 && gives_up(polls, abort, status, status_bit)) return false;
+    return true;
 }
 // The same for the lanes of a warp, which leave together.
 __device__ __forceinline__ bool mbar_wait_soon_lanes(uint32_t bar, uint32_t parity, volatile int *abort, int *status, int status_bit)

@@ -32,7 +32,7 @@ struct TilesCfg {
     static constexpr int NG = TT / 16;
     static constexpr int WARPS = 4 * NQ + CW + 4, THREADS = 32 * WARPS;       // the last four: one issues the products
     // registers a thread: of the launch (65536 over the threads, whole eights), and of the softmax, converter and last warps
-    static constexpr int REGS = NQ == 2 ? 96 : 128, SOFT_REGS = NQ == 2 ? 144 : 200, CONV_REGS = NQ == 2 ? 72 : 104, REST_REGS = 48;
+    static constexpr int REGS = NQ == 2 ? 96 : 128, SOFT_REGS = NQ == 2 ? 120 : 176, CONV_REGS = NQ == 2 ? 80 : 104, REST_REGS = NQ == 2 ? 80 : 128;
     static_assert(NQ * SOFT_REGS + 2 * CONV_REGS + REST_REGS <= (NQ + 3) * REGS, "the shares of the registers fit the launch's");
     static constexpr uint32_t QTILE = 128 * DC * 2, SLOT = TT * DC * 2;
     static constexpr uint32_t O_Q = 0, O_K = NQ * SPL * QTILE, O_V = O_K + SLOTS * SLOT, O_HEAD = O_V + SLOTS * SLOT, SMEM = O_HEAD + 2048 + 1024;
