@@ -87,12 +87,6 @@ __device__ __forceinline__ Unit unit_of(const AttendArgs &p, const Sequence &s, 
     u.nt = u.hi > u.lo ? (u.hi + TT - 1) / TT - u.t0 : 1;
     return u;
 }
-template <int R, int TT>
-__device__ __forceinline__ Unit unit_of(const AttendArgs &p, int b, int h, int rc)
-{
-    return unit_of<R, TT>(p, sequence_at(p, b), b, h, rc);
-}
-
 // The tokens row `at` of a unit's sequence sees.
 __device__ __forceinline__ void row_limits(const AttendArgs &p, const Unit &u, int at, int &lo, int &hi)
 {
@@ -102,22 +96,17 @@ __device__ __forceinline__ void row_limits(const AttendArgs &p, const Unit &u, i
 }
 
 // ---------------------------------------------------------------------------------- shares
-template <int R>
-__device__ __forceinline__ int chunks_of(const AttendArgs &p, int b)
-{
-    int row, n;
-    bool bad;
-    seq_rows(p.seq, b, row, n, bad);
-    return (n * p.group + R - 1) / R;
-}
-
-// a / b for 0 <= a < 2^52, b > 0: a double's quotient, put right
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b)
+// a / b for 0 <= a < 2^52, b > 0.  Lines longer than 2^31 are rare: a double's quotient, put right.
+static __device__ __noinline__ int64_t long_quotient(int64_t a, int64_t b)
 {
     int64_t q = (int64_t)((double)a / (double)b);
     if (q * b > a) q--;
     if ((q + 1) * b <= a) q++;
     return q;
+}
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b)
+{
+    return (a | b) >> 31 ? long_quotient(a, b) : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
 struct Start {
@@ -126,125 +115,81 @@ struct Start {
 };
 
 // The line of work: sequence after sequence, head after head, unit after unit, a unit taking unit_pad places for itself and
-// then one a tile.  The functions below are called by a whole warp.  Few sequences: a lane a unit; many: a lane a sequence.
-constexpr int FEW_SEQUENCES = 8;
+// then one a tile.  It is cut into shares, one a block, but none of less than LEAST_TOKENS tokens unless every unit has one;
+// shares are equally long, but for one place.
+struct Line {
+    Start start;                               // of the share asked for
+    int64_t each;                              // places a share,
+    int more, shares;                          // and one more in the first `more` of them
+    __device__ __forceinline__ int64_t at(int block) const { return each * block + min(block, more); }
+};
 
-// The length of one head of sequence b: this lane's part of it (few sequences), or all.
+// Called by a whole warp, a lane a sequence (32 at a time).  This is the first thing a block does, and its instructions have
+// to be fetched before they run: it is written for little code, not for few steps.
 template <int R, int TT>
-__device__ __forceinline__ int64_t tiles_of(const AttendArgs &p, int b, int first, int step)
-{
-    int64_t sum = 0;
-    const Sequence s = sequence_at(p, b);
-    const int chunks = (s.n * p.group + R - 1) / R;
-#pragma unroll 1
-    for (int rc = first; rc < chunks; rc += step) sum += unit_of<R, TT>(p, s, b, 0, rc).nt + unit_pad(TT);
-    return sum;
-}
-__device__ __forceinline__ int64_t warp_sum(int64_t x)
-{
-#pragma unroll
-    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    return x;
-}
-__device__ __forceinline__ int64_t warp_upto(int64_t x)          // the sum over this lane and those before it
+__device__ __noinline__ Line line_of(const AttendArgs &p, int block)
 {
     const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const int64_t other = __shfl_up_sync(0xffffffffu, x, d);
-        if (lane >= d) x += other;
-    }
-    return x;
-}
-template <int R, int TT>
-__device__ __forceinline__ int64_t line_length(const AttendArgs &p)
-{
-    const int lane = threadIdx.x & 31;
-    int64_t sum = 0;
-    if (p.seq.count <= FEW_SEQUENCES)
+    Line line = {{p.seq.count, 0, 0, 0, 0}, 0, 0, 1};
+    int64_t total = 0, x = -1, tiles = 0;      // x: the place looked for, from the first of the sequences at hand; -1: none yet
 #pragma unroll 1
-        for (int b = 0; b < p.seq.count; b++) sum += tiles_of<R, TT>(p, b, lane, 32);
-    else
-#pragma unroll 1
-        for (int b = lane; b < p.seq.count; b += 32) sum += tiles_of<R, TT>(p, b, 0, 1);
-    return warp_sum(sum) * p.heads;
-}
-// Where place x of the line is; x is below its length.
-template <int R, int TT>
-__device__ __forceinline__ Start place_on_line(const AttendArgs &p, int64_t x)
-{
-    const int lane = threadIdx.x & 31;
-    Start s = {p.seq.count, 0, 0, 0, 0};
-    int64_t tiles = 0;                         // the length of one head of the sequence found
-    if (p.seq.count <= FEW_SEQUENCES) {
-#pragma unroll 1
-        for (int b = 0; b < p.seq.count; b++) {
-            tiles = warp_sum(tiles_of<R, TT>(p, b, lane, 32));
-            if (x < tiles * p.heads) { s.b = b; break; }
-            x -= tiles * p.heads;
-        }
-    } else {
+    for (int pass = 0; pass < 2; pass++) {
 #pragma unroll 1
         for (int base = 0; base < p.seq.count; base += 32) {
-            const int64_t mine = base + lane < p.seq.count ? tiles_of<R, TT>(p, base + lane, 0, 1) : 0, upto = warp_upto(mine) * p.heads;
+            // the length of one head of this lane's sequence
+            int64_t mine = 0;
+            if (base + lane < p.seq.count) {
+                const Sequence s = sequence_at(p, base + lane);
+                const int chunks = (s.n * p.group + R - 1) / R;
+#pragma unroll 1
+                for (int rc = 0; rc < chunks; rc++) mine += unit_of<R, TT>(p, s, 0, 0, rc).nt + unit_pad(TT);
+            }
+            int64_t upto = mine * p.heads;     // and of those before it, all heads
+#pragma unroll 1
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t other = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += other;
+            }
+            const int64_t all = __shfl_sync(0xffffffffu, upto, 31);
+            if (pass == 0) {
+                total += all;
+                continue;
+            }
             const unsigned after = __ballot_sync(0xffffffffu, upto > x);
             if (after) {
                 const int k = __ffs(after) - 1;
-                s.b = base + k;
+                line.start.b = base + k;
                 tiles = __shfl_sync(0xffffffffu, mine, k);
                 x -= __shfl_sync(0xffffffffu, upto, k) - tiles * p.heads;
                 break;
             }
-            x -= __shfl_sync(0xffffffffu, upto, 31);
+            x -= all;
+        }
+        if (pass == 0) {
+            const int64_t units = (int64_t)p.seq.count * p.heads * p.chunks;
+            line.shares = (int)max((int64_t)1, min(min((int64_t)p.grid, total), max(units, total / (LEAST_TOKENS / TT))));
+            if (block >= line.shares || total == 0) return line;
+            line.each = quotient(total, line.shares);
+            line.more = (int)(total - line.each * line.shares);
+            x = line.at(block);
+            line.start.left = line.at(block + 1) - x;
         }
     }
-    if (s.b == p.seq.count || tiles == 0) { s.b = p.seq.count; return s; }
-    s.h = (int)quotient(x, tiles);
-    x -= s.h * tiles;
-    const Sequence q = sequence_at(p, s.b);
-    const int chunks = (q.n * p.group + R - 1) / R;
-#pragma unroll 1
-    for (int base = 0; base < chunks; base += 32) {
-        const int64_t upto = warp_upto(base + lane < chunks ? unit_of<R, TT>(p, q, s.b, s.h, base + lane).nt + unit_pad(TT) : 0);
-        const unsigned after = __ballot_sync(0xffffffffu, upto > x);
-        if (after) {
-            const int k = __ffs(after) - 1;
-            s.rc = base + k;
-            const int64_t before = __shfl_sync(0xffffffffu, upto, k > 0 ? k - 1 : 0);
-            s.at = (int)(x - (k > 0 ? before : 0));
-            return s;
-        }
-        x -= __shfl_sync(0xffffffffu, upto, 31);
+    if (line.start.b == p.seq.count || tiles == 0) {
+        line.start.left = 0;
+        return line;
     }
-    s.b = p.seq.count;
-    return s;
-}
-// Shares there are: one a block, but none of less than LEAST_TOKENS tokens unless every unit has one.
-template <int TT>
-__device__ __forceinline__ int shares_of(const AttendArgs &p, int64_t total)
-{
-    const int64_t units = (int64_t)p.seq.count * p.heads * p.chunks;
-    return (int)max((int64_t)1, min(min((int64_t)p.grid, total), max(units, total / (LEAST_TOKENS / TT))));
-}
-// Where share `block` begins: shares are equally long, but for one place.
-struct Shares {
-    int64_t each;
-    int more;                                  // the first `more` of them have one place more
-    __device__ __forceinline__ Shares(int64_t total, int shares) { each = quotient(total, shares); more = (int)(total - each * shares); }
-    __device__ __forceinline__ int64_t at(int block) const { return each * block + min(block, more); }
-};
-template <int R, int TT>
-__device__ __noinline__ Start start_of(const AttendArgs &p, int block)
-{
-    const int64_t total = line_length<R, TT>(p);
-    const int shares = shares_of<TT>(p, total);
-    Start s = {0, 0, 0, 0, 0};
-    if (block >= shares) return s;
-    const Shares cuts(total, shares);
-    const int64_t from = cuts.at(block), to = cuts.at(block + 1);
-    if (to > from) s = place_on_line<R, TT>(p, from);
-    s.left = to - from;
-    return s;
+    line.start.h = (int)quotient(x, tiles);
+    x -= line.start.h * tiles;
+    const Sequence s = sequence_at(p, line.start.b);
+    for (;;) {
+        const int length = unit_of<R, TT>(p, s, 0, 0, line.start.rc).nt + unit_pad(TT);
+        if (x < length) break;
+        x -= length;
+        line.start.rc++;
+    }
+    line.start.at = (int)x;
+    return line;
 }
 
 struct Cut {
@@ -252,24 +197,17 @@ struct Cut {
     int block, parts;                          // parts: 0, or how many blocks from block - 1 on hold parts of the unit
 };
 template <int R, int TT>
-__device__ __noinline__ Cut cut_of(const AttendArgs &p, int block)
+__device__ __forceinline__ Cut cut_of(const AttendArgs &p, int block)
 {
-    const int64_t total = line_length<R, TT>(p);
-    const int shares = shares_of<TT>(p, total);
-    Cut c = {0, 0, 0, block, 0};
-    if (block >= shares) return c;
-    const Shares cuts(total, shares);
-    const int64_t from = cuts.at(block), before = cuts.at(block - 1);
-    const Start s = place_on_line<R, TT>(p, from);
+    const Line line = line_of<R, TT>(p, block);
+    const Start &s = line.start;
+    Cut c = {s.b, s.h, s.rc, block, 0};
     // not inside a unit's tiles, or not the first boundary inside them
-    if (s.b >= p.seq.count || s.at <= unit_pad(TT) || before > from - s.at + unit_pad(TT)) return c;
-    const int64_t end = from - s.at + unit_pad(TT) + unit_of<R, TT>(p, s.b, s.h, s.rc).nt;
-    c.b = s.b;
-    c.h = s.h;
-    c.rc = s.rc;
+    if (s.left == 0 || s.at <= unit_pad(TT) || s.at - unit_pad(TT) > line.at(block) - line.at(block - 1)) return c;
+    const int64_t end = line.at(block) - s.at + unit_pad(TT) + unit_of<R, TT>(p, sequence_at(p, s.b), s.b, s.h, s.rc).nt;
     c.parts = 1;
 #pragma unroll 1
-    for (int k = block; k < shares && cuts.at(k) < end; k++) c.parts++;
+    for (int k = block; k < line.shares && line.at(k) < end; k++) c.parts++;
     return c;
 }
 

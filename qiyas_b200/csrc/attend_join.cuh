@@ -17,7 +17,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");         // (what a call is cut by was there before either kernel)
     if (cut.parts == 0) return;
-    const Unit u = unit_of<R, TT>(p, cut.b, cut.h, cut.rc);
+    const Unit u = unit_of<R, TT>(p, sequence_at(p, cut.b), cut.b, cut.h, cut.rc);
     const int rows = u.r1 - u.r0, quads = p.dim / 4;
     const size_t size = part_floats(R, p.dim);
     const float *first = (const float *)p.workspace + (size_t)((cut.block - 1) * 2 + 1) * size;      // the part that begins the unit

@@ -87,7 +87,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
         mbar_fence_init();
     }
     if (warp == 0) {
-        const Start s = p.whole ? Start{} : start_of<C::R, 32>(p, blockIdx.x);
+        const Start s = p.whole ? Start{} : line_of<C::R, 32>(p, blockIdx.x).start;
         if (lane == 0) head->start = s;
     }
     __syncthreads();

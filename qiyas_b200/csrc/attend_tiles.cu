@@ -32,7 +32,7 @@ struct TilesCfg {
     static constexpr int NG = TT / 16;
     static constexpr int WARPS = 4 * NQ + CW + 4, THREADS = 32 * WARPS;       // the last four: one issues the products
     // registers a thread: of the launch (65536 over the threads, whole eights), and of the softmax, converter and last warps
-    static constexpr int REGS = NQ == 2 ? 96 : 128, SOFT_REGS = NQ == 2 ? 120 : 176, CONV_REGS = NQ == 2 ? 80 : 104, REST_REGS = NQ == 2 ? 80 : 128;
+    static constexpr int REGS = NQ == 2 ? 96 : 128, SOFT_REGS = NQ == 2 ? 136 : 176, CONV_REGS = NQ == 2 ? 72 : 104, REST_REGS = NQ == 2 ? 64 : 128;
     static_assert(NQ * SOFT_REGS + 2 * CONV_REGS + REST_REGS <= (NQ + 3) * REGS, "the shares of the registers fit the launch's");
     static constexpr uint32_t QTILE = 128 * DC * 2, SLOT = TT * DC * 2;
     static constexpr uint32_t O_Q = 0, O_K = NQ * SPL * QTILE, O_V = O_K + SLOTS * SLOT, O_HEAD = O_V + SLOTS * SLOT, SMEM = O_HEAD + 2048 + 1024;
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         mbar_fence_init();
     }
     if (warp == 0) {
-        const Start s = start_of<R, TT>(p, blockIdx.x);
+        const Start s = line_of<R, TT>(p, blockIdx.x).start;
         if (lane == 0) head->start = s;
     }
     if (warp == 4 * NQ + CW) tmem_alloc(smem_u32(&head->tmem), 512);
@@ -377,6 +377,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             float *part = slot + R * 2 + (size_t)r * p.dim;
             const float f = complete ? v0 * inverse_of(l) : v0;
             T *dst = out_row<T>(p, u, min(at, u.r1 - 1));
+#pragma unroll 1
             for (int d = 0; d < p.dim; d += 16) {
                 uint32_t v[16];
                 tmem_ld16(tmem + lanes + C::o_col(t) + d, v);
@@ -403,8 +404,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         const uint32_t full = kv ? vfull : kfull, empty = kv ? vempty : kempty;
         uint8_t *slots = smem + (kv ? C::O_V : C::O_K);
         constexpr int GROUPS = TT / 32, HALVES = DC / 64;        // groups of 8 tokens a warp; a lane: a token and every fourth chunk of 16 dims
-        constexpr int BATCH = 8 / (GROUPS * HALVES), LOADS = GROUPS * HALVES;        // tiles whose loads, eight a lane, are under way together
-        static_assert(BATCH * LOADS == 8 && BATCH <= SLOTS, "eight loads a lane");
+        constexpr int LOADS = GROUPS * HALVES;
         const int r8 = lane & 7, c4 = lane >> 3, chunks = p.dim >> 4;
         // where a chunk's two halves of 8 dims go.  K: core matrices, [8 dims][8 tokens]; V: rows of 64 dims, 128 bytes, with
         // the chunks of a row exchanged by its number (the 128-byte swizzle)
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         auto page_of = [&](const KvTile<R, TT> &t) {             // lane i: the page of this warp's i-th group
             return page_at(p, t.b, t.base + (lane * 4 + w) * 8, 8, t.lo, t.hi, t.there && lane < GROUPS);
         };
-        auto load = [&](const KvTile<R, TT> &t, int id, uint4 *raw) {
+        auto load = [&](const KvTile<R, TT> &t, int id, uint4 (&raw)[LOADS]) {
 #pragma unroll
             for (int i = 0; i < GROUPS; i++) {
                 const int page = __shfl_sync(0xffffffffu, id, i);
@@ -425,33 +425,20 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                     raw[i * HALVES + k] = page >= 0 && c4 + 4 * k < chunks ? __ldg((const uint4 *)row + c4 + 4 * k) : make_uint4(0, 0, 0, 0);
             }
         };
-        KvTile<R, TT> next[BATCH];
-        Page page[BATCH];
-#pragma unroll
-        for (int i = 0; i < BATCH; i++) {
-            next[i] = tiles.next();
-            page[i] = page_of(next[i]);
-        }
-        for (uint32_t seq = 0; next[0].there; seq += BATCH) {
-            // the loads are under way while the slots are waited for
-            uint4 raw[8];
-            bool there[BATCH];
-#pragma unroll
-            for (int i = 0; i < BATCH; i++) {
-                there[i] = next[i].there;
-                load(next[i], page_number(p, page[i], false), raw + i * LOADS);
-            }
-#pragma unroll
-            for (int i = 0; i < BATCH; i++) {
-                next[i] = tiles.next();
-                page[i] = page_of(next[i]);
-            }
-            bool ok = true;
-#pragma unroll
-            for (int n = 0; n < BATCH; n++) {
-                if (!there[n]) break;
-                const uint32_t slot = (seq + n) % SLOTS, use = (seq + n) / SLOTS;
-                if (use > 0 && !mbar_wait_soon_lanes(empty + 8 * slot, (use - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
+        // three tiles at a time: one is converted, the next one's loads are under way, the page of the one after is asked for
+        KvTile<R, TT> now, next;
+        now.there = next.there = false;
+        Page page = {-1, false};
+        uint4 raw[LOADS], coming[LOADS];
+        uint32_t seq = 0;
+#pragma unroll 1
+        do {
+            if (next.there) load(next, page_number(p, page, false), coming);
+            const KvTile<R, TT> after = tiles.next();
+            page = page_of(after);
+            if (now.there) {
+                const uint32_t slot = seq % SLOTS, use = seq / SLOTS;
+                if (use > 0 && !mbar_wait_soon_lanes(empty + 8 * slot, (use - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) break;
                 uint8_t *dst = slots + slot * C::SLOT;
 #pragma unroll
                 for (int i = 0; i < GROUPS; i++)
@@ -461,7 +448,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                             uint32_t h[8];
 #pragma unroll
                             for (int q = 0; q < 4; q++) {
-                                const uint32_t x = word(raw[n * LOADS + i * HALVES + k], q) ^ 0x80808080u;
+                                const uint32_t x = word(raw[i * HALVES + k], q) ^ 0x80808080u;
                                 h[2 * q] = codes_lo(x);
                                 h[2 * q + 1] = codes_hi(x);
                             }
@@ -473,9 +460,13 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full + 8 * slot);
+                seq++;
             }
-            if (!ok) break;
-        }
+            now = next;
+            next = after;
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) raw[i] = coming[i];
+        } while (now.there || next.there);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REST_REGS));
         const int issuer = warp - 4 * NQ - CW;
@@ -484,15 +475,19 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             // a lane a group of 16 tokens; pages are asked for two tiles ahead, scales one
             KvWalk<R, TT> walk(p, head->start);
             auto page_of = [&](const KvTile<R, TT> &t) { return page_at(p, t.b, t.base + lane * 16, 16, t.lo, t.hi, t.there && lane < NG); };
-            KvTile<R, TT> now = walk.next();
-            float2 sc = scales_at(p, page_number(p, page_of(now), true), now.h);
-            KvTile<R, TT> next = walk.next();
-            Page page = page_of(next);
+            KvTile<R, TT> now, next;
+            now.there = next.there = false;
+            Page page = {-1, false};
+            float2 sc = make_float2(0.f, -1.f);
             float vref = 0.f;
-            for (uint32_t seq = 0; now.there; seq++) {
-                const float2 sc_next = scales_at(p, page_number(p, page, true), next.h);
+            uint32_t seq = 0;
+#pragma unroll 1
+            do {
+                float2 sc_next = make_float2(0.f, -1.f);
+                if (next.there) sc_next = scales_at(p, page_number(p, page, true), next.h);
                 const KvTile<R, TT> after = walk.next();
                 page = page_of(after);
+                if (now.there) {
                 if (now.starts) vref = 0.f;
                 // V's scales against the first of the piece that is not zero
                 const unsigned some = __ballot_sync(0xffffffffu, sc.y > 0.f);
@@ -507,10 +502,12 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 // (an arrival of the slot's next use must not count for this one)
                 if (seq >= SLOTS && !mbar_wait_soon_lanes(kempty + 8 * (seq % SLOTS), (seq / SLOTS - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) break;
                 if (lane == 0) mbar_arrive(kfull + 8 * (seq % SLOTS));
+                seq++;
+                }
                 now = next;
                 sc = sc_next;
                 next = after;
-            }
+            } while (now.there || next.there);
         }
         if (issuer < 2 && lane == 0) {
         // ------------------------------------------------------------------ a thread a row tile issues its products
