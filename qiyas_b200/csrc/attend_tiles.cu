@@ -44,9 +44,8 @@ struct TilesCfg {
 struct TilesHead {
     uint64_t qfull, ofull, drain;
     uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-    uint64_t sfull[4], pfull[4], odone[2];     // of the S buffers, two a row tile; of O, one a row tile
-    uint64_t sempty[4];                        // of `scales`
-    float4 scales[4][4];                       // of a tile's groups of 16 tokens: sk, log2(sv / v0), v0 / sv, v0
+    uint64_t sfull[4], pfull[4];               // of the S buffers, two a row tile
+    float4 scales[4][4];                       // beside K's slots, of a tile's groups of 16 tokens: sk, log2(sv / v0), v0 / sv, v0
     Start start;
     uint32_t tmem;
     int abort;
@@ -166,20 +165,19 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
     const uint32_t base_u32 = smem_u32(smem);
     const uint32_t qfull = smem_u32(&head->qfull), ofull = smem_u32(&head->ofull), drain = smem_u32(&head->drain);
     const uint32_t kfull = smem_u32(head->kfull), kempty = smem_u32(head->kempty), vfull = smem_u32(head->vfull), vempty = smem_u32(head->vempty);
-    const uint32_t sfull = smem_u32(head->sfull), pfull = smem_u32(head->pfull), odone = smem_u32(head->odone), sempty = smem_u32(head->sempty);
+    const uint32_t sfull = smem_u32(head->sfull), pfull = smem_u32(head->pfull);
 
     if (threadIdx.x == 0) {
         head->abort = 0;
         mbar_init(qfull, 4 * NQ);
         mbar_init(ofull, 2);
         mbar_init(drain, 2);
-        for (int i = 0; i < 2; i++) mbar_init(odone + 8 * i, 1);
         for (int i = 0; i < 4; i++) {
             mbar_init(kfull + 8 * i, 5);           // the converters', and the tile's scales
-            mbar_init(sempty + 8 * i, 2);
-            mbar_init(kempty + 8 * i, 2);
+
+            mbar_init(kempty + 8 * i, 8);          // the softmax warps' (with one row tile they arrive twice)
             mbar_init(vfull + 8 * i, 4);
-            mbar_init(vempty + 8 * i, 2);
+            mbar_init(vempty + 8 * i, 2);          // the products' ends, of both row tiles (or twice of one)
             mbar_init(sfull + 8 * i, 1);
             mbar_init(pfull + 8 * i, 4);
         }
@@ -214,7 +212,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             const int at = u.r0 + t * 128 + quarter * 32 + lane;
             if (active) {
                 // q: half a warp a row of up to 128 dims, a warp a row beyond; a row's address comes from the lane whose row it is
-                constexpr int PER = DC == 128 ? 2 : 1, WIDTH = 32 / PER, BATCH = sizeof(T) == 4 ? 4 : 8;
+                constexpr int PER = DC == 128 ? 2 : 1, WIDTH = 32 / PER, BATCH = sizeof(T) == 4 ? 2 : 4;
                 uint8_t *tile = smem + C::O_Q + t * SPL * C::QTILE;
                 const int col = lane % WIDTH;
                 const T *mine = q_row<T>(p, u, min(at, u.r1 - 1));
@@ -280,10 +278,12 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                     tmem_ld32(s_at + 32, v[1]);
                     float4 sc[NG];
 #pragma unroll
-                    for (int e = 0; e < NG; e++) sc[e] = head->scales[(seq + j) & 3][e];
+                    for (int e = 0; e < NG; e++) sc[e] = head->scales[(seq + j) % SLOTS][e];
                     vref = sc[NG - 1].w;
                     tmem_ld_landed32(v[0]);
                     tmem_ld_landed32(v[1]);
+                    __syncwarp();
+                    if (lane < 3 - nq) mbar_arrive(kempty + 8 * ((seq + j) % SLOTS));        // K and the scales have been read
                     float x[64];                                 // scores, in powers of two against mm
 #pragma unroll
                     for (int i = 0; i < 64; i += 2) {
@@ -318,7 +318,8 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
 #pragma unroll
                         for (int i = 0; i < 64; i++) x[i] -= up;
                         if (j > 0) {                             // O so far, once the product before has ended
-                            if (!mbar_wait_soon_lanes(odone + 8 * t, (tiles + j - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
+                            const uint32_t was = seq + j - 1;
+                            if (!mbar_wait_soon_lanes(vempty + 8 * (was % SLOTS), was / SLOTS & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
                             tc_fence_after();
 #pragma unroll 1
                             for (int d = 0; d < p.dim; d += 16) {
@@ -496,11 +497,9 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 float lr = 0.f, rinv = 1.f;
                 if (sc.y < 0.f) { lr = -INFINITY; rinv = 0.f; }
                 else if (sc.y > 0.f && sc.y != vref) { lr = log2_ratio(sc.y, vref); rinv = __fdividef(vref, sc.y); }
-                if (seq >= 4 && !mbar_wait_soon_lanes(sempty + 8 * (seq & 3), (seq / 4 - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) break;
-                if (lane < NG) head->scales[seq & 3][lane] = make_float4(sc.x, lr, rinv, vref);
-                __syncwarp();
-                // (an arrival of the slot's next use must not count for this one)
                 if (seq >= SLOTS && !mbar_wait_soon_lanes(kempty + 8 * (seq % SLOTS), (seq / SLOTS - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) break;
+                if (lane < NG) head->scales[seq % SLOTS][lane] = make_float4(sc.x, lr, rinv, vref);
+                __syncwarp();
                 if (lane == 0) mbar_arrive(kfull + 8 * (seq % SLOTS));
                 seq++;
                 }
@@ -522,12 +521,12 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         const uint64_t q_desc = smem_desc(base_u32 + C::O_Q, 2048, 128), k_desc = smem_desc(base_u32 + C::O_K, TT * 16, 128);
         const uint64_t v_desc = smem_desc(base_u32 + C::O_V, TT * 128, 1024) | (uint64_t)2 << 61;      // 128-byte swizzle
         const int steps = p.dim / 16;
-        // K's slots, and V's, are released by two arrivals: with one row tile both come from its thread
+        // V's slots are released by two arrivals: with one row tile both come from its thread
         auto release = [&](uint32_t bar, int nq) {
             mma_commit(bar);
             if (nq == 1) mma_commit(bar);
         };
-        auto scores = [&](int j, int nq) {
+        auto scores = [&](int j) {
             const uint32_t slot = (seq + j) % SLOTS;
             const int buf = (tiles + j) & 1;
             if (!wait(kfull + 8 * slot, (seq + j) / SLOTS)) return;
@@ -545,7 +544,6 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 }
             }
             mma_commit(sfull + 8 * (2 * t + buf));
-            release(kempty + 8 * slot, nq);
         };
         auto sums = [&](int j, int nq) {
             const uint32_t slot = (seq + j) % SLOTS;
@@ -566,9 +564,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 col += SPL == 2 ? 32 : 16;
                 accumulate = 1;
             }
-            mma_commit(odone + 8 * t);
             release(vempty + 8 * slot, nq);
-            release(sempty + 8 * ((seq + j) & 3), nq);
         };
         while (ok && walk.next(piece)) {
             const int n = piece.count, nq = NQ == 2 && piece.unit.r1 - piece.unit.r0 > 128 ? 2 : 1;
@@ -576,9 +572,9 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             tc_fence_after();
             if (t < nq) {
                 // S of a tile takes the place of the weights two tiles back: behind their product, in this thread's order
-                scores(0, nq);
+                scores(0);
                 for (int j = 0; j < n && ok; j++) {
-                    if (j + 1 < n) scores(j + 1, nq);
+                    if (j + 1 < n) scores(j + 1);
                     if (ok) sums(j, nq);
                 }
                 if (!ok) break;
