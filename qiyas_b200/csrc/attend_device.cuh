@@ -192,23 +192,25 @@ __device__ __noinline__ Line line_of(const AttendArgs &p, int block)
     return line;
 }
 
-struct Cut {
-    int b, h, rc;
-    int block, parts;                          // parts: 0, or how many blocks from block - 1 on hold parts of the unit
+// What a block leaves at the head of the workspace for the kernel that joins the parts: where its share begins.
+struct Mark {
+    Line line;
+    int nt;                                    // tiles of the unit
 };
+__host__ __device__ constexpr size_t marks_bytes(int grid) { return ((size_t)grid * sizeof(Mark) + 255) / 256 * 256; }
+__device__ __forceinline__ float *parts_of(const AttendArgs &p) { return (float *)((uint8_t *)p.workspace + marks_bytes(p.grid)); }
+
 template <int R, int TT>
-__device__ __forceinline__ Cut cut_of(const AttendArgs &p, int block)
+__device__ __forceinline__ Start share_of(const AttendArgs &p, int block)        // by a whole warp
 {
     const Line line = line_of<R, TT>(p, block);
-    const Start &s = line.start;
-    Cut c = {s.b, s.h, s.rc, block, 0};
-    // not inside a unit's tiles, or not the first boundary inside them
-    if (s.left == 0 || s.at <= unit_pad(TT) || s.at - unit_pad(TT) > line.at(block) - line.at(block - 1)) return c;
-    const int64_t end = line.at(block) - s.at + unit_pad(TT) + unit_of<R, TT>(p, sequence_at(p, s.b), s.b, s.h, s.rc).nt;
-    c.parts = 1;
-#pragma unroll 1
-    for (int k = block; k < line.shares && line.at(k) < end; k++) c.parts++;
-    return c;
+    if ((threadIdx.x & 31) == 0) {
+        Mark m;
+        m.line = line;
+        m.nt = line.start.left > 0 ? unit_of<R, TT>(p, sequence_at(p, line.start.b), line.start.b, line.start.h, line.start.rc).nt : 0;
+        ((Mark *)p.workspace)[block] = m;
+    }
+    return line.start;
 }
 
 struct Piece {                                 // tiles first .. first + count - 1 of a unit

@@ -9,31 +9,35 @@ namespace qb {
 template <int R, int TT, typename T>
 __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttendArgs p)
 {
-    __shared__ Cut cut;
-    if (threadIdx.x < 32) {
-        const Cut c = cut_of<R, TT>(p, blockIdx.x + 1);
-        if (threadIdx.x == 0) cut = c;
-    }
-    __syncthreads();
-    asm volatile("griddepcontrol.wait;" ::: "memory");         // (what a call is cut by was there before either kernel)
-    if (cut.parts == 0) return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int block = blockIdx.x + 1;
+    const Mark mark = ((const Mark *)p.workspace)[block];
+    const Line &line = mark.line;
+    const Start &cut = line.start;
+    const int64_t place = line.at(block);
+    // not inside a unit's tiles, or not the first boundary inside them
+    if (block >= line.shares || cut.left == 0 || cut.at <= unit_pad(TT) || cut.at - unit_pad(TT) > place - line.at(block - 1)) return;
+    const int64_t end = place - cut.at + unit_pad(TT) + mark.nt;
+    int parts = 1;
+#pragma unroll 1
+    for (int k = block; k < line.shares && line.at(k) < end; k++) parts++;
     const Unit u = unit_of<R, TT>(p, sequence_at(p, cut.b), cut.b, cut.h, cut.rc);
     const int rows = u.r1 - u.r0, quads = p.dim / 4;
     const size_t size = part_floats(R, p.dim);
-    const float *first = (const float *)p.workspace + (size_t)((cut.block - 1) * 2 + 1) * size;      // the part that begins the unit
+    const float *first = parts_of(p) + (size_t)((block - 1) * 2 + 1) * size;      // the part that begins the unit
     for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * quads; i += 256 * gridDim.y) {
         const int r = i / quads, d = (i - r * quads) * 4;
         float m = NOTHING, sum = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-        for (int k0 = 0; k0 < cut.parts; k0 += 8) {            // eight parts' loads at a time, in the order of the tokens
+        for (int k0 = 0; k0 < parts; k0 += 8) {            // eight parts' loads at a time, in the order of the tokens
             float2 s[8];
             float4 x[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 s[k] = make_float2(NOTHING, 0.f);
                 x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (k0 + k < cut.parts) {
+                if (k0 + k < parts) {
                     const float *part = first + (k0 + k ? (size_t)(2 * (k0 + k) - 1) * size : 0);
                     s[k] = *(const float2 *)(part + r * 2);
                     x[k] = *(const float4 *)(part + R * 2 + r * p.dim + d);
@@ -69,7 +73,7 @@ static int launch_join(const AttendArgs &args, cudaStream_t stream)
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(args.grid - 1, R > 16 ? R / 16 : 1);
+    cfg.gridDim = dim3(args.grid - 1, R > 16 ? R / 32 : 1);
     cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cfg.attrs = &attr;

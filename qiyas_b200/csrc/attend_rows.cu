@@ -87,7 +87,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
         mbar_fence_init();
     }
     if (warp == 0) {
-        const Start s = p.whole ? Start{} : line_of<C::R, 32>(p, blockIdx.x).start;
+        const Start s = p.whole ? Start{} : share_of<C::R, 32>(p, blockIdx.x);
         if (lane == 0) head->start = s;
     }
     __syncthreads();
@@ -454,7 +454,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
             }
             if (complete) finish_row<T>(p, u, u.r0 + r, d, acc, m, sum);
             else {
-                float *slot = (float *)p.workspace + (size_t)(blockIdx.x * 2 + (piece.first ? 0 : 1)) * part_floats(C::R, p.dim);
+                float *slot = parts_of(p) + (size_t)(blockIdx.x * 2 + (piece.first ? 0 : 1)) * part_floats(C::R, p.dim);
                 *(float4 *)(slot + C::R * 2 + r * p.dim + d) = acc;
                 if (d == 0) *(float2 *)(slot + r * 2) = make_float2(m, sum);
             }

@@ -14,6 +14,7 @@
 //  * A thread reads its row of S once, 32 tokens at a time, and takes the weights against the exponent it has: only where one
 //    would pass 2^15 does it go back over what the row has of O and of the tile's weights, in place, by a power of two.
 // Scales, exponents and the cut of q and w are those of attend_rows.cu; so are the shares of the grid's blocks.
+#include <type_traits>
 #include "common.cuh"
 #include "attend_device.cuh"
 #include "attend_join.cuh"
@@ -49,7 +50,6 @@ struct TilesHead {
     Start start;
     uint32_t tmem;
     int abort;
-    float factor[256];
 };
 static_assert(sizeof(TilesHead) <= 2048, "the header fits");
 
@@ -111,6 +111,12 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
+}
+
+// 16 bytes of global memory into shared memory.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 // Pairs of f32 in one instruction.
@@ -184,7 +190,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         mbar_fence_init();
     }
     if (warp == 0) {
-        const Start s = line_of<R, TT>(p, blockIdx.x).start;
+        const Start s = share_of<R, TT>(p, blockIdx.x);
         if (lane == 0) head->start = s;
     }
     if (warp == 4 * NQ + CW) tmem_alloc(smem_u32(&head->tmem), 512);
@@ -210,44 +216,62 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             const bool active = t < nq;
             const int n = piece.count;
             const int at = u.r0 + t * 128 + quarter * 32 + lane;
+            float factor = p.scale * 1.4426950408889634f;
             if (active) {
-                // q: half a warp a row of up to 128 dims, a warp a row beyond; a row's address comes from the lane whose row it is
-                constexpr int PER = DC == 128 ? 2 : 1, WIDTH = 32 / PER, BATCH = sizeof(T) == 4 ? 2 : 4;
+                // q: its rows are copied as they are to where their core matrices will be (8 f16 dims, or 4 of f32: 16 bytes), all
+                // copies under way at once; then each thread scales and cuts its own row in place (f16 lanes stay as they are)
                 uint8_t *tile = smem + C::O_Q + t * SPL * C::QTILE;
-                const int col = lane % WIDTH;
                 const T *mine = q_row<T>(p, u, min(at, u.r1 - 1));
+                const int groups = p.dim / 8, rows = min(32, u.r1 - (at - lane));
+                if (p.q_wide) {
+                    constexpr int PER = DC == 128 ? 2 : 1, WIDTH = 32 / PER;
+                    const int col = lane % WIDTH;
 #pragma unroll 1
-                for (int i0 = 0; i0 < 32 / PER; i0 += BATCH) {
-                    Vec8<T> raw[BATCH];
-#pragma unroll
-                    for (int i = 0; i < BATCH; i++) {
-                        const int r = (i0 + i) * PER + lane / WIDTH;
-                        const T *src = (const T *)__shfl_sync(0xffffffffu, (unsigned long long)mine, r);
-                        raw[i] = u.r0 + t * 128 + quarter * 32 + r < u.r1 && col < p.dim / 8 ? load8<T>(src + col * 8, p.q_wide) : zero8<T>();
+                    for (int i = lane / WIDTH; i - lane / WIDTH < rows; i += PER) {
+                        const T *src = (const T *)__shfl_sync(0xffffffffu, (unsigned long long)mine, i & 31) + col * 8;
+                        const int r = quarter * 32 + i;
+                        const uint32_t dst = smem_u32(tile) + col * 2048 + (r >> 3) * 128 + (r & 7) * 16;
+                        if (col < groups && i < rows) {
+                            copy16(dst, src);
+                            if (SPL == 2) copy16(dst + C::QTILE, src + 4);
+                        }
                     }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    __syncwarp();
+                }
+                uint8_t *row = tile + ((at - u.r0 - t * 128) >> 3) * 128 + (lane & 7) * 16;
+                const bool valid = lane < rows;
+                if (!p.q_wide || !valid || !std::is_same<T, __half>::value) {
+                    float top = 0.f, up = 1.f, down = 1.f;
+#pragma unroll 1
+                    for (int pass = 0; pass < 2; pass++) {
+#pragma unroll 2
+                        for (int g = 0; g < groups; g++) {
+                            Vec8<T> raw = zero8<T>();
+                            if (valid && p.q_wide) {
+                                const uint4 a = *(const uint4 *)(row + g * 2048);
+                                raw.w[0] = a.x; raw.w[1] = a.y; raw.w[2] = a.z; raw.w[3] = a.w;
+                                if (SPL == 2) {
+                                    const uint4 b = *(const uint4 *)(row + g * 2048 + C::QTILE);
+                                    raw.w[sizeof(T) * 2 - 4] = b.x; raw.w[sizeof(T) * 2 - 3] = b.y; raw.w[sizeof(T) * 2 - 2] = b.z; raw.w[sizeof(T) * 2 - 1] = b.w;
+                                }
+                            } else if (valid) raw = load8<T>(mine + g * 8, false);
+                            float x[8];
+                            unpack8(raw, x);
+                            if (pass == 0) {
 #pragma unroll
-                    for (int i = 0; i < BATCH; i++) {
-                        const int r = quarter * 32 + (i0 + i) * PER + lane / WIDTH;
-                        float x[8];
-                        unpack8(raw[i], x);
-                        float top = 0.f;
-#pragma unroll
-                        for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[k]));
-#pragma unroll
-                        for (int d = WIDTH / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        float up, down;
-                        power_scale(top, up, down);
-                        if (p.scale < 0.f) up = -up;           // the factor stays positive, so maxima can be taken of the sums
-                        if (col < p.dim / 8) {
+                                for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[k]));
+                                continue;
+                            }
                             uint32_t hi[4], lo[4];
 #pragma unroll
                             for (int k = 0; k < 4; k++) split2(x[2 * k] * up, x[2 * k + 1] * up, hi[k], lo[k]);
-                            uint8_t *dst = tile + col * 2048 + (r >> 3) * 128 + (r & 7) * 16;
-                            *(uint4 *)dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                            if (SPL == 2) *(uint4 *)(dst + C::QTILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            *(uint4 *)(row + g * 2048) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            if (SPL == 2) *(uint4 *)(row + g * 2048 + C::QTILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                         }
-                        if (col == 0) head->factor[t * 128 + r] = fabsf(p.scale) * 1.4426950408889634f * down;
+                        if (pass == 0) power_scale(top, up, down);
                     }
+                    factor *= down;
                 }
                 fence_proxy_async();
             }
@@ -259,7 +283,6 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             bool fresh = true;                                   // nothing seen yet: mm says nothing
             bool ok = true;
             if (active) {
-                const float factor = head->factor[t * 128 + quarter * 32 + lane];
                 int lo, hi;
                 row_limits(p, u, min(at, u.r1 - 1), lo, hi);
                 const int lo_most = __reduce_max_sync(0xffffffffu, lo), hi_least = __reduce_min_sync(0xffffffffu, hi);
@@ -374,7 +397,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             const float v0 = vref > 0.f ? vref : 1.f;
             const bool complete = piece.first == 0 && n == u.nt;
             const int r = at - u.r0;
-            float *slot = (float *)p.workspace + (size_t)(blockIdx.x * 2 + (piece.first ? 0 : 1)) * part_floats(R, p.dim);
+            float *slot = parts_of(p) + (size_t)(blockIdx.x * 2 + (piece.first ? 0 : 1)) * part_floats(R, p.dim);
             float *part = slot + R * 2 + (size_t)r * p.dim;
             const float f = complete ? v0 * inverse_of(l) : v0;
             T *dst = out_row<T>(p, u, min(at, u.r1 - 1));
