@@ -182,23 +182,31 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
     uint2 *qs = (uint2 *)(smem + C::O_Q);
     float *merge = (float *)(smem + C::O_MERGE);
     float2 *ml = (float2 *)(smem + C::O_ML);
-    Piece piece;
-    bool gone = false;
-    while (walk.next(piece)) {
+    // this warp's rows of q for a piece: asked for while the piece before it runs
+    auto rows_of = [&](const Unit &u, Vec8<T> (&q)[NB]) {
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            const int at = u.r0 + warp + i * RW;
+            q[i] = at < u.r1 && lane < p.dim / 8 ? load8<T>(q_row<T>(p, u, at) + lane * 8, p.q_wide) : zero8<T>();
+        }
+    };
+    Piece piece, coming;
+    Vec8<T> q[NB];
+    bool gone = false, more = walk.next(coming);
+    if (more) rows_of(coming.unit, q);
+    while (more) {
+        piece = coming;
         const Unit &u = piece.unit;
         // the rows of q, scaled and cut, in the order of the products' operands
         named_bar_sync(1, 32 * RW);            // the last piece's buffers are free
-        for (int r = warp; r < C::R; r += RW) {
-            const int at = u.r0 + r;
-            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (at < u.r1 && lane < p.dim / 8) {
-                const T *src = q_row<T>(p, u, at) + lane * 8;
-                const Vec8<T> v = load8<T>(src, p.q_wide);
-                unpack8(v, x);
-            }
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            const int r = warp + i * RW, at = u.r0 + r;
+            float x[8];
+            unpack8(q[i], x);
             float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[i]));
+            for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[k]));
 #pragma unroll
             for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             float up, down;
@@ -225,6 +233,8 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                 head->hi[r] = hi;
             }
         }
+        more = walk.next(coming);
+        if (more) rows_of(coming.unit, q);
         named_bar_sync(1, 32 * RW);
         float factor[NB][2];
         int lo[NB][2], hi[NB][2];
