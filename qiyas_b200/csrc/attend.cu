@@ -1,6 +1,6 @@
 // Attention over the 8-bit cache: which kernel takes a call, and how its work is cut.
 //
-//  * attend_rows.cu: at most 16 rows (query heads x tokens that share a head of the cache): the cache's bytes bound it.
+//  * attend_rows.cu: few rows (query heads x tokens that share a head of the cache): the cache's bytes bound it.
 //  * attend_tiles.cu: more rows: the tensor cores (tcgen05) take 128 rows of queries at a time.
 #include <cuda.h>
 #include "common.cuh"
@@ -40,9 +40,19 @@ static Plan plan_of(const qb200_cache_t &c, const qb200_sequences_t &s, const qb
 {
     const int64_t rows = (int64_t)(a.q_heads / c.heads) * a.max_queries;
     Plan plan;
-    plan.tiles = rows > 16;
+    // Few rows: attend_rows.cu, which reads the cache (from the L2 after the first time) once for every 16 rows of a head, 8
+    // where dim is over 128.  Measured at 8 sequences of 6000 tokens, 4 heads, bf16, us (rows, then tiles): dim 128: 16 rows
+    // 26 and 51, 32 rows 36 and 52, 64 rows 47 and 53, 96 rows 74 and 55; dim 256: 16 rows 44 and 86, 40 rows 81 and 88, 64
+    // rows 121 and 92; dim 64: 64 rows 32 and 39, 96 rows 49 and 41.
+    plan.tiles = rows > (c.dim <= 128 ? 64 : 48);
     plan.r = plan.tiles ? (c.dim <= 128 ? 256 : 128) : c.dim <= 128 && rows > 8 ? 16 : 8;
-    plan.whole = !plan.tiles && a.max_length <= 1024 && (int64_t)s.count * c.heads * rows < 1 << 30;
+    // Units cut (equal shares, a second kernel) or each to a block of its own.  In tokens of 128 dims a block takes (about 11
+    // cycles each): a unit costs 256 besides its tokens where the blocks stay, 556 where each has its own, the cut ones' partition
+    // and second kernel 1500 once.  Measured, 8 heads, bf16, us (whole, cut): 1 sequence of 500 tokens 6.9 and 10.1, of 1000
+    // 9.4 and 10.7, of 2000 14.6 and 11.6; 16 sequences of 2000 18 and 23; 64 of 1000 42 and 38.
+    const int64_t units = (int64_t)s.count * c.heads * ((rows + plan.r - 1) / plan.r);
+    const int64_t length = (int64_t)a.max_length * c.dim / 128, waves = (units + g_attend_sms - 1) / (g_attend_sms > 0 ? g_attend_sms : 1);
+    plan.whole = !plan.tiles && units < 1 << 30 && waves * (length + 556) <= units * (length + 256) / (g_attend_sms > 0 ? g_attend_sms : 1) + 1500;
     return plan;
 }
 

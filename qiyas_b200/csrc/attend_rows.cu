@@ -17,8 +17,9 @@
 //    token g, and V's chunk g of tokens 2t, 2t+1, 2t+8, 2t+9.
 //  * sk goes into the score's factor.  sv goes into the exponent: with v0 the first V scale a warp meets, the weights are
 //    w = 2^(s + log2(sv / v0) - m), the sum of them with v0 / sv as factor is the denominator, and O = v0 * sum w cv.
-//    m is chosen so that w lies at 2^7 at its largest when it is set and is kept while w stays below 2^15: f16 then holds
-//    weights down to 2^-29 of the largest with all its bits, and the accumulators are seldom rescaled.
+//    m is chosen so that w lies at 2^11 at its largest when it is set and is kept while w stays below 2^15: f16 then holds
+//    weights down to 2^-24 of the largest with all its bits and errs by 2^-35 of it below, and the accumulators are seldom
+//    rescaled.
 //  * q is scaled by a power of two to a row's maximum of 2^13 and cut to f16; with f32 lanes q and w enter as the sum of
 //    two f16 (SPL 2), which loses 2^-22.
 #include <cuda.h>
@@ -355,7 +356,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                         float top = fmaxf(fmaxf(s[0][nb][c], s[0][nb][c + 2]), fmaxf(s[1][nb][c], s[1][nb][c + 2]));
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        const float next = fmaxf(mm[nb][c], top - 7.f), less = exp2_fast(mm[nb][c] - next);
+                        const float next = fmaxf(mm[nb][c], top - 11.f), less = exp2_fast(mm[nb][c] - next);
                         mm[nb][c] = next;
                         l[nb][c] *= less;
 #pragma unroll

@@ -33,7 +33,7 @@ struct TilesCfg {
     static constexpr int NG = TT / 16;
     static constexpr int WARPS = 4 * NQ + CW + 4, THREADS = 32 * WARPS;       // the last four: one issues the products
     // registers a thread: of the launch (65536 over the threads, whole eights), and of the softmax, converter and last warps
-    static constexpr int REGS = NQ == 2 ? 96 : 128, SOFT_REGS = NQ == 2 ? 136 : 176, CONV_REGS = NQ == 2 ? 72 : 104, REST_REGS = NQ == 2 ? 64 : 128;
+    static constexpr int REGS = NQ == 2 ? 96 : 128, SOFT_REGS = NQ == 2 ? 128 : 176, CONV_REGS = NQ == 2 ? 80 : 104, REST_REGS = NQ == 2 ? 64 : 128;
     static_assert(NQ * SOFT_REGS + 2 * CONV_REGS + REST_REGS <= (NQ + 3) * REGS, "the shares of the registers fit the launch's");
     static constexpr uint32_t QTILE = 128 * DC * 2, SLOT = TT * DC * 2;
     static constexpr uint32_t O_Q = 0, O_K = NQ * SPL * QTILE, O_V = O_K + SLOTS * SLOT, O_HEAD = O_V + SLOTS * SLOT, SMEM = O_HEAD + 2048 + 1024;
@@ -45,7 +45,7 @@ struct TilesCfg {
 struct TilesHead {
     uint64_t qfull, ofull, drain;
     uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-    uint64_t sfull[4], pfull[4];               // of the S buffers, two a row tile
+    uint64_t sfull[4], pfull[4], odone[2];     // of the S buffers, two a row tile; of O, one a row tile
     float4 scales[4][4];                       // beside K's slots, of a tile's groups of 16 tokens: sk, log2(sv / v0), v0 / sv, v0
     Start start;
     uint32_t tmem;
@@ -140,25 +140,6 @@ __device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b)
     return d;
 }
 
-// 2^x0, 2^x1 without the exponential unit: x = n + f with |f| <= 1/2, 2^f by its Taylor polynomial of degree 5 (what is
-// left out is below 0.00016 * 2^-6, 4e-6 of the value), n added to the exponent.  Below 2^-120: 2^-120.
-__device__ __forceinline__ void exp2_pair(float x0, float x1, float &e0, float &e1)
-{
-    constexpr float MAGIC = 12582912.f;                        // 1.5 * 2^23: the sum's low bits are the integer
-    const uint64_t x = pair(fmaxf(x0, -120.f), fmaxf(x1, -120.f)), n = pair_add(x, pair(MAGIC, MAGIC));
-    const uint64_t f = pair_fma(pair_add(n, pair(-MAGIC, -MAGIC)), pair(-1.f, -1.f), x);
-    uint64_t y = pair_fma(f, pair(0.0013333558f, 0.0013333558f), pair(0.009618129f, 0.009618129f));
-    y = pair_fma(y, f, pair(0.055504109f, 0.055504109f));
-    y = pair_fma(y, f, pair(0.240226507f, 0.240226507f));
-    y = pair_fma(y, f, pair(0.693147181f, 0.693147181f));
-    y = pair_fma(y, f, pair(1.f, 1.f));
-    float n0, n1, y0, y1;
-    unpair(n, n0, n1);
-    unpair(y, y0, y1);
-    e0 = __int_as_float(__float_as_int(y0) + (__float_as_int(n0) << 23));
-    e1 = __int_as_float(__float_as_int(y1) + (__float_as_int(n1) << 23));
-}
-
 template <int DC, int SPL, typename T>
 __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_kernel(const __grid_constant__ AttendArgs p)
 {
@@ -171,13 +152,14 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
     const uint32_t base_u32 = smem_u32(smem);
     const uint32_t qfull = smem_u32(&head->qfull), ofull = smem_u32(&head->ofull), drain = smem_u32(&head->drain);
     const uint32_t kfull = smem_u32(head->kfull), kempty = smem_u32(head->kempty), vfull = smem_u32(head->vfull), vempty = smem_u32(head->vempty);
-    const uint32_t sfull = smem_u32(head->sfull), pfull = smem_u32(head->pfull);
+    const uint32_t sfull = smem_u32(head->sfull), pfull = smem_u32(head->pfull), odone = smem_u32(head->odone);
 
     if (threadIdx.x == 0) {
         head->abort = 0;
         mbar_init(qfull, 4 * NQ);
         mbar_init(ofull, 2);
         mbar_init(drain, 2);
+        for (int i = 0; i < 2; i++) mbar_init(odone + 8 * i, 1);
         for (int i = 0; i < 4; i++) {
             mbar_init(kfull + 8 * i, 5);           // the converters', and the tile's scales
 
@@ -332,7 +314,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                     if (__any_sync(0xffffffffu, above)) {
                         float up = 0.f, less = 1.f;
                         if (above) {
-                            up = ceilf(top) - 7.f;
+                            up = ceilf(top) - 11.f;
                             if (!fresh) less = exp2_fast(-up);
                             fresh = false;
                         }
@@ -341,8 +323,9 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
 #pragma unroll
                         for (int i = 0; i < 64; i++) x[i] -= up;
                         if (j > 0) {                             // O so far, once the product before has ended
-                            const uint32_t was = seq + j - 1;
-                            if (!mbar_wait_soon_lanes(vempty + 8 * (was % SLOTS), was / SLOTS & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
+                            // (the barrier is at this phase or just past it: S of this tile was issued behind the product before
+                            // the last, and the next product needs this tile's weights)
+                            if (!mbar_wait_soon_lanes(odone + 8 * t, (tiles + j - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
                             tc_fence_after();
 #pragma unroll 1
                             for (int d = 0; d < p.dim; d += 16) {
@@ -364,10 +347,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
 #pragma unroll
                             for (int i = 0; i < 16; i += 4) {
                                 const float *y = x + 32 * c + 16 * e + i;
-                                float e0 = exp2_fast(y[0]), e1 = exp2_fast(y[1]), e2, e3;
-                                // a quarter of the exponentials on the fma pipe, where their cut to f16 hides the polynomial's error
-                                if (SPL == 1 && i % 8 == 0) exp2_pair(y[2], y[3], e2, e3);
-                                else { e2 = exp2_fast(y[2]); e3 = exp2_fast(y[3]); }
+                                const float e0 = exp2_fast(y[0]), e1 = exp2_fast(y[1]), e2 = exp2_fast(y[2]), e3 = exp2_fast(y[3]);
                                 sum0 = pair_add(sum0, pair(e0, e1));
                                 sum1 = pair_add(sum1, pair(e2, e3));
                                 split2(e0, e1, w[8 * e + i / 2], w2[8 * e + i / 2]);
@@ -393,7 +373,6 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             pieces++;
             if (!active) continue;
             tc_fence_after();
-            if (fresh) l = 0.f;                                  // (what is hidden weighs 2^-120 at most, not always nothing)
             const float v0 = vref > 0.f ? vref : 1.f;
             const bool complete = piece.first == 0 && n == u.nt;
             const int r = at - u.r0;
@@ -587,6 +566,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 col += SPL == 2 ? 32 : 16;
                 accumulate = 1;
             }
+            mma_commit(odone + 8 * t);
             release(vempty + 8 * slot, nq);
         };
         while (ok && walk.next(piece)) {

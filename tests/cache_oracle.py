@@ -45,7 +45,7 @@ class Cache:
 
 def attend(q, k, v, scale, causal=True, window=0):
     """q [n, heads, dim], k and v [tokens, kv heads, dim], all float64 -> out, lse, and what the tolerances are made of:
-    sum p |v| and the largest scale * sum |q| |k| of a row."""
+    sum p |v|, and the largest scale * sum |q| |k| of a row."""
     n, heads, dim = q.shape
     length, kv = k.shape[:2]
     group = heads // kv

@@ -225,7 +225,9 @@ def check_attention(s, kind, lens, counts, heads, group, causal=True, window=0, 
     """CacheAttention on a setup against the definition.  The tolerance, for a row with weights p: the scores are sums of dim
     products in f32 (an error of (dim + 8) * 2^-24 of scale * sum |q||k| each, 2^-20 for the cut of q, the exponentials and
     V's scales), the weights are cut to f16 (half a step, 2^-11; f32 lanes: two f16, 2^-21), and the sums over tokens run in
-    f32 over tokens / 128 + 64 steps.  All of that is relative to sum p |v|; the output is rounded once more to its type."""
+    f32 over tokens / 128 + 64 steps.  All of that is relative to sum p |v|; the output is rounded once more to its type.  Below
+    f16's normal numbers a weight is off by half of 2^-24 whatever its size: the largest weight is 2^10 at least, so that is
+    2^-35 of the largest of p * (V's scale), each time a code of V, 127 at most."""
     import torch
     o = H.ops()
     cache = s.on_gpu()
@@ -251,7 +253,9 @@ def check_attention(s, kind, lens, counts, heads, group, causal=True, window=0, 
         want, want_lse, weight, size = attend(qn[at].astype(np.float64), k, v, scale, causal, window)
         score = (s.dim + 8) * 2.0 ** -24 * size + 2.0 ** -20 * (1 + np.abs(size))
         sums = (length / 128 + 64) * 2.0 ** -24
-        bound = weight * (2 * score[..., None] + cut + sums) + np.abs(want) * eps + 1e-30
+        # (p <= 1, so the largest V scale of the sequence bounds p * scale)
+        floor = 2.0 ** -35 * length * 127 * max([s.v.scales[x].max() for x in s.table[b][:(length + s.page - 1) // s.page]], default=0)
+        bound = weight * (2 * score[..., None] + cut + sums) + np.abs(want) * eps + floor + 1e-30
         if kind != "f32":
             bound = bound + (2.0 ** -25 if kind == "f16" else 0)            # f16 output below its normal numbers
         err = np.abs(got[at] - want)
@@ -285,6 +289,7 @@ def test_attention_of_several_rows(kind, heads, group, page, dim, window, causal
     counts = [5, 7, 2, 9, 0, 50, 1, 33]                # the third and fourth have rows that see nothing
     s = Setup(dim + group, len(lens), 200, heads, page, dim)
     check_attention(s, kind, lens, counts, heads * group, group, causal, window)
+    check_attention(s, kind, lens, counts, heads * group, group, causal, window, max_queries=1)        # the kernel for few rows
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -292,6 +297,36 @@ def test_attention_cut_over_many_blocks(kind):
     s = Setup(77, 3, 5000, 2, 16, 128)
     check_attention(s, kind, [5000, 1, 2777], [1, 1, 1], 16, 8)
     check_attention(s, kind, [5000, 1, 2777], [2, 0, 3], 8, 4, window=1500)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,group,page,dim,window", [(2, 4, 64, 128, 0), (1, 3, 16, 256, 0), (1, 8, 32, 64, 700), (2, 2, 128, 112, 100)])
+def test_attention_of_pieces_of_prompts(kind, heads, group, page, dim, window):
+    """Row tiles of 128 and 256, whole and not, over contexts that several blocks share."""
+    lens, counts = [900, 1300, 70, 333], [40, 130, 70, 1]
+    s = Setup(dim * 2 + group, len(lens), 1300, heads, page, dim)
+    check_attention(s, kind, lens, counts, heads * group, group, True, window)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_of_many_sequences(kind):
+    """More sequences than a warp has lanes, some without rows, some without tokens, their work cut into equal shares."""
+    rng = np.random.default_rng(5)
+    lens = [int(x) for x in rng.integers(0, 200, 75)]
+    lens[3], lens[40], lens[74] = 3000, 2500, 0
+    counts = [int(x) for x in rng.integers(0, 3, 75)]
+    s = Setup(85, 75, 3000, 1, 16, 64)
+    check_attention(s, kind, lens, counts, 2, 2, max_queries=2)
+    check_attention(s, kind, lens, counts, 2, 2)
+    counts = [1] * 75
+    check_attention(s, kind, lens, counts, 2, 2, with_offsets=False)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.5])
+def test_attention_with_other_scales(scale):
+    s = Setup(86, 2, 300, 1, 32, 128)
+    check_attention(s, "f32", [300, 41], [3, 30], 4, 4, scale=scale)
+    check_attention(s, "bf16", [300, 41], [3, 30], 4, 4, scale=scale, max_queries=1)
 
 
 def test_bounds_that_are_too_small_change_nothing():
@@ -422,6 +457,57 @@ def test_same_bits_every_time_and_on_another_stream_and_as_a_graph():
                 g.replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+def test_a_captured_step_writes_and_attends_with_new_lengths():
+    """Write and attention in one graph, replayed as the sequences grow: lengths and rows are read on the device."""
+    import torch
+    s = Setup(87, 3, 100, 2, 16, 64)
+    o, cache = H.ops(), s.on_gpu()
+    table, before, after = gpu(s.table), ints([0, 15, 40]), ints([1, 16, 41])
+    k, v, q = (torch.zeros(3, h, 64, device="cuda") for h in (2, 2, 6))
+    out = torch.empty_like(q)
+    o.CacheWrite(cache, k, v, table, ints([0, 0, 0]))          # once outside the capture; the page is written again below
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        st = torch.cuda.current_stream()
+        o.CacheWrite(cache, k, v, table, before, stream=st)
+        o.CacheAttention(cache, q, out, table, after, stream=st)
+    cache.k_codes.copy_(gpu(s.k.codes)), cache.v_codes.copy_(gpu(s.v.codes))
+    cache.k_scales.copy_(gpu(s.k.scales)), cache.v_scales.copy_(gpu(s.v.scales))
+    for step in range(20):
+        lens = [step, 15 + step, 40 + step]
+        rows = [s.rows(3, h, "f32")[1] for h in (2, 2, 6)]
+        for t, x in zip((k, v, q), rows):
+            t.copy_(gpu(x))
+        before.copy_(ints(lens)), after.copy_(ints([n + 1 for n in lens]))
+        graph.replay()
+        for b, n in enumerate(lens):
+            s.k.write(s.table[b], n, rows[0][b:b + 1])
+            s.v.write(s.table[b], n, rows[1][b:b + 1])
+            kk, vv = s.k.values(s.table[b], 0, n + 1), s.v.values(s.table[b], 0, n + 1)
+            want = attend(rows[2][b:b + 1].astype(np.float64), kk, vv, 0.125)[0]
+            assert np.abs(out[b:b + 1].double().cpu().numpy() - want).max() <= 2e-5 * np.abs(vv).max()
+    assert np.array_equal(cache.k_codes.cpu().numpy(), s.k.codes)
+    assert o.gpu.status() == 0
+
+
+def test_empty_calls_do_nothing():
+    import torch
+    s = Setup(88, 2, 32, 1, 16, 32)
+    o, cache = H.ops(), s.on_gpu()
+    none = torch.empty(0, 1, 32, device="cuda")
+    o.CacheWrite(cache, none, none, gpu(s.table), ints([0, 0]), offsets=ints([0, 0, 0]))
+    o.CacheRead(cache, none, none, gpu(s.table), ints([0, 0]), offsets=ints([0, 0, 0]))
+    o.CacheAttention(cache, none, none, gpu(s.table), ints([5, 5]), offsets=ints([0, 0, 0]))
+    empty = torch.empty(0, 2, dtype=torch.int32, device="cuda")
+    o.CacheAttention(cache, none, none, empty, ints([]))
+    rows = torch.full((4, 1, 32), 3.0, device="cuda")                   # rows, but of no sequence
+    o.CacheWrite(cache, rows, rows, gpu(s.table), ints([0, 0]), offsets=ints([0, 0, 0]))
+    out = torch.full_like(rows, 9.0)
+    o.CacheAttention(cache, rows, out, gpu(s.table), ints([5, 5]), offsets=ints([0, 0, 0]))
+    assert (out == 9).all() and o.gpu.status() == 0
+    assert np.array_equal(cache.k_codes.cpu().numpy(), s.k.codes)
 
 
 def test_a_layer_as_it_is_used():
