@@ -5,7 +5,7 @@
 // of 128 x 128 x 128, 2048 cycles of the tensor pipe, and as many cycles of the exponential unit.  So:
 //  * S = q K^T and O += P V are tcgen05.mma kind::f16 (codes are exact in f16), issued by one thread, S, P and O in tensor
 //    memory: P replaces S in place as f16 and is read from there as the second product's A operand.
-//  * Eight converter warps fetch the codes (16 bytes a load) and store them as f16: K as core matrices of 8 tokens x 8 dims,
+//  * Four converter warps (eight for dims over 128) fetch the codes (16 bytes a load) and store them as f16: K as core matrices of 8 tokens x 8 dims,
 //    V as rows of 64 dims with the 128-byte swizzle, which the second product reads across (a row a dim: MN-major).  Every
 //    byte of the cache is converted once for the 256 rows of a block.
 //  * A group of four softmax warps a row tile, a thread a row, with two buffers of S: the tensor pipe is a tile of tokens
@@ -22,8 +22,6 @@
 
 namespace qb {
 
-constexpr int CW = 8;                          // converter warps: four for K, four for V
-
 template <int DC, int SPL>
 struct TilesCfg {
     static constexpr int TT = 64;                               // tokens a tile
@@ -31,10 +29,11 @@ struct TilesCfg {
     static constexpr int R = 128 * NQ;
     static constexpr int SLOTS = (SPL == 1 ? 2 : 1) * (DC == 128 ? 2 : 1);      // of K and of V
     static constexpr int NG = TT / 16;
+    static constexpr int CW = DC == 128 ? 4 : 8, KW = CW / 2;   // converter warps: half of them for K, half for V
     static constexpr int WARPS = 4 * NQ + CW + 4, THREADS = 32 * WARPS;       // the last four: one issues the products
     // registers a thread: of the launch (65536 over the threads, whole eights), and of the softmax, converter and last warps
-    static constexpr int REGS = NQ == 2 ? 96 : 128, SOFT_REGS = NQ == 2 ? 128 : 176, CONV_REGS = NQ == 2 ? 80 : 104, REST_REGS = NQ == 2 ? 64 : 128;
-    static_assert(NQ * SOFT_REGS + 2 * CONV_REGS + REST_REGS <= (NQ + 3) * REGS, "the shares of the registers fit the launch's");
+    static constexpr int REGS = 128, SOFT_REGS = NQ == 2 ? 152 : 176, CONV_REGS = NQ == 2 ? 128 : 104, REST_REGS = NQ == 2 ? 80 : 128;
+    static_assert(NQ * SOFT_REGS + CW / 4 * CONV_REGS + REST_REGS <= WARPS / 4 * REGS, "the shares of the registers fit the launch's");
     static constexpr uint32_t QTILE = 128 * DC * 2, SLOT = TT * DC * 2;
     static constexpr uint32_t O_Q = 0, O_K = NQ * SPL * QTILE, O_V = O_K + SLOTS * SLOT, O_HEAD = O_V + SLOTS * SLOT, SMEM = O_HEAD + 2048 + 1024;
     static_assert(SMEM <= 232448, "227 KB of shared memory");
@@ -45,7 +44,7 @@ struct TilesCfg {
 struct TilesHead {
     uint64_t qfull, ofull, drain;
     uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-    uint64_t sfull[4], pfull[4], odone[2];     // of the S buffers, two a row tile; of O, one a row tile
+    uint64_t sfull[4], pfull[4], odone[2];     // of the S buffers, two a row tile; of O before a piece's last tile
     float4 scales[4][4];                       // beside K's slots, of a tile's groups of 16 tokens: sk, log2(sv / v0), v0 / sv, v0
     Start start;
     uint32_t tmem;
@@ -144,7 +143,7 @@ template <int DC, int SPL, typename T>
 __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_kernel(const __grid_constant__ AttendArgs p)
 {
     using C = TilesCfg<DC, SPL>;
-    constexpr int TT = C::TT, NQ = C::NQ, R = C::R, SLOTS = C::SLOTS, NG = C::NG;
+    constexpr int TT = C::TT, NQ = C::NQ, R = C::R, SLOTS = C::SLOTS, NG = C::NG, CW = C::CW, KW = C::KW;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     TilesHead *head = (TilesHead *)(smem + C::O_HEAD);
@@ -161,10 +160,10 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         mbar_init(drain, 2);
         for (int i = 0; i < 2; i++) mbar_init(odone + 8 * i, 1);
         for (int i = 0; i < 4; i++) {
-            mbar_init(kfull + 8 * i, 5);           // the converters', and the tile's scales
+            mbar_init(kfull + 8 * i, KW + 1);           // the converters', and the tile's scales
 
             mbar_init(kempty + 8 * i, 8);          // the softmax warps' (with one row tile they arrive twice)
-            mbar_init(vfull + 8 * i, 4);
+            mbar_init(vfull + 8 * i, KW);
             mbar_init(vempty + 8 * i, 2);          // the products' ends, of both row tiles (or twice of one)
             mbar_init(sfull + 8 * i, 1);
             mbar_init(pfull + 8 * i, 4);
@@ -191,7 +190,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         Walk<R, TT, false> walk(p, head->start);
         Piece piece;
-        uint32_t pieces = 0, seq = 0, tiles = 0;                 // so far: pieces, tiles of the block, of this row tile
+        uint32_t pieces = 0, seq = 0, tiles = 0, ends = 0;       // so far: pieces, tiles of the block, of this row tile; phases of odone
         while (walk.next(piece)) {
             const Unit &u = piece.unit;
             const int nq = NQ == 2 && u.r1 - u.r0 > 128 ? 2 : 1;
@@ -323,9 +322,11 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
 #pragma unroll
                         for (int i = 0; i < 64; i++) x[i] -= up;
                         if (j > 0) {                             // O so far, once the product before has ended
-                            // (the barrier is at this phase or just past it: S of this tile was issued behind the product before
-                            // the last, and the next product needs this tile's weights)
-                            if (!mbar_wait_soon_lanes(odone + 8 * t, (tiles + j - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) { ok = false; break; }
+                            // S of the next tile is issued behind that product, so its end is the product's too; the last tile has
+                            // no next one, and a barrier of its own
+                            const bool last = j + 1 == n;
+                            if (!mbar_wait_soon_lanes(last ? odone + 8 * t : sfull + 8 * (2 * t + (buf ^ 1)), (last ? ends : (tiles + j + 1) >> 1) & 1, abort, status,
+                                                      STATUS_ATTEND_WAIT)) { ok = false; break; }
                             tc_fence_after();
 #pragma unroll 1
                             for (int d = 0; d < p.dim; d += 16) {
@@ -367,7 +368,10 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 }
             }
             seq += n;
-            if (active) tiles += n;
+            if (active) {
+                tiles += n;
+                ends += n > 1;
+            }
             ok = __all_sync(0xffffffffu, ok);
             if (!ok || !mbar_wait_lanes(ofull, pieces & 1, abort, status, STATUS_ATTEND_WAIT)) break;
             pieces++;
@@ -402,11 +406,11 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
     } else if (warp < 4 * NQ + CW) {
         // ------------------------------------------------------------------ converters
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::CONV_REGS));
-        const int kv = (warp - 4 * NQ) >> 2, w = (warp - 4 * NQ) & 3;
+        const int kv = (warp - 4 * NQ) / KW, w = (warp - 4 * NQ) % KW;
         const int8_t *codes = kv ? p.v_codes : p.k_codes;
         const uint32_t full = kv ? vfull : kfull, empty = kv ? vempty : kempty;
         uint8_t *slots = smem + (kv ? C::O_V : C::O_K);
-        constexpr int GROUPS = TT / 32, HALVES = DC / 64;        // groups of 8 tokens a warp; a lane: a token and every fourth chunk of 16 dims
+        constexpr int GROUPS = TT / 8 / KW, HALVES = DC / 64;        // groups of 8 tokens a warp; a lane: a token and every fourth chunk of 16 dims
         constexpr int LOADS = GROUPS * HALVES;
         const int r8 = lane & 7, c4 = lane >> 3, chunks = p.dim >> 4;
         // where a chunk's two halves of 8 dims go.  K: core matrices, [8 dims][8 tokens]; V: rows of 64 dims, 128 bytes, with
@@ -415,13 +419,13 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
         const int at1 = kv ? w * 1024 + r8 * 128 + (((2 * c4 + 1) ^ r8) << 4) : at0 + TT * 16;
         KvWalk<R, TT> tiles(p, head->start);
         auto page_of = [&](const KvTile<R, TT> &t) {             // lane i: the page of this warp's i-th group
-            return page_at(p, t.b, t.base + (lane * 4 + w) * 8, 8, t.lo, t.hi, t.there && lane < GROUPS);
+            return page_at(p, t.b, t.base + (lane * KW + w) * 8, 8, t.lo, t.hi, t.there && lane < GROUPS);
         };
         auto load = [&](const KvTile<R, TT> &t, int id, uint4 (&raw)[LOADS]) {
 #pragma unroll
             for (int i = 0; i < GROUPS; i++) {
                 const int page = __shfl_sync(0xffffffffu, id, i);
-                const int token = t.base + (i * 4 + w) * 8 + r8;
+                const int token = t.base + (i * KW + w) * 8 + r8;
                 const int8_t *row = codes + ((((int64_t)page * p.heads + t.h) << p.log_page) + (token & ((1 << p.log_page) - 1))) * p.dim;
 #pragma unroll
                 for (int k = 0; k < HALVES; k++)
@@ -455,7 +459,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                                 h[2 * q] = codes_lo(x);
                                 h[2 * q + 1] = codes_hi(x);
                             }
-                            uint8_t *at = dst + i * (kv ? 4096 : 512) + k * (TT * 128);
+                            uint8_t *at = dst + i * (KW * (kv ? 1024 : 128)) + k * (TT * 128);
                             *(uint4 *)(at + at0) = make_uint4(h[0], h[1], h[2], h[3]);
                             *(uint4 *)(at + at1) = make_uint4(h[4], h[5], h[6], h[7]);
                         }
@@ -547,7 +551,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             }
             mma_commit(sfull + 8 * (2 * t + buf));
         };
-        auto sums = [&](int j, int nq) {
+        auto sums = [&](int j, int nq, bool last) {          // last: of those that another tile's weights follow
             const uint32_t slot = (seq + j) % SLOTS;
             const int buf = (tiles + j) & 1;
             if (!wait(vfull + 8 * slot, (seq + j) / SLOTS) || !wait(pfull + 8 * (2 * t + buf), (tiles + j) >> 1)) return;
@@ -566,7 +570,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 col += SPL == 2 ? 32 : 16;
                 accumulate = 1;
             }
-            mma_commit(odone + 8 * t);
+            if (last) mma_commit(odone + 8 * t);
             release(vempty + 8 * slot, nq);
         };
         while (ok && walk.next(piece)) {
@@ -578,7 +582,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 scores(0);
                 for (int j = 0; j < n && ok; j++) {
                     if (j + 1 < n) scores(j + 1);
-                    if (ok) sums(j, nq);
+                    if (ok) sums(j, nq, j + 2 == n);
                 }
                 if (!ok) break;
                 release(ofull, nq);
