@@ -297,7 +297,8 @@ int qb200_ipc_close(void *ptr);
  *
  * qb200_lanes: an array of rows in f32, f16 or bf16 (`type` of the call); element (row, head, i) is at base + row *
  * row_stride + head * head_stride + i, strides in elements.  Where base and strides are multiples of 16 bytes the loads
- * are wide. */
+ * are wide.  Rows that are read may repeat (a stride of 0); rows that are written lie apart from each other (strides of dim
+ * at least) and from everything the call reads. */
 typedef struct qb200_cache {
     void *k_codes, *v_codes;
     float *k_scales, *v_scales;

@@ -472,13 +472,16 @@ static int check_cache(const qb200_cache_t *c, const qb200_sequences_t *s, int t
     return 0;
 }
 
-static int check_lanes(const char *name, int type, const qb200_lanes_t &x, int rows, int heads)
+// dim: 0, or (written lanes) the values of a head, which have to lie apart from those of other rows and heads
+static int check_lanes(const char *name, int type, const qb200_lanes_t &x, int rows, int heads, int dim = 0)
 {
     if (rows > 0 && !x.base) return fail(QB200_E_POINTER, "%s: null", name);
     if ((uintptr_t)x.base & (type == QB200_F32 ? 3 : 1)) return fail(QB200_E_POINTER, "%s: misaligned", name);
     const int64_t most = (int64_t)1 << 55;        // products with 32-bit counts stay inside 64 bits of bytes
     if (x.row_stride < 0 || x.head_stride < 0 || x.row_stride > most / ((int64_t)rows + 1) || x.head_stride > most / ((int64_t)heads + 1))
         return fail(QB200_E_SHAPE, "%s: strides %lld, %lld", name, (long long)x.row_stride, (long long)x.head_stride);
+    if ((rows > 1 && x.row_stride < dim) || (heads > 1 && x.head_stride < dim))
+        return fail(QB200_E_SHAPE, "%s: strides %lld, %lld: rows of %d values that are written overlap", name, (long long)x.row_stride, (long long)x.head_stride, dim);
     return 0;
 }
 
@@ -499,8 +502,8 @@ int qb200_cache_read(const qb200_cache_t *cache, const qb200_sequences_t *sequen
     int rc = check_cache(cache, sequences, type);
     if (rc) return rc;
     if (!k && !v) return fail(QB200_E_POINTER, "neither k nor v is asked for");
-    if (k && (rc = check_lanes("k", type, *k, sequences->rows, cache->heads))) return rc;
-    if (v && (rc = check_lanes("v", type, *v, sequences->rows, cache->heads))) return rc;
+    if (k && (rc = check_lanes("k", type, *k, sequences->rows, cache->heads, cache->dim))) return rc;
+    if (v && (rc = check_lanes("v", type, *v, sequences->rows, cache->heads, cache->dim))) return rc;
     OnDevice on;
     if (!g_ready) return fail(QB200_E_DEVICE, "qb200_init has not succeeded");
     if (on.e) return cuda_fail(on.e, "cudaSetDevice");
@@ -515,6 +518,7 @@ static void attention_bounds(const qb200_cache_t &c, const qb200_sequences_t &s,
     const int64_t most = (int64_t)s.width * c.page;
     if (a.max_queries <= 0 || a.max_queries > rows) a.max_queries = rows > 0 ? rows : 1;
     if (a.max_length <= 0 || a.max_length > most) a.max_length = most > 0 ? (int)most : 1;
+    if (a.window >= most) a.window = 0;       // as much as any sequence has; differences with it stay inside 32 bits
 }
 
 size_t qb200_cache_attention_workspace_bytes(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const qb200_attention_t *attention)
@@ -533,7 +537,7 @@ int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *s
     qb200_attention_t a = *attention;
     if (a.q_heads <= 0 || a.q_heads % cache->heads) return fail(QB200_E_SHAPE, "%d query heads over %d heads of the cache: a whole group each", a.q_heads, cache->heads);
     if ((int64_t)a.q_heads * sequences->rows > 2147483647LL - 65536) return fail(QB200_E_LIMIT, "%d rows x %d heads: at most 2^31 - 65537", sequences->rows, a.q_heads);
-    if ((rc = check_lanes("q", type, a.q, sequences->rows, a.q_heads)) || (rc = check_lanes("out", type, a.out, sequences->rows, a.q_heads))) return rc;
+    if ((rc = check_lanes("q", type, a.q, sequences->rows, a.q_heads)) || (rc = check_lanes("out", type, a.out, sequences->rows, a.q_heads, cache->dim))) return rc;
     if ((uintptr_t)a.lse & 3) return fail(QB200_E_POINTER, "misaligned lse");
     if (a.window < 0 || (a.window > 0 && !a.causal)) return fail(QB200_E_SHAPE, "window %d: a window looks back from a row's own token, so it needs causal", a.window);
     if (!(a.scale == a.scale) || a.scale - a.scale != 0.f) return fail(QB200_E_SHAPE, "scale is not a finite number");

@@ -1,19 +1,28 @@
-// Attention over the 8-bit cache for many rows (prompts, guessed tokens, large groups) on the fifth-generation tensor cores.
+// Attention over the 8-bit cache for many rows (prompts, large groups) on the fifth-generation tensor cores.
 //
-// out = softmax(scale * q K^T) V as in attend_rows.cu, with 128 rows (tokens x the query heads of a group) a tile and tiles
-// of TT tokens of the cache.  Here the operations bound it: a pair of row tiles and 128 tokens of 128 dims are 2 x 2 products
-// of 128 x 128 x 128, 2048 cycles of the tensor pipe, and as many cycles of the exponential unit.  So:
-//  * S = q K^T and O += P V are tcgen05.mma kind::f16 (codes are exact in f16), issued by one thread, S, P and O in tensor
-//    memory: P replaces S in place as f16 and is read from there as the second product's A operand.
-//  * Four converter warps (eight for dims over 128) fetch the codes (16 bytes a load) and store them as f16: K as core matrices of 8 tokens x 8 dims,
-//    V as rows of 64 dims with the 128-byte swizzle, which the second product reads across (a row a dim: MN-major).  Every
-//    byte of the cache is converted once for the 256 rows of a block.
-//  * A group of four softmax warps a row tile, a thread a row, with two buffers of S: the tensor pipe is a tile of tokens
-//    ahead, so the chain from a product's end through the barrier, the softmax and the next product's issue is hidden (with
-//    one buffer of 128 tokens a row tile it was not: 7700 cycles for 128 tokens, 2048 of them the tensor pipe's).
-//  * A thread reads its row of S once, 32 tokens at a time, and takes the weights against the exponent it has: only where one
-//    would pass 2^15 does it go back over what the row has of O and of the tile's weights, in place, by a power of two.
+// out = softmax(scale * q K^T) V as in attend_rows.cu, with 128 rows (tokens x the query heads of a group) a row tile, up to
+// two row tiles a block, and tiles of 64 tokens of the cache.  Here the operations bound it: two row tiles, 64 tokens and 128
+// dims are 1280 cycles of the tensor pipe and 1024 of the exponential unit.  So:
+//  * S = q K^T and O += P V are tcgen05.mma kind::f16 (codes are exact in f16), a thread a row tile issuing them, S, P and O
+//    in tensor memory: P replaces S in place as f16 and is read from there as the second product's A operand.
+//  * Four converter warps (eight for dims over 128) fetch the codes, 16 bytes a load, a tile ahead in registers, and store
+//    them as f16: K as core matrices of 8 tokens x 8 dims, V as rows of 64 dims with the 128-byte swizzle, which the second
+//    product reads across (a row a dim: MN-major; from unswizzled core matrices it took half as long again).  Every byte of
+//    the cache is converted once for the 256 rows of a block.  One warp fetches the tiles' scales.
+//  * Four softmax warps a row tile, a thread a row, with two buffers of S: the tensor pipe is a tile of tokens ahead.
+//  * A thread reads its row of S once and takes the weights against the exponent it has: only where one would pass 2^15 does
+//    it raise the exponent and go back over what the row has of O, by a power of two.
+//  * The registers are shared out between the warps' kinds (setmaxnreg), so that none spills.
 // Scales, exponents and the cut of q and w are those of attend_rows.cu; so are the shares of the grid's blocks.
+//
+// Measured: 7894 queries of 32 heads (8 of the cache) over up to 8192 tokens, causal, 128 dims, bf16: 1.18 ms, 666 TFLOP/s, 39 %
+// of the library's bf16 product.  Three chains are near one another there (with the work of one left out in a copy): the
+// converters 1.01 ms, the softmax 1.00 ms, the products with their barriers 0.82 ms; what they wait for is mostly
+// instructions (16 warps of four kinds, 90 KB of code).  Tried and dropped: tiles of 128 tokens with one buffer of S a row tile
+// (1.3 ms: the chain from a product through softmax to the next is not hidden), a maximum pass over S before the weights
+// (1.7 ms), one issuing thread (1.3 ms), issue by a whole warp (1.56 ms), a quarter or half of the exponentials as
+// polynomials on the fma pipe (4 and 18 % slower: the exponential unit is not the bound), five commits a tile
+// instead of two (3 %).
 #include <type_traits>
 #include "common.cuh"
 #include "attend_device.cuh"
@@ -30,8 +39,9 @@ struct TilesCfg {
     static constexpr int SLOTS = (SPL == 1 ? 2 : 1) * (DC == 128 ? 2 : 1);      // of K and of V
     static constexpr int NG = TT / 16;
     static constexpr int CW = DC == 128 ? 4 : 8, KW = CW / 2;   // converter warps: half of them for K, half for V
-    static constexpr int WARPS = 4 * NQ + CW + 4, THREADS = 32 * WARPS;       // the last four: one issues the products
-    // registers a thread: of the launch (65536 over the threads, whole eights), and of the softmax, converter and last warps
+    static constexpr int WARPS = 4 * NQ + CW + 4, THREADS = 32 * WARPS;       // the last four: two issue the products, one fetches scales
+    // registers a thread: of the launch, and of the softmax, converter and last warps (checked against the build when the
+    // library is bound: a share above the launch's would wait for good)
     static constexpr int REGS = 128, SOFT_REGS = NQ == 2 ? 152 : 176, CONV_REGS = NQ == 2 ? 128 : 104, REST_REGS = NQ == 2 ? 80 : 128;
     static_assert(NQ * SOFT_REGS + CW / 4 * CONV_REGS + REST_REGS <= WARPS / 4 * REGS, "the shares of the registers fit the launch's");
     static constexpr uint32_t QTILE = 128 * DC * 2, SLOT = TT * DC * 2;

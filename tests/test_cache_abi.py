@@ -97,6 +97,16 @@ def test_attention_refuses(lib):
     assert attention(lib, workspace=4104) == WORKSPACE
 
 
+@pytest.mark.parametrize("row,head", [(0, 64), (63, 64), (512, 0), (512, 48)])
+def test_written_rows_that_overlap_are_refused(lib, row, head):
+    from qiyas_b200 import _lib
+    bad, good = lanes(256, row, head), lanes(256, 512, 64)
+    assert lib.qb200_cache_read(parts(), sequences(), B.F16, bad, good, None) == SHAPE
+    assert lib.qb200_cache_read(parts(), sequences(), B.F16, None, bad, None) == SHAPE
+    args = _lib.ATTENTION(256, 512, 64, 256, row, head, 0, 4096, 1 << 40, 8, 0, 0, 0.125, 1, 0)
+    assert lib.qb200_cache_attention(parts(), sequences(), B.F16, args, None) == SHAPE
+
+
 def test_a_good_call_needs_a_device(lib):
     import torch
     if torch.cuda.is_available():

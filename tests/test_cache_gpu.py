@@ -322,6 +322,32 @@ def test_attention_of_many_sequences(kind):
     check_attention(s, kind, lens, counts, 2, 2, with_offsets=False)
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 100, 320, 319])
+@pytest.mark.parametrize("max_queries", [0, 1])
+def test_windows_of_all_there_is_and_more_rows_than_tokens(window, max_queries):
+    s = Setup(35, 4, 320, 1, 64, 128)
+    check_attention(s, "bf16", [320, 5, 0, 300], [9, 40, 30, 70], 2, 2, window=window, max_queries=max_queries)
+
+
+def test_repeated_rows_of_q_and_of_what_is_written():
+    """Rows read with a stride of 0: the same row for every token."""
+    import torch
+    o = H.ops()
+    s = Setup(36, 2, 96, 2, 16, 64)
+    cache = s.on_gpu()
+    q = torch.randn(1, 4, 64, device="cuda").to(torch.bfloat16)
+    out, wide = (torch.zeros(2, 4, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    o.CacheAttention(cache, q.expand(2, 4, 64), out, gpu(s.table), ints([40, 90]))
+    o.CacheAttention(cache, q.repeat(2, 1, 1), wide, gpu(s.table), ints([40, 90]))
+    assert torch.equal(out, wide)
+    k, back, v_back = torch.randn(1, 1, 64, device="cuda"), torch.zeros(2, 2, 64, device="cuda"), torch.zeros(2, 2, 64, device="cuda")
+    o.CacheWrite(cache, k.expand(2, 2, 64), k.expand(2, 2, 64), gpu(s.table), ints([0, 0]))
+    o.CacheRead(cache, back, v_back, gpu(s.table), ints([0, 0]))
+    assert torch.equal(back, v_back) and torch.equal(back[0, 0], back[1, 1])
+    assert (back[0, 0] - k[0, 0]).abs().max() <= 0.5001 * k.abs().max() / 127
+    assert o.gpu.status() == 0
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 2.5])
 def test_attention_with_other_scales(scale):
     s = Setup(86, 2, 300, 1, 32, 128)
