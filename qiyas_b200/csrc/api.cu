@@ -526,7 +526,7 @@ size_t qb200_cache_attention_workspace_bytes(const qb200_cache_t *cache, const q
     if (!attention || check_cache(cache, sequences, type) || attention->q_heads <= 0 || attention->q_heads % cache->heads) return 0;
     qb200_attention_t a = *attention;
     attention_bounds(*cache, *sequences, a);
-    return qb::attend_workspace_bytes(*cache, *sequences, a);
+    return qb::attend_workspace_bytes(*cache, *sequences, type, a);
 }
 
 int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const qb200_attention_t *attention, void *stream)
@@ -543,7 +543,7 @@ int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *s
     if (!(a.scale == a.scale) || a.scale - a.scale != 0.f) return fail(QB200_E_SHAPE, "scale is not a finite number");
     if (a.max_queries < 0 || a.max_length < 0) return fail(QB200_E_SHAPE, "max_queries %d, max_length %d", a.max_queries, a.max_length);
     attention_bounds(*cache, *sequences, a);
-    const size_t need = qb::attend_workspace_bytes(*cache, *sequences, a);
+    const size_t need = qb::attend_workspace_bytes(*cache, *sequences, type, a);
     if (need && (!a.workspace || a.workspace_bytes < need))
         return fail(QB200_E_WORKSPACE, "workspace of %zu bytes, %zu needed", a.workspace ? a.workspace_bytes : (size_t)0, need);
     if ((uintptr_t)a.workspace & 15) return fail(QB200_E_WORKSPACE, "workspace not 16-byte aligned");

@@ -56,10 +56,12 @@ static Plan plan_of(const qb200_cache_t &c, const qb200_sequences_t &s, const qb
     return plan;
 }
 
-size_t attend_workspace_bytes(const qb200_cache_t &c, const qb200_sequences_t &s, const qb200_attention_t &a)
+size_t attend_workspace_bytes(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const qb200_attention_t &a)
 {
     const Plan plan = plan_of(c, s, a);
-    return plan.whole ? 0 : marks_bytes(g_attend_sms) + (size_t)g_attend_sms * 2 * part_floats(plan.r, c.dim) * 4;
+    if (plan.whole) return 0;
+    const size_t kept = plan.tiles && type == QB200_F32 ? (size_t)plan.r * c.dim : 0;
+    return marks_bytes(g_attend_sms) + (size_t)g_attend_sms * (2 * part_floats(plan.r, c.dim) + kept) * 4;
 }
 
 // The codes as rows of dim bytes, fetched box_rows tokens and box_dim dims at a time (zeros past dim).

@@ -200,6 +200,9 @@ struct Mark {
 __host__ __device__ constexpr size_t marks_bytes(int grid) { return ((size_t)grid * sizeof(Mark) + 255) / 256 * 256; }
 __device__ __forceinline__ float *parts_of(const AttendArgs &p) { return (float *)((uint8_t *)p.workspace + marks_bytes(p.grid)); }
 
+// attend_tiles.cu, f32 lanes: a block's sums so far, behind the parts.
+__device__ __forceinline__ float *kept_of(const AttendArgs &p, int r) { return parts_of(p) + (size_t)p.grid * 2 * part_floats(r, p.dim); }
+
 template <int R, int TT>
 __device__ __forceinline__ Start share_of(const AttendArgs &p, int block)        // by a whole warp
 {

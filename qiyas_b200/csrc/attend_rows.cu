@@ -73,6 +73,22 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void *map, int x
                  : "memory");
 }
 
+// c += A.b.  The tensor cores cut their sums off, where f32 additions round: with f32 lanes (b = b[0] + b[1]) the products of 16
+// are summed by themselves, what the cut left first, and added with a rounding.
+template <int SPL>
+__device__ __forceinline__ void add_products(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint2 (&b)[SPL])
+{
+    if (SPL == 1) {
+        mma16816(c, a0, a1, a2, a3, b[0].x, b[0].y);
+        return;
+    }
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
+    mma16816(d, a0, a1, a2, a3, b[SPL - 1].x, b[SPL - 1].y);
+    mma16816(d, a0, a1, a2, a3, b[0].x, b[0].y);
+#pragma unroll
+    for (int i = 0; i < 4; i++) c[i] += d[i];
+}
+
 template <int DT, int NB, int SPL, typename T>
 __global__ void __launch_bounds__(RTHREADS, 1)
 attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap)
@@ -313,9 +329,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                             const uint32_t w0 = word(a[mt][0], q) ^ 0x80808080u, w1 = word(a[mt][1], q) ^ 0x80808080u;
                             const uint32_t a0 = codes_lo(w0), a1 = codes_lo(w1), a2 = codes_hi(w0), a3 = codes_hi(w1);
 #pragma unroll
-                            for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                                for (int x = 0; x < SPL; x++) mma16816(s[mt][nb], a0, a1, a2, a3, b[nb][x].x, b[nb][x].y);
+                            for (int nb = 0; nb < NB; nb++) add_products<SPL>(s[mt][nb], a0, a1, a2, a3, b[nb]);
                         }
                     }
                 }
@@ -373,11 +387,12 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                             }
                     }
             }
-            uint32_t w[2][NB][SPL][2];
+            uint2 w[2][NB][SPL];
 #pragma unroll
             for (int mt = 0; mt < 2; mt++)
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++) {
+                    uint32_t half[SPL][2];
                     float e[4];
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
@@ -388,9 +403,11 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                     for (int k = 0; k < 2; k++) {
                         uint32_t a, b;
                         split2(e[2 * k], e[2 * k + 1], a, b);
-                        w[mt][nb][0][k] = transposed8(a);
-                        if (SPL == 2) w[mt][nb][SPL - 1][k] = transposed8(b);
+                        half[0][k] = transposed8(a);
+                        if (SPL == 2) half[SPL - 1][k] = transposed8(b);
                     }
+#pragma unroll
+                    for (int z = 0; z < SPL; z++) w[mt][nb][z] = make_uint2(half[z][0], half[z][1]);
                 }
 
             // ---- O^T += V^T P^T
@@ -418,9 +435,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                             const uint32_t x = k ? x1 : x0, y = k ? y1 : y0;
                             const uint32_t a0 = codes_lo(x), a1 = codes_hi(x), a2 = codes_lo(y), a3 = codes_hi(y);
 #pragma unroll
-                            for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                                for (int z = 0; z < SPL; z++) mma16816(o[sub * 4 + q][k][nb], a0, a1, a2, a3, w[mt][nb][z][0], w[mt][nb][z][1]);
+                            for (int nb = 0; nb < NB; nb++) add_products<SPL>(o[sub * 4 + q][k][nb], a0, a1, a2, a3, w[mt][nb]);
                         }
                     }
                 }

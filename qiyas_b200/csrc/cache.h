@@ -22,7 +22,7 @@ int cache_read(const qb200_cache_t &c, const qb200_sequences_t &s, int type, con
 
 // max_queries and max_length have been given values
 cudaError_t attend_init(int sm_count, int max_smem, int *status);
-size_t attend_workspace_bytes(const qb200_cache_t &c, const qb200_sequences_t &s, const qb200_attention_t &a);
+size_t attend_workspace_bytes(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const qb200_attention_t &a);
 int attend(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const qb200_attention_t &a, cudaStream_t stream);
 
 }  // namespace qb

@@ -322,6 +322,43 @@ def test_attention_of_many_sequences(kind):
     check_attention(s, kind, lens, counts, 2, 2, with_offsets=False)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,rising", [(128, 1.0), (128, 8.0), (192, 8.0)])
+def test_long_parts_of_prompts(kind, dim, rising):
+    """Parts of a thousand tokens and more in one block, of keys that stay as large or grow, so that the largest score comes
+    late.  The definition in 64 bits, with torch; the tolerance of check_attention."""
+    import torch
+    o = H.ops()
+    heads, group, lens, counts = 8, 4, [3000, 1300, 2100], [300, 257, 40]
+    s = Setup(37, 3, 3000, heads, 64, dim)
+    for row in s.table:
+        s.k.scales[row] *= np.linspace(1 / rising, rising, s.width)[:, None].astype(np.float32)
+    q, qn = s.rows(sum(counts), heads * group, kind)
+    out, lse = torch.zeros_like(q), torch.zeros(sum(counts), heads * group, device="cuda")
+    offsets = offsets_of(counts)
+    scale = dim ** -0.5
+    o.CacheAttention(s.on_gpu(), q, out, gpu(s.table), ints(lens), offsets=ints(offsets), lse=lse)
+    assert o.gpu.status() == 0
+    cut = 2.0 ** -21 if kind == "f32" else 2.0 ** -11
+    for b, (length, n) in enumerate(zip(lens, counts)):
+        at = slice(offsets[b], offsets[b] + n)
+        k, v = (gpu(x.values(s.table[b], 0, length)).double().transpose(0, 1).repeat_interleave(group, 0) for x in (s.k, s.v))
+        x = q[at].double().transpose(0, 1)
+        scores = torch.matmul(x, k.transpose(1, 2)) * scale
+        unseen = torch.arange(length, device="cuda") > length - n + torch.arange(n, device="cuda")[:, None]
+        size = (torch.matmul(x.abs(), k.abs().transpose(1, 2)) * scale).masked_fill_(unseen, 0).amax(-1)
+        scores.masked_fill_(unseen, -float("inf"))
+        want_lse = torch.logsumexp(scores, -1)
+        p = torch.exp(scores - want_lse[..., None])
+        want, weight = torch.matmul(p, v), torch.matmul(p, v.abs())
+        score = (dim + 8) * 2.0 ** -24 * size + 2.0 ** -20 * (1 + size)
+        sums = (length / 128 + 64) * 2.0 ** -24
+        floor = 2.0 ** -35 * length * 127 * float(s.v.scales[s.table[b]].max())
+        bound = weight * (2 * score[..., None] + cut + sums) + want.abs() * torch.finfo(kind_of(kind)).eps / 2 + floor + 2.0 ** -25
+        assert bool(((out[at].double().transpose(0, 1) - want).abs() <= bound).all()), b
+        assert bool(((lse[at].double().transpose(0, 1) - want_lse).abs() <= score + sums + 2.0 ** -21 * (1 + want_lse.abs())).all()), b
+
+
 @pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 100, 320, 319])
 @pytest.mark.parametrize("max_queries", [0, 1])
 def test_windows_of_all_there_is_and_more_rows_than_tokens(window, max_queries):
