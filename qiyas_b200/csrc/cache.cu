@@ -10,9 +10,9 @@
 // writer and nothing is atomic.  A group holds everything it writes in registers: each value is read once.  Which sequence
 // and page a group has follows from the rows' offsets alone: sequence b gets rows/page + 2 places, as many as it can touch.
 //
-// The memory bounds long prompts: 25 370 tokens of 8 heads x 128 in f16, pages of 64, are written in 42 us and read back in 31,
-// 4.2 TB/s together (65 % of the copy peak); 43 288 tokens in bf16, pages of 16, are read back at 5.2 TB/s (79 %).  A write is 10 instructions
-// a value: the largest magnitude as bits, two values at a time (it was 5 a value in floats, 65 us), and the check of the
+// The memory bounds long prompts: 25 370 tokens of 8 heads x 128 in f16, pages of 64, are written in 42 us and read back in 27,
+// 4.5 TB/s together (69 % of the copy peak); 43 288 tokens in bf16, pages of 16, are read back at 5.4 TB/s (83 %).  A write is
+// 10 instructions a value, and three quarters of the issue slots are taken: the largest magnitude as bits, two values at a time (it was 5 a value in floats, 65 us), and the check of the
 // rounding eight values at a time.  One token a sequence is a launch's latency, 5 us.
 #include "common.cuh"
 #include "cache.h"
@@ -246,6 +246,13 @@ __global__ void __launch_bounds__(item_threads(LANES)) cache_write_kernel(const 
     }
 }
 
+// Byte i of a word of codes as a float: under the exponent of 2^23 the code + 128 is the last byte.  (Conversions from integers
+// run on the unit of the exponentials, a quarter as wide: it was 81 % busy, and reading took 31 us where it takes 27.)
+__device__ __forceinline__ float code_at(uint32_t w, int i)
+{
+    return __fsub_rn(__uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7440 + i)), 8388736.f);
+}
+
 template <typename T, int LANES>
 __global__ void __launch_bounds__(item_threads(LANES)) cache_read_kernel(const __grid_constant__ CacheArgs p)
 {
@@ -274,7 +281,7 @@ __global__ void __launch_bounds__(item_threads(LANES)) cache_read_kernel(const _
         if (tid + j * LANES >= total) break;
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = __fmul_rn((float)(int8_t)((i < 4 ? c[j].x : c[j].y) >> 8 * (i & 3)), scale);
+        for (int i = 0; i < 8; i++) v[i] = __fmul_rn(code_at(i < 4 ? c[j].x : c[j].y, i & 3), scale);
         store8<T>(dst + row * stride + col * 8, v, wide);
         row += drow;
         col += dcol;
