@@ -522,6 +522,41 @@ def test_same_bits_every_time_and_on_another_stream_and_as_a_graph():
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
 
 
+def test_calls_at_once_on_two_streams():
+    """Both kernels and products of blocks beside each other: each call gives the bits it gives alone."""
+    import torch
+    from qiyas_b200 import blocks as B
+    o = H.ops()
+    s = Setup(38, 4, 2000, 2, 32, 128)
+    cache, table, lens = s.on_gpu(), gpu(s.table), ints([2000, 700, 1999, 3])
+    calls = []
+    for n, kind in ((1, "bf16"), (100, "f32"), (60, "f16")):
+        q = s.rows(4 * n, 8, kind)[0]
+        calls.append((q, ints([0, n, 2 * n, 3 * n, 4 * n]), torch.empty_like(q)))
+    rows, cols = 515, 4096
+    a, x = gpu(B.make_weights(B.Q4_0, rows, cols, 5)), gpu(B.make_activations(cols, 6))
+    y = torch.empty(rows, device="cuda")
+    for q, at, out in calls:
+        o.CacheAttention(cache, q, out, table, lens, offsets=at)
+    o.GemvBlocks(B.Q4_0, a, x, y, rows, cols, fmt_x=B.F32)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[torch.empty_like(out) for _ in range(2)] for _, _, out in calls]
+    ys = [torch.empty_like(y) for _ in range(2)]
+    torch.cuda.synchronize()
+    for turn in range(10):
+        for i, stream in enumerate(streams):
+            for k in range(3):
+                q, at, _ = calls[(k + i) % 3]
+                o.CacheAttention(cache, q, got[(k + i) % 3][i], table, lens, offsets=at, stream=stream)
+            o.GemvBlocks(B.Q4_0, a, x, ys[i], rows, cols, fmt_x=B.F32, stream=stream)
+    torch.cuda.synchronize()
+    assert o.gpu.status() == 0
+    for (_, _, out), pair in zip(calls, got):
+        assert torch.equal(out, pair[0]) and torch.equal(out, pair[1])
+    assert torch.equal(y, ys[0]) and torch.equal(y, ys[1])
+
+
 def test_a_captured_step_writes_and_attends_with_new_lengths():
     """Write and attention in one graph, replayed as the sequences grow: lengths and rows are read on the device."""
     import torch
