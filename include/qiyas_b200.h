@@ -317,11 +317,11 @@ typedef struct qb200_lanes {
 
 /* Writes the rows of k and v as tokens lengths[b], lengths[b] + 1, ... of their sequences (lengths[b] = tokens that are
  * in the cache already).  The definition, block by block: let a be the largest magnitude written into the block, s the
- * block's scale if earlier tokens of the sequence lie in it, else 0, n = a * (1/127) in f32 (both rounded).  Where n <= s the scale stays s;
- * else it becomes max(n, 1.25 * s), and the earlier tokens' codes c become the integer nearest c * s / scale (a scale
+ * block's scale if earlier tokens of the sequence lie in it, else 0, n = a * (1/127) in f32 (both rounded).  Where n <= |s| the scale stays s;
+ * else it becomes max(n, 1.25 * |s|), and the earlier tokens' codes c become the integer nearest c * s / scale (a scale
  * that has to grow grows by a quarter at least, so that however many tokens arrive one by one, rounding again and again
  * costs a code 2.5 steps at most).  New codes are the integers nearest x / scale, ties to even, from the exact quotients.  A block of zeros has
- * scale 0.  A NaN is stored as 0 and an infinity as the code +-127; neither enters a, and both set bit 5 of the status word.
+ * scale 0.  A NaN is stored as 0 and an infinity as the code +-127 that gives its sign; neither enters a, and both set bit 5 of the status word.
  * Two calls that write the same block must be ordered (one stream, or an event); a page written to must not belong to two
  * sequences of a call. */
 int qb200_cache_write(const qb200_cache_t *cache, const qb200_sequences_t *sequences, int type, const qb200_lanes_t *k, const qb200_lanes_t *v,

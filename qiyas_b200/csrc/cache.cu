@@ -1,8 +1,8 @@
 // A cache of keys and values in 8 bits: what is written is quantised on the way in, and read back.
 //
 // A block is `page` tokens of one sequence in one head: int8 codes [page][dim], contiguous, and one f32 scale.  The
-// arithmetic (also in the header): n = max|x| * (1/127); the scale s of a block that holds earlier tokens stays where n <= s,
-// else it becomes max(n, 1.25 s) and the earlier codes c are rounded again to rn(c * s / scale); new codes are
+// arithmetic (also in the header): n = max|x| * (1/127); the scale s of a block that holds earlier tokens stays where n <= |s|,
+// else it becomes max(n, 1.25 |s|) and the earlier codes c are rounded again to rn(c * s / scale); new codes are
 // rn(x / scale).  Growth by a quarter at least bounds what repeated rounding costs: the errors of the earlier roundings
 // shrink by 4/5 with each later one, half a step * 1 / (1 - 4/5) = 2.5 steps, whatever the number of tokens.
 //
@@ -123,11 +123,12 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], float scale, floa
     return w;
 }
 
-// The same for scales whose reciprocal leaves the type's range or whose half is not exact, and for NaN and infinities.
+// The same for scales whose reciprocal leaves the type's range or whose half is not exact, for a caller's scales below zero, and
+// for NaN and infinities.
 __device__ __noinline__ uint32_t code_of_any(float x, float scale)
 {
     if (scale == 0.f || x != x) return 0;
-    if (fabsf(x) > 3.402823466e38f) return (uint32_t)(x > 0.f ? 127 : -127) & 0xffu;
+    if (fabsf(x) > 3.402823466e38f) return (uint32_t)((x > 0.f) == (scale > 0.f) ? 127 : -127) & 0xffu;
     const double q = rint((double)x / (double)scale);
     return (uint32_t)(int)fmin(fmax(q, -127.), 127.) & 0xffu;
 }
@@ -208,9 +209,9 @@ __global__ void __launch_bounds__(item_threads(LANES)) cache_write_kernel(const 
     if (odd && tid == 0) atomicOr(p.status, STATUS_CACHE_VALUE);
 
     const float need = __fmul_rn(top, 1.f / 127.f);
-    const float scale = need <= had ? had : fmaxf(need, __fmul_rn(had, 1.25f));
-    if (scale != had && it.first && had > 0.f) {
-        // the earlier tokens' codes in the new scale (exact products, correctly rounded quotients)
+    const float scale = need <= fabsf(had) ? had : fmaxf(need, __fmul_rn(fabsf(had), 1.25f));
+    if (scale != had && it.first) {
+        // the earlier tokens' codes in the new scale (exact products, correctly rounded quotients): zeros where it was 0
         const int words = it.first * p.dim >> 2;
         uint32_t *old = (uint32_t *)codes;
         const double s0 = had, s1 = scale;
