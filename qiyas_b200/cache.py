@@ -7,7 +7,7 @@ has no counterpart (it keeps keys and values in its plain types).
 ========  ======================================  ============================================================
 k_codes   int8 [pages, heads, page, dim]          page: 16, 32, 64 or 128 tokens; dim: a multiple of 16 up to 256
 v_codes   int8 [pages, heads, page, dim]
-k_scales  float32 [pages, heads]                  a stored value is code * scale
+k_scales  float32 [pages, heads]                  a stored value is code * scale, any finite number
 v_scales  float32 [pages, heads]
 ========  ======================================  ============================================================
 

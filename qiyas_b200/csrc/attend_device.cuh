@@ -345,12 +345,46 @@ __device__ __forceinline__ int page_number(const AttendArgs &p, const Page &g, b
     if (g.wanted && report) atomicOr(p.status, STATUS_CACHE_RANGE);
     return -1;
 }
-__device__ __forceinline__ float2 scales_at(const AttendArgs &p, int page, int h)      // of K and of V; V's below zero: no page
+__device__ __forceinline__ float2 scales_at(const AttendArgs &p, int page, int h)      // of K and of V
 {
-    if (page < 0) return make_float2(0.f, -1.f);
+    if (page < 0) return make_float2(0.f, 0.f);
     const int64_t i = (int64_t)page * p.heads + h;
     return make_float2(__ldg(p.k_scales + i), __ldg(p.v_scales + i));
 }
+// What V's scale may be the reference for others: its size, or 0.
+__device__ __forceinline__ float reference_of(bool there, float sv) { return there && fabsf(sv) <= 3.402823466e38f ? fabsf(sv) : 0.f; }
+// How the tokens of a page are weighted: against the reference v0, which is above zero where some scale met so far is not 0.
+struct Weighted {
+    float log_ratio, inverse;                  // log2(|sv| / v0), added to the scores; v0 / |sv|, a weight's part of the denominator
+    uint32_t mark;                             // what else V's scale asks for
+};
+constexpr uint32_t MARK_ZERO = 1, MARK_MINUS = 2;      // of a scale of 0 (in the denominator, nothing to the sums), and below 0
+__device__ __forceinline__ Weighted weighted(float size, float v0)          // size: |sv|, above 0 and finite
+{
+    Weighted w = {0.f, 1.f, 0};
+    if (size != v0) {
+        w.log_ratio = log2_ratio(size, v0);
+        w.inverse = __fdividef(v0, size);
+    }
+    return w;
+}
+__device__ __forceinline__ Weighted weighted(bool there, float sv, float v0)
+{
+    Weighted w = {0.f, 1.f, 0};
+    const float size = fabsf(sv);
+    if (!there) {
+        w.log_ratio = -INFINITY;
+        w.inverse = 0.f;
+    } else if (size == 0.f) w.mark = MARK_ZERO;
+    else if (!(size <= 3.402823466e38f)) w.log_ratio = __int_as_float(0x7fffffff);     // rows that see it get NaN, others nothing of it
+    else {
+        w = weighted(size, v0);
+        w.mark = sv < 0.f ? MARK_MINUS : 0;
+    }
+    return w;
+}
+// Pairs of weights as the product with V takes them.
+__device__ __forceinline__ uint32_t marked(uint32_t pair, bool zero, bool minus) { return zero ? 0u : pair ^ (minus ? 0x80008000u : 0u); }
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)

@@ -18,6 +18,8 @@
 //    token g, and V's chunk g of tokens 2t, 2t+1, 2t+8, 2t+9.
 //  * sk goes into the score's factor.  sv goes into the exponent: with v0 the first V scale a warp meets, the weights are
 //    w = 2^(s + log2(sv / v0) - m), the sum of them with v0 / sv as factor is the denominator, and O = v0 * sum w cv.
+//    (|sv| is meant: where sv is below 0 the weights change sign, where it is 0 they are zeros in the second product, and a page
+//    that is not there has weights of 0 in the denominator too.)
 //    m is chosen so that w lies at 2^11 at its largest when it is set and is kept while w stays below 2^15: f16 then holds
 //    weights down to 2^-24 of the largest with all its bits and errs by 2^-35 of it below, and the accumulators are seldom
 //    rescaled.
@@ -57,6 +59,7 @@ struct RowsCfg {
 struct RowsHead {                              // at O_HEAD
     uint64_t full[24], empty[24];
     float4 scales[24];                         // of a stage: sk, sv of its first and second 16 tokens
+    uint32_t odd[24];                          // 0: both pages are there and sv is above 0 and finite; else 4, and bits 0 and 1 if they are there
     float factor[16];                          // rows: scale * log2 e / (what q was scaled by)
     int lo[16], hi[16];                        // rows: tokens they see
     Start start;
@@ -159,6 +162,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
             const int id_then = page_number(p, id_next, mine == 0);
             const float2 sc_then = scales_at(p, id_then, next.h);
             id_next = page_of(after);
+            const unsigned usual = __ballot_sync(0xffffffffu, id >= 0 && sc.y > 0.f && sc.y <= 3.402823466e38f);
             for (int k = (mine - seq) & (RP - 1); k < now.count; k += RP) {
                 const uint32_t tile = seq + k;
                 const int stage = tile % C::S;
@@ -170,6 +174,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                 if (lane == 0) {
                     const int live = (id0 >= 0 ? 1 : 0) + (per == 2 && id1 >= 0 ? 1 : 0);
                     head->scales[stage] = make_float4(k0, v0, k1, v1);
+                    head->odd[stage] = (usual >> l0 & usual >> l1 & 1) ? 0 : 4 | (id0 >= 0 ? 1 : 0) | (id1 >= 0 ? 2 : 0);
                     if (live) mbar_arrive_expect_tx(full0 + 8 * stage, live * 2 * C::SUB * bytes);
                     else mbar_arrive(full0 + 8 * stage);
                 }
@@ -297,6 +302,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
             const int stage = at % C::S;
             if (!mbar_wait_soon_lanes(full0 + 8 * stage, (at / C::S) & 1, abort, p.status, STATUS_ATTEND_WAIT)) { gone = true; break; }
             const float4 sc = head->scales[stage];
+            const uint32_t odd = head->odd[stage];
             const uint8_t *kt = smem + stage * C::STAGE, *vt = kt + C::HALF;
             const int base = (u.t0 + piece.first + j) * 32;
 
@@ -335,19 +341,21 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                 }
 
             // ---- weights
-            float lr[2], rinv[2];
+            Weighted v[2];
 #pragma unroll
             for (int mt = 0; mt < 2; mt++) {
                 const float sk = mt ? sc.z : sc.x, sv = mt ? sc.w : sc.y;
-                if (vref == 0.f && sv > 0.f) vref = sv;
-                lr[mt] = 0.f;
-                rinv[mt] = 1.f;
-                if (sv < 0.f) { lr[mt] = -INFINITY; rinv[mt] = 0.f; }          // a page that is not there
-                else if (sv > 0.f && sv != vref) { lr[mt] = log2_ratio(sv, vref); rinv[mt] = __fdividef(vref, sv); }
+                if (odd) {
+                    if (vref == 0.f) vref = reference_of(odd >> mt & 1, sv);
+                    v[mt] = weighted(odd >> mt & 1, sv, vref);
+                } else {
+                    if (vref == 0.f) vref = sv;
+                    v[mt] = weighted(sv, vref);
+                }
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) s[mt][nb][c] = __fmaf_rn(s[mt][nb][c], factor[nb][c & 1] * sk, lr[mt]);
+                    for (int c = 0; c < 4; c++) s[mt][nb][c] = __fmaf_rn(s[mt][nb][c], factor[nb][c & 1] * sk, v[mt].log_ratio);
             }
             if (base < lo_most || base + 32 > hi_least) {
 #pragma unroll
@@ -397,7 +405,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
                         e[c] = exp2_fast(s[mt][nb][c] - mm[nb][c & 1]);
-                        l[nb][c & 1] = __fmaf_rn(e[c], rinv[mt], l[nb][c & 1]);
+                        l[nb][c & 1] = __fmaf_rn(e[c], v[mt].inverse, l[nb][c & 1]);
                     }
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
@@ -409,6 +417,17 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
 #pragma unroll
                     for (int z = 0; z < SPL; z++) w[mt][nb][z] = make_uint2(half[z][0], half[z][1]);
                 }
+            if (odd) {                         // seldom: scales of 0 or below
+#pragma unroll
+                for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                        for (int z = 0; z < SPL; z++) {
+                            w[mt][nb][z].x = marked(w[mt][nb][z].x, v[mt].mark == MARK_ZERO, v[mt].mark == MARK_MINUS);
+                            w[mt][nb][z].y = marked(w[mt][nb][z].y, v[mt].mark == MARK_ZERO, v[mt].mark == MARK_MINUS);
+                        }
+            }
 
             // ---- O^T += V^T P^T
 #pragma unroll

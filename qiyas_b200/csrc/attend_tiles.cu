@@ -60,7 +60,8 @@ struct TilesHead {
     uint64_t qfull, ofull, drain;
     uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
     uint64_t sfull[4], pfull[4], odone[2];     // of the S buffers, two a row tile; of O before a piece's last tile
-    float4 scales[4][4];                       // beside K's slots, of a tile's groups of 16 tokens: sk, log2(sv / v0), v0 / sv, v0
+    float4 scales[4][4];                       // beside K's slots, of a tile's groups of 16 tokens: sk, log2(|sv| / v0), v0 / |sv|, and v0
+                                               // (the first group's: a bit a group, V's scale is 0, and from bit 16 on, it is below 0)
     Start start;
     uint32_t tmem;
     int abort;
@@ -302,6 +303,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
 #pragma unroll
                     for (int e = 0; e < NG; e++) sc[e] = head->scales[(seq + j) % SLOTS][e];
                     vref = sc[NG - 1].w;
+                    const uint32_t marks = __float_as_uint(sc[0].w);
                     tmem_ld_landed32(v[0]);
                     tmem_ld_landed32(v[1]);
                     __syncwarp();
@@ -394,6 +396,21 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                         if (SPL == 2) tmem_st16(s_at + 32 * c + 16, w2);
                     }
                     tmem_st_wait();
+                    if (marks) {                                 // seldom: scales of 0 or below; what was stored is put right
+#pragma unroll 1
+                        for (int c = 0; c < 2 * SPL; c++) {
+                            uint32_t w[16];
+                            tmem_ld16(s_at + 16 * c, w);
+                            tmem_ld_landed16(w);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                const int e = 2 * (c / SPL) + i / 8;
+                                w[i] = marked(w[i], marks >> e & 1, marks >> (16 + e) & 1);
+                            }
+                            tmem_st16(s_at + 16 * c, w);
+                        }
+                        tmem_st_wait();
+                    }
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(pfull + 8 * (2 * t + buf));
@@ -522,32 +539,39 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             KvTile<R, TT> now, next;
             now.there = next.there = false;
             Page page = {-1, false};
-            float2 sc = make_float2(0.f, -1.f);
+            float2 sc = make_float2(0.f, 0.f);
+            bool there = false;
             float vref = 0.f;
             uint32_t seq = 0;
 #pragma unroll 1
             do {
-                float2 sc_next = make_float2(0.f, -1.f);
-                if (next.there) sc_next = scales_at(p, page_number(p, page, true), next.h);
+                float2 sc_next = make_float2(0.f, 0.f);
+                bool there_next = false;
+                if (next.there) {
+                    const int id = page_number(p, page, true);
+                    sc_next = scales_at(p, id, next.h);
+                    there_next = id >= 0;
+                }
                 const KvTile<R, TT> after = walk.next();
                 page = page_of(after);
                 if (now.there) {
                 if (now.starts) vref = 0.f;
                 // V's scales against the first of the piece that is not zero
-                const unsigned some = __ballot_sync(0xffffffffu, sc.y > 0.f);
-                const float found = __shfl_sync(0xffffffffu, sc.y, some ? __ffs(some) - 1 : 0);
+                const float size = reference_of(there, sc.y);
+                const unsigned some = __ballot_sync(0xffffffffu, size > 0.f);
+                const float found = __shfl_sync(0xffffffffu, size, some ? __ffs(some) - 1 : 0);
                 if (vref == 0.f && some) vref = found;
-                float lr = 0.f, rinv = 1.f;
-                if (sc.y < 0.f) { lr = -INFINITY; rinv = 0.f; }
-                else if (sc.y > 0.f && sc.y != vref) { lr = log2_ratio(sc.y, vref); rinv = __fdividef(vref, sc.y); }
+                const Weighted v = weighted(there, sc.y, vref);
+                const uint32_t marks = __ballot_sync(0xffffffffu, v.mark == MARK_ZERO) | __ballot_sync(0xffffffffu, v.mark == MARK_MINUS) << 16;
                 if (seq >= SLOTS && !mbar_wait_soon_lanes(kempty + 8 * (seq % SLOTS), (seq / SLOTS - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) break;
-                if (lane < NG) head->scales[seq % SLOTS][lane] = make_float4(sc.x, lr, rinv, vref);
+                if (lane < NG) head->scales[seq % SLOTS][lane] = make_float4(sc.x, v.log_ratio, v.inverse, lane ? vref : __uint_as_float(marks));
                 __syncwarp();
                 if (lane == 0) mbar_arrive(kfull + 8 * (seq % SLOTS));
                 seq++;
                 }
                 now = next;
                 sc = sc_next;
+                there = there_next;
                 next = after;
             } while (now.there || next.there);
         }

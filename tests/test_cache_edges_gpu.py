@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from . import helpers as H
-from .test_cache_gpu import Setup, gpu, ints, kind_of
+from .test_cache_gpu import Setup, gpu, ints, kind_of, offsets_of
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,127 @@ def test_writes_behind_blocks_of_any_scale(kind, page, dim):
     out = H.empty(len(scales) * at * 2 * dim, t.dtype).view(-1, 2, dim)
     o.CacheRead(cache, out, None, gpu(s.table), ints([0] * len(scales)), offsets=ints(np.arange(len(scales) + 1) * at))
     assert (out[:at] == 0).all() and o.gpu.status() == 0                         # what a scale of zero held is zero still
+
+
+# query heads of a head of the cache, rows of each sequence: the kernel for few rows (one token, and a few), and the tile
+# kernel (more than 64 rows a head, 48 above 128 dims), one and two row tiles a unit
+ROWS = [(1, [1, 1, 1, 1]), (5, [3, 1, 2, 0]), (4, [1, 40, 17, 3]), (2, [130, 3, 200, 70])]
+KINDS = ["f32", "f16", "bf16"]
+
+
+def check(s, kind, lens, counts, group, causal=True, window=0, absent=(), status=0, q=None, out=None, table=None, **more):
+    """CacheAttention against the definition in 64 bits, for scales of any sign and size.  absent: (sequence, slot) pairs whose
+    pages `table` does not name.  The tolerance, for a row with weights p: the scores are sums of dim products in f32 ((dim + 8) *
+    2^-24 of scale * sum |q||k|), 2^-20 for the cut of q, the exponentials and the logarithms of V's scales, the weights are cut to
+    f16 (half a step, 2^-11; f32 lanes: two f16, 2^-21), the sums over tokens run in f32 over tokens / 128 + 64 steps: all relative
+    to sum p |v|.  The output is rounded once to its type.  Below f16's normal numbers a weight is off by 2^-35 of the largest of
+    p * |V's scale|, each time a code of V, 128 at most."""
+    import torch
+    o, heads, rows = H.ops(), s.heads * group, int(sum(counts))
+    if q is None:
+        q = s.rows(rows, heads, kind)[0]
+    if out is None:
+        out = torch.full_like(q, 5.0)
+    lse = torch.full((rows, heads), 5.0, device="cuda")
+    offsets, scale = offsets_of(counts), s.dim ** -0.5
+    o.CacheAttention(s.on_gpu(), q, out, gpu(s.table if table is None else table), ints(lens), offsets=ints(offsets), causal=causal, window=window,
+                     lse=lse, **more)
+    assert o.gpu.status() == status
+    eps, cut = torch.finfo(q.dtype).eps / 2, 2.0 ** -21 if kind == "f32" else 2.0 ** -11
+    for b, (length, n) in enumerate(zip(lens, counts)):
+        if n == 0:
+            continue
+        length = min(length, s.width * s.page)
+        at = slice(int(offsets[b]), int(offsets[b]) + n)
+        token = np.arange(length)
+        place = (length - n + np.arange(n))[:, None]
+        seen = token <= place if causal else np.ones((n, length), bool)
+        if window:
+            seen &= token > place - window
+        for x, slot in absent:
+            if x == b:
+                seen &= token // s.page != slot
+        k, v = (gpu(c.values(s.table[b], 0, length)).permute(1, 0, 2).repeat_interleave(group, 0) for c in (s.k, s.v))
+        x, seen = q[at].double().transpose(0, 1), gpu(seen)
+        scores = (x @ k.transpose(1, 2) * scale).masked_fill(~seen, -float("inf"))
+        size = (x.abs() @ k.abs().transpose(1, 2) * scale).masked_fill(~seen, 0).amax(-1) if length else torch.zeros(heads, n, device="cuda")
+        want_lse = torch.logsumexp(scores, -1)
+        p = torch.exp(scores - want_lse.masked_fill(want_lse.isneginf(), 0)[..., None])
+        want, weight = p @ v, p @ v.abs()
+        score = (s.dim + 8) * 2.0 ** -24 * size + 2.0 ** -20 * (1 + size)
+        sums = (length / 128 + 64) * 2.0 ** -24
+        most = np.abs(s.v.scales[s.table[b][:(length + s.page - 1) // s.page]])
+        floor = 2.0 ** -35 * length * 128 * float(most[np.isfinite(most)].max(initial=0))
+        bound = weight * (2 * score[..., None] + cut + sums) + want.abs() * eps + floor + (2.0 ** -25 if kind == "f16" else 1e-30)
+        err = (out[at].double().transpose(0, 1) - want).abs()
+        assert bool((err <= bound).all()), (b, float((err / bound).max()))
+        nothing = want_lse.isneginf()
+        got = lse[at].double().transpose(0, 1)
+        assert torch.equal(got.isneginf(), nothing) and bool((out[at].transpose(0, 1)[nothing] == 0).all())
+        off = (got - want_lse).masked_fill(nothing, 0).abs()
+        assert bool((off <= score + sums + 2.0 ** -21 * (1 + want_lse.masked_fill(nothing, 0).abs())).all()), b
+    return out, lse
+
+
+def odd_scales(s, rng, both=True):
+    """Scales of zero (and -0) and below zero among the others, under codes that are not zero; the first page, the last and a
+    whole sequence of zeros among them."""
+    for c in (s.k, s.v) if both else (s.v,):
+        pick = rng.integers(0, 10, c.scales.shape)
+        c.scales[pick < 3] *= -1
+        c.scales[pick == 3], c.scales[pick == 4] = 0.0, -0.0
+    s.v.scales[s.table[0, 0]] = 0
+    s.v.scales[s.table[0, -1]] = 0
+    s.v.scales[s.table[1]] = 0
+    s.v.scales[s.table[2, 0]] = -np.abs(s.v.scales[s.table[2, 0]])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("group,counts", ROWS)
+@pytest.mark.parametrize("page,dim", [(16, 64), (32, 128), (16, 192), (128, 96), (64, 256)])
+def test_attention_over_scales_of_zero_and_below(kind, group, counts, page, dim):
+    s = Setup(43 + dim, 4, 400, 2, page, dim)
+    odd_scales(s, s.rng)
+    for c in (s.k, s.v):
+        c.scales[s.table[:, 1]] = np.abs(c.scales).max()
+    check(s, kind, [400, 131, 399, 50], counts, group)
+    check(s, kind, [400, 131, 399, 50], counts, group, window=70, max_length=400)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("counts", [[1, 2], [100, 40]])
+def test_attention_over_nothing_but_scales_of_zero(kind, counts):
+    """Codes other than zero under scales of zero are zeros: they count in the denominator and add nothing."""
+    import torch
+    s = Setup(44, 2, 1500, 1, 16, 128)
+    s.v.scales[s.table[0]] = 0
+    s.v.scales[s.table[1, :40]], s.v.scales[s.table[1, 80:]] = 0, -0.0
+    check(s, kind, [1500, 1500], counts, 4)
+    o, cache, n = H.ops(), s.on_gpu(), sum(counts)
+    q, _ = s.rows(n, 4, kind)
+    out = torch.full_like(q, 3.0)
+    o.CacheAttention(cache, q, out, gpu(s.table), ints([1500, 1500]), offsets=ints([0, counts[0], n]))
+    assert (out[:counts[0]] == 0).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("counts", [[3, 2], [90, 40]])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_scales_that_are_not_finite_reach_the_rows_that_see_them_only(kind, counts, bad):
+    import torch
+    s = Setup(45, 2, 200, 1, 16, 64)
+    o, n = H.ops(), sum(counts)
+    q, _ = s.rows(n, 4, kind)
+    window, lens = 20, [200, 150]
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    args = (gpu(s.table), ints(lens))
+    o.CacheAttention(s.on_gpu(), q, want, *args, offsets=ints([0, counts[0], n]), window=window)
+    slot = (lens[0] - 1) // 16                           # of the first sequence, seen by its last rows
+    s.v.scales[s.table[0, slot]] = bad
+    o.CacheAttention(s.on_gpu(), q, out, *args, offsets=ints([0, counts[0], n]), window=window)
+    place = np.arange(lens[0] - counts[0], lens[0])
+    sees = np.zeros(n, bool)
+    sees[:counts[0]] = place >= slot * 16
+    sees = torch.from_numpy(sees).cuda()
+    assert sees.any() and out[sees].isnan().all()
+    assert torch.equal(out[~sees], want[~sees]) and o.gpu.status() == 0
