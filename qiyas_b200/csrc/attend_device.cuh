@@ -294,9 +294,16 @@ __device__ __forceinline__ float exp2_fast(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float log2_ratio(float a, float b)
+// A part of a row's sums, o * v0 and sum with weights against 2^m, is handed on with the sum brought to 2^-16 .. 2^-15 by a power of
+// two (less where v0 times that would leave f32): parts then join whatever reference each had, and values next to f32's
+// largest do not leave it.  Gives what o is to be multiplied by.
+__device__ __forceinline__ float part_scale(float &m, float &sum, float v0)
 {
-    return __log2f(__fdiv_rn(a, b));
+    const int e = sum == 0.f ? 0 : max(min((int)(__float_as_uint(sum) >> 23) - 127 + 16, 126), (__float_as_int(v0) >> 23) - 253);
+    const float up = __uint_as_float((uint32_t)(127 - e) << 23);
+    sum *= up;
+    m += (float)e;
+    return v0 * up;
 }
 // A power of two that brings `top` to 2^13 .. 2^14, and its reciprocal; 1 for zero, infinities and NaN.
 __device__ __forceinline__ void power_scale(float top, float &up, float &down)
@@ -351,34 +358,41 @@ __device__ __forceinline__ float2 scales_at(const AttendArgs &p, int page, int h
     const int64_t i = (int64_t)page * p.heads + h;
     return make_float2(__ldg(p.k_scales + i), __ldg(p.v_scales + i));
 }
-// What V's scale may be the reference for others: its size, or 0.
-__device__ __forceinline__ float reference_of(bool there, float sv) { return there && fabsf(sv) <= 3.402823466e38f ? fabsf(sv) : 0.f; }
-// How the tokens of a page are weighted: against the reference v0, which is above zero where some scale met so far is not 0.
+// V's scales enter the weights against a reference v0, a power of two: the largest scale of those first met, rounded down.  A
+// scale more than 2^FAR above v0 sets a new one, one more than 2^FAR below counts as 0.  So weights of up to 2^15 against a page FAR
+// above v0 leave those against one FAR below above f32's least normal number, down to 2^-35 of the largest, and the denominator (at most
+// 2^17 tokens of 2^(15 + FAR) a part) below its largest, whatever the scales are.
+constexpr int FAR = 50;
+__device__ __forceinline__ int exponent_of(float x) { return (__float_as_int(x) >> 23) & 255; }
+// The bits of what V's scale asks of the reference: its size, or 0 where there is nothing to measure.
+__device__ __forceinline__ uint32_t reference_of(bool there, float sv) { return there && fabsf(sv) <= 3.402823466e38f ? __float_as_uint(fabsf(sv)) : 0u; }
+__device__ __forceinline__ void raise(float &v0, uint32_t largest)       // largest: of what several scales ask
+{
+    const float to = __uint_as_float(min(max(largest & 0x7f800000u, 1u << 23), 253u << 23));      // its inverse is a normal number too
+    if (largest && (v0 == 0.f || exponent_of(to) > exponent_of(v0) + FAR)) v0 = to;
+}
+// Where the reference rises by 2^step, the weights of what a row has seen get smaller by as much and O is scaled down; the exponent m
+// of a row that sees tokens of the tile falls by FALL first, or what was large against the old reference (its weights lie at 2^11
+// against a scale 2^FAR above it at most) would leave the new ones f16's least numbers.
+constexpr float FALL = 45.f;
+// How the tokens of a page are weighted.
 struct Weighted {
     float log_ratio, inverse;                  // log2(|sv| / v0), added to the scores; v0 / |sv|, a weight's part of the denominator
     uint32_t mark;                             // what else V's scale asks for
 };
 constexpr uint32_t MARK_ZERO = 1, MARK_MINUS = 2;      // of a scale of 0 (in the denominator, nothing to the sums), and below 0
-__device__ __forceinline__ Weighted weighted(float size, float v0)          // size: |sv|, above 0 and finite
-{
-    Weighted w = {0.f, 1.f, 0};
-    if (size != v0) {
-        w.log_ratio = log2_ratio(size, v0);
-        w.inverse = __fdividef(v0, size);
-    }
-    return w;
-}
 __device__ __forceinline__ Weighted weighted(bool there, float sv, float v0)
 {
     Weighted w = {0.f, 1.f, 0};
-    const float size = fabsf(sv);
+    const float ratio = fabsf(sv) * __uint_as_float((uint32_t)(254 - exponent_of(v0)) << 23);
     if (!there) {
         w.log_ratio = -INFINITY;
         w.inverse = 0.f;
-    } else if (size == 0.f) w.mark = MARK_ZERO;
-    else if (!(size <= 3.402823466e38f)) w.log_ratio = __int_as_float(0x7fffffff);     // rows that see it get NaN, others nothing of it
+    } else if (!(fabsf(sv) <= 3.402823466e38f)) w.log_ratio = __int_as_float(0x7fffffff);     // rows that see it get NaN, others nothing of it
+    else if (exponent_of(ratio) < 127 - FAR) w.mark = MARK_ZERO;
     else {
-        w = weighted(size, v0);
+        w.log_ratio = __log2f(ratio);
+        w.inverse = __fdividef(1.f, ratio);
         w.mark = sv < 0.f ? MARK_MINUS : 0;
     }
     return w;

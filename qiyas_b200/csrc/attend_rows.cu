@@ -16,8 +16,9 @@
 //    The codes become f16 exactly (byte permute under an exponent of 1024, subtract 1152).  An order of dims or tokens
 //    inside a product is free, so both operands are read as whole 16-byte chunks: lane (g, t) holds K's chunks 2t, 2t+1 of
 //    token g, and V's chunk g of tokens 2t, 2t+1, 2t+8, 2t+9.
-//  * sk goes into the score's factor.  sv goes into the exponent: with v0 the first V scale a warp meets, the weights are
-//    w = 2^(s + log2(sv / v0) - m), the sum of them with v0 / sv as factor is the denominator, and O = v0 * sum w cv.
+//  * sk goes into the score's factor.  sv goes into the exponent: with a reference v0 for a piece (a power of two, the
+//    largest of its first pages' scales; `raise`), the weights are w = 2^(s + log2(sv / v0) - m), the sum of them with v0 / sv as
+//    factor is the denominator, and O = v0 * sum w cv.  The producers take logarithms and quotients, a lane a page.
 //    (|sv| is meant: where sv is below 0 the weights change sign, where it is 0 they are zeros in the second product, and a page
 //    that is not there has weights of 0 in the denominator too.)
 //    m is chosen so that w lies at 2^11 at its largest when it is set and is kept while w stays below 2^15: f16 then holds
@@ -58,8 +59,7 @@ struct RowsCfg {
 
 struct RowsHead {                              // at O_HEAD
     uint64_t full[24], empty[24];
-    float4 scales[24];                         // of a stage: sk, sv of its first and second 16 tokens
-    uint32_t odd[24];                          // 0: both pages are there and sv is above 0 and finite; else 4, and bits 0 and 1 if they are there
+    float4 scales[24][2];                      // of a stage's page, or two of 16 tokens: sk, log2(|sv| / v0), v0 / |sv|, v0
     float factor[16];                          // rows: scale * log2 e / (what q was scaled by)
     int lo[16], hi[16];                        // rows: tokens they see
     Start start;
@@ -67,7 +67,7 @@ struct RowsHead {                              // at O_HEAD
 };
 static_assert(sizeof(RowsHead) <= ROWS_HEADER, "the header fits");
 
-struct Batch { int b, h, lo, hi, tile, count; };       // tiles of one piece
+struct Batch { int b, h, lo, hi, tile, count; bool starts; };      // tiles of one piece; starts: its first
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void *map, int x, int y, uint32_t bar)
 {
@@ -140,6 +140,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
             t.lo = piece.unit.lo;
             t.hi = piece.unit.hi;
             t.tile = piece.unit.t0 + piece.first + at;
+            t.starts = at == 0;
             t.count = more ? min(most, piece.count - at) : 0;
             at += t.count;
             return t;
@@ -157,27 +158,30 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
         float2 sc = scales_at(p, id, now.h);
         Batch next = next_batch();
         Page id_next = page_of(next);
+        float vref = 0.f;                      // what V's scales of the piece are taken against
         while (now.count) {
             const Batch after = next_batch();
             const int id_then = page_number(p, id_next, mine == 0);
             const float2 sc_then = scales_at(p, id_then, next.h);
             id_next = page_of(after);
-            const unsigned usual = __ballot_sync(0xffffffffu, id >= 0 && sc.y > 0.f && sc.y <= 3.402823466e38f);
+            float4 own;                        // this lane's page, for the consumers
+            bool made = false;
+            auto make = [&]() {                // by every producer for every batch: they all have the same reference
+                made = true;
+                if (now.starts) vref = 0.f;
+                raise(vref, __reduce_max_sync(0xffffffffu, reference_of(id >= 0, sc.y)));
+                // what is seldom needed lies in the signs: V's scale is below 0; it counts as 0
+                const Weighted v = weighted(id >= 0, sc.y, vref);
+                own = make_float4(sc.x, v.log_ratio, v.mark == MARK_MINUS ? -v.inverse : v.inverse, v.mark == MARK_ZERO ? -vref : vref);
+            };
             for (int k = (mine - seq) & (RP - 1); k < now.count; k += RP) {
                 const uint32_t tile = seq + k;
                 const int stage = tile % C::S;
                 if (tile >= C::S && !mbar_wait_soon_lanes(empty0 + 8 * stage, (tile / C::S - 1) & 1, abort, p.status, STATUS_ATTEND_WAIT)) goto done;
                 const int base = (now.tile + k) * 32, l0 = k * per, l1 = l0 + per - 1;
                 const int id0 = __shfl_sync(0xffffffffu, id, l0), id1 = __shfl_sync(0xffffffffu, id, l1);
-                const float k0 = __shfl_sync(0xffffffffu, sc.x, l0), k1 = __shfl_sync(0xffffffffu, sc.x, l1);
-                const float v0 = __shfl_sync(0xffffffffu, sc.y, l0), v1 = __shfl_sync(0xffffffffu, sc.y, l1);
-                if (lane == 0) {
-                    const int live = (id0 >= 0 ? 1 : 0) + (per == 2 && id1 >= 0 ? 1 : 0);
-                    head->scales[stage] = make_float4(k0, v0, k1, v1);
-                    head->odd[stage] = (usual >> l0 & usual >> l1 & 1) ? 0 : 4 | (id0 >= 0 ? 1 : 0) | (id1 >= 0 ? 2 : 0);
-                    if (live) mbar_arrive_expect_tx(full0 + 8 * stage, live * 2 * C::SUB * bytes);
-                    else mbar_arrive(full0 + 8 * stage);
-                }
+                const int live = (id0 >= 0 ? 1 : 0) + (per == 2 && id1 >= 0 ? 1 : 0);
+                if (lane == 0 && live) mbar_expect_tx(full0 + 8 * stage, live * 2 * C::SUB * bytes);
                 issued++;
                 __syncwarp();
                 const int page = second ? id1 : id0;
@@ -185,7 +189,12 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                     const int row = ((page * p.heads + now.h) << p.log_page) + ((base + second * 16) & ((1 << p.log_page) - 1));
                     tma_load_2d(ring + stage * C::STAGE + offset, which ? &vmap : &kmap, sub * 128, row, full0 + 8 * stage);
                 }
+                if (!made) make();             // beside the first copy
+                if (lane == l0 || lane == l1) head->scales[stage][lane - l0] = own;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full0 + 8 * stage);
             }
+            if (!made) make();
             seq += now.count;
             now = next;
             id = id_then;
@@ -301,8 +310,6 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
             const uint32_t at = seq + j;
             const int stage = at % C::S;
             if (!mbar_wait_soon_lanes(full0 + 8 * stage, (at / C::S) & 1, abort, p.status, STATUS_ATTEND_WAIT)) { gone = true; break; }
-            const float4 sc = head->scales[stage];
-            const uint32_t odd = head->odd[stage];
             const uint8_t *kt = smem + stage * C::STAGE, *vt = kt + C::HALF;
             const int base = (u.t0 + piece.first + j) * 32;
 
@@ -341,22 +348,13 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                 }
 
             // ---- weights
-            Weighted v[2];
+            const float4 *sc[2] = { &head->scales[stage][0], &head->scales[stage][p.log_page == 4] };
 #pragma unroll
-            for (int mt = 0; mt < 2; mt++) {
-                const float sk = mt ? sc.z : sc.x, sv = mt ? sc.w : sc.y;
-                if (odd) {
-                    if (vref == 0.f) vref = reference_of(odd >> mt & 1, sv);
-                    v[mt] = weighted(odd >> mt & 1, sv, vref);
-                } else {
-                    if (vref == 0.f) vref = sv;
-                    v[mt] = weighted(sv, vref);
-                }
+            for (int mt = 0; mt < 2; mt++)
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) s[mt][nb][c] = __fmaf_rn(s[mt][nb][c], factor[nb][c & 1] * sk, v[mt].log_ratio);
-            }
+                    for (int c = 0; c < 4; c++) s[mt][nb][c] = __fmaf_rn(s[mt][nb][c], factor[nb][c & 1] * sc[mt]->x, sc[mt]->y);
             if (base < lo_most || base + 32 > hi_least) {
 #pragma unroll
                 for (int mt = 0; mt < 2; mt++)
@@ -367,6 +365,27 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                             const int token = base + mt * 16 + g + (c >> 1) * 8;
                             if (token < lo[nb][c & 1] || token >= hi[nb][c & 1]) s[mt][nb][c] = -INFINITY;
                         }
+            }
+            if (fabsf(sc[1]->w) != vref) {     // what V's scales are taken against: the first, seldom another
+                const float step = vref == 0.f ? 0.f : (float)(exponent_of(sc[1]->w) - exponent_of(vref));
+                vref = fabsf(sc[1]->w);
+                if (step > 0.f) {
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            const float fall = lo[nb][c] < base + 32 && hi[nb][c] > base ? FALL : 0.f, less = exp2_fast(fall - step);
+                            mm[nb][c] -= fall;
+                            l[nb][c] *= exp2_fast(fall);
+#pragma unroll
+                            for (int i = 0; i < C::SUB * (DT == 64 ? 2 : 4); i++)
+#pragma unroll
+                                for (int k = 0; k < 2; k++) {
+                                    o[i][k][nb][c] *= less;
+                                    o[i][k][nb][c + 2] *= less;
+                                }
+                        }
+                }
             }
             bool above = false;
 #pragma unroll
@@ -405,7 +424,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
                         e[c] = exp2_fast(s[mt][nb][c] - mm[nb][c & 1]);
-                        l[nb][c & 1] = __fmaf_rn(e[c], v[mt].inverse, l[nb][c & 1]);
+                        l[nb][c & 1] = __fmaf_rn(e[c], fabsf(sc[mt]->z), l[nb][c & 1]);
                     }
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
@@ -417,16 +436,18 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
 #pragma unroll
                     for (int z = 0; z < SPL; z++) w[mt][nb][z] = make_uint2(half[z][0], half[z][1]);
                 }
-            if (odd) {                         // seldom: scales of 0 or below
+            if (__float_as_int(sc[0]->z) < 0 || __float_as_int(sc[0]->w) < 0 || __float_as_int(sc[1]->z) < 0 || __float_as_int(sc[1]->w) < 0) {   // seldom: scales of V of 0 or below
 #pragma unroll
-                for (int mt = 0; mt < 2; mt++)
+                for (int mt = 0; mt < 2; mt++) {
+                    const bool minus = __float_as_int(sc[mt]->z) < 0, zero = __float_as_int(sc[mt]->w) < 0;
 #pragma unroll
                     for (int nb = 0; nb < NB; nb++)
 #pragma unroll
                         for (int z = 0; z < SPL; z++) {
-                            w[mt][nb][z].x = marked(w[mt][nb][z].x, v[mt].mark == MARK_ZERO, v[mt].mark == MARK_MINUS);
-                            w[mt][nb][z].y = marked(w[mt][nb][z].y, v[mt].mark == MARK_ZERO, v[mt].mark == MARK_MINUS);
+                            w[mt][nb][z].x = marked(w[mt][nb][z].x, zero, minus);
+                            w[mt][nb][z].y = marked(w[mt][nb][z].y, zero, minus);
                         }
+                }
             }
 
             // ---- O^T += V^T P^T
@@ -473,12 +494,13 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                 const int r = nb * 8 + 2 * t + c;
+                const float times = part_scale(mm[nb][c], sum, v0);
                 if (g == 0) ml[warp * C::R + r] = make_float2(mm[nb][c], sum);
                 float *row = merge + (warp * C::R + r) * C::MROW;
 #pragma unroll
                 for (int i = 0; i < C::SUB * (DT == 64 ? 2 : 4); i++) {
                     const int dim = DT == 64 ? 8 * g + 4 * i : (i / 4) * 128 + 16 * g + 4 * (i % 4);
-                    *(float4 *)(row + dim) = make_float4(o[i][0][nb][c] * v0, o[i][0][nb][c + 2] * v0, o[i][1][nb][c] * v0, o[i][1][nb][c + 2] * v0);
+                    *(float4 *)(row + dim) = make_float4(o[i][0][nb][c] * times, o[i][0][nb][c + 2] * times, o[i][1][nb][c] * times, o[i][1][nb][c + 2] * times);
                 }
             }
         named_bar_sync(1, 32 * RW);

@@ -61,7 +61,8 @@ struct TilesHead {
     uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
     uint64_t sfull[4], pfull[4], odone[2];     // of the S buffers, two a row tile; of O before a piece's last tile
     float4 scales[4][4];                       // beside K's slots, of a tile's groups of 16 tokens: sk, log2(|sv| / v0), v0 / |sv|, and v0
-                                               // (the first group's: a bit a group, V's scale is 0, and from bit 16 on, it is below 0)
+                                               // (the first group's: a bit a group, V's scale counts as 0, and from bit 16 on, it is below 0;
+                                               // the second's: by how many powers of two v0 rose with this tile)
     Start start;
     uint32_t tmem;
     int abort;
@@ -304,6 +305,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                     for (int e = 0; e < NG; e++) sc[e] = head->scales[(seq + j) % SLOTS][e];
                     vref = sc[NG - 1].w;
                     const uint32_t marks = __float_as_uint(sc[0].w);
+                    const float step = sc[1].w;
                     tmem_ld_landed32(v[0]);
                     tmem_ld_landed32(v[1]);
                     __syncwarp();
@@ -331,15 +333,21 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                     // seldom: the exponent the weights are taken against goes up, by whole powers of two
                     const bool above = fresh ? top > -INFINITY : top > 15.f;
                     const bool keep = SPL == 2 && j > 0 && j % C::KEEP == 0;
-                    if (keep || __any_sync(0xffffffffu, above)) {
-                        float up = 0.f, less = 1.f;
-                        if (above) {
-                            up = ceilf(top) - 11.f;
-                            if (!fresh) less = exp2_fast(-up);
-                            fresh = false;
+                    if (keep || step > 0.f || __any_sync(0xffffffffu, above)) {
+                        // (or what V's scales are taken against does, seldom: the sums keep their values)
+                        float up = 0.f, less = 1.f, o_less = 1.f;
+                        if (fresh) {
+                            if (top > -INFINITY) up = ceilf(top) - 11.f;
+                            fresh = top == -INFINITY;
+                        } else {
+                            const float down = step > 0.f && (top > -INFINITY || l < 1.f) ? FALL : 0.f;      // (l < 1: so that v0 / l stays inside f32)
+                            up = top + down > 15.f ? ceilf(top) - 11.f : -down;
+                            less = exp2_fast(-up);
+                            o_less = exp2_fast(-up - step);
                         }
                         mm += up;
                         l *= less;
+                        kept_mm -= step;
 #pragma unroll
                         for (int i = 0; i < 64; i++) x[i] -= up;
                         if (j > 0) {                             // O so far, once the product before has ended
@@ -356,7 +364,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                                 tmem_ld16(o_at + d, w);
                                 tmem_ld_landed16(w);
 #pragma unroll
-                                for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__uint_as_float(w[i]) * less);
+                                for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__uint_as_float(w[i]) * o_less);
                                 if (keep) {
                                     if (j != C::KEEP) {
 #pragma unroll
@@ -426,14 +434,18 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             pieces++;
             if (!active) continue;
             tc_fence_after();
-            const float v0 = vref > 0.f ? vref : 1.f;
             const bool complete = piece.first == 0 && n == u.nt;
             const int r = at - u.r0;
             float *slot = parts_of(p) + (size_t)(blockIdx.x * 2 + (piece.first ? 0 : 1)) * part_floats(R, p.dim);
             float *part = slot + R * 2 + (size_t)r * p.dim;
-            const float f = complete ? v0 * inverse_of(l) : v0;
             T *dst = out_row<T>(p, u, min(at, u.r1 - 1));
             const float kept_less = exp2_fast(kept_mm - mm);
+            const float v0 = vref > 0.f ? vref : 1.f;
+            float f = v0 * inverse_of(l);
+            if (!complete) {
+                if (fresh) mm = NOTHING;
+                f = part_scale(mm, l, v0);
+            }
 #pragma unroll 1
             for (int d = 0; d < p.dim; d += 16) {
                 uint32_t v[16];
@@ -454,7 +466,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             }
             if (at < u.r1) {
                 if (complete) store_lse(p, u, at, mm, l);
-                else *(float2 *)(slot + r * 2) = make_float2(fresh ? NOTHING : mm, l);
+                else *(float2 *)(slot + r * 2) = make_float2(mm, l);
             }
         }
     } else if (warp < 4 * NQ + CW) {
@@ -556,15 +568,12 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                 page = page_of(after);
                 if (now.there) {
                 if (now.starts) vref = 0.f;
-                // V's scales against the first of the piece that is not zero
-                const float size = reference_of(there, sc.y);
-                const unsigned some = __ballot_sync(0xffffffffu, size > 0.f);
-                const float found = __shfl_sync(0xffffffffu, size, some ? __ffs(some) - 1 : 0);
-                if (vref == 0.f && some) vref = found;
+                const float before = vref;
+                raise(vref, __reduce_max_sync(0xffffffffu, reference_of(there, sc.y)));
                 const Weighted v = weighted(there, sc.y, vref);
                 const uint32_t marks = __ballot_sync(0xffffffffu, v.mark == MARK_ZERO) | __ballot_sync(0xffffffffu, v.mark == MARK_MINUS) << 16;
                 if (seq >= SLOTS && !mbar_wait_soon_lanes(kempty + 8 * (seq % SLOTS), (seq / SLOTS - 1) & 1, abort, status, STATUS_ATTEND_WAIT)) break;
-                if (lane < NG) head->scales[seq % SLOTS][lane] = make_float4(sc.x, v.log_ratio, v.inverse, lane ? vref : __uint_as_float(marks));
+                if (lane < NG) head->scales[seq % SLOTS][lane] = make_float4(sc.x, v.log_ratio, v.inverse, lane == 0 ? __uint_as_float(marks) : lane == 1 && before > 0.f ? (float)(exponent_of(vref) - exponent_of(before)) : lane == 1 ? 0.f : vref);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(kfull + 8 * (seq % SLOTS));
                 seq++;

@@ -85,13 +85,15 @@ ROWS = [(1, [1, 1, 1, 1]), (5, [3, 1, 2, 0]), (4, [1, 40, 17, 3]), (2, [130, 3, 
 KINDS = ["f32", "f16", "bf16"]
 
 
-def check(s, kind, lens, counts, group, causal=True, window=0, absent=(), status=0, q=None, out=None, table=None, **more):
+def check(s, kind, lens, counts, group, causal=True, window=0, absent=(), status=0, q=None, out=None, table=None, far=False, **more):
     """CacheAttention against the definition in 64 bits, for scales of any sign and size.  absent: (sequence, slot) pairs whose
     pages `table` does not name.  The tolerance, for a row with weights p: the scores are sums of dim products in f32 ((dim + 8) *
-    2^-24 of scale * sum |q||k|), 2^-20 for the cut of q, the exponentials and the logarithms of V's scales, the weights are cut to
-    f16 (half a step, 2^-11; f32 lanes: two f16, 2^-21), the sums over tokens run in f32 over tokens / 128 + 64 steps: all relative
+    2^-24 of scale * sum |q||k|), 2^-20 for the cut of q and the exponentials; the logarithm r of a ratio of V's scales has two ulps,
+    and four sums with it round by half an ulp each: r * 2^-21, r the logarithm of the sequence's largest scale to its smallest, 50 at
+    most.  The weights are cut to f16 (half a step, 2^-11; f32 lanes: two f16, 2^-21), the sums over tokens run in f32 over tokens / 128 + 64 steps: all relative
     to sum p |v|.  The output is rounded once to its type.  Below f16's normal numbers a weight is off by 2^-35 of the largest of
-    p * |V's scale|, each time a code of V, 128 at most."""
+    p * |V's scale| that the row sees, each time a code of V, 128 at most; far: scales more than 2^50 apart may count as 0, so the
+    largest of the sequence, seen or not, takes that place."""
     import torch
     o, heads, rows = H.ops(), s.heads * group, int(sum(counts))
     if q is None:
@@ -124,12 +126,20 @@ def check(s, kind, lens, counts, group, causal=True, window=0, absent=(), status
         want_lse = torch.logsumexp(scores, -1)
         p = torch.exp(scores - want_lse.masked_fill(want_lse.isneginf(), 0)[..., None])
         want, weight = p @ v, p @ v.abs()
-        score = (s.dim + 8) * 2.0 ** -24 * size + 2.0 ** -20 * (1 + size)
+        held = np.abs(s.v.scales[s.table[b][:(length + s.page - 1) // s.page]]).astype(np.float64)
+        held = held[(held > 0) & np.isfinite(held)]
+        ratio = min(50.0, np.log2(held.max() / held.min())) if held.size else 0.0
+        score = (s.dim + 8) * 2.0 ** -24 * size + 2.0 ** -20 * (1 + size) + 2.0 ** -21 * ratio
         sums = (length / 128 + 64) * 2.0 ** -24
-        most = np.abs(s.v.scales[s.table[b][:(length + s.page - 1) // s.page]])
-        floor = 2.0 ** -35 * length * 128 * float(most[np.isfinite(most)].max(initial=0))
+        most = gpu(np.where(np.isfinite(s.v.scales), np.abs(s.v.scales), 0)[s.table[b][token // s.page]].astype(np.float64))     # [tokens, heads]
+        most = most.t().repeat_interleave(group, 0)[:, None].expand(heads, n, length)
+        most = (most if far else most.masked_fill(~seen, 0)).amax(-1, keepdim=True) if length else 0
+        floor = 2.0 ** -35 * length * 128 * most
         bound = weight * (2 * score[..., None] + cut + sums) + want.abs() * eps + floor + (2.0 ** -25 if kind == "f16" else 1e-30)
         err = (out[at].double().transpose(0, 1) - want).abs()
+        if kind == "f16":                                # from 65520 on (65504 and half a step) f16 rounds to infinity
+            got = out[at].double().transpose(0, 1)
+            err = err.masked_fill(got.isinf() & (got.sign() == want.sign()) & (want.abs() + bound >= 65520), 0)
         assert bool((err <= bound).all()), (b, float((err / bound).max()))
         nothing = want_lse.isneginf()
         got = lse[at].double().transpose(0, 1)
@@ -201,3 +211,60 @@ def test_scales_that_are_not_finite_reach_the_rows_that_see_them_only(kind, coun
     sees = torch.from_numpy(sees).cuda()
     assert sees.any() and out[sees].isnan().all()
     assert torch.equal(out[~sees], want[~sees]) and o.gpu.status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("group,counts", ROWS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("order", ["up", "down", "any"])
+def test_attention_over_scales_of_very_different_sizes(kind, group, counts, dim, order):
+    """V's scales up to 2^49 apart: a row's result is right against what it sees, whatever else its neighbours see."""
+    s = Setup(46 + dim, 4, 1300, 1, 16, dim)
+    size = s.rng.uniform(-39, 10, (4, s.width, 1))
+    if order != "any":
+        size = np.sort(size, 1)[:, ::1 if order == "up" else -1]
+    s.v.scales[s.table] = np.exp2(size).astype(np.float32)
+    s.v.scales[s.table[3, 2]] *= -1
+    s.v.scales[s.table[2, 5:7]] = 0
+    check(s, kind, [1300, 131, 399, 50], counts, group)
+    check(s, kind, [1300, 131, 399, 50], counts, group, window=9)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("group,counts", ROWS)
+@pytest.mark.parametrize("order", ["up", "down", "any"])
+def test_attention_over_scales_that_the_type_hardly_holds(kind, group, counts, order):
+    """V's scales from f32's least numbers (what a write of subnormal values leaves) to 2^112, and with them values next to the largest."""
+    most = 112 if kind != "f16" else 0
+    s = Setup(47, 4, 1300, 2, 16, 128)
+    size = s.rng.uniform(-149, most, (4, s.width, 2))
+    size[:, ::5] = s.rng.uniform(-149, -140, size[:, ::5].shape)
+    if order != "any":
+        size = np.sort(size, 1)[:, ::1 if order == "up" else -1]
+    s.v.scales[s.table] = np.exp2(size).astype(np.float32)
+    check(s, kind, [1300, 131, 399, 50], counts, group, far=True)
+    check(s, kind, [1300, 131, 399, 50], counts, group, far=True, window=40)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("group,counts", ROWS)
+@pytest.mark.parametrize("page,dim", [(32, 256), (16, 128)])
+def test_scales_that_rise_behind_what_a_row_sees(kind, group, counts, page, dim):
+    """Rows that see tokens close below a scale which only their neighbours see, far above those before."""
+    s = Setup(49, 4, 1300, 2, page, dim)
+    steps = np.linspace(-140, 112, s.width)              # rising evenly, and by jumps
+    s.v.scales[s.table, 0] = np.exp2(steps)
+    s.v.scales[s.table, 1] = np.exp2(np.floor(steps / 40) * 40 + s.rng.uniform(0, 17, s.width))
+    for window in (70, 0):
+        out, _ = check(s, kind, [1300, 131, 399, 50], counts, group, far=True, window=window)
+        assert bool(out.isfinite().all())
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("counts", [[1, 2], [100, 40]])
+def test_attention_over_values_next_to_the_largest(kind, counts):
+    s = Setup(48, 2, 3000, 2, 32, 64)
+    s.v.scales[:] = np.float32(3.3e38 / 128)
+    s.v.codes[:] = np.abs(s.v.codes.astype(np.int32)).clip(0, 127)
+    out, _ = check(s, kind, [3000, 70], counts, 4)
+    assert bool(out.isfinite().all())
