@@ -655,9 +655,9 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                     if (ok) sums(j, nq, j + 2 == n);
                 }
                 if (!ok) break;
-                release(ofull, nq);
+                mma_commit(ofull);
                 tiles += n;
-            }
+            } else mbar_arrive(ofull);                         // it has looked at qfull, which may go on to its next phase
             seq += n;
             pieces++;
         }

@@ -268,3 +268,24 @@ def test_attention_over_values_next_to_the_largest(kind, counts):
     s.v.codes[:] = np.abs(s.v.codes.astype(np.int32)).clip(0, 127)
     out, _ = check(s, kind, [3000, 70], counts, 4)
     assert bool(out.isfinite().all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [128, 256])
+def test_one_and_two_row_tiles_in_turn(kind, dim):
+    """Many short units one after the other in a block, with one row tile and with two: the second issuing thread sits out runs
+    of them and has to be back in step with the others."""
+    import torch
+    rng = np.random.default_rng(6)
+    counts = [int(x) for x in rng.choice([1, 30, 127, 128, 129, 200, 256], 60)]
+    counts[20:40] = [1] * 20
+    lens = [n + int(x) for n, x in zip(counts, rng.integers(0, 70, 60))]
+    s = Setup(50, 60, 330, 8, 16, dim)
+    q = s.rows(sum(counts), 8, kind)[0]
+    want, lse = check(s, kind, lens, counts, 1, q=q)
+    o, cache, args = H.ops(), s.on_gpu(), (gpu(s.table), ints(lens), ints(offsets_of(counts)))
+    for _ in range(20):
+        out, out_lse = torch.full_like(q, 5.0), torch.empty_like(lse)
+        o.CacheAttention(cache, q, out, *args, lse=out_lse)
+        assert torch.equal(out, want) and torch.equal(out_lse, lse)
+    assert o.gpu.status() == 0
