@@ -23,11 +23,13 @@ _kinds = {}
 
 
 def _lane_kinds():
-    """Lane types by torch's: filled on first use, since importing this module needs no torch."""
+    """Lane types by torch's, and what else is torch's: filled on first use, since importing this module needs no torch."""
     if not _kinds:
         import torch
         _kinds.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
         _kinds["i32"] = torch.int32
+        # the handle of torch's current stream on a device (the quick way takes 0.2 us where a Stream object takes 2)
+        _kinds["stream"] = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
     return _kinds
 
 
@@ -264,13 +266,14 @@ class GpuOps:
     def CacheWrite(self, cache, k, v, table, lengths, offsets=None, stream=None):
         """Quantises the rows of k and v ([rows, heads, dim], f32, f16 or bf16) into `cache` as tokens lengths[b], lengths[b] + 1,
         ... of their sequences.  table: int32 [sequences, width] of pages; lengths: int32, tokens already there; offsets: int32
-        [sequences + 1], the rows of each sequence (None: one row each).  All on the device; nothing is synchronised."""
+        [sequences + 1], the rows of each sequence (None: one row each).  All on the device; nothing is synchronised.  stream None:
+        torch's current stream, as for the other cache operators."""
         kind, rows, base, row, head = self._lanes(cache, k, "k", cache.heads)
         other, same, v_base, v_row, v_head = self._lanes(cache, v, "v", cache.heads)
         if other != kind or same != rows:
             raise ValueError("k and v have the same rows and type")
         rc = self.lib.qb200_cache_write(cache.parts, self._sequences(cache, table, lengths, offsets, rows), kind, _lib.LANES(base, row, head),
-                                        _lib.LANES(v_base, v_row, v_head), _stream(stream))
+                                        _lib.LANES(v_base, v_row, v_head), self._current(stream))
         if rc:
             self.gpu.check(rc, "CacheWrite")
         return "s8 cache blocks"
@@ -290,7 +293,7 @@ class GpuOps:
             if other != kind or same != rows:
                 raise ValueError("k and v have the same rows and type")
             v_at = _lib.LANES(base, row, head)
-        rc = self.lib.qb200_cache_read(cache.parts, self._sequences(cache, table, starts, offsets, rows), kind, at, v_at, _stream(stream))
+        rc = self.lib.qb200_cache_read(cache.parts, self._sequences(cache, table, starts, offsets, rows), kind, at, v_at, self._current(stream))
         if rc:
             self.gpu.check(rc, "CacheRead")
         return "s8 cache blocks"
@@ -302,6 +305,7 @@ class GpuOps:
         (0: all).  lse: optional f32 [rows, query heads].  max_queries, max_length: bounds on the rows of a sequence and on
         lengths, known to the host, for the choice of kernel (0: rows, or 1 without offsets; all the table holds).  scale None:
         1 / sqrt(dim).  workspace None: one of the call's own, from torch's allocator on the call's stream."""
+        stream = self._current(stream)
         heads = q.shape[1] if q.dim() == 3 else 0
         kind, rows, base, row, head = self._lanes(cache, q, "q", heads)
         other, same, out_base, out_row, out_head = self._lanes(cache, out, "out", heads)
@@ -322,7 +326,7 @@ class GpuOps:
             if need:
                 held = self._scratch_on(stream, need)          # until the call is in its stream
                 args = _lib.ATTENTION(base, row, head, out_base, out_row, out_head, lse_at, held.data_ptr(), need, *rest)
-        rc = self.lib.qb200_cache_attention(cache.parts, seq, kind, args, _stream(stream))
+        rc = self.lib.qb200_cache_attention(cache.parts, seq, kind, args, stream)
         if rc:
             self.gpu.check(rc, "CacheAttention")
         return "f16 mma cache blocks"
@@ -358,11 +362,16 @@ class GpuOps:
                              ", ".join(f"{t.dtype} {t.stride()} on {t.device}" for t in (table, lengths, offsets) if t is not None))
         return _lib.SEQUENCES(table.data_ptr(), lengths.data_ptr(), at, count, width, rows)
 
+    def _current(self, stream):
+        """The stream a cache operator runs on, as the C ABI takes it; None: torch's current one on the library's device, where the
+        tensors it is given were made."""
+        return _lane_kinds()["stream"](self.gpu.device) or None if stream is None else _stream(stream)
+
     def _scratch_on(self, stream, nbytes_):
         """A buffer of torch's allocator that belongs to `stream`: freed in its order, and the graph's own under capture."""
         import torch
         device = torch.device("cuda", self.gpu.device)
-        want = _stream(stream) or 0
+        want = stream or 0
         if torch.cuda.current_stream(device).cuda_stream == want:
             return torch.empty(nbytes_, dtype=torch.uint8, device=device)
         with torch.cuda.stream(torch.cuda.ExternalStream(want, device=device) if want else torch.cuda.default_stream(device)):

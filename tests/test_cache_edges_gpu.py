@@ -289,3 +289,47 @@ def test_one_and_two_row_tiles_in_turn(kind, dim):
         o.CacheAttention(cache, q, out, *args, lse=out_lse)
         assert torch.equal(out, want) and torch.equal(out_lse, lse)
     assert o.gpu.status() == 0
+
+
+def test_calls_without_a_stream_run_on_torchs_current_one():
+    """Inside a side stream's context, and while a graph is captured: behind the torch operations that made their arguments."""
+    import torch
+    s = Setup(51, 3, 500, 2, 16, 64)
+    o, cache, table = H.ops(), s.on_gpu(), gpu(s.table)
+    before, after, offsets = ints([0, 100, 250]), ints([200, 250, 500]), ints([0, 200, 350, 600])
+    x = [s.rows(600, h, "f32")[0] for h in (2, 2, 4)]
+    k, v, q = (torch.zeros_like(t) for t in x)
+    want_k, want_out = torch.empty_like(k), torch.empty_like(q)
+    o.CacheWrite(cache, x[0], x[1], table, before, offsets=offsets)
+    o.CacheRead(cache, want_k, None, table, before, offsets=offsets)
+    o.CacheAttention(cache, x[2], want_out, table, after, offsets=offsets)
+    slow = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        cache = s.on_gpu()
+        got_k, got_out = torch.zeros_like(k), torch.zeros_like(q)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(10):
+                slow = slow @ slow                           # milliseconds before the rows are there
+            for t, made in zip((k, v, q), x):
+                t.copy_(made)
+            o.CacheWrite(cache, k, v, table, before, offsets=offsets)
+            o.CacheRead(cache, got_k, None, table, before, offsets=offsets)
+            o.CacheAttention(cache, q, got_out, table, after, offsets=offsets)
+            sums = got_k.clone(), got_out.clone()
+            for t in (k, v, q):
+                t.zero_()
+        side.synchronize()
+        assert torch.equal(sums[0], want_k) and torch.equal(sums[1], want_out)
+    cache = s.on_gpu()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o.CacheWrite(cache, x[0], x[1], table, before, offsets=offsets)
+        o.CacheRead(cache, got_k, None, table, before, offsets=offsets)
+        o.CacheAttention(cache, x[2], got_out, table, after, offsets=offsets)
+    for t in (got_k, got_out):
+        t.fill_(float("nan"))
+    graph.replay()
+    assert torch.equal(got_k, want_k) and torch.equal(got_out, want_out) and o.gpu.status() == 0
