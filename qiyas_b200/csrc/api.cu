@@ -47,7 +47,9 @@ int finish(int rc, const char *what)
 }
 
 // A launch that is not a gemv: the gemv's record of launches in flight (which lets an unrelated gemv start beside its
-// predecessors) does not describe what this one touches, so the next gemv on the stream orders itself after everything.
+// predecessors) does not describe what this one touches, so the next gemv on the stream orders itself after everything, which
+// is to wait for this launch, which waited for all before it.  A call that launches nothing must not come here: gemvs of
+// a burst may still be running side by side, and to wait for the newest is not to wait for all.
 int finish_other(int rc, const char *what, void *stream)
 {
     if (rc == 0) qb::gemv_history_everything((cudaStream_t)stream);
@@ -418,6 +420,7 @@ int qb200_encode(int fmt, const float *lanes, void *blocks, int64_t n, void *str
     if (!qb::block_values(fmt)) return fail(QB200_E_FORMAT, "%s: not a block format", fmt_name(fmt));
     if (n < 0 || n > 2147483647LL) return fail(QB200_E_SHAPE, "count %lld", (long long)n);
     if (n && (!lanes || !blocks || ((uintptr_t)lanes & 3))) return fail(QB200_E_POINTER, "null or misaligned operand");
+    if (n == 0) return 0;
     return finish_other(qb::encode_launch(fmt, lanes, blocks, n, (cudaStream_t)stream), "encode", stream);
 }
 
@@ -427,6 +430,7 @@ int qb200_decode(int fmt, const void *blocks, float *lanes, int64_t n, void *str
     if (!qb::block_values(fmt)) return fail(QB200_E_FORMAT, "%s: not a block format", fmt_name(fmt));
     if (n < 0 || n > 2147483647LL) return fail(QB200_E_SHAPE, "count %lld", (long long)n);
     if (n && (!lanes || !blocks || ((uintptr_t)lanes & 3))) return fail(QB200_E_POINTER, "null or misaligned operand");
+    if (n == 0) return 0;
     return finish_other(qb::decode_launch(fmt, blocks, lanes, n, (cudaStream_t)stream), "decode", stream);
 }
 
@@ -494,6 +498,7 @@ int qb200_cache_write(const qb200_cache_t *cache, const qb200_sequences_t *seque
     OnDevice on;
     if (!g_ready) return fail(QB200_E_DEVICE, "qb200_init has not succeeded");
     if (on.e) return cuda_fail(on.e, "cudaSetDevice");
+    if (sequences->count == 0 || sequences->rows == 0) return 0;
     return finish_other(qb::cache_write(*cache, *sequences, type, *k, *v, (cudaStream_t)stream), "cache_write", stream);
 }
 
@@ -508,6 +513,7 @@ int qb200_cache_read(const qb200_cache_t *cache, const qb200_sequences_t *sequen
     if (!g_ready) return fail(QB200_E_DEVICE, "qb200_init has not succeeded");
     if (on.e) return cuda_fail(on.e, "cudaSetDevice");
     const qb200_lanes_t none = { nullptr, 0, 0 };
+    if (sequences->count == 0 || sequences->rows == 0) return 0;
     return finish_other(qb::cache_read(*cache, *sequences, type, k ? *k : none, v ? *v : none, (cudaStream_t)stream), "cache_read", stream);
 }
 
@@ -550,6 +556,7 @@ int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *s
     OnDevice on;
     if (!g_ready) return fail(QB200_E_DEVICE, "qb200_init has not succeeded");
     if (on.e) return cuda_fail(on.e, "cudaSetDevice");
+    if (sequences->count == 0 || sequences->rows == 0) return 0;
     return finish_other(qb::attend(*cache, *sequences, type, a, (cudaStream_t)stream), "cache_attention", stream);
 }
 

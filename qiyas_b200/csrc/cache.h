@@ -15,6 +15,8 @@ constexpr int STATUS_ATTEND_WAIT = 8;
 constexpr int STATUS_CACHE_RANGE = 16;
 constexpr int STATUS_CACHE_VALUE = 32;
 
+// Of the calls below each launches something: there are sequences, and there are rows (rows of no sequence would have no
+// lengths and offsets to look at).
 cudaError_t cache_init(int *status);
 int cache_write(const qb200_cache_t &c, const qb200_sequences_t &s, int type, const qb200_lanes_t &k, const qb200_lanes_t &v, cudaStream_t stream);
 // either of k and v may have no base

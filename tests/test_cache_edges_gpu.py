@@ -333,3 +333,40 @@ def test_calls_without_a_stream_run_on_torchs_current_one():
         t.fill_(float("nan"))
     graph.replay()
     assert torch.equal(got_k, want_k) and torch.equal(got_out, want_out) and o.gpu.status() == 0
+
+
+@pytest.mark.parametrize("what", ["write", "read", "attention", "encode", "decode"])
+def test_a_call_with_nothing_to_do_orders_nothing(what):
+    """Gemvs of a burst run side by side; a call between them that launches nothing says nothing about when they end, so a gemv
+    that reads what an earlier one writes still waits for that one."""
+    import torch
+    from qiyas_b200 import blocks as B
+    o = H.ops()
+    s = Setup(52, 1, 16, 1, 16, 32)
+    cache, table, lengths = s.on_gpu(), gpu(s.table), ints([0])
+    none, offsets = torch.empty(0, 1, 32, device="cuda"), ints([0, 0])
+    rows, cols = 8192, 8192
+    big, small, last = (gpu(B.make_weights(B.Q8_0, r, c, i)) for i, (r, c) in enumerate([(rows, cols), (64, 256), (96, rows)]))
+    xs = [torch.randn(cols, device="cuda") for _ in range(12)]
+    x = torch.randn(256, device="cuda")
+    y, z, out = torch.empty(rows, device="cuda"), torch.empty(64, device="cuda"), torch.empty(96, device="cuda")
+    nothing = {"write": lambda: o.CacheWrite(cache, none, none, table, lengths, offsets=offsets, stream=0),
+               "read": lambda: o.CacheRead(cache, none, none, table, lengths, offsets=offsets, stream=0),
+               "attention": lambda: o.CacheAttention(cache, none, none, table, lengths, offsets=offsets, stream=0),
+               "encode": lambda: o.Back(B.Q8_0, x, small, 0), "decode": lambda: o.Lanes(B.Q8_0, small, x, 0)}[what]
+    want = []
+    for v in xs:
+        o.GemvBlocks(B.Q8_0, big, v, y, rows, cols, fmt_x=B.F32)
+        torch.cuda.synchronize()
+        o.GemvBlocks(B.Q8_0, last, y, out, 96, rows, fmt_x=B.F32)
+        want.append(out.clone())
+    got = [torch.empty_like(out) for _ in xs]
+    torch.cuda.synchronize()
+    for v, g in zip(xs, got):
+        o.GemvBlocks(B.Q8_0, big, v, y, rows, cols, fmt_x=B.F32)
+        o.GemvBlocks(B.Q8_0, small, x, z, 64, 256, fmt_x=B.F32)
+        nothing()
+        o.GemvBlocks(B.Q8_0, last, y, g, 96, rows, fmt_x=B.F32)
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert torch.equal(w, g)
