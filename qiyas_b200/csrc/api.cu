@@ -21,6 +21,7 @@ struct Kept {
 };
 Kept g_stage_a, g_stage_x, g_stage_y, g_scratch;
 int *g_status = nullptr;      // device word the kernels OR their STATUS_* bits into
+cudaError_t g_attend_error = cudaSuccess;      // what keeps qb200_cache_attention from running on the bound device
 int g_bound = -1;             // the device the kept buffers and the status word live on
 
 int fail(int code, const char *fmt, ...)
@@ -165,7 +166,8 @@ int qb200_init(int device)
     if ((e = qb::matmul_init(g_caps.sm_count, g_caps.max_shared_bytes, g_status))) return cuda_fail(e, "matmul attributes");
     if ((e = qb::shard_init(g_status))) return cuda_fail(e, "shard set-up");
     if ((e = qb::cache_init(g_status))) return cuda_fail(e, "cache set-up");
-    if ((e = qb::attend_init(g_caps.sm_count, g_caps.max_shared_bytes, g_status))) return cuda_fail(e, "attention set-up");
+    g_attend_error = qb::attend_init(g_caps.sm_count, g_caps.max_shared_bytes, g_status);
+    cudaGetLastError();           // what attention misses (qb200_cache_attention says so) is no launch's error
     g_ready = true;
     t_error[0] = 0;
     return 0;
@@ -556,6 +558,7 @@ int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *s
     OnDevice on;
     if (!g_ready) return fail(QB200_E_DEVICE, "qb200_init has not succeeded");
     if (on.e) return cuda_fail(on.e, "cudaSetDevice");
+    if (g_attend_error) return fail(QB200_E_DEVICE, "attention cannot run on this device: %s", cudaGetErrorString(g_attend_error));
     if (sequences->count == 0 || sequences->rows == 0) return 0;
     return finish_other(qb::attend(*cache, *sequences, type, a, (cudaStream_t)stream), "cache_attention", stream);
 }

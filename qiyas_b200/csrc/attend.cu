@@ -13,11 +13,15 @@ typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, 
 static EncodeTiled g_attend_encode = nullptr;
 static int *g_attend_status = nullptr;
 static int g_attend_sms = 0;
+static bool g_attend_tiles = false;        // the tile kernel can run as it is built
 
+// Attention's kernels ask for more of the device and the build than the products do; what they miss is theirs alone.  Without
+// the tile kernel the other takes every call; without that, calls are refused.
 cudaError_t attend_init(int sm_count, int max_smem, int *status)
 {
     g_attend_status = status;
     g_attend_sms = sm_count;
+    g_attend_tiles = false;
     if (max_smem < 232448) return cudaErrorInvalidValue;
     void *fn = nullptr;
     cudaDriverEntryPointQueryResult found;
@@ -26,7 +30,8 @@ cudaError_t attend_init(int sm_count, int max_smem, int *status)
     if (found != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
     g_attend_encode = (EncodeTiled)fn;
     if ((e = attend_rows_init())) return e;
-    return attend_tiles_init();
+    g_attend_tiles = attend_tiles_init() == cudaSuccess;
+    return cudaSuccess;
 }
 
 // What a call is cut into: rows a unit, by the kernel that takes it.
@@ -44,7 +49,7 @@ static Plan plan_of(const qb200_cache_t &c, const qb200_sequences_t &s, const qb
     // where dim is over 128.  Measured at 8 sequences of 6000 tokens, 4 heads, bf16, us (rows, then tiles): dim 128: 16 rows
     // 26 and 51, 32 rows 36 and 52, 64 rows 47 and 53, 96 rows 74 and 55; dim 256: 16 rows 44 and 86, 40 rows 81 and 88, 64
     // rows 121 and 92; dim 64: 64 rows 32 and 39, 96 rows 49 and 41.
-    plan.tiles = rows > (c.dim <= 128 ? 64 : 48);
+    plan.tiles = g_attend_tiles && rows > (c.dim <= 128 ? 64 : 48);
     plan.r = plan.tiles ? (c.dim <= 128 ? 256 : 128) : c.dim <= 128 && rows > 8 ? 16 : 8;
     // Units cut (equal shares, a second kernel) or each to a block of its own.  In tokens of 128 dims a block takes (about 11
     // cycles each): a unit costs 256 besides its tokens where the blocks stay, 556 where each has its own, the cut ones' partition

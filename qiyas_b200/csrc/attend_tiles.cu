@@ -41,7 +41,7 @@ struct TilesCfg {
     static constexpr int CW = DC == 128 ? 4 : 8, KW = CW / 2;   // converter warps: half of them for K, half for V
     static constexpr int WARPS = 4 * NQ + CW + 4, THREADS = 32 * WARPS;       // the last four: two issue the products, one fetches scales
     // registers a thread: of the launch, and of the softmax, converter and last warps (checked against the build when the
-    // library is bound: a share above the launch's would wait for good)
+    // library is bound, and the kernel left aside where it differs: a share above the launch's would wait for good)
     static constexpr int REGS = 128, SOFT_REGS = NQ == 2 ? 152 : 176, CONV_REGS = NQ == 2 ? 128 : 104, REST_REGS = NQ == 2 ? 80 : 128;
     static_assert(NQ * SOFT_REGS + CW / 4 * CONV_REGS + REST_REGS <= WARPS / 4 * REGS, "the shares of the registers fit the launch's");
     static constexpr uint32_t QTILE = 128 * DC * 2, SLOT = TT * DC * 2;

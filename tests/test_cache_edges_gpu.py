@@ -370,3 +370,45 @@ def test_a_call_with_nothing_to_do_orders_nothing(what):
     torch.cuda.synchronize()
     for w, g in zip(want, got):
         assert torch.equal(w, g)
+
+
+def test_a_tile_kernel_that_was_built_otherwise_is_left_aside(tmp_path):
+    """A library whose tile kernel says at set-up that it cannot run (another number of registers than its warps share out): the
+    products are as they were, and attention's other kernel takes prompts."""
+    import os
+    import shutil
+    import subprocess
+    import sys
+    from qiyas_b200 import build
+    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+    objects = [build._object(src) for src in build.SOURCES if src != "attend_tiles.cu"]
+    if not shutil.which(nvcc) or not all(os.path.exists(f) for f in objects):
+        pytest.skip("no compiler, or the package was not built here")
+    stub = tmp_path / "stub.cu"
+    stub.write_text("""#include "attend_device.cuh"
+namespace qb {
+cudaError_t attend_tiles_init() { return cudaErrorInvalidConfiguration; }
+int attend_tiles(const AttendArgs &, int, cudaStream_t) { return (int)cudaErrorInvalidConfiguration; }
+}
+""")
+    library = tmp_path / "libother.so"
+    subprocess.check_call([nvcc, *build.FLAGS[:2], "-std=c++17", "-Xcompiler", "-fPIC", "-I", build.CSRC, "-shared", "-o", str(library), str(stub)] + objects)
+    program = """
+import sys
+from qiyas_b200 import _lib, blocks as B
+_lib.LIBRARY = sys.argv[1]
+import numpy as np
+from tests import helpers as H
+from tests.test_cache_edges_gpu import Setup, check, gpu
+import torch
+y = torch.empty(64, device="cuda")
+H.ops().GemvBlocks(B.Q8_0, gpu(B.make_weights(B.Q8_0, 64, 256, 1)), torch.ones(256, device="cuda"), y, 64, 256, fmt_x=B.F32)
+assert y.isfinite().all() and (y != 0).any()
+for kind in ("f32", "f16", "bf16"):
+    for dim in (64, 128, 256):
+        check(Setup(53, 3, 400, 2, 16, dim), kind, [400, 131, 399], [130, 3, 200], 4)
+print("as it should be")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    ran = subprocess.run([sys.executable, "-c", program, str(library)], cwd=root, capture_output=True, text=True, timeout=300)
+    assert "as it should be" in ran.stdout, ran.stderr[-2000:]
