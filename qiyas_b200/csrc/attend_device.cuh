@@ -64,7 +64,7 @@ __device__ __forceinline__ Sequence sequence_at(const AttendArgs &p, int b)
     const int most = p.seq.width << p.log_page;
     bad |= s.len < 0 || s.len > most;
     s.len = max(0, min(s.len, most));
-    if (bad && (threadIdx.x & 31) == 0) atomicOr(p.status, STATUS_CACHE_RANGE);
+    if (bad) atomicOr(p.status, STATUS_CACHE_RANGE);           // (by any lane: where a share is found each looks at another sequence)
     return s;
 }
 

@@ -412,3 +412,40 @@ print("as it should be")
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     ran = subprocess.run([sys.executable, "-c", program, str(library)], cwd=root, capture_output=True, text=True, timeout=300)
     assert "as it should be" in ran.stdout, ran.stderr[-2000:]
+
+
+def bad_cases():
+    """(lengths, offsets) of 70 sequences that do not fit 100 rows or 64 tokens: one of them only, in every place."""
+    for b in (0, 1, 31, 32, 33, 69):
+        for what in ("offset past the rows", "offsets that fall", "length", "negative length"):
+            yield b, what
+
+
+@pytest.mark.parametrize("max_queries", [0, 1])
+@pytest.mark.parametrize("most", [64, 4096])
+@pytest.mark.parametrize("b,what", list(bad_cases()))
+def test_attention_reports_what_does_not_fit(b, what, most, max_queries):
+    """Whichever sequence it is, cut into shares or not: bit 4, and the others have their results."""
+    import torch
+    s = Setup(54, 70, 64, 1, 16, 32)
+    o, cache = H.ops(), s.on_gpu()
+    q = s.rows(100, 2, "f32")[0]
+    lens, offsets = np.full(70, 50, np.int32), np.arange(71, dtype=np.int32)
+    want, out = torch.full_like(q, 7.0), torch.full_like(q, 7.0)
+    o.CacheAttention(cache, q, want, gpu(s.table), ints(lens), offsets=ints(offsets), max_queries=max_queries, max_length=most)
+    assert o.gpu.status() == 0
+    bad_lens, bad_offsets = lens.copy(), offsets.copy()
+    if what == "length":
+        bad_lens[b] = 65
+    elif what == "negative length":
+        bad_lens[b] = -1
+    elif what == "offset past the rows":
+        bad_offsets[b + 1:] = 101 + np.arange(70 - b)
+    else:
+        bad_offsets[b + 1] = b - 1
+    o.CacheAttention(cache, q, out, gpu(s.table), ints(bad_lens), offsets=ints(bad_offsets), max_queries=max_queries, max_length=most)
+    assert o.gpu.status() == 16
+    assert torch.equal(out[:max(0, b - 1)], want[:max(0, b - 1)])
+    if "length" in what:
+        assert torch.equal(out[b + 1:70], want[b + 1:70])
+    assert (out[70:] == 7).all() or what == "offset past the rows"
