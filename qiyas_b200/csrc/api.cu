@@ -478,6 +478,19 @@ static int check_cache(const qb200_cache_t *c, const qb200_sequences_t *s, int t
     return 0;
 }
 
+// Do rows of dim values at i * a + j * b, 0 <= i < n, 0 <= j < m, lie apart?  a, b >= dim where there are several.
+static bool apart(int64_t a, int64_t n, int64_t b, int64_t m, int64_t dim)
+{
+    if (n < 2 || m < 2 || a >= (m - 1) * b + dim || b >= (n - 1) * a + dim) return true;      // one axis, or one inside the other
+    if (n < m) return apart(b, m, a, n, dim);
+    // one between the other: the distance of i * a and j * b, for every j (the smaller count: below 2^16 where the counts' product is below 2^31)
+    for (int64_t j = 1; j < m; j++) {
+        const int64_t i = j * b / a, over = j * b - i * a;
+        if ((i < n && over < dim) || (i + 1 < n && a - over < dim)) return false;
+    }
+    return true;
+}
+
 // dim: 0, or (written lanes) the values of a head, which have to lie apart from those of other rows and heads
 static int check_lanes(const char *name, int type, const qb200_lanes_t &x, int rows, int heads, int dim = 0)
 {
@@ -486,7 +499,7 @@ static int check_lanes(const char *name, int type, const qb200_lanes_t &x, int r
     const int64_t most = (int64_t)1 << 55;        // products with 32-bit counts stay inside 64 bits of bytes
     if (x.row_stride < 0 || x.head_stride < 0 || x.row_stride > most / ((int64_t)rows + 1) || x.head_stride > most / ((int64_t)heads + 1))
         return fail(QB200_E_SHAPE, "%s: strides %lld, %lld", name, (long long)x.row_stride, (long long)x.head_stride);
-    if ((rows > 1 && x.row_stride < dim) || (heads > 1 && x.head_stride < dim))
+    if (dim && ((rows > 1 && x.row_stride < dim) || (heads > 1 && x.head_stride < dim) || !apart(x.row_stride, rows, x.head_stride, heads, dim)))
         return fail(QB200_E_SHAPE, "%s: strides %lld, %lld: rows of %d values that are written overlap", name, (long long)x.row_stride, (long long)x.head_stride, dim);
     return 0;
 }

@@ -1,0 +1,43 @@
+"""Refusals of the cache operators at the edges of what they take (no GPU needed: arguments are looked at before the device;
+where one is there and the library bound, calls that are not refused have no sequences and launch nothing)."""
+import numpy as np
+import pytest
+
+from .test_cache_abi import SHAPE, lanes, lib, parts, sequences        # noqa: F401 (lib: a fixture)
+from qiyas_b200 import blocks as B
+
+
+def overlaps(row, head, rows, heads, dim):
+    starts = np.sort((np.arange(rows)[:, None] * row + np.arange(heads) * head).ravel())
+    return bool((np.diff(starts) < dim).any())
+
+
+@pytest.mark.parametrize("rows,heads,row,head", [(9, 2, 64, 64), (9, 2, 128, 128), (9, 2, 128, 1151), (9, 2, 100, 150), (9, 2, 128, 64), (9, 2, 64, 576), (9, 2, 64, 575),
+                                                 (9, 8, 64, 128), (9, 8, 130, 65), (9, 8, 128, 1024 + 64), (9, 8, 192, 64 + 9 * 192), (3, 2, 640, 320), (9, 8, 512, 64),
+                                                 (2, 8, 64, 128), (2, 8, 65, 130), (9, 4, 256, 320), (9, 4, 300, 100), (1, 8, 0, 64), (9, 2, 576, 64)])
+def test_written_rows_have_to_lie_apart(lib, rows, heads, row, head):      # noqa: F811
+    """Rows of 64 values: strides that bring a head of one row onto another row's are refused, all others are not."""
+    from qiyas_b200 import _lib
+    cache, seq, at = parts(heads=heads), sequences(rows=rows, count=0), lanes(256, row, head)
+    bad = overlaps(row, head, rows, heads, 64)
+    rc = lib.qb200_cache_read(cache, seq, B.F16, at, None, None)
+    assert (rc == SHAPE) == bad, rc
+    rc = lib.qb200_cache_read(cache, seq, B.F16, None, at, None)
+    assert (rc == SHAPE) == bad, rc
+    cache = parts(heads=1)
+    args = _lib.ATTENTION(256, 64 * heads, 64, 256, row, head, 0, 4096, 1 << 40, heads, 0, 0, 0.125, 1, 0)
+    rc = lib.qb200_cache_attention(cache, seq, B.F16, args, None)
+    assert (rc == SHAPE) == bad, rc
+    assert lib.qb200_cache_write(parts(heads=heads), seq, B.F16, at, at, None) != SHAPE      # what is read may overlap
+
+
+def test_strides_of_all_kinds(lib):                                         # noqa: F811
+    rng = np.random.default_rng(7)
+    refused = 0
+    for _ in range(3000):
+        rows, heads = int(rng.integers(1, 12)), int(rng.integers(1, 12))
+        row, head = (int(rng.choice([64, 65, 80, 96, 100, 128, 130, 192, 256, 512, 640, 700, 777])) for _ in range(2))
+        rc = lib.qb200_cache_read(parts(heads=heads), sequences(rows=rows, count=0), B.F16, lanes(256, row, head), None, None)
+        assert (rc == SHAPE) == overlaps(row, head, rows, heads, 64), (rows, heads, row, head)
+        refused += rc == SHAPE
+    assert 500 < refused < 2500
