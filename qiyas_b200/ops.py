@@ -304,7 +304,8 @@ class GpuOps:
         call's own among them.  causal: the rows of a sequence are its last tokens; window: how many tokens a row sees at most
         (0: all).  lse: optional f32 [rows, query heads].  max_queries, max_length: bounds on the rows of a sequence and on
         lengths, known to the host, for the choice of kernel (0: rows, or 1 without offsets; all the table holds).  scale None:
-        1 / sqrt(dim).  workspace None: one of the call's own, from torch's allocator on the call's stream."""
+        1 / sqrt(dim).  workspace: a tensor (or address) of attention_workspace_bytes(...) bytes, private to the call until it has
+        run; None: one of the call's own, from torch's allocator on the call's stream."""
         stream = self._current(stream)
         heads = q.shape[1] if q.dim() == 3 else 0
         kind, rows, base, row, head = self._lanes(cache, q, "q", heads)
@@ -318,6 +319,10 @@ class GpuOps:
                 raise ValueError(f"lse: contiguous float32 {(rows, heads)} on the cache's device")
             lse_at = lse.data_ptr()
         scale = cache.dim ** -0.5 if scale is None else scale
+        if workspace is not None and not isinstance(workspace, int):
+            if workspace.get_device() != cache.index or not workspace.is_contiguous():
+                raise ValueError(f"workspace: contiguous, on the cache's device; got {workspace.stride()} on {workspace.device}")
+            workspace_bytes = workspace_bytes or workspace.numel() * workspace.element_size()
         workspace = _ptr(workspace) or 0
         rest = (heads, max_queries, max_length, scale, 1 if causal else 0, window)
         args = _lib.ATTENTION(base, row, head, out_base, out_row, out_head, lse_at, workspace, workspace_bytes, *rest)
@@ -330,6 +335,13 @@ class GpuOps:
         if rc:
             self.gpu.check(rc, "CacheAttention")
         return "f16 mma cache blocks"
+
+    def attention_workspace_bytes(self, cache, q, table, lengths, offsets=None, max_queries=0, max_length=0):
+        """What a CacheAttention call with these arguments needs of a caller's own workspace (0: none)."""
+        heads = q.shape[1] if q.dim() == 3 else 0
+        kind, rows, base, row, head = self._lanes(cache, q, "q", heads)
+        args = _lib.ATTENTION(base, row, head, base, row, head, 0, 0, 0, heads, max_queries, max_length, 1.0, 1, 0)
+        return int(self.lib.qb200_cache_attention_workspace_bytes(cache.parts, self._sequences(cache, table, lengths, offsets, rows), kind, args))
 
     def _lanes(self, cache, t, name, heads):
         """Rows [rows, heads, dim] of a cache operator as the C ABI takes them: (lane type, rows, address, row stride, head stride)."""

@@ -449,3 +449,40 @@ def test_attention_reports_what_does_not_fit(b, what, most, max_queries):
     if "length" in what:
         assert torch.equal(out[b + 1:70], want[b + 1:70])
     assert (out[70:] == 7).all() or what == "offset past the rows"
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("counts,dim", [([1, 1, 1], 128), ([1, 1, 1], 256), ([100, 3, 140], 64), ([60, 3, 40], 192)])
+def test_a_workspace_of_the_callers_own(kind, counts, dim):
+    """The size asked for is enough, nothing behind it is touched, less is refused, and one serves calls (and replays) in turn."""
+    import torch
+    s = Setup(55, 3, 3000, 2, 16, dim)
+    o, cache, lens = H.ops(), s.on_gpu(), ints([3000, 1, 2049])
+    q = s.rows(sum(counts), 8, kind)[0]
+    args, bounds = (gpu(s.table), lens), dict(offsets=ints(offsets_of(counts)), max_queries=max(counts), max_length=3000)
+    want, out = torch.empty_like(q), torch.full_like(q, 5.0)
+    o.CacheAttention(cache, q, want, *args, **bounds)
+    need = o.attention_workspace_bytes(cache, q, *args, **bounds)
+    assert need > 0
+    room = torch.full((need + 4096,), 0xa5, dtype=torch.uint8, device="cuda")
+    for extra in (dict(workspace=room[:need]), dict(workspace=room.data_ptr(), workspace_bytes=need)):
+        for _ in range(2):
+            out.fill_(5.0)
+            o.CacheAttention(cache, q, out, *args, **bounds, **extra)
+            assert torch.equal(out, want)
+    assert (room[need:] == 0xa5).all()
+    for bad in (dict(workspace=room[:need - 1]), dict(workspace=room[8:]), dict(workspace=room, workspace_bytes=need - 1), dict(workspace=room.cpu()),
+                dict(workspace=room[::2])):
+        with pytest.raises(ValueError):
+            o.CacheAttention(cache, q, out, *args, **bounds, **bad)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], [torch.empty_like(q) for _ in range(2)]
+    for g, t in zip(graphs, outs):
+        with torch.cuda.graph(g):
+            o.CacheAttention(cache, q, t, *args, **bounds, workspace=room[:need])
+    for _ in range(5):
+        for g, t in zip(graphs, outs):
+            t.fill_(5.0)
+            g.replay()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+    short = o.attention_workspace_bytes(cache, q[:1], args[0][:1], lens[:1], max_length=40)
+    assert short == 0 and o.gpu.status() == 0            # short sequences are not cut
