@@ -486,3 +486,117 @@ def test_a_workspace_of_the_callers_own(kind, counts, dim):
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
     short = o.attention_workspace_bytes(cache, q[:1], args[0][:1], lens[:1], max_length=40)
     assert short == 0 and o.gpu.status() == 0            # short sequences are not cut
+
+
+# ------------------------------------------------------------------------------------------------ the tile kernel's own paths
+
+TILES = [(2, [90, 40], [400, 70]), (1, [260, 129], [700, 129]), (4, [70, 1], [1300, 1100])]        # query heads a head, rows, tokens
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("group,counts,lens", TILES)
+@pytest.mark.parametrize("dim", [48, 128, 192])
+def test_tiles_with_strides(kind, group, counts, lens, dim):
+    """q and out as slices of wider rows, with a head order of their own, and from bases that are not 16-byte aligned; what lies
+    between the rows of out stays."""
+    import torch
+    s = Setup(56, 2, max(lens), 2, 32, dim)
+    rows, heads = sum(counts), 2 * group
+    x = s.rows(rows, heads + 2, kind, 2.0)[0]
+    flat = torch.cat([torch.zeros(1, dtype=x.dtype, device="cuda"), x.reshape(-1)])
+    qs = (x[:, 1:heads + 1], flat[1:].view(rows, heads + 2, dim)[:, 1:heads + 1], x.transpose(0, 1).contiguous().transpose(0, 1)[:, 1:heads + 1])
+    for i, q in enumerate(qs):
+        room = torch.full((rows * (heads + 2) * dim + 1,), 9.0, dtype=x.dtype, device="cuda")
+        whole = (room[1:].view(rows, heads + 2, dim), room[:-1].view(rows, heads + 2, dim), room[:-1].view(heads + 2, rows, dim).transpose(0, 1))[i]
+        out = whole[:, 1:heads + 1]
+        check(s, kind, lens, counts, group, q=q, out=out, window=0 if i else 90)
+        assert (whole[:, 0] == 9).all() and (whole[:, heads + 1] == 9).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("group,counts,lens", TILES)
+@pytest.mark.parametrize("page,dim", [(16, 64), (16, 128), (32, 256), (128, 192)])
+def test_tiles_with_pages_that_are_not_there(kind, group, counts, lens, page, dim):
+    """Pages the table does not name, inside tiles, whole tiles and the first and last: left out, and reported."""
+    s = Setup(57, 2, max(lens), 2, page, dim)
+    table, absent = s.table.copy(), []
+    for b, length in enumerate(lens):
+        last = (length - 1) // page
+        for slot in {0, 3, 4, 5, 6, 7, 11, last} if b == 0 else {last // 2}:
+            if slot <= last:
+                table[b, slot] = -1 if slot % 2 else s.pages + slot
+                absent.append((b, slot))
+    check(s, kind, lens, counts, group, table=table, absent=absent, status=16)
+    check(s, kind, lens, counts, group, table=table, absent=absent, status=16, window=page)      # some rows see nothing else
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("group,counts,lens", TILES)
+@pytest.mark.parametrize("dim", [64, 192])
+def test_tiles_with_pages_missing_and_scales_of_all_kinds(kind, group, counts, lens, dim):
+    s = Setup(58, 4, max(lens), 2, 16, dim)
+    odd_scales(s, s.rng)
+    table, absent = s.table.copy(), [(0, 2), (0, 17), (1, 1), (2, 0), (2, 40)]
+    lens, counts = [*lens, *lens[::-1]], [*counts, 30, 2]
+    for b, slot in absent:
+        if slot < s.width:
+            table[b, slot] = -7
+    absent = [(b, slot) for b, slot in absent if slot < s.width]
+    check(s, kind, lens, counts, group, table=table, absent=absent, status=16)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("group,counts,lens", TILES)
+@pytest.mark.parametrize("dim", [128, 256])
+def test_tiles_with_nan_rows_and_unwritten_places(kind, group, counts, lens, dim):
+    """NaN and infinities in rows of q stay in their rows; codes and scales that no row sees do not matter."""
+    import torch
+    s = Setup(59, 2, max(lens) + 40, 2, 16, dim)
+    o, cache, heads, rows = H.ops(), s.on_gpu(), 2 * group, sum(counts)
+    q = s.rows(rows, heads, kind)[0]
+    args = gpu(s.table), ints(lens), ints(offsets_of(counts))
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    lse, want_lse = (torch.empty(rows, heads, device="cuda") for _ in range(2))
+    o.CacheAttention(cache, q, want, *args, lse=want_lse)
+    used = np.concatenate([s.table[b, :(n + 15) // 16] for b, n in enumerate(lens)])
+    rest = torch.from_numpy(np.setdiff1d(np.arange(s.pages), used)).cuda()
+    for c in (cache.k_scales, cache.v_scales):
+        c[rest] = float("nan")
+    for c in (cache.k_codes, cache.v_codes):
+        c[rest] = 127
+        for b, n in enumerate(lens):
+            if n % 16:
+                c[int(s.table[b, n // 16]), :, n % 16:] = -128
+    o.CacheAttention(cache, q, out, *args, lse=lse)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    marks = [(0, 0, float("nan")), (rows - 1, heads - 1, float("inf")), (rows // 2, 1, -float("inf")), (3, heads - 1, float("nan"))]
+    for r, h, x in marks:
+        q[r, h, 5] = x
+    o.CacheAttention(cache, q, out, *args, lse=lse)
+    for r, h, _ in marks:
+        assert out[r, h].isnan().all() and lse[r, h].isnan()
+        out[r, h], lse[r, h] = want[r, h], want_lse[r, h]
+    assert torch.equal(out, want) and torch.equal(lse, want_lse) and o.gpu.status() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_tiles_over_a_dominant_token(dim):
+    """One token takes nearly all the weight and its value is zero: the small weights' sum is left, in every row.  The tolerance is
+    `check`'s: scores of up to 15.3, two f16 a weight, and 2^-35 of the largest weight for each token."""
+    s = Setup(60, 1, 2048, 1, 16, dim)
+    s.v.scales[:] = 0.01
+    p = s.table[0, 0]
+    s.v.codes[p, 0, 0] = 0
+    s.k.codes[p, 0, 0], s.k.scales[p, 0] = 127, 0.05
+    import torch
+    o, n = H.ops(), 150
+    q = torch.full((n, 1, dim), 0.3 * 8 / dim ** 0.5, device="cuda")
+    out = torch.empty_like(q)
+    o.CacheAttention(s.on_gpu(), q, out, gpu(s.table), ints([2048]), offsets=ints([0, n]))
+    k, v = (gpu(c.values(s.table[0], 0, 2048))[:, 0] for c in (s.k, s.v))
+    scores = (q[:, 0].double() @ k.t() * dim ** -0.5).masked_fill(torch.arange(2048, device="cuda") > 2048 - n + torch.arange(n, device="cuda")[:, None], -float("inf"))
+    weights = torch.softmax(scores, -1)
+    assert weights[:, 0].min() > 0.99
+    score = ((dim + 8) * 2.0 ** -24 + 2.0 ** -20) * 16.3
+    bound = weights @ v.abs() * (2 * score + 2.0 ** -21 + (2048 / 128 + 64) * 2.0 ** -24) + 2.0 ** -35 * 2048 * 128 * 0.01
+    assert bool(((out[:, 0].double() - weights @ v).abs() <= bound).all())
