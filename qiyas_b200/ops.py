@@ -11,6 +11,7 @@ Errors follow the reference: a format or shape the block product does not take r
 ``RuntimeError`` (its InvalidOperationException).  Nothing here computes on the CPU.
 """
 import ctypes as C
+import struct
 from dataclasses import dataclass
 
 from . import _lib
@@ -325,7 +326,10 @@ class GpuOps:
             workspace_bytes = workspace_bytes or workspace.numel() * workspace.element_size()
         workspace = _ptr(workspace) or 0
         rest = (heads, max_queries, max_length, scale, 1 if causal else 0, window)
-        args = _lib.ATTENTION(base, row, head, out_base, out_row, out_head, lse_at, workspace, workspace_bytes, *rest)
+        try:
+            args = _lib.ATTENTION(base, row, head, out_base, out_row, out_head, lse_at, workspace, workspace_bytes, *rest)
+        except (struct.error, OverflowError) as e:
+            raise ValueError(f"max_queries {max_queries}, max_length {max_length}, scale {scale}, window {window}, workspace_bytes {workspace_bytes}: {e}") from None
         if not workspace:
             need = self.lib.qb200_cache_attention_workspace_bytes(cache.parts, seq, kind, args)
             if need:
@@ -340,7 +344,10 @@ class GpuOps:
         """What a CacheAttention call with these arguments needs of a caller's own workspace (0: none)."""
         heads = q.shape[1] if q.dim() == 3 else 0
         kind, rows, base, row, head = self._lanes(cache, q, "q", heads)
-        args = _lib.ATTENTION(base, row, head, base, row, head, 0, 0, 0, heads, max_queries, max_length, 1.0, 1, 0)
+        try:
+            args = _lib.ATTENTION(base, row, head, base, row, head, 0, 0, 0, heads, max_queries, max_length, 1.0, 1, 0)
+        except (struct.error, OverflowError) as e:
+            raise ValueError(f"max_queries {max_queries}, max_length {max_length}: {e}") from None
         return int(self.lib.qb200_cache_attention_workspace_bytes(cache.parts, self._sequences(cache, table, lengths, offsets, rows), kind, args))
 
     def _lanes(self, cache, t, name, heads):

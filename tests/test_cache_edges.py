@@ -41,3 +41,26 @@ def test_strides_of_all_kinds(lib):                                         # no
         assert (rc == SHAPE) == overlaps(row, head, rows, heads, 64), (rows, heads, row, head)
         refused += rc == SHAPE
     assert 500 < refused < 2500
+
+
+@pytest.mark.parametrize("change", [dict(max_queries=2 ** 31), dict(max_length=2 ** 40), dict(max_length=-2 ** 31 - 1), dict(window=2 ** 31), dict(max_queries=1.5),
+                                    dict(window="16"), dict(workspace_bytes=-1), dict(scale="large")])
+def test_numbers_the_library_cannot_hold_are_argument_errors(change):
+    """As every other argument error of the mirror: ValueError, before the library is called."""
+    import torch
+    from qiyas_b200 import BlockCache
+    from qiyas_b200.ops import GpuOps
+
+    class Host:                     # the checks alone: tensors and "device" of the host, and no library
+        device = -1
+    ops = GpuOps.__new__(GpuOps)
+    ops.gpu, ops.lib, ops._scratch = Host(), None, {}
+    codes, scales = torch.zeros(4, 2, 16, 64, dtype=torch.int8), torch.zeros(4, 2)
+    cache = BlockCache(codes, codes.clone(), scales, scales.clone())
+    q, table, lengths = torch.zeros(3, 4, 64), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        ops.CacheAttention(cache, q, torch.zeros_like(q), table, lengths, workspace=4096, stream=0, **change)
+    bounds = {k: v for k, v in change.items() if k.startswith("max")}
+    if bounds:
+        with pytest.raises(ValueError):
+            ops.attention_workspace_bytes(cache, q, table, lengths, **bounds)
