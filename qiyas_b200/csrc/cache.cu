@@ -223,6 +223,7 @@ __global__ void __launch_bounds__(item_threads(LANES)) cache_write_kernel(const 
             old[i] = n;
         }
     }
+    if (LANES == 32) __syncwarp();                 // every lane has read the scale (a block of several warps met above)
     if (tid == 0 && (scale != had || !it.first)) *scale_at = scale;
 
     uint2 *dst = (uint2 *)(codes + it.first * p.dim);

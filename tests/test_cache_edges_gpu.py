@@ -600,3 +600,22 @@ def test_tiles_over_a_dominant_token(dim):
     score = ((dim + 8) * 2.0 ** -24 + 2.0 ** -20) * 16.3
     bound = weights @ v.abs() * (2 * score + 2.0 ** -21 + (2048 / 128 + 64) * 2.0 ** -24) + 2.0 ** -35 * 2048 * 128 * 0.01
     assert bool(((out[:, 0].double() - weights @ v).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("page,dim", [(16, 16), (16, 128), (32, 64)])
+def test_scales_that_grow_with_every_token(page, dim):
+    """Blocks that a single warp writes, whose scale is read by all lanes and replaced by one, again and again: bit for bit."""
+    s = Setup(61, 200, page, 3, page, dim)
+    o, cache, table = H.ops(), s.on_gpu(), gpu(s.table)
+    rng = s.rng
+    for at in range(page):
+        x = (rng.standard_normal((200, 3, dim)) * np.exp(at * rng.uniform(0, 0.5, (200, 3, 1)))).astype(np.float32)
+        t = gpu(x)
+        o.CacheWrite(cache, t, -t, table, ints([at] * 200))
+        for b in range(200):
+            p = s.table[b, 0]
+            for h in range(3):
+                s.k.codes[p, h], s.k.scales[p, h] = written(s.k.codes[p, h], s.k.scales[p, h], at, x[b:b + 1, h])
+    pages = s.table[:, 0]
+    assert np.array_equal(cache.k_codes.cpu().numpy()[pages], s.k.codes[pages]) and np.array_equal(cache.k_scales.cpu().numpy()[pages], s.k.scales[pages])
+    assert np.array_equal(cache.v_scales.cpu().numpy()[pages], s.k.scales[pages]) and o.gpu.status() == 0
