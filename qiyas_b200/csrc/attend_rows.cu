@@ -21,9 +21,9 @@
 //    factor is the denominator, and O = v0 * sum w cv.  The producers take logarithms and quotients, a lane a page.
 //    (|sv| is meant: where sv is below 0 the weights change sign, where it is 0 they are zeros in the second product, and a page
 //    that is not there has weights of 0 in the denominator too.)
-//    m is chosen so that w lies at 2^11 at its largest when it is set and is kept while w stays below 2^15: f16 then holds
-//    weights down to 2^-24 of the largest with all its bits and errs by 2^-35 of it below, and the accumulators are seldom
-//    rescaled.
+//    m is a whole number, so that the powers of two which parts are scaled by add to it exactly.  It is chosen so that w lies at
+//    2^10 .. 2^11 at its largest when it is set and is kept while w stays below 2^15: f16 then holds weights down to 2^-24 of the
+//    largest with all its bits and errs by 2^-35 of it below, and the accumulators are seldom rescaled.
 //  * q is scaled by a power of two to a row's maximum of 2^13 and cut to f16; with f32 lanes q and w enter as the sum of
 //    two f16 (SPL 2), which loses 2^-22.
 //
@@ -52,7 +52,7 @@ struct RowsCfg {
     static constexpr int S = DT == 64 ? 24 : DT == 128 ? 16 : 8;
     static constexpr uint32_t MROW = DT + 4;                    // floats a row of the joining buffer
     static constexpr uint32_t O_RING = 0, O_Q = S * STAGE, O_MERGE = O_Q + KS * NB * SPL * 256, O_ML = O_MERGE + RW * R * MROW * 4;
-    static constexpr uint32_t O_HEAD = O_ML + RW * R * 8, SMEM = O_HEAD + ROWS_HEADER + 1024;
+    static constexpr uint32_t O_HEAD = O_ML + RW * R * 16, SMEM = O_HEAD + ROWS_HEADER + 1024;
     static_assert(S % RW == 0 && S % RP == 0, "a stage has one consumer warp and one producer");
     static_assert(SMEM <= 232448, "227 KB of shared memory");
 };
@@ -214,10 +214,10 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
     }
 
     // ---------------------------------------------------------------------- consumers
-    const int g = lane >> 2, t = lane & 3;
+    const int g = lane >> 2, t = lane & 3, pages16 = p.log_page == 4;
     uint2 *qs = (uint2 *)(smem + C::O_Q);
     float *merge = (float *)(smem + C::O_MERGE);
-    float2 *ml = (float2 *)(smem + C::O_ML);
+    float4 *ml = (float4 *)(smem + C::O_ML);       // of a warp's part of a row: exponent, sum, what its O is to be multiplied by
     // this warp's rows of q for a piece: asked for while the piece before it runs
     auto rows_of = [&](const Unit &u, Vec8<T> (&q)[NB]) {
 #pragma unroll
@@ -348,7 +348,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                 }
 
             // ---- weights
-            const float4 *sc[2] = { &head->scales[stage][0], &head->scales[stage][p.log_page == 4] };
+            const float4 *sc[2] = { &head->scales[stage][0], &head->scales[stage][pages16] };
 #pragma unroll
             for (int mt = 0; mt < 2; mt++)
 #pragma unroll
@@ -402,7 +402,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                         float top = fmaxf(fmaxf(s[0][nb][c], s[0][nb][c + 2]), fmaxf(s[1][nb][c], s[1][nb][c + 2]));
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        const float next = fmaxf(mm[nb][c], top - 11.f), less = exp2_fast(mm[nb][c] - next);
+                        const float next = fmaxf(mm[nb][c], ceilf(top) - 11.f), less = exp2_fast(mm[nb][c] - next);
                         mm[nb][c] = next;
                         l[nb][c] *= less;
 #pragma unroll
@@ -494,8 +494,9 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                 const int r = nb * 8 + 2 * t + c;
-                const float times = part_scale(mm[nb][c], sum, v0);
-                if (g == 0) ml[warp * C::R + r] = make_float2(mm[nb][c], sum);
+                // O is multiplied where the parts are joined (window, f32: 38.7 us here, 36.9 there; at dim 256 it costs registers: 57.6, 60.5)
+                const float scale = part_scale(mm[nb][c], sum, v0), times = DT == 256 ? scale : 1.f;
+                if (g == 0) ml[warp * C::R + r] = make_float4(mm[nb][c], sum, DT == 256 ? 1.f : scale, 0.f);
                 float *row = merge + (warp * C::R + r) * C::MROW;
 #pragma unroll
                 for (int i = 0; i < C::SUB * (DT == 64 ? 2 : 4); i++) {
@@ -515,14 +516,14 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int k = 0; k < RW; k++) {
-                const float2 part = ml[k * C::R + r];
-                const float f = exp2_fast(part.x - m);
+                const float4 part = ml[k * C::R + r];
+                const float f = exp2_fast(part.x - m), fo = DT == 256 ? f : f * part.z;
                 const float4 x = *(const float4 *)(merge + (k * C::R + r) * C::MROW + d);
                 sum = __fmaf_rn(part.y, f, sum);
-                acc.x = __fmaf_rn(x.x, f, acc.x);
-                acc.y = __fmaf_rn(x.y, f, acc.y);
-                acc.z = __fmaf_rn(x.z, f, acc.z);
-                acc.w = __fmaf_rn(x.w, f, acc.w);
+                acc.x = __fmaf_rn(x.x, fo, acc.x);
+                acc.y = __fmaf_rn(x.y, fo, acc.y);
+                acc.z = __fmaf_rn(x.z, fo, acc.z);
+                acc.w = __fmaf_rn(x.w, fo, acc.w);
             }
             if (complete) finish_row<T>(p, u, u.r0 + r, d, acc, m, sum);
             else {
