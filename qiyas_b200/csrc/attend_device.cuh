@@ -359,9 +359,9 @@ __device__ __forceinline__ float2 scales_at(const AttendArgs &p, int page, int h
     return make_float2(__ldg(p.k_scales + i), __ldg(p.v_scales + i));
 }
 // V's scales enter the weights against a reference v0, a power of two: the largest scale of those first met, rounded down.  A
-// scale more than 2^FAR above v0 sets a new one, one more than 2^FAR below counts as 0.  So weights of up to 2^15 against a page FAR
-// above v0 leave those against one FAR below above f32's least normal number, down to 2^-35 of the largest, and the denominator (at most
-// 2^17 tokens of 2^(15 + FAR) a part) below its largest, whatever the scales are.
+// scale more than 2^FAR above v0 sets a new reference, one more than 2^FAR below counts as 0.  So whatever the scales are, f32
+// holds a weight beside one that is 2^(2 FAR) larger by their scales and 2^35 by their scores, and the denominator of a part
+// (2^17 tokens of 2^15 * 2^FAR at most).
 constexpr int FAR = 50;
 __device__ __forceinline__ int exponent_of(float x) { return (__float_as_int(x) >> 23) & 255; }
 // The bits of what V's scale asks of the reference: its size, or 0 where there is nothing to measure.
@@ -371,9 +371,9 @@ __device__ __forceinline__ void raise(float &v0, uint32_t largest)       // larg
     const float to = __uint_as_float(min(max(largest & 0x7f800000u, 1u << 23), 253u << 23));      // its inverse is a normal number too
     if (largest && (v0 == 0.f || exponent_of(to) > exponent_of(v0) + FAR)) v0 = to;
 }
-// Where the reference rises by 2^step, the weights of what a row has seen get smaller by as much and O is scaled down; the exponent m
-// of a row that sees tokens of the tile falls by FALL first, or what was large against the old reference (its weights lie at 2^11
-// against a scale 2^FAR above it at most) would leave the new ones f16's least numbers.
+// Where the reference rises by 2^step, the weights of what a row has seen get smaller by as much: O goes down.  A row's exponent m
+// may have stood for scales up to 2^FAR above the old reference, and against it the new tokens' weights would be f16's least
+// numbers, so m falls by FALL before the tile is looked at (2^6 is then the least that the largest new weight can be).
 constexpr float FALL = 45.f;
 // How the tokens of a page are weighted.
 struct Weighted {

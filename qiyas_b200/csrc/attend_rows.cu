@@ -25,10 +25,16 @@
 //    2^10 .. 2^11 at its largest when it is set and is kept while w stays below 2^15: f16 then holds weights down to 2^-24 of the
 //    largest with all its bits and errs by 2^-35 of it below, and the accumulators are seldom rescaled.
 //  * q is scaled by a power of two to a row's maximum of 2^13 and cut to f16; with f32 lanes q and w enter as the sum of
-//    two f16 (SPL 2), which loses 2^-22.
+//    two f16 (SPL 2), which loses 2^-22.  With 16-bit lanes w is one f16, half a step of 2^-11 each, independent of one
+//    another, and out = sum w v / sum w (the denominator has all 24 bits) is off by less than 2^-11 of sum p |v|, by a third of
+//    that or less in the mean.  The output's own rounding is as large (f16) or 8 times as large (bf16).  Measured, f16, relative: prompts
+//    2.9e-4 where f32 weights give 2.1e-4, 40 rows at dim 256 2.5e-4 and 2.1e-4, 131072 tokens 2.5e-4 and 2.3e-4; bf16 1.67e-3 and
+//    1.66e-3.  Two f16 a weight bring it to what f32 weights give and cost f16 prompts 20 % (1164 -> 1391 us), dim 256 7 %,
+//    steps 3 %, long documents 1 %: not taken, since a caller who needs more than f16's own rounding has f32 lanes.
 //
-// Measured (bf16, 8 heads of the cache, 128 dims): 32 sequences of 500 to 8000 tokens, 4 query heads a head 64 us = 4.65 TB/s of
-// codes, 71 % of the copy peak; one of 131072 tokens, 8 a head 57 us, 71 %; 129 tokens 7 us on the device.  Of the 64 us, 45
+// Measured (bf16, 8 heads of the cache, 128 dims): 32 sequences of 500 to 8000 tokens, 4 query heads a head 64 us = 4.6 TB/s of
+// codes, 70 % of the copy peak; one of 131072 tokens, 8 a head 58 us, 71 %; a window of 1024 in f32, one row a head, 37 us, 25 %;
+// 129 tokens 7 us on the device.  Of the 64 us, 45
 // are the memory's; the partition at the start takes 3, the join's launch 4, and a piece's beginning and end 1.5 each.
 #include <cuda.h>
 #include "common.cuh"
@@ -494,7 +500,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                 const int r = nb * 8 + 2 * t + c;
-                // O is multiplied where the parts are joined (window, f32: 38.7 us here, 36.9 there; at dim 256 it costs registers: 57.6, 60.5)
+                // O's factor is taken below, where the parts are joined (f32 window: 38.0 us, taken here 38.6); at dim 256 that spills (60.5 us, here 58.6)
                 const float scale = part_scale(mm[nb][c], sum, v0), times = DT == 256 ? scale : 1.f;
                 if (g == 0) ml[warp * C::R + r] = make_float4(mm[nb][c], sum, DT == 256 ? 1.f : scale, 0.f);
                 float *row = merge + (warp * C::R + r) * C::MROW;

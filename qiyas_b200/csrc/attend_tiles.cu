@@ -12,11 +12,14 @@
 //  * Four softmax warps a row tile, a thread a row, with two buffers of S: the tensor pipe is a tile of tokens ahead.
 //  * A thread reads its row of S once and takes the weights against the exponent it has: only where one would pass 2^15 does
 //    it raise the exponent and go back over what the row has of O, by a power of two.
-//  * The registers are shared out between the warps' kinds (setmaxnreg), so that none spills.
-// Scales, exponents and the cut of q and w are those of attend_rows.cu; so are the shares of the grid's blocks.
+//  * The registers are shared out between the warps' kinds (setmaxnreg): up to 128 dims 16-bit lanes spill nothing, f32 lanes 12 bytes,
+//    over 128 dims 72 to 76.
+// Scales, exponents and the cut of q and w (what it costs, and why) are those of attend_rows.cu; so are the shares of the
+// grid's blocks.  One warp takes the logarithms of V's scales; where a tile has scales of 0 or below, the stored weights are put right
+// after the fact, out of the way of the others (in their loop it took prompts from 1.18 to 1.21 ms).
 //
-// Measured: 7894 queries of 32 heads (8 of the cache) over up to 8192 tokens, causal, 128 dims, bf16: 1.18 ms, 666 TFLOP/s, 39 %
-// of the library's bf16 product.  Three chains are near one another there (with the work of one left out in a copy): the
+// Measured: 7894 queries of 32 heads (8 of the cache) over up to 8192 tokens, causal, 128 dims, bf16: 1.2 ms, 650 TFLOP/s, 39 %
+// of the library's bf16 product; 3900 of them over up to 4000 tokens: f32 626 us, at 256 dims in bf16 955 us.  Three chains are near one another there (with the work of one left out in a copy): the
 // converters 1.01 ms, the softmax 1.00 ms, the products with their barriers 0.82 ms; what they wait for is mostly
 // instructions (16 warps of four kinds, 90 KB of code).  Tried and dropped: tiles of 128 tokens with one buffer of S a row tile
 // (1.3 ms: the chain from a product through softmax to the next is not hidden), a maximum pass over S before the weights

@@ -13,7 +13,9 @@
 // The memory bounds long prompts: 25 370 tokens of 8 heads x 128 in f16, pages of 64, are written in 42 us and read back in 27,
 // 4.5 TB/s together (69 % of the copy peak); 43 288 tokens in bf16, pages of 16, are read back at 5.4 TB/s (83 %).  A write is
 // 10 instructions a value, and three quarters of the issue slots are taken: the largest magnitude as bits, two values at a time (it was 5 a value in floats, 65 us), and the check of the
-// rounding eight values at a time.  One token a sequence is a launch's latency, 5 us.
+// rounding eight values at a time.  One token a sequence is a launch's latency, 3 to 5 us
+// (64 sequences, 8 heads x 128, pages of 16, replayed: 3.2 us); where a block's scale grows the serial loop over its earlier codes
+// shows: 12 us if a tenth of the blocks grow, 13 if all do (pages of 64: 5.7, 18.6, 24.8).
 #include "common.cuh"
 #include "cache.h"
 #include "cache_device.cuh"

@@ -619,3 +619,15 @@ def test_scales_that_grow_with_every_token(page, dim):
     pages = s.table[:, 0]
     assert np.array_equal(cache.k_codes.cpu().numpy()[pages], s.k.codes[pages]) and np.array_equal(cache.k_scales.cpu().numpy()[pages], s.k.scales[pages])
     assert np.array_equal(cache.v_scales.cpu().numpy()[pages], s.k.scales[pages]) and o.gpu.status() == 0
+
+
+def test_codes_of_subnormal_scales_are_held_to_127():
+    """Where the scale is f32's least number its rounding can leave quotients above 127."""
+    s = Setup(62, 1, 16, 1, 16, 16)
+    o, cache = H.ops(), s.on_gpu()
+    least = np.float32(2.0 ** -149)
+    x = (np.array([150, -150, 190, -190, 127, 100, -3, 0] * 2, np.float32) * least).reshape(1, 1, 16)
+    o.CacheWrite(cache, gpu(x), gpu(x), gpu(s.table), ints([0]))
+    p = int(s.table[0, 0])
+    assert cache.k_scales[p, 0].item() == least and o.gpu.status() == 0
+    assert cache.k_codes[p, 0, 0].tolist() == [127, -127, 127, -127, 127, 100, -3, 0] * 2
