@@ -118,7 +118,7 @@ __device__ __forceinline__ void seq_rows(const qb200_sequences_t &s, int b, int 
     const int lo = s.offsets[b], hi = s.offsets[b + 1];
     bad = lo < 0 || hi < lo || hi > s.rows;
     row = max(0, min(lo, s.rows));
-    n = max(0, min(hi, s.rows) - row);
+    n = max(row, min(hi, s.rows)) - row;           // (whatever hi is, the difference stays inside 32 bits)
 }
 
 }  // namespace qb

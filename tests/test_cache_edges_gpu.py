@@ -631,3 +631,31 @@ def test_codes_of_subnormal_scales_are_held_to_127():
     p = int(s.table[0, 0])
     assert cache.k_scales[p, 0].item() == least and o.gpu.status() == 0
     assert cache.k_codes[p, 0, 0].tolist() == [127, -127, 127, -127, 127, 100, -3, 0] * 2
+
+
+@pytest.mark.parametrize("op", ["write", "read", "rows", "tiles"])
+@pytest.mark.parametrize("least", [-2 ** 31, -2 ** 31 + 1, -2 ** 31 + 39, -1, 2 ** 31 - 1])
+def test_offsets_of_any_32_bits(op, least):
+    """Offsets at both ends of their type: no rows for the sequences they are of, nothing touched outside the rows given."""
+    import torch
+    from qiyas_b200 import BlockCache
+    s = Setup(63, 3, 200, 2, 16, 64)
+    o, heads, rows, guard = H.ops(), 2 if op in ("write", "read") else 4, 90, 1 << 16
+    room = torch.full((rows * heads * 64 + 2 * guard,), 7.0, device="cuda")
+    x, table = room[guard:-guard].view(rows, heads, 64), gpu(s.table)
+    x.copy_(torch.randn(rows, heads, 64, device="cuda"))
+    codes = torch.full((s.k.codes.size + 2 * guard,), 7, dtype=torch.int8, device="cuda")
+    scales = torch.full((s.k.scales.size + 2 * guard,), 7.0, device="cuda")
+    codes[guard:-guard], scales[guard:-guard] = gpu(s.k.codes).reshape(-1), gpu(s.k.scales).reshape(-1)
+    cache = BlockCache(codes[guard:-guard].view(s.k.codes.shape), gpu(s.v.codes), scales[guard:-guard].view(s.k.scales.shape), gpu(s.v.scales))
+    for offsets in ([0, 40, least, 90], [0, least, least, 90], [least, 40, 60, least], [40, least, 50, 90]):
+        if op == "write":
+            o.CacheWrite(cache, x, x, table, ints([0, 10, 20]), offsets=ints(offsets))
+        elif op == "read":
+            o.CacheRead(cache, x, None, table, ints([0, 10, 20]), offsets=ints(offsets))
+        else:
+            q = torch.randn(rows, heads, 64, device="cuda")
+            o.CacheAttention(cache, q, x, table, ints([200, 150, 100]), offsets=ints(offsets), max_queries=1 if op == "rows" else 0)
+        assert o.gpu.status() == 16
+        assert (room[:guard] == 7).all() and (room[-guard:] == 7).all()
+        assert (codes[:guard] == 7).all() and (codes[-guard:] == 7).all() and (scales[:guard] == 7).all() and (scales[-guard:] == 7).all()
