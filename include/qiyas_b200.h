@@ -288,7 +288,7 @@ int qb200_ipc_close(void *ptr);
  * 32, 64 or 128 tokens, dim a multiple of 16 up to 256.  Nothing needs initialising: a block's scale and codes are read
  * only once a token of the sequence has been written into it.
  * The codes and scales may be the caller's own: a scale may be any finite number, zero and below zero too.  A scale of V that is
- * not finite makes the rows of an attention call that see its tokens NaN, and no others; scales of V more than 2^50 below
+ * not finite makes the rows of an attention call that see its tokens NaN, and no others; scales of V more than 2^85 below
  * others of the sequence and head may count as 0 there.
  *
  * qb200_sequences: `count` sequences whose rows (a row = one token of the call) lie behind one another.  table[b * width + i]

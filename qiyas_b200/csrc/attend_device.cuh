@@ -359,22 +359,21 @@ __device__ __forceinline__ float2 scales_at(const AttendArgs &p, int page, int h
     return make_float2(__ldg(p.k_scales + i), __ldg(p.v_scales + i));
 }
 // V's scales enter the weights against a reference v0, a power of two: the largest scale of those first met, rounded down.  A
-// scale more than 2^FAR above v0 sets a new reference, one more than 2^FAR below counts as 0.  So whatever the scales are, f32
-// holds a weight beside one that is 2^(2 FAR) larger by their scales and 2^35 by their scores, and the denominator of a part
-// (2^17 tokens of 2^15 * 2^FAR at most).
-constexpr int FAR = 50;
+// scale more than 2^ABOVE above v0 sets a new reference, one more than 2^BELOW below counts as 0.  So whatever the scales are, f32
+// holds a weight (2^11 at its largest) beside one that is 2^(ABOVE + BELOW) larger by their scales and 2^30 by their scores, and the
+// denominator of a part (2^17 tokens of 2^15 * 2^BELOW at most).
+constexpr int ABOVE = 10, BELOW = 85;
 __device__ __forceinline__ int exponent_of(float x) { return (__float_as_int(x) >> 23) & 255; }
 // The bits of what V's scale asks of the reference: its size, or 0 where there is nothing to measure.
 __device__ __forceinline__ uint32_t reference_of(bool there, float sv) { return there && fabsf(sv) <= 3.402823466e38f ? __float_as_uint(fabsf(sv)) : 0u; }
 __device__ __forceinline__ void raise(float &v0, uint32_t largest)       // largest: of what several scales ask
 {
     const float to = __uint_as_float(min(max(largest & 0x7f800000u, 1u << 23), 253u << 23));      // its inverse is a normal number too
-    if (largest && (v0 == 0.f || exponent_of(to) > exponent_of(v0) + FAR)) v0 = to;
+    if (largest && (v0 == 0.f || exponent_of(to) > exponent_of(v0) + ABOVE)) v0 = to;
 }
-// Where the reference rises by 2^step, the weights of what a row has seen get smaller by as much: O goes down.  A row's exponent m
-// may have stood for scales up to 2^FAR above the old reference, and against it the new tokens' weights would be f16's least
-// numbers, so m falls by FALL before the tile is looked at (2^6 is then the least that the largest new weight can be).
-constexpr float FALL = 45.f;
+// Where the reference rises by 2^step, a row's exponent m falls by as much, so that its weights stay what they are, and so does O; the
+// denominator rises, and where that would leave f32 (e: its exponent_of) m falls by less and O goes down for the rest.
+__device__ __forceinline__ int fall_of(int step, int e) { return min(step, 127 + 100 - e); }
 // How the tokens of a page are weighted.
 struct Weighted {
     float log_ratio, inverse;                  // log2(|sv| / v0), added to the scores; v0 / |sv|, a weight's part of the denominator
@@ -389,7 +388,7 @@ __device__ __forceinline__ Weighted weighted(bool there, float sv, float v0)
         w.log_ratio = -INFINITY;
         w.inverse = 0.f;
     } else if (!(fabsf(sv) <= 3.402823466e38f)) w.log_ratio = __int_as_float(0x7fffffff);     // rows that see it get NaN, others nothing of it
-    else if (exponent_of(ratio) < 127 - FAR) w.mark = MARK_ZERO;
+    else if (exponent_of(ratio) < 127 - BELOW) w.mark = MARK_ZERO;
     else {
         w.log_ratio = __log2f(ratio);
         w.inverse = __fdividef(1.f, ratio);

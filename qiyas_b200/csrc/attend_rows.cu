@@ -373,14 +373,17 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                         }
             }
             if (fabsf(sc[1]->w) != vref) {     // what V's scales are taken against: the first, seldom another
-                const float step = vref == 0.f ? 0.f : (float)(exponent_of(sc[1]->w) - exponent_of(vref));
+                const int step = vref == 0.f ? 0 : exponent_of(sc[1]->w) - exponent_of(vref);
                 vref = fabsf(sc[1]->w);
-                if (step > 0.f) {
+                if (step) {
 #pragma unroll
                     for (int nb = 0; nb < NB; nb++)
 #pragma unroll
                         for (int c = 0; c < 2; c++) {
-                            const float fall = lo[nb][c] < base + 32 && hi[nb][c] > base ? FALL : 0.f, less = exp2_fast(fall - step);
+                            int e = exponent_of(l[nb][c]);
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, d));
+                            const float fall = (float)fall_of(step, e), less = exp2_fast(fall - (float)step);
                             mm[nb][c] -= fall;
                             l[nb][c] *= exp2_fast(fall);
 #pragma unroll

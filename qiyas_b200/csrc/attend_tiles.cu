@@ -343,7 +343,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                             if (top > -INFINITY) up = ceilf(top) - 11.f;
                             fresh = top == -INFINITY;
                         } else {
-                            const float down = step > 0.f && (top > -INFINITY || l < 1.f) ? FALL : 0.f;      // (l < 1: so that v0 / l stays inside f32)
+                            const float down = step > 0.f ? (float)fall_of((int)step, exponent_of(l)) : 0.f;
                             up = top + down > 15.f ? ceilf(top) - 11.f : -down;
                             less = exp2_fast(-up);
                             o_less = exp2_fast(-up - step);
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
             T *dst = out_row<T>(p, u, min(at, u.r1 - 1));
             const float kept_less = exp2_fast(kept_mm - mm);
             const float v0 = vref > 0.f ? vref : 1.f;
-            float f = v0 * inverse_of(l);
+            float f = v0 * inverse_of(l);                        // (l is 1/2 at least where a row has seen something)
             if (!complete) {
                 if (fresh) mm = NOTHING;
                 f = part_scale(mm, l, v0);
