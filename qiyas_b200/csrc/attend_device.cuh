@@ -388,8 +388,11 @@ __device__ __forceinline__ Weighted weighted(bool there, float sv, float v0)
         w.log_ratio = -INFINITY;
         w.inverse = 0.f;
     } else if (!(fabsf(sv) <= 3.402823466e38f)) w.log_ratio = __int_as_float(0x7fffffff);     // rows that see it get NaN, others nothing of it
-    else if (exponent_of(ratio) < 127 - BELOW) w.mark = MARK_ZERO;
-    else {
+    else if (exponent_of(ratio) < 127 - BELOW) {       // as if it were the least that counts, so that it sets no row's exponent
+        w.mark = MARK_ZERO;
+        w.log_ratio = -BELOW;
+        w.inverse = __uint_as_float((uint32_t)(127 + BELOW) << 23);
+    } else {
         w.log_ratio = __log2f(ratio);
         w.inverse = __fdividef(1.f, ratio);
         w.mark = sv < 0.f ? MARK_MINUS : 0;

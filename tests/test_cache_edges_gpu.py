@@ -232,6 +232,21 @@ def test_attention_over_scales_of_very_different_sizes(kind, group, counts, dim,
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("group,counts", ROWS)
+@pytest.mark.parametrize("page,dim", [(16, 64), (16, 128), (32, 192)])
+@pytest.mark.parametrize("small", [2.0 ** -30, 2.0 ** -70])
+def test_small_scales_beside_scales_of_zero(kind, group, counts, page, dim, small):
+    """Rows that see tokens of small scales and of scales of zero, and whose neighbours see large ones: the zeros weigh in the
+    denominator alone, and what the small ones give is not lost beside them."""
+    s = Setup(64 + dim, 4, 1300, 2, page, dim)
+    for b in range(4):
+        pattern = np.array([small, 0, small, -small, 0, 0, small, 1, small, 0, 0, -1, 0, small], np.float32)
+        s.v.scales[s.table[b]] = np.resize(np.roll(pattern, b), s.width)[:, None]
+    for window in (9, page + 3, 0):
+        check(s, kind, [1300, 131, 399, 50], counts, group, window=window)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("group,counts", ROWS)
 @pytest.mark.parametrize("order", ["up", "down", "any"])
 def test_attention_over_scales_that_the_type_hardly_holds(kind, group, counts, order):
     """V's scales from f32's least numbers (what a write of subnormal values leaves) to 2^112, and with them values next to the largest."""
