@@ -564,6 +564,8 @@ int qb200_cache_attention(const qb200_cache_t *cache, const qb200_sequences_t *s
     if (!(a.scale == a.scale) || a.scale - a.scale != 0.f) return fail(QB200_E_SHAPE, "scale is not a finite number");
     if (a.max_queries < 0 || a.max_length < 0) return fail(QB200_E_SHAPE, "max_queries %d, max_length %d", a.max_queries, a.max_length);
     attention_bounds(*cache, *sequences, a);
+    // a row's first token is (tokens - rows + its place) - window: inside 32 bits
+    if ((int64_t)a.window + sequences->rows > 2147483647LL) return fail(QB200_E_LIMIT, "window %d with %d rows: together at most 2^31 - 1", a.window, sequences->rows);
     const size_t need = qb::attend_workspace_bytes(*cache, *sequences, type, a);
     if (need && (!a.workspace || a.workspace_bytes < need))
         return fail(QB200_E_WORKSPACE, "workspace of %zu bytes, %zu needed", a.workspace ? a.workspace_bytes : (size_t)0, need);

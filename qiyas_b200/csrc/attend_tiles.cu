@@ -13,7 +13,7 @@
 //  * A thread reads its row of S once and takes the weights against the exponent it has: only where one would pass 2^15 does
 //    it raise the exponent and go back over what the row has of O, by a power of two.
 //  * The registers are shared out between the warps' kinds (setmaxnreg): up to 128 dims 16-bit lanes spill nothing, f32 lanes 12 bytes,
-//    over 128 dims 72 to 76.
+//    over 128 dims all 72.
 // Scales, exponents and the cut of q and w (what it costs, and why) are those of attend_rows.cu; so are the shares of the
 // grid's blocks.  One warp takes the logarithms of V's scales; where a tile has scales of 0 or below, the stored weights are put right
 // after the fact, out of the way of the others (in their loop it took prompts from 1.18 to 1.21 ms).

@@ -3,7 +3,7 @@ where one is there and the library bound, calls that are not refused have no seq
 import numpy as np
 import pytest
 
-from .test_cache_abi import SHAPE, lanes, lib, parts, sequences        # noqa: F401 (lib: a fixture)
+from .test_cache_abi import LIMIT, SHAPE, lanes, lib, parts, sequences        # noqa: F401 (lib: a fixture)
 from qiyas_b200 import blocks as B
 
 
@@ -41,6 +41,16 @@ def test_strides_of_all_kinds(lib):                                         # no
         assert (rc == SHAPE) == overlaps(row, head, rows, heads, 64), (rows, heads, row, head)
         refused += rc == SHAPE
     assert 500 < refused < 2500
+
+
+@pytest.mark.parametrize("window,rows,refused", [(2 ** 31 - 2000, 100, False), (2 ** 31 - 3000, 3001, True), (2 ** 31 - 1, 2 ** 30, False), (2 ** 30, 2 ** 30, True), (2 ** 30, 2 ** 30 - 1, False)])
+def test_windows_and_rows_that_leave_32_bits_together(lib, window, rows, refused):      # noqa: F811
+    """Differences of a row's place and the window are taken in 32 bits; a window of all a sequence can have is none."""
+    from qiyas_b200 import _lib
+    cache, seq = parts(pages=2 ** 27 - 1, heads=1), sequences(rows=rows, count=0, width=2 ** 27 - 70)
+    args = _lib.ATTENTION(256, 64, 64, 256, 64, 64, 0, 4096, 1 << 40, 1, 0, 0, 0.125, 1, window)
+    rc = lib.qb200_cache_attention(cache, seq, B.F16, args, None)
+    assert (rc == LIMIT) == refused, (rc, lib.qb200_last_error())
 
 
 @pytest.mark.parametrize("change", [dict(max_queries=2 ** 31), dict(max_length=2 ** 40), dict(max_length=-2 ** 31 - 1), dict(window=2 ** 31), dict(max_queries=1.5),
