@@ -345,7 +345,7 @@ int qb200_cache_read(const qb200_cache_t *cache, const qb200_sequences_t *sequen
  *   the work; the results do not depend on them beyond the order of sums.  0: rows (1 without offsets), width * page.
  *   Sums, softmax statistics and the accumulators are f32; q and the weights enter the tensor cores in f16 (f32 lanes: as
  *   the sum of two f16), the codes exactly.  With 16-bit lanes that is off by less than 2^-11 of sum p |v|, the size of f16's own
- *   rounding of the output (measured: 2.9e-4 against 2.1e-4 with f32 weights at most).
+ *   rounding of the output (measured: 2.7e-4 against 2.1e-4 with f32 weights at most).
  *   workspace: device scratch of qb200_cache_attention_workspace_bytes(...) bytes, 16-byte aligned, private to the call
  *   until it completes on `stream`; the function gives 0, and workspace may be NULL, where no sequence is ever split. */
 typedef struct qb200_attention {

@@ -21,14 +21,14 @@
 //    factor is the denominator, and O = v0 * sum w cv.  The producers take logarithms and quotients, a lane a page.
 //    (|sv| is meant: where sv is below 0 the weights change sign, where it is 0 they are zeros in the second product, and a page
 //    that is not there has weights of 0 in the denominator too.)
-//    m is a whole number, so that the powers of two which parts are scaled by add to it exactly.  It is chosen so that w lies at
-//    2^10 .. 2^11 at its largest when it is set and is kept while w stays below 2^15: f16 then holds weights down to 2^-24 of the
-//    largest with all its bits and errs by 2^-35 of it below, and the accumulators are seldom rescaled.
+//    m is chosen so that w lies at 2^11 at its largest when it is set (`exponent_for`) and is kept while w stays below 2^15: f16
+//    then holds weights down to 2^-24 of the largest with all its bits and errs by 2^-35 of it below, and the accumulators are
+//    seldom rescaled.
 //  * q is scaled by a power of two to a row's maximum of 2^13 and cut to f16; with f32 lanes q and w enter as the sum of
 //    two f16 (SPL 2), which loses 2^-22.  With 16-bit lanes w is one f16, half a step of 2^-11 each, independent of one
 //    another, and out = sum w v / sum w (the denominator has all 24 bits) is off by less than 2^-11 of sum p |v|, by a third of
 //    that or less in the mean.  The output's own rounding is as large (f16) or 8 times as large (bf16).  Measured, f16, relative: prompts
-//    2.9e-4 where f32 weights give 2.1e-4, 40 rows at dim 256 2.5e-4 and 2.1e-4, 131072 tokens 2.5e-4 and 2.3e-4; bf16 1.67e-3 and
+//    2.7e-4 where f32 weights give 2.1e-4, 40 rows at dim 256 2.5e-4 and 2.1e-4, 131072 tokens 2.4e-4 and 2.1e-4; bf16 1.67e-3 and
 //    1.66e-3.  Two f16 a weight bring it to what f32 weights give and cost f16 prompts 20 % (1164 -> 1391 us), dim 256 7 %,
 //    steps 3 %, long documents 1 %: not taken, since a caller who needs more than f16's own rounding has f32 lanes.
 //
@@ -411,7 +411,7 @@ attend_rows_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__
                         float top = fmaxf(fmaxf(s[0][nb][c], s[0][nb][c + 2]), fmaxf(s[1][nb][c], s[1][nb][c + 2]));
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        const float next = fmaxf(mm[nb][c], ceilf(top) - 11.f), less = exp2_fast(mm[nb][c] - next);
+                        const float next = fmaxf(mm[nb][c], exponent_for(top, 11.f)), less = exp2_fast(mm[nb][c] - next);
                         mm[nb][c] = next;
                         l[nb][c] *= less;
 #pragma unroll

@@ -11,15 +11,16 @@
 //    the cache is converted once for the 256 rows of a block.  One warp fetches the tiles' scales.
 //  * Four softmax warps a row tile, a thread a row, with two buffers of S: the tensor pipe is a tile of tokens ahead.
 //  * A thread reads its row of S once and takes the weights against the exponent it has: only where one would pass 2^15 does
-//    it raise the exponent and go back over what the row has of O, by a power of two.
+//    it raise the exponent and go back over what the row has of O.
 //  * The registers are shared out between the warps' kinds (setmaxnreg): up to 128 dims 16-bit lanes spill nothing, f32 lanes 12 bytes,
 //    over 128 dims all 72.
 // Scales, exponents and the cut of q and w (what it costs, and why) are those of attend_rows.cu; so are the shares of the
 // grid's blocks.  One warp takes the logarithms of V's scales; where a tile has scales of 0 or below, the stored weights are put right
 // after the fact, out of the way of the others (in their loop it took prompts from 1.18 to 1.21 ms).
 //
-// Measured: 7894 queries of 32 heads (8 of the cache) over up to 8192 tokens, causal, 128 dims, bf16: 1.2 ms, 650 TFLOP/s, 39 %
-// of the library's bf16 product; 3900 of them over up to 4000 tokens: f32 626 us, at 256 dims in bf16 955 us.  Three chains are near one another there (with the work of one left out in a copy): the
+// Measured: 7894 queries of 32 heads (8 of the cache) over up to 8192 tokens, causal, 128 dims, bf16: 1.14 ms, 690 TFLOP/s, 41 %
+// of the library's bf16 product; 3900 of them over up to 4000 tokens: f32 603 us, at 256 dims in bf16 947 us.  Three chains are
+// near one another there (measured at 1.18 ms, with the work of one left out in a copy): the
 // converters 1.01 ms, the softmax 1.00 ms, the products with their barriers 0.82 ms; what they wait for is mostly
 // instructions (16 warps of four kinds, 90 KB of code).  Tried and dropped: tiles of 128 tokens with one buffer of S a row tile
 // (1.3 ms: the chain from a product through softmax to the next is not hidden), a maximum pass over S before the weights
@@ -333,18 +334,18 @@ __global__ void __launch_bounds__((TilesCfg<DC, SPL>::THREADS), 1) attend_tiles_
                         tops[q] = fmaxf(tops[q], x[16 * q + 15]);
                     }
                     const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
-                    // seldom: the exponent the weights are taken against goes up, by whole powers of two
+                    // seldom: the exponent the weights are taken against goes up
                     const bool above = fresh ? top > -INFINITY : top > 15.f;
                     const bool keep = SPL == 2 && j > 0 && j % C::KEEP == 0;
                     if (keep || step > 0.f || __any_sync(0xffffffffu, above)) {
                         // (or what V's scales are taken against does, seldom: the sums keep their values)
                         float up = 0.f, less = 1.f, o_less = 1.f;
                         if (fresh) {
-                            if (top > -INFINITY) up = ceilf(top) - 11.f;
+                            if (top > -INFINITY) up = exponent_for(top, 10.f);
                             fresh = top == -INFINITY;
                         } else {
                             const float down = step > 0.f ? (float)fall_of((int)step, exponent_of(l)) : 0.f;
-                            up = top + down > 15.f ? ceilf(top) - 11.f : -down;
+                            up = top + down > 15.f ? exponent_for(top, 10.f) : -down;
                             less = exp2_fast(-up);
                             o_less = exp2_fast(-up - step);
                         }
