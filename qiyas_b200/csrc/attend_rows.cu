@@ -33,7 +33,7 @@
 //    steps 3 %, long documents 1 %: not taken, since a caller who needs more than f16's own rounding has f32 lanes.
 //
 // Measured (bf16, 8 heads of the cache, 128 dims): 32 sequences of 500 to 8000 tokens, 4 query heads a head 64 us = 4.6 TB/s of
-// codes, 70 % of the copy peak; one of 131072 tokens, 8 a head 58 us, 71 %; a window of 1024 in f32, one row a head, 37 us, 25 %;
+// codes, 71 % of the copy peak; one of 131072 tokens, 8 a head 58 us, 71 %; a window of 1024 in f32, one row a head, 37 us, 25 %;
 // 129 tokens 7 us on the device.  Of the 64 us, 45
 // are the memory's; the partition at the start takes 3, the join's launch 4, and a piece's beginning and end 1.5 each.
 #include <cuda.h>

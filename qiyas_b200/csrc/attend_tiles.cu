@@ -18,7 +18,7 @@
 // grid's blocks.  One warp takes the logarithms of V's scales; where a tile has scales of 0 or below, the stored weights are put right
 // after the fact, out of the way of the others (in their loop it took prompts from 1.18 to 1.21 ms).
 //
-// Measured: 7894 queries of 32 heads (8 of the cache) over up to 8192 tokens, causal, 128 dims, bf16: 1.14 ms, 690 TFLOP/s, 41 %
+// Measured: 7894 queries of 32 heads (8 of the cache) over up to 8192 tokens, causal, 128 dims, bf16: 1.13 to 1.15 ms, 680 TFLOP/s, 40 %
 // of the library's bf16 product; 3900 of them over up to 4000 tokens: f32 603 us, at 256 dims in bf16 947 us.  Three chains are
 // near one another there (measured at 1.18 ms, with the work of one left out in a copy): the
 // converters 1.01 ms, the softmax 1.00 ms, the products with their barriers 0.82 ms; what they wait for is mostly
